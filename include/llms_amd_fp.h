@@ -64,7 +64,7 @@ const char* fp_status_string(int status);
 /* ABI version of this library: (major << 16) | minor. Minor 5 adds
  * fp_rmsnorm_qkv_bf16_noalloc and FP_ERR_SCRATCH, and sizes
  * fp_rmsnorm_workspace_bytes for the normalised rows of every call. Minor 6
- * adds fp_attention_bf16. */
+ * adds fp_attention_bf16. Minor 7 adds fp_token_logprobs. */
 int fp_abi_version(void);
 
 /*
@@ -324,6 +324,31 @@ int64_t fp_attention_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int6
                                      int64_t head_dim, int64_t keys);
 int fp_attention_bf16(const fp_attention_args* args, void* workspace, int64_t workspace_bytes,
                       void* stream);
+
+/*
+ * Log-probabilities of given tokens, entropy and top alternatives of every row
+ * of logits (no reference counterpart: the reference scores with torch's
+ * log_softmax), in one pass over the logits.
+ *   logits        [M, V] of dtype, row stride ld
+ *   tokens        [M] int64. A negative token asks for none (logprob 0); one of V
+ *                 or more has logprob NaN
+ *   logprob       [M] fp32: x_t - m - log l with m = max x, l = sum e^(x-m)
+ *   entropy       [M] fp32: log l - sum (x-m) e^(x-m) / l  (logits of -inf add 0)
+ *   top_ids       [M, top_k] int64, by value, ties to the lowest token; NULL with top_k 0
+ *   top_logprobs  [M, top_k] fp32
+ * Sums in fp32. A row with a NaN or +inf, or of nothing but -inf, has logprob and
+ * entropy NaN; NaN logits come first among the top. V <= 2^20, top_k <= 64 and <= V;
+ * M times the pieces of a row (at most 64, one per 16384 logits or fewer) <= 2^23.
+ * logits, tokens and outputs are aligned to their elements. workspace: at least
+ * fp_logprob_workspace_bytes(M, V, top_k), 16-byte aligned, written before it is read.
+ */
+typedef enum fp_dtype { FP_BF16 = 0, FP_F16 = 1, FP_F32 = 2 } fp_dtype;
+
+int64_t fp_logprob_workspace_bytes(int64_t M, int64_t V, int64_t top_k);
+int fp_token_logprobs(const void* logits, int dtype, int64_t ld, const int64_t* tokens,
+                      float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs,
+                      int64_t M, int64_t V, int64_t top_k,
+                      void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Per-output-channel symmetric int8 quantisation on the device (the packing

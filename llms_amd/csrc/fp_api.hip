@@ -341,7 +341,7 @@ const char* fp_status_string(int status) {
   }
 }
 
-int fp_abi_version(void) { return (1 << 16) | 6; }
+int fp_abi_version(void) { return (1 << 16) | 7; }
 
 int64_t fp_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up) {
   if (M < 1 || N < 1 || K < 1) return 0;
@@ -606,6 +606,33 @@ int fp_attention_bf16(const fp_attention_args* g, void* workspace, int64_t works
   a.pos = g->pos;
   a.pos_dev = g->pos_dev;
   return fp::launch_status(fp::launch_attention(a, D, keys, workspace, (hipStream_t)stream));
+}
+
+int64_t fp_logprob_workspace_bytes(int64_t M, int64_t V, int64_t top_k) {
+  return fp::logprob_supported(M, V, top_k) ? fp::logprob_workspace_bytes(M, V, top_k) : 0;
+}
+
+int fp_token_logprobs(const void* logits, int dtype, int64_t ld, const int64_t* tokens,
+                      float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs,
+                      int64_t M, int64_t V, int64_t top_k, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  if (dtype < FP_BF16 || dtype > FP_F32) return FP_ERR_SHAPE;
+  if (!fp::logprob_supported(M < 1 ? M + 1 : M, V, top_k)) return FP_ERR_SHAPE;
+  if (ld < V) return FP_ERR_STRIDE;
+  if (M == 0) return FP_OK;
+  if (!logits || !tokens || !logprob || !entropy || (top_k > 0 && (!top_ids || !top_logprobs)))
+    return FP_ERR_NULL;
+  const auto off = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
+  if (off(logits, dtype == FP_F32 ? 4 : 2) || off(tokens, 8) || off(logprob, 4) || off(entropy, 4) ||
+      off(top_ids, 8) || off(top_logprobs, 4))
+    return FP_ERR_STRIDE;
+  const int64_t need = fp::logprob_workspace_bytes(M, V, top_k);
+  if (workspace_bytes < need || (need > 0 && !workspace) || !fp::al16(workspace))
+    return FP_ERR_WORKSPACE;
+  fp::LogprobArgs a{};
+  a.x = logits, a.ld = ld, a.tokens = tokens, a.M = M, a.V = V, a.k = (int)top_k;
+  a.logprob = logprob, a.entropy = entropy, a.top_ids = top_ids, a.top_logprobs = top_logprobs;
+  return fp::launch_status(fp::launch_logprobs(a, dtype, workspace, (hipStream_t)stream));
 }
 
 int fp_quantize_w8_per_row(const void* w, int64_t ldw, int8_t* q, int64_t ldq, float* scale,

@@ -194,6 +194,28 @@ struct AttnArgs {
 int64_t attn_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
 int launch_attention(AttnArgs a, int64_t D, int64_t keys, void* ws, hipStream_t s);
 
+// Log-probabilities of the rows of logits x [M][V] (fp_logprob.hip).
+struct LogprobArgs {
+  const void* x;
+  int64_t ld;
+  const int64_t* tokens;
+  int64_t M, V;
+  int k;  // top alternatives per row
+  float *logprob, *entropy;
+  int64_t* top_ids;
+  float* top_logprobs;
+  // pieces of `per` elements per row; workspace: each piece's {max, sum, sum about
+  // the maximum} and sorted top keys
+  int pieces;
+  int64_t per;
+  float* stat;
+  uint64_t* keys;
+};
+bool logprob_supported(int64_t M, int64_t V, int64_t k);
+int64_t logprob_workspace_bytes(int64_t M, int64_t V, int64_t k);
+// dtype: an fp_dtype.
+int launch_logprobs(LogprobArgs a, int dtype, void* ws, hipStream_t s);
+
 // Device-side per-row int8 quantisation.
 int launch_quantize_w8(const uint16_t* w, int64_t ldw, int8_t* q, int64_t ldq,
                        float* scale, int64_t N, int64_t K, hipStream_t s);

@@ -381,6 +381,38 @@ std::tuple<at::Tensor, at::Tensor> quantize_w8(const at::Tensor& w) {
   return {q, s};
 }
 
+// ---- log-probabilities of tokens ----
+
+// x [M, V], tokens [M]: {logprob [M], entropy [M], top_ids [M, k], top_logprobs [M, k]}.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
+    const at::Tensor& x, const at::Tensor& tokens, int64_t top_k) {
+  const at::ScalarType dt = x.scalar_type();
+  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat,
+              "logits must be bfloat16, float16 or float32, got ", c10::toString(dt));
+  check_2d(x, "logits", dt);
+  TORCH_CHECK(!x.is_neg(), "logits must not be a lazily negated view");
+  const int64_t M = x.size(0), V = x.size(1);
+  TORCH_CHECK(tokens.dim() == 1 && tokens.scalar_type() == at::kLong && tokens.is_contiguous() &&
+                  tokens.size(0) == M,
+              "tokens must be a contiguous 1-D int64 tensor of ", M, " elements");
+  check_same_device(x, tokens, "tokens");
+  TORCH_CHECK(top_k >= 0, "top_k must be at least 0, got ", top_k);
+  const c10::DeviceGuard guard(x.device());
+  const at::TensorOptions f = x.options().dtype(at::kFloat), i = x.options().dtype(at::kLong);
+  at::Tensor lp = at::empty({M}, f), h = at::empty({M}, f);
+  at::Tensor ids = at::empty({M, top_k}, i), top = at::empty({M, top_k}, f);
+  const int64_t bytes = fp_logprob_workspace_bytes(M, V, top_k);
+  at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  const int dtype = dt == at::kBFloat16 ? FP_BF16 : dt == at::kHalf ? FP_F16 : FP_F32;
+  check_status(fp_token_logprobs(x.data_ptr(), dtype, M > 1 ? x.stride(0) : V,
+                                 tokens.data_ptr<int64_t>(), lp.data_ptr<float>(),
+                                 h.data_ptr<float>(), ids.data_ptr<int64_t>(),
+                                 top.data_ptr<float>(), M, V, top_k,
+                                 bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(x)),
+               "fp_token_logprobs");
+  return {lp, h, ids, top};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(llms_amd, m) {
@@ -399,6 +431,8 @@ TORCH_LIBRARY(llms_amd, m) {
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_gamma, Tensor? k_gamma, float q_eps, "
         "float k_eps, Tensor cos, Tensor sin, Tensor(a!) cache_k, Tensor(b!) cache_v, "
         "int n_heads, int start_pos, Tensor? pos) -> Tensor");
+  m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k) -> (Tensor, Tensor, Tensor, "
+        "Tensor)");
   m.def("quantize_w8(Tensor w) -> (Tensor, Tensor)");
 }
 
@@ -414,5 +448,6 @@ TORCH_LIBRARY_IMPL(llms_amd, CUDA, m) {
   m.impl("rmsnorm_qkv_w8", rmsnorm_qkv_w8);
   m.impl("rmsnorm_gate_up_silu_w8", rmsnorm_gate_up_silu_w8);
   m.impl("attention", attention);
+  m.impl("token_logprobs", token_logprobs);
   m.impl("quantize_w8", quantize_w8);
 }

@@ -38,6 +38,7 @@ from torch import nn
 
 from .kernels._eager import RMSNorm, apply_rope, attend, build_rope_tables, write_kv
 from .kernels.fused_norm import fused_rmsnorm_head
+from .kernels.logprobs import TokenLogprobs, token_logprobs
 
 
 @dataclass(frozen=True)
@@ -246,6 +247,17 @@ def teacher_forced_logits(model: Qwen3Model, tokens: list[int], device) -> torch
     ids = torch.tensor([tokens], dtype=torch.long, device=device)
     with torch.inference_mode():
         return model(ids, model.alloc_cache(len(tokens) + 4), start_pos=0)[0].float()
+
+
+def teacher_forced_logprobs(model: Qwen3Model, tokens: list[int], device, *,
+                            top_k: int = 0) -> TokenLogprobs:
+    """How likely the model finds ``tokens``, fed as one prefill: of each token but
+    the first its log-probability after the ones before it, with the entropy there
+    and the ``top_k`` most likely tokens (``[len(tokens) - 1]`` each; a HIP device)."""
+    ids = torch.tensor([tokens], dtype=torch.long, device=device)
+    with torch.inference_mode():
+        logits = model(ids, model.alloc_cache(len(tokens) + 4), start_pos=0)
+        return token_logprobs(logits[0, :-1], ids[0, 1:], top_k)
 
 
 class StepGraph:

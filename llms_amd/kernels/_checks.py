@@ -58,6 +58,14 @@ def transformed(*tensors: torch.Tensor) -> bool:
             or _functorch.peek_interpreter_stack() is not None)
 
 
+def refuse_grad(fn: str, *tensors: torch.Tensor) -> None:
+    """The inference-only operators raise where a gradient or a torch.func
+    transform would have to follow them."""
+    if transformed(*tensors):
+        raise RuntimeError(f"{fn}: no gradients or torch.func transforms; call it under "
+                           "torch.no_grad() or torch.inference_mode()")
+
+
 def autocast() -> bool:
     """Whether torch's autocast would choose the types of a matmul here."""
     return torch.is_autocast_enabled("cuda")
