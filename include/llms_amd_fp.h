@@ -64,7 +64,8 @@ const char* fp_status_string(int status);
 /* ABI version of this library: (major << 16) | minor. Minor 5 adds
  * fp_rmsnorm_qkv_bf16_noalloc and FP_ERR_SCRATCH, and sizes
  * fp_rmsnorm_workspace_bytes for the normalised rows of every call. Minor 6
- * adds fp_attention_bf16. Minor 7 adds fp_token_logprobs. */
+ * adds fp_attention_bf16. Minor 7 adds fp_token_logprobs
+ * and the 4-bit projections. */
 int fp_abi_version(void);
 
 /*
@@ -324,6 +325,49 @@ int64_t fp_attention_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int6
                                      int64_t head_dim, int64_t keys);
 int fp_attention_bf16(const fp_attention_args* args, void* workspace, int64_t workspace_bytes,
                       void* stream);
+
+/*
+ * Projections on 4-bit weights with a scale for each group of `group` (32, 64 or
+ * 128) inputs (no reference counterpart).
+ *   q  [N, ceil(K/2)] bytes, row stride ldq (bytes): byte j holds the codes of inputs
+ *      2j (low half) and 2j + 1, each code + 8; the last half byte of an odd K is unused
+ *   s  [N, ceil(K/group)] bf16, row stride lds, of five significant bits, so that
+ *      code * s is exact in bf16
+ *   y = x W^T with W[n,k] = code[n,k] * s[n, k/group], in the bf16 contract above
+ * gamma [K], when not NULL, is an RMSNorm weight applied to x first (the contract of
+ * fp_rmsnorm_qkv_bf16; eps finite and >= 0). Up to 64 rows the weights are read as they
+ * are; above that their bf16 values go to the workspace and the bf16 tiles run.
+ * A row of x with an infinity has NaN outputs (also where its codes are zero).
+ * workspace: at least fp_w4_workspace_bytes(M, N, K, gate_up), 16-byte aligned.
+ * ldq < 2^26 and lds < 2^26.
+ */
+int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up);
+
+int fp_linear_w4(const void* x, int64_t ldx, const void* gamma, float eps,
+                 const uint8_t* q, int64_t ldq, const void* s, int64_t lds, int64_t group,
+                 void* y, int64_t ldy,
+                 int64_t M, int64_t N, int64_t K,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+int fp_gate_up_silu_w4(const void* x, int64_t ldx, const void* gamma, float eps,
+                       const uint8_t* qg, int64_t ldqg, const void* sg, int64_t ldsg,
+                       const uint8_t* qu, int64_t ldqu, const void* su, int64_t ldsu,
+                       int64_t group,
+                       void* y, int64_t ldy,
+                       int64_t M, int64_t N, int64_t K,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The packing of a bf16 weight [N, K] for them (once, at swap time):
+ *   s = max |w| / 7 over the group in fp32, rounded to five significant bits (ties to
+ *       even); 0, with all codes 0, where that is under 2^-126; NaN where the group
+ *       holds an infinity or a NaN
+ *   code = rne(w / s), within -7 .. 7
+ */
+int fp_quantize_w4(const void* w, int64_t ldw,
+                   uint8_t* q, int64_t ldq, void* s, int64_t lds,
+                   int64_t N, int64_t K, int64_t group,
+                   void* stream);
 
 /*
  * Log-probabilities of given tokens, entropy and top alternatives of every row

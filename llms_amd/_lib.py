@@ -57,6 +57,11 @@ CAPI_SIGNATURES: dict[str, list] = {
                                    _I64, _P, _I64, _P],
     "fp_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64],
     "fp_attention_bf16": [_P, _P, _I64, _P],
+    "fp_w4_workspace_bytes": [_I64, _I64, _I64, ctypes.c_int],
+    "fp_linear_w4": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "fp_gate_up_silu_w4": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64,
+                           _I64, _I64, _P, _I64, _P],
+    "fp_quantize_w4": [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P],
     "fp_logprob_workspace_bytes": [_I64, _I64, _I64],
     "fp_token_logprobs": [_P, ctypes.c_int, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P],
     "fp_rmsnorm_qkv_bf16_noalloc": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P],
@@ -101,6 +106,7 @@ def capi() -> ctypes.CDLL:
                               "fp_workspace_bytes_w8": ctypes.c_int64,
                               "fp_rmsnorm_workspace_bytes": ctypes.c_int64,
                               "fp_attention_workspace_bytes": ctypes.c_int64,
+                              "fp_w4_workspace_bytes": ctypes.c_int64,
                               "fp_logprob_workspace_bytes": ctypes.c_int64}.get(name, ctypes.c_int)
             _capi = lib
         return _capi

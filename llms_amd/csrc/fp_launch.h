@@ -194,6 +194,33 @@ struct AttnArgs {
 int64_t attn_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
 int launch_attention(AttnArgs a, int64_t D, int64_t keys, void* ws, hipStream_t s);
 
+// Projections on 4-bit weights (fp_w4.hip). q: rows of ceil(K / 2) bytes, s: rows
+// of ceil(K / group) bf16 (strides in elements); gate-up has two of each.
+struct W4Args {
+  const uint16_t* x;
+  int64_t ldx;
+  const uint8_t *q0, *q1;
+  int64_t ldq0, ldq1;
+  const uint16_t *s0, *s1;
+  int64_t lds0, lds1;
+  uint16_t* y;
+  int64_t ldy;
+  int64_t M, N, K;
+  int group;  // 32, 64 or 128
+};
+constexpr int64_t kW4RowsMaxM = 64;
+// M <= kW4RowsMaxM rows of x, 16-byte aligned, of K rounded up to 8 elements (zeros past
+// K), 128 ldx and 16 ldq bytes under 2^31. aligned: weight rows on 16 bytes.
+int launch_w4_rows(const W4Args& a, bool gateup, bool aligned, hipStream_t s);
+// The weights as bf16 [N][Kp], zero from K on (Kp a multiple of 32).
+int launch_w4_dequantize(const uint8_t* q, int64_t ldq, const uint16_t* sc, int64_t lds, int group,
+                         uint16_t* out, int64_t N, int64_t K, int64_t Kp, hipStream_t s);
+// x [M][K] as [M][Kp], zero from K on (Kp a multiple of 8).
+int launch_w4_pad(const uint16_t* x, int64_t ldx, uint16_t* out, int64_t M, int64_t K, int64_t Kp,
+                  hipStream_t s);
+int launch_w4_quantize(const uint16_t* w, int64_t ldw, uint8_t* q, int64_t ldq, uint16_t* sc,
+                       int64_t lds, int64_t N, int64_t K, int group, hipStream_t s);
+
 // Log-probabilities of the rows of logits x [M][V] (fp_logprob.hip).
 struct LogprobArgs {
   const void* x;

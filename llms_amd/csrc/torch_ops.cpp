@@ -381,6 +381,83 @@ std::tuple<at::Tensor, at::Tensor> quantize_w8(const at::Tensor& w) {
   return {q, s};
 }
 
+// ---- 4-bit weights ----
+
+// Row stride of a matrix (a single row may carry any).
+int64_t ld(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// Codes q [N, ceil(K/2)] and scales s [N, ceil(K/group)] of one weight, on x's device.
+void check_w4(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s, int64_t group) {
+  check_2d(q, "q", at::kByte);
+  check_2d(s, "scale", at::kBFloat16);
+  check_same_device(x, q, "q");
+  check_same_device(x, s, "scale");
+  TORCH_CHECK(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128, got ", group);
+  const int64_t K = x.size(1);
+  TORCH_CHECK(q.size(1) == (K + 1) / 2, "q has ", q.size(1), " bytes a row, x has K = ", K);
+  TORCH_CHECK(s.size(0) == q.size(0) && s.size(1) == (K + group - 1) / group, "scale ", s.sizes(),
+              " does not fit ", q.size(0), " rows of K = ", K, " in groups of ", group);
+}
+
+const void* gamma_ptr(const at::Tensor& x, const c10::optional<at::Tensor>& gamma) {
+  if (!gamma.has_value()) return nullptr;
+  check_gamma(x, *gamma);
+  return gamma->data_ptr();
+}
+
+at::Tensor linear_w4(const at::Tensor& x, const c10::optional<at::Tensor>& gamma, double eps,
+                     const at::Tensor& q, const at::Tensor& s, int64_t group) {
+  check_2d(x, "x", at::kBFloat16);
+  check_w4(x, q, s, group);
+  const void* g = gamma_ptr(x, gamma);
+  const c10::DeviceGuard guard(x.device());
+  const int64_t M = x.size(0), K = x.size(1), N = q.size(0);
+  at::Tensor y = at::empty({M, N}, x.options());
+  const int64_t bytes = fp_w4_workspace_bytes(M, N, K, 0);
+  at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check_status(fp_linear_w4(x.data_ptr(), ld(x), g, (float)eps, q.data_ptr<uint8_t>(),
+                            ld(q), s.data_ptr(), ld(s), group, y.data_ptr(),
+                            y.stride(0), M, N, K, bytes ? ws.data_ptr() : nullptr, bytes,
+                            cur_stream(x)),
+               "fp_linear_w4");
+  return y;
+}
+
+at::Tensor gate_up_silu_w4(const at::Tensor& x, const c10::optional<at::Tensor>& gamma, double eps,
+                           const at::Tensor& qg, const at::Tensor& sg, const at::Tensor& qu,
+                           const at::Tensor& su, int64_t group) {
+  check_2d(x, "x", at::kBFloat16);
+  check_w4(x, qg, sg, group);
+  check_w4(x, qu, su, group);
+  check_pair(qg, qu, "qg", "qu");
+  const void* g = gamma_ptr(x, gamma);
+  const c10::DeviceGuard guard(x.device());
+  const int64_t M = x.size(0), K = x.size(1), N = qg.size(0);
+  at::Tensor y = at::empty({M, N}, x.options());
+  const int64_t bytes = fp_w4_workspace_bytes(M, N, K, 1);
+  at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check_status(fp_gate_up_silu_w4(x.data_ptr(), ld(x), g, (float)eps, qg.data_ptr<uint8_t>(),
+                                  ld(qg), sg.data_ptr(), ld(sg),
+                                  qu.data_ptr<uint8_t>(), ld(qu), su.data_ptr(),
+                                  ld(su), group, y.data_ptr(), y.stride(0), M, N, K,
+                                  bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(x)),
+               "fp_gate_up_silu_w4");
+  return y;
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_w4(const at::Tensor& w, int64_t group) {
+  check_2d(w, "W", at::kBFloat16);
+  TORCH_CHECK(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128, got ", group);
+  const c10::DeviceGuard guard(w.device());
+  const int64_t N = w.size(0), K = w.size(1);
+  at::Tensor q = at::empty({N, (K + 1) / 2}, w.options().dtype(at::kByte));
+  at::Tensor s = at::empty({N, (K + group - 1) / group}, w.options());
+  check_status(fp_quantize_w4(w.data_ptr(), ld(w), q.data_ptr<uint8_t>(), ld(q),
+                              s.data_ptr(), ld(s), N, K, group, cur_stream(w)),
+               "fp_quantize_w4");
+  return {q, s};
+}
+
 // ---- log-probabilities of tokens ----
 
 // x [M, V], tokens [M]: {logprob [M], entropy [M], top_ids [M, k], top_logprobs [M, k]}.
@@ -431,6 +508,10 @@ TORCH_LIBRARY(llms_amd, m) {
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_gamma, Tensor? k_gamma, float q_eps, "
         "float k_eps, Tensor cos, Tensor sin, Tensor(a!) cache_k, Tensor(b!) cache_v, "
         "int n_heads, int start_pos, Tensor? pos) -> Tensor");
+  m.def("linear_w4(Tensor x, Tensor? gamma, float eps, Tensor q, Tensor scale, int group) -> Tensor");
+  m.def("gate_up_silu_w4(Tensor x, Tensor? gamma, float eps, Tensor qg, Tensor sg, Tensor qu, "
+        "Tensor su, int group) -> Tensor");
+  m.def("quantize_w4(Tensor w, int group) -> (Tensor, Tensor)");
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k) -> (Tensor, Tensor, Tensor, "
         "Tensor)");
   m.def("quantize_w8(Tensor w) -> (Tensor, Tensor)");
@@ -448,6 +529,9 @@ TORCH_LIBRARY_IMPL(llms_amd, CUDA, m) {
   m.impl("rmsnorm_qkv_w8", rmsnorm_qkv_w8);
   m.impl("rmsnorm_gate_up_silu_w8", rmsnorm_gate_up_silu_w8);
   m.impl("attention", attention);
+  m.impl("linear_w4", linear_w4);
+  m.impl("gate_up_silu_w4", gate_up_silu_w4);
+  m.impl("quantize_w4", quantize_w4);
   m.impl("token_logprobs", token_logprobs);
   m.impl("quantize_w8", quantize_w8);
 }

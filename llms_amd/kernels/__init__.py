@@ -11,8 +11,10 @@ from .fused_norm import (fused_rmsnorm_gate_up_silu, fused_rmsnorm_gate_up_silu_
                          fused_rmsnorm_qkv, fused_rmsnorm_qkv_w8)
 from .linear import FusedLinear, fused_linear, fused_linear_w8
 from .logprobs import TokenLogprobs, token_logprobs
-from .quant import dequantize_w8, quantize_w8_per_row
+from .quant import dequantize_w4, dequantize_w8, quantize_w4, quantize_w8_per_row
 from .swap import apply_triton_kernels, prewarm_triton_kernels
+from .w4 import (fused_gate_up_silu_w4, fused_linear_w4, fused_qkv_w4, fused_rmsnorm_gate_up_silu_w4,
+                 fused_rmsnorm_qkv_w4)
 
 __all__ = [
     "FusedLinear",
@@ -32,6 +34,13 @@ __all__ = [
     "fused_gate_up_silu",
     "fused_qkv_w8",
     "fused_gate_up_silu_w8",
+    "fused_linear_w4",
+    "fused_qkv_w4",
+    "fused_gate_up_silu_w4",
+    "fused_rmsnorm_qkv_w4",
+    "fused_rmsnorm_gate_up_silu_w4",
+    "quantize_w4",
+    "dequantize_w4",
     "TokenLogprobs",
     "token_logprobs",
     "quantize_w8_per_row",

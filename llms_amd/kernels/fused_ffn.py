@@ -20,6 +20,8 @@ from torch import nn
 
 from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
+from .quant import pack_weight
+from .w4 import fused_gate_up_silu_w4, fused_rmsnorm_gate_up_silu_w4
 
 
 def triton_fused_gate_up_silu(
@@ -104,10 +106,15 @@ class TritonFFN(nn.Module):
     ``gate``/``up``/``down`` match the eager ``FFN``.
 
     ``from_eager(..., int8=True)`` keeps per-row int8 gate/up weights
-    (``qg``, ``sg``, ``qu``, ``su`` buffers) and runs the int8 kernel.
+    (``qg``, ``sg``, ``qu``, ``su`` buffers) and runs the int8 kernel, with
+    ``w4_group=32, 64 or 128`` 4-bit ones with their group scales.
     ``prenorm`` (set by ``apply_triton_kernels(..., fuse_norm=True)``) is the
     block's pre-FFN RMSNorm, run inside the projection call.
     """
+
+    # The group size of 4-bit weights, 0 for the other forms; on the class, so that a
+    # module saved whole without it loads and runs as it did.
+    w4_group = 0
 
     def __init__(self, hidden_size: int, intermediate_size: int) -> None:
         super().__init__()
@@ -121,6 +128,11 @@ class TritonFFN(nn.Module):
         """The fused projection alone: ``silu(x Wg^T) * (x Wu^T)`` (of the
         RMS-normalised x when a ``prenorm`` was fused in)."""
         pn = getattr(self, "prenorm", None)
+        if self.w4_group:
+            w = (self.qg, self.sg, self.qu, self.su)
+            if pn is not None:
+                return fused_rmsnorm_gate_up_silu_w4(x, pn.weight, pn.eps, *w, group=self.w4_group)
+            return fused_gate_up_silu_w4(x, *w, group=self.w4_group)
         if pn is not None:
             from .fused_norm import fused_rmsnorm_gate_up_silu, fused_rmsnorm_gate_up_silu_w8
 
@@ -137,20 +149,20 @@ class TritonFFN(nn.Module):
         return self.down(self.gate_up(x))
 
     @classmethod
-    def from_eager(cls, eager: nn.Module, *, int8: bool = False) -> "TritonFFN":
+    def from_eager(cls, eager: nn.Module, *, int8: bool = False, w4_group: int = 0) -> "TritonFFN":
         """Wrap a module with ``gate``/``up``/``down`` Linears, sharing their
         parameters (no copy). int8=True quantises gate and up per output row
-        and drops the bf16 gate/up modules."""
+        and drops the bf16 gate/up modules; w4_group does so in 4 bits."""
         out = cls.__new__(cls)
         nn.Module.__init__(out)
         out.down = eager.down
         out.int8 = bool(int8)
         out.prenorm = None
-        if out.int8:
-            from .quant import quantize_w8_per_row
-
-            qg, sg = quantize_w8_per_row(eager.gate.weight.detach())
-            qu, su = quantize_w8_per_row(eager.up.weight.detach())
+        if w4_group:
+            out.w4_group, out.in_features = w4_group, eager.gate.in_features
+        if out.int8 or w4_group:
+            qg, sg = pack_weight(eager.gate.weight.detach(), w4_group)
+            qu, su = pack_weight(eager.up.weight.detach(), w4_group)
             for name, t in (("qg", qg), ("sg", sg), ("qu", qu), ("su", su)):
                 out.register_buffer(name, t)
             out.gate = None

@@ -18,6 +18,8 @@ from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
 from ._eager import RMSNorm, apply_rope, attend, write_kv
 from .fused_attention import attention_core
+from .quant import pack_weight
+from .w4 import fused_qkv_w4, fused_rmsnorm_qkv_w4
 
 
 def triton_fused_qkv(
@@ -134,10 +136,15 @@ class TritonAttention(nn.Module):
     reference's causal semantics); ``o`` is the module's own Linear.
 
     With ``from_eager(..., int8=True)`` the stacked weight is kept as
-    per-row int8 (``q_qkv``, ``s_qkv`` buffers) and the int8 kernel runs.
+    per-row int8 (``q_qkv``, ``s_qkv`` buffers) and the int8 kernel runs; with
+    ``w4_group=32, 64 or 128`` in 4 bits with group scales.
     ``prenorm`` (set by ``apply_triton_kernels(..., fuse_norm=True)``) is the
     block's pre-attention RMSNorm, run inside the projection call.
     """
+
+    # The group size of 4-bit weights, 0 for the other forms; on the class, so that a
+    # module saved whole without it loads and runs as it did.
+    w4_group = 0
 
     def __init__(
         self,
@@ -164,12 +171,13 @@ class TritonAttention(nn.Module):
         self.prenorm = None
 
     @classmethod
-    def from_eager(cls, eager: nn.Module, *, int8: bool = False) -> "TritonAttention":
+    def from_eager(cls, eager: nn.Module, *, int8: bool = False, w4_group: int = 0) -> "TritonAttention":
         """Build from an eager ``Attention`` with loaded weights: row-stack
         ``[Wq; Wk; Wv]`` once, reuse ``o``, ``q_norm`` and ``k_norm`` (no copy).
 
         int8=True quantises the stacked weight per output row on the device
-        and keeps only the int8 weight and its scales.
+        and keeps only the int8 weight and its scales; w4_group does so in 4
+        bits.
         """
         out = cls.__new__(cls)
         nn.Module.__init__(out)
@@ -181,10 +189,10 @@ class TritonAttention(nn.Module):
         out.n_k = eager.num_kv_heads * eager.head_dim
         W_qkv = torch.cat([eager.q.weight, eager.k.weight, eager.v.weight], dim=0)
         out.int8 = bool(int8)
-        if out.int8:
-            from .quant import quantize_w8_per_row
-
-            q, s = quantize_w8_per_row(W_qkv.detach())
+        if w4_group:
+            out.w4_group, out.in_features = w4_group, eager.q.in_features
+        if out.int8 or w4_group:
+            q, s = pack_weight(W_qkv.detach(), w4_group)
             out.register_buffer("q_qkv", q)
             out.register_buffer("s_qkv", s)
             out.W_qkv = None
@@ -200,6 +208,11 @@ class TritonAttention(nn.Module):
         """The fused projection alone: ``(q, k, v)`` flat views (of the
         RMS-normalised x when a ``prenorm`` was fused in)."""
         pn = getattr(self, "prenorm", None)
+        if self.w4_group:
+            n = dict(n_q=self.n_q, n_k=self.n_k, group=self.w4_group)
+            if pn is not None:
+                return fused_rmsnorm_qkv_w4(x, pn.weight, pn.eps, self.q_qkv, self.s_qkv, **n)
+            return fused_qkv_w4(x, self.q_qkv, self.s_qkv, **n)
         if pn is not None:
             from .fused_norm import fused_rmsnorm_qkv, fused_rmsnorm_qkv_w8
 

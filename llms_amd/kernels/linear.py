@@ -18,6 +18,8 @@ from torch import nn
 
 from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
+from .quant import pack_weight
+from .w4 import fused_linear_w4
 
 
 def fused_linear(x: torch.Tensor, W: torch.Tensor) -> torch.Tensor:
@@ -75,8 +77,12 @@ class FusedLinear(nn.Module):
 
     bf16: keeps the wrapped Linear's ``weight`` Parameter (same state-dict
     key, no copy). int8: keeps ``q`` (int8) and ``s`` (float32 row scales)
-    buffers instead.
+    buffers instead. 4 bits: ``q`` (uint8) and ``s`` (bfloat16 group scales).
     """
+
+    # The group size of 4-bit weights, 0 for the other forms; on the class, so that a
+    # module saved whole without it loads and runs as it did.
+    w4_group = 0
 
     def __init__(self, in_features: int, out_features: int) -> None:
         super().__init__()
@@ -86,14 +92,17 @@ class FusedLinear(nn.Module):
         self.int8 = False
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.w4_group:
+            return fused_linear_w4(x, self.q, self.s, group=self.w4_group)
         if self.int8:
             return fused_linear_w8(x, self.q, self.s)
         return fused_linear(x, self.weight)
 
     @classmethod
-    def from_linear(cls, lin: nn.Linear, *, int8: bool = False) -> "FusedLinear":
+    def from_linear(cls, lin: nn.Linear, *, int8: bool = False, w4_group: int = 0) -> "FusedLinear":
         """Wrap a bias-free ``nn.Linear`` (its weight is shared, not copied);
-        ``int8=True`` quantises it per output row on its device instead."""
+        ``int8=True`` quantises it per output row on its device instead,
+        ``w4_group`` in 4 bits in groups of that many inputs."""
         if getattr(lin, "bias", None) is not None:
             raise ValueError("FusedLinear wraps bias-free Linears only")
         out = cls.__new__(cls)
@@ -101,10 +110,10 @@ class FusedLinear(nn.Module):
         out.in_features = lin.in_features
         out.out_features = lin.out_features
         out.int8 = bool(int8)
-        if out.int8:
-            from .quant import quantize_w8_per_row
-
-            q, s = quantize_w8_per_row(lin.weight.detach())
+        if w4_group:
+            out.w4_group = w4_group
+        if out.int8 or w4_group:
+            q, s = pack_weight(lin.weight.detach(), w4_group)
             out.register_buffer("q", q)
             out.register_buffer("s", s)
             out.weight = None
@@ -113,4 +122,4 @@ class FusedLinear(nn.Module):
         return out
 
     def extra_repr(self) -> str:
-        return f"in_features={self.in_features}, out_features={self.out_features}, int8={self.int8}"
+        return f"in_features={self.in_features}, out_features={self.out_features}, int8={self.int8}, w4_group={self.w4_group}"
