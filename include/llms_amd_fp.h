@@ -64,8 +64,8 @@ const char* fp_status_string(int status);
 /* ABI version of this library: (major << 16) | minor. Minor 5 adds
  * fp_rmsnorm_qkv_bf16_noalloc and FP_ERR_SCRATCH, and sizes
  * fp_rmsnorm_workspace_bytes for the normalised rows of every call. Minor 6
- * adds fp_attention_bf16. Minor 7 adds fp_token_logprobs
- * and the 4-bit projections. */
+ * adds fp_attention_bf16. Minor 7 adds fp_token_logprobs, the 4-bit projections and
+ * the 8-bit cache. */
 int fp_abi_version(void);
 
 /*
@@ -325,6 +325,68 @@ int64_t fp_attention_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int6
                                      int64_t head_dim, int64_t keys);
 int fp_attention_bf16(const fp_attention_args* args, void* workspace, int64_t workspace_bytes,
                       void* stream);
+
+/*
+ * A layer's key/value cache in 8 bits, one scale for each block of 64 positions and
+ * kv head (no reference counterpart). All buffers are contiguous, NB = ceil(cache_len /
+ * 64) blocks:
+ *   k_codes     [B][n_kv_heads][NB][64][head_dim] int8     k_scale [B][n_kv_heads][NB] fp32
+ *   v_codes     [B][n_kv_heads][NB][head_dim][64] int8     v_scale [B][n_kv_heads][NB] fp32
+ *   k_tail      [B][n_kv_heads][2][64][head_dim]  bf16     tail_block [B][n_kv_heads][2]
+ *   v_tail      [B][n_kv_heads][2][head_dim][64]  bf16       int32, -1 in a new cache
+ * A block is packed when its last position is written: with top the largest finite |x|
+ * of its 64 x head_dim entries, the scale is top / 127 and a code rne(127 x / top), the
+ * division correctly rounded; its values are code * scale. An entry that is not finite
+ * has the code -128 (a NaN) and makes the scale negative (values use its magnitude).
+ * Positions of the unfinished block are in bf16 in slot (block & 1) of the tail, which
+ * tail_block names; the last two blocks written stay there.
+ *   q, k, v    rows m = b*T + t of n_heads / n_kv_heads heads of head_dim, bf16, 8-byte
+ *              aligned, row strides ld* multiples of 4
+ *   cos, sin   [T, head_dim] bf16 (the two halves share frequencies), or both NULL: q and
+ *              k are normalised and rotated already. q_gamma, k_gamma [head_dim] bf16, or
+ *              both NULL: no QK-norm (always so without cos). Rounded as fp_attention_bf16
+ *   y          [B*T, n_heads*head_dim] bf16, contiguous
+ *   pos        position of token 0 of every sequence; pos_dev, when not NULL, replaces it
+ *              by pos_dev[b * pos_stride] (int64 on the device; pos_stride 0 or 1)
+ *   lengths    NULL, or each sequence's number of new tokens (int64 on the device), taken
+ *              into 0 .. T; the rows behind them are neither written nor attended
+ * fp_kv8_attention writes the new keys and values, then attends (scale head_dim^-0.5, key
+ * position <= query position, grouped-query heads sharing their kv head), over the
+ * cache as it then is. Rows that see no key (behind a sequence's length, at a position outside
+ * the cache) are zero. fp_kv8_write only writes. Both may start anywhere up to the
+ * number of positions written so far: what is behind is dropped. (A call that starts
+ * later than that leaves a gap: the unfinished block before it is lost.)
+ * fp_kv8_read gives k_out, v_out [B][T][n_kv_heads][head_dim] fp32, the values at
+ * positions pos .. pos+T-1 of sequences that end there (0 outside the cache).
+ * head_dim is 64 or 128; cache_len at most 2^23; codes, scales and tails 16-byte
+ * aligned. With pos, [pos, pos+T) has to lie in the cache (FP_ERR_SHAPE). Calls on one
+ * cache must not overlap. workspace: at least fp_kv8_workspace_bytes(..., keys) with keys
+ * = pos + T, or cache_len with pos_dev; 16-byte aligned; written before it is read.
+ */
+typedef struct fp_kv8_args {
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  const void *q_gamma, *k_gamma;
+  const void *cos, *sin;
+  int64_t ld_cos, ld_sin;
+  int8_t *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  void *k_tail, *v_tail;
+  int32_t* tail_block;
+  void* y;
+  int64_t B, T, n_heads, n_kv_heads, head_dim, cache_len, pos;
+  const int64_t* pos_dev;
+  int64_t pos_stride;
+  const int64_t* lengths;
+  float q_eps, k_eps;
+} fp_kv8_args;
+
+int64_t fp_kv8_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int64_t n_kv_heads,
+                               int64_t head_dim, int64_t keys);
+int fp_kv8_attention(const fp_kv8_args* args, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+int fp_kv8_write(const fp_kv8_args* args, void* stream);
+int fp_kv8_read(const fp_kv8_args* args, float* k_out, float* v_out, void* stream);
 
 /*
  * Projections on 4-bit weights with a scale for each group of `group` (32, 64 or

@@ -57,6 +57,10 @@ CAPI_SIGNATURES: dict[str, list] = {
                                    _I64, _P, _I64, _P],
     "fp_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64],
     "fp_attention_bf16": [_P, _P, _I64, _P],
+    "fp_kv8_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64],
+    "fp_kv8_attention": [_P, _P, _I64, _P],
+    "fp_kv8_write": [_P, _P],
+    "fp_kv8_read": [_P, _P, _P, _P],
     "fp_w4_workspace_bytes": [_I64, _I64, _I64, ctypes.c_int],
     "fp_linear_w4": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
     "fp_gate_up_silu_w4": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64,
@@ -106,6 +110,7 @@ def capi() -> ctypes.CDLL:
                               "fp_workspace_bytes_w8": ctypes.c_int64,
                               "fp_rmsnorm_workspace_bytes": ctypes.c_int64,
                               "fp_attention_workspace_bytes": ctypes.c_int64,
+                              "fp_kv8_workspace_bytes": ctypes.c_int64,
                               "fp_w4_workspace_bytes": ctypes.c_int64,
                               "fp_logprob_workspace_bytes": ctypes.c_int64}.get(name, ctypes.c_int)
             _capi = lib

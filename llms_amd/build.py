@@ -32,8 +32,8 @@ TORCH_OPS_SO = PKG / "_torch_ops.so"
 
 HIP_SOURCES = ["fp_api.hip", "fp_stream.hip", "fp_rows.hip", "fp_splitk.hip", "fp_tiled.hip",
                "fp_gemm.hip", "fp_scratch.hip", "fp_xpanel.hip", "fp_attn.hip", "fp_logprob.hip",
-               "fp_w4.hip"]
-HIP_HEADERS = ["fp_common.h", "fp_launch.h"]
+               "fp_w4.hip", "fp_kv8.hip"]
+HIP_HEADERS = ["fp_common.h", "fp_launch.h", "fp_norm.h", "fp_rope.h"]
 
 # gfx950 only. Packed-fp32 VALU ops (v_pk_*_f32) are disabled for all device
 # code: hipcc -O3 would otherwise form them from ordinary float code.

@@ -322,6 +322,52 @@ int check_attention(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
   return FP_OK;
 }
 
+// ---- 8-bit cache ----
+
+// The checks and the kernels' form of an 8-bit cache call: new tokens (k, v), queries
+// (q, y).
+int kv8_args(const fp_kv8_args& g, bool tokens, bool queries, Kv8Args* out) {
+  const int64_t D = g.head_dim, S = g.cache_len;
+  const int st = check_attention(g.B, g.T, queries ? g.n_heads : g.n_kv_heads, g.n_kv_heads, D);
+  if (st) return st;
+  if (S < 1 || S > (int64_t)1 << 23 || g.pos_stride < 0 || g.pos_stride > 1) return FP_ERR_SHAPE;
+  if (!g.pos_dev && (g.pos < 0 || g.pos + g.T > S)) return FP_ERR_SHAPE;
+  // workgroups of the write and of the read, in threads within 2^32
+  if (g.B * g.n_kv_heads * ((g.T + 126) / 64 + (g.T + 15) / 16) > (int64_t)1 << 23) return FP_ERR_SHAPE;
+  if (tokens && (g.ldk < g.n_kv_heads * D || g.ldv < g.n_kv_heads * D || ((g.ldk | g.ldv) & 3)))
+    return FP_ERR_STRIDE;
+  if (queries && (g.ldq < g.n_heads * D || (g.ldq & 3))) return FP_ERR_STRIDE;
+  if (g.cos && (g.ld_cos < D || g.ld_sin < D)) return FP_ERR_STRIDE;
+  if (g.cos && (!(g.q_eps >= 0.f) || !(g.k_eps >= 0.f))) return FP_ERR_SHAPE;
+  if (!g.k_codes || !g.v_codes || !g.k_scale || !g.v_scale || !g.k_tail || !g.v_tail || !g.tail_block)
+    return FP_ERR_NULL;
+  if ((tokens && (!g.k || !g.v)) || (queries && (!g.q || !g.y))) return FP_ERR_NULL;
+  if (!g.cos != !g.sin || !g.q_gamma != !g.k_gamma || (g.q_gamma && !g.cos)) return FP_ERR_NULL;
+  const auto off = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
+  for (const void* p : {(const void*)g.k_codes, (const void*)g.v_codes, (const void*)g.k_scale,
+                        (const void*)g.v_scale, (const void*)g.k_tail, (const void*)g.v_tail})
+    if (off(p, 16)) return FP_ERR_STRIDE;
+  if (off(g.tail_block, 4) || (tokens && (off(g.k, 8) || off(g.v, 8))) || (queries && (off(g.q, 8) || off(g.y, 8))) ||
+      off(g.q_gamma, 8) || off(g.k_gamma, 8) || off(g.cos, 2) || off(g.sin, 2) || off(g.pos_dev, 8) ||
+      off(g.lengths, 8))
+    return FP_ERR_STRIDE;
+  Kv8Args a{};
+  a.q = (const uint16_t*)g.q, a.k = (const uint16_t*)g.k, a.v = (const uint16_t*)g.v;
+  a.ldq = g.ldq, a.ldk = g.ldk, a.ldv = g.ldv;
+  a.gq = (const uint16_t*)g.q_gamma, a.gk = (const uint16_t*)g.k_gamma;
+  a.epsq = g.q_eps, a.epsk = g.k_eps;
+  a.cos = (const uint16_t*)g.cos, a.sin = (const uint16_t*)g.sin;
+  a.ldc = g.ld_cos, a.lds = g.ld_sin;
+  a.k_codes = g.k_codes, a.v_codes = g.v_codes, a.k_scale = g.k_scale, a.v_scale = g.v_scale;
+  a.k_tail = (uint16_t*)g.k_tail, a.v_tail = (uint16_t*)g.v_tail, a.tail_block = g.tail_block;
+  a.y = (uint16_t*)g.y;
+  a.B = (int)g.B, a.T = (int)g.T, a.Hq = queries ? (int)g.n_heads : 0, a.Hk = (int)g.n_kv_heads;
+  a.S = (int)S, a.NB = (int)((S + 63) / 64);
+  a.pos = g.pos, a.pos_dev = g.pos_dev, a.pos_stride = g.pos_stride, a.lengths = g.lengths;
+  *out = a;
+  return FP_OK;
+}
+
 // A dimension of a strided layout, in elements.
 struct Dim {
   int64_t size, stride;
@@ -675,6 +721,42 @@ int fp_attention_bf16(const fp_attention_args* g, void* workspace, int64_t works
   a.pos = g->pos;
   a.pos_dev = g->pos_dev;
   return fp::launch_status(fp::launch_attention(a, D, keys, workspace, (hipStream_t)stream));
+}
+
+int64_t fp_kv8_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int64_t n_kv_heads,
+                               int64_t head_dim, int64_t keys) {
+  if (fp::check_attention(B, T, n_heads, n_kv_heads, head_dim) || keys < 1) return 0;
+  return fp::kv8_workspace_bytes(B, T, n_heads, n_kv_heads, head_dim, keys);
+}
+
+int fp_kv8_attention(const fp_kv8_args* g, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!g) return FP_ERR_NULL;
+  fp::Kv8Args a;
+  const int st = fp::kv8_args(*g, true, true, &a);
+  if (st) return st;
+  const int64_t keys = g->pos_dev ? g->cache_len : g->pos + g->T;
+  if (!workspace || !fp::al16(workspace) ||
+      workspace_bytes < fp::kv8_workspace_bytes(g->B, g->T, g->n_heads, g->n_kv_heads, g->head_dim, keys))
+    return FP_ERR_WORKSPACE;
+  return fp::launch_status(fp::launch_kv8_attention(a, g->head_dim, keys, workspace, (hipStream_t)stream));
+}
+
+int fp_kv8_write(const fp_kv8_args* g, void* stream) {
+  if (!g) return FP_ERR_NULL;
+  fp::Kv8Args a;
+  const int st = fp::kv8_args(*g, true, false, &a);
+  if (st) return st;
+  return fp::launch_status(fp::launch_kv8_write(a, g->head_dim, (hipStream_t)stream));
+}
+
+int fp_kv8_read(const fp_kv8_args* g, float* k_out, float* v_out, void* stream) {
+  if (!g) return FP_ERR_NULL;
+  fp::Kv8Args a;
+  const int st = fp::kv8_args(*g, false, false, &a);
+  if (st) return st;
+  if (!k_out || !v_out) return FP_ERR_NULL;
+  if (!fp::al16(k_out) || !fp::al16(v_out)) return FP_ERR_STRIDE;
+  return fp::launch_status(fp::launch_kv8_read(a, g->head_dim, k_out, v_out, (hipStream_t)stream));
 }
 
 int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up) {

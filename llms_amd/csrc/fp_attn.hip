@@ -39,7 +39,7 @@
 // the tied head 1468 -> 553 us. Against 64 bits the layer's error is unchanged.
 #include "fp_common.h"
 #include "fp_launch.h"
-#include "fp_norm.h"
+#include "fp_rope.h"
 
 namespace fp {
 
@@ -78,16 +78,6 @@ __device__ __forceinline__ int first_pos(const AttnArgs& a) {
   return (int)(p < -kFar ? -kFar : p > kFar ? kFar : p);
 }
 
-// Sum over the LPH (8 or 16) consecutive lanes of a head.
-template <int LPH>
-__device__ __forceinline__ float head_sum(float v) {
-  v += dpp_f32<0xb1>(v);                            // quad_perm [1,0,3,2]
-  v += dpp_f32<0x4e>(v);                            // quad_perm [2,3,0,1]
-  v += dpp_f32<0x141>(v);                           // row_half_mirror: sums of 8
-  if constexpr (LPH == 16) v += dpp_f32<0x140>(v);  // row_mirror: sums of 16
-  return v;
-}
-
 // One head row per LPH = D / 8 lanes: lane j holds elements 4j .. 4j+3 of the
 // first half and of the second, so a rotate-half pair sits in one lane.
 // gamma NULL: no norm (the caller has normalised q and k).
@@ -110,41 +100,9 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
                               : a.v + m * a.ldv + (int64_t)hk * D;
   u32x2 lo = *reinterpret_cast<const u32x2*>(src + 4 * j);
   u32x2 hi = *reinterpret_cast<const u32x2*>(src + D / 2 + 4 * j);
-  const uint16_t* g = isq ? a.gq : a.gk;
-  if (isq || isk) {
-    uint32_t x[8] = {lo.x & 0xffffu, lo.x >> 16, lo.y & 0xffffu, lo.y >> 16,
-                     hi.x & 0xffffu, hi.x >> 16, hi.y & 0xffffu, hi.y >> 16};
-    if (g) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = bf16_bits_to_f32(x[e]);
-        s += __fmul_rn(f, f);
-      }
-      const float r = rms_scale(head_sum<LPH>(s), D, isq ? a.epsq : a.epsk);
-      const u32x2 gl = *reinterpret_cast<const u32x2*>(g + 4 * j);
-      const u32x2 gh = *reinterpret_cast<const u32x2*>(g + D / 2 + 4 * j);
-      const uint32_t gb[8] = {gl.x & 0xffffu, gl.x >> 16, gl.y & 0xffffu, gl.y >> 16,
-                              gh.x & 0xffffu, gh.x >> 16, gh.y & 0xffffu, gh.y >> 16};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = norm_bf16(x[e], gb[e], r);
-    }
-    // RoPE, each product and the sum rounded to bf16 as torch's bf16 ops do
-    const uint16_t* cr = a.cos + t * a.ldc;
-    const uint16_t* sr = a.sin + t * a.lds;
-    uint32_t y[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x1 = bf16_bits_to_f32(x[e]), x2 = bf16_bits_to_f32(x[4 + e]);
-      const int d = 4 * j + e;
-      const float c1 = bf16_bits_to_f32(cr[d]), c2 = bf16_bits_to_f32(cr[D / 2 + d]);
-      const float s1 = bf16_bits_to_f32(sr[d]), s2 = bf16_bits_to_f32(sr[D / 2 + d]);
-      y[e] = f32_to_bf16_bits(round_bf16(__fmul_rn(x1, c1)) + round_bf16(__fmul_rn(-x2, s1)));
-      y[4 + e] = f32_to_bf16_bits(round_bf16(__fmul_rn(x2, c2)) + round_bf16(__fmul_rn(x1, s2)));
-    }
-    lo = u32x2{y[0] | (y[1] << 16), y[2] | (y[3] << 16)};
-    hi = u32x2{y[4] | (y[5] << 16), y[6] | (y[7] << 16)};
-  }
+  if (isq || isk)
+    norm_rope_row<D>(lo, hi, isq ? a.gq : a.gk, isq ? a.epsq : a.epsk, a.cos + t * a.ldc,
+                     a.sin + t * a.lds, j);
   uint16_t* dst;
   if (isq) {
     dst = a.qn + (m * a.Hq + h) * D;

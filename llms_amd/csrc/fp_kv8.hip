@@ -1,0 +1,1048 @@
+// fp_kv8.hip — a key/value cache in 8 bits with one scale for each block of 64
+// tokens and head, and causal attention over it.
+//
+//   top = max |x| over a block's 64 x D finite entries,  s = top / 127
+//   code = rne(127 x / top);  the block's value is code * s
+//
+// Only whole blocks are packed, from their bf16 tokens, when the last token
+// arrives; the tokens of the unfinished block stay in bf16 in a ring of two blocks per
+// head (`tail`, `tail_block` says which block a slot holds), so what the cache
+// holds does not depend on how its tokens were cut into calls. A call that goes back
+// within the ring finds its bf16 tokens there; further back, the block's codes are
+// expanded into the ring first. Keys are held [64][D], values [D][64] (codes and
+// ring): a value column then is 16 contiguous bytes per lane of a V^T operand.
+// Code -128 stands for an entry that was not finite; a block with one has its scale
+// negated, so that only such blocks pay for the check.
+//
+//   - kv8_write_kernel: a workgroup per touched block and kv head; QK-norm and RoPE of
+//     the new keys on the way where the caller asks (and of q, in more workgroups).
+//   - kv8_rows_kernel (T * group <= 64 query rows per kv head) and kv8_tiles_kernel
+//     (prompts): S^T = K Q^T and O^T = V^T P^T as in fp_attn.hip. Tile n of a block
+//     takes keys 16 (i / 4) + 4 n + i % 4 as rows i, so that a lane's accumulators of
+//     the four tiles are keys 16 g .. 16 g + 15 of its lane group g: the order of the 16
+//     bytes it loads of a V row.
+//   - kv8_combine_kernel: sums a split's partials in split order.
+//
+// Precision: codes are exact in bf16 (keys) and fp16 (values), scores exact products
+// summed in fp32 and scaled after the sum, softmax and its sum in fp32. p enters the
+// matrix core in fp16 (2^-12 of itself, an eighth of the output's rounding): the codes
+// carry no more than 8 bits, so the parts that fp_attn.hip adds would be lost on
+// them. A block's product is scaled by s_v in fp32.
+#include "fp_common.h"
+#include "fp_launch.h"
+#include "fp_rope.h"
+
+#include <type_traits>
+
+namespace fp {
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+constexpr int kBlk = 64;
+constexpr int kKv8MaxSplit = 64;  // one lane per split in kv8_combine_kernel
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ f32x4 mfma16h(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, int64_t bytes) {
+  constexpr int kRsrcFlags = 0x00020000;  // raw buffer, 32-bit data format
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, kRsrcFlags);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
+}
+// max / sum over the four lane groups that share a row column.
+__device__ __forceinline__ float col_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float col_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// Four codes of a dword as bf16 (BAD: -128 as NaN).
+template <bool BAD>
+__device__ __forceinline__ u32x2 codes4_bf16(uint32_t w) {
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = (float)(int8_t)(w >> (8 * i));
+    if (BAD && f[i] == -128.f) f[i] = __uint_as_float(0x7fc00000u);
+  }
+  // the low halves are zero: every code has at most 8 significant bits
+  return u32x2{__builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u),
+               __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u)};
+}
+template <bool BAD>
+__device__ __forceinline__ u32x4 codes8_bf16(uint32_t a, uint32_t b) {
+  const u32x2 lo = codes4_bf16<BAD>(a), hi = codes4_bf16<BAD>(b);
+  return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+// Four codes as fp16: 1024 + (code + 128) is exact, and so is 1152 less.
+template <bool BAD>
+__device__ __forceinline__ u32x2 codes4_f16(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  u32x2 v;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t biased = __builtin_amdgcn_perm(0x64646464u, u, i ? 0x04030402u : 0x04010400u);
+    const f16x2 h = __builtin_bit_cast(f16x2, biased) + f16x2{(_Float16)-1152.f, (_Float16)-1152.f};
+    uint32_t w2 = __builtin_bit_cast(uint32_t, h);
+    if constexpr (BAD) {
+      if ((w2 & 0xffffu) == 0xd800u) w2 = (w2 & 0xffff0000u) | 0x7e00u;  // -128
+      if ((w2 >> 16) == 0xd800u) w2 = (w2 & 0xffffu) | 0x7e000000u;
+    }
+    v[i] = w2;
+  }
+  return v;
+}
+template <bool BAD>
+__device__ __forceinline__ u32x4 codes8_f16(uint32_t a, uint32_t b) {
+  const u32x2 lo = codes4_f16<BAD>(a), hi = codes4_f16<BAD>(b);
+  return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+// Eight codes at scale s as bf16 values (what a block going back into the ring holds).
+__device__ __forceinline__ u32x4 expand8(u32x2 w, float s) {
+  const float a = fabsf(s);
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = (int8_t)(w[i / 2] >> (16 * (i & 1) + 8 * e));
+      v[e] = c == -128 ? __uint_as_float(0x7fc00000u) : (float)c * a;
+    }
+    o[i] = pack_bf16x2(v[0], v[1]);
+  }
+  return o;
+}
+
+// Where one sequence's new tokens go, within 32 bits.
+struct Span {
+  int first;   // position of token 0
+  int tokens;  // of this call
+  int beg, end;  // positions written: those within the cache
+};
+__device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
+  constexpr int64_t kFar = 1 << 30;
+  const int64_t p = a.pos_dev ? a.pos_dev[b * a.pos_stride] : a.pos;
+  int64_t n = a.lengths ? a.lengths[b] : a.T;
+  n = n < 0 ? 0 : n > a.T ? a.T : n;
+  Span s;
+  s.first = (int)(p < -kFar ? -kFar : p > kFar ? kFar : p);
+  s.tokens = (int)n;
+  s.beg = s.first < 0 ? 0 : s.first;
+  s.end = s.first + s.tokens < a.S ? s.first + s.tokens : a.S;
+  if (s.end < s.beg) s.end = s.beg;
+  return s;
+}
+
+// ---- write ------------------------------------------------------------------
+
+constexpr int kVRow = kBlk + 8;  // LDS row of a value column, padded against bank conflicts
+
+template <int D>
+struct WriteLds {
+  uint16_t k[kBlk * D];
+  uint16_t v[D * kVRow];
+  float top[2][4];
+  int bad[2][4];
+};
+
+// The largest finite |x| of eight bf16, and whether one is not finite.
+__device__ __forceinline__ void top8(u32x4 v, float& top, int& bad) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float f = fabsf(__uint_as_float(e ? v[i] & 0xffff0000u : v[i] << 16));
+      if (f < INFINITY) top = fmaxf(top, f);
+      else bad = 1;
+    }
+}
+__device__ __forceinline__ u32x2 code8(u32x4 v, float top) {
+  u32x2 o = {0u, 0u};
+  const float down = top > 1.f ? 0x1p-7f : 1.f;  // 127 f stays finite
+  const float div = top * down;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float f = __uint_as_float(e ? v[i] & 0xffff0000u : v[i] << 16);
+      // 127 f is exact: a tie of the quotient is seen as one
+      const int c = !(fabsf(f) < INFINITY) ? -128 : top > 0.f ? (int)rintf(127.f * (f * down) / div) : 0;
+      o[i / 2] |= (uint32_t)(uint8_t)(int8_t)c << (16 * (i & 1) + 8 * e);
+    }
+  return o;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
+  constexpr int LPH = D / 8, RPP = 256 / LPH;  // lanes per row, rows per pass
+  __shared__ __attribute__((aligned(16))) WriteLds<D> sm;
+  const int tid = threadIdx.x, j = tid % LPH;
+
+  if ((int64_t)blockIdx.x >= (int64_t)a.B * a.Hk * a.touch) {  // q heads
+    const int64_t items = (int64_t)a.B * a.T * a.Hq;
+    int64_t item = ((int64_t)blockIdx.x - (int64_t)a.B * a.Hk * a.touch) * RPP + tid / LPH;
+    const bool live = item < items;  // dead lanes stay for the cross-lane sums
+    if (!live) item = items - 1;
+    const int64_t m = item / a.Hq, h = item - m * a.Hq, t = m % a.T;
+    const uint16_t* src = a.q + m * a.ldq + h * D;
+    u32x2 lo = *reinterpret_cast<const u32x2*>(src + 4 * j);
+    u32x2 hi = *reinterpret_cast<const u32x2*>(src + D / 2 + 4 * j);
+    norm_rope_row<D>(lo, hi, a.gq, a.epsq, a.cos + t * a.ldc, a.sin + t * a.lds, j);
+    if (!live) return;
+    uint16_t* dst = a.qn + item * D;
+    *reinterpret_cast<u32x2*>(dst + 4 * j) = lo;
+    *reinterpret_cast<u32x2*>(dst + D / 2 + 4 * j) = hi;
+    return;
+  }
+
+  const int bh = blockIdx.x / a.touch, b = bh / a.Hk, h = bh - b * a.Hk;
+  const Span s = span_of(a, b);
+  if (s.beg >= s.end) return;
+  const int fb = s.beg / kBlk, lb = (s.end - 1) / kBlk;  // blocks touched
+  const int blk = fb + (int)(blockIdx.x - (int64_t)bh * a.touch);
+  if (blk > lb) return;
+  const int row0 = blk == fb ? s.beg - fb * kBlk : 0;
+  const int row1 = blk == lb ? s.end - lb * kBlk : kBlk;
+  const int slot = blk & 1;
+  const bool complete = row1 == kBlk, in_tail = blk >= lb - 1, have_old = row0 > 0;
+  // Of the last two blocks, which stay in bf16, the one in the slot that the first
+  // block's old rows are read from is stored by that block's workgroup, after it has
+  // read them.
+  const bool old_first = s.beg % kBlk != 0 && fb < lb - 1;
+  const int after = ((lb ^ fb) & 1) ? lb - 1 : lb;  // of {lb - 1, lb}, the one in fb's slot
+  const bool tag_ok = have_old && a.tail_block[bh * 2 + slot] == blk;
+  const int64_t at = (int64_t)bh * a.NB + blk;
+  int8_t* kc = a.k_codes + at * (kBlk * D);
+  int8_t* vc = a.v_codes + at * (kBlk * D);
+  auto tail_k = [&](int sl) { return a.k_tail + ((int64_t)bh * 2 + sl) * (kBlk * D); };
+  auto tail_v = [&](int sl) { return a.v_tail + ((int64_t)bh * 2 + sl) * (kBlk * D); };
+
+  // rows r0 .. r1-1 of block w: into the ring (tail) and into LDS (lds)
+  auto put = [&](int w, int r0, int r1, bool tail, bool lds) {
+    uint16_t* tk = tail_k(w & 1);
+    uint16_t* tv = tail_v(w & 1);
+    for (int r = r0 + tid / LPH; r < r1; r += RPP) {
+      const int t = w * kBlk + r - s.first;
+      const int64_t m = (int64_t)b * a.T + t;
+      const uint16_t* ks = a.k + m * a.ldk + (int64_t)h * D;
+      const uint16_t* vs = a.v + m * a.ldv + (int64_t)h * D;
+      u32x2 lo = *reinterpret_cast<const u32x2*>(ks + 4 * j);
+      u32x2 hi = *reinterpret_cast<const u32x2*>(ks + D / 2 + 4 * j);
+      const u32x2 v0 = *reinterpret_cast<const u32x2*>(vs + 8 * j);
+      const u32x2 v1 = *reinterpret_cast<const u32x2*>(vs + 8 * j + 4);
+      if (a.cos) norm_rope_row<D>(lo, hi, a.gk, a.epsk, a.cos + t * a.ldc, a.sin + t * a.lds, j);
+      const uint32_t vv[4] = {v0.x, v0.y, v1.x, v1.y};
+      if (tail) {
+        *reinterpret_cast<u32x2*>(tk + r * D + 4 * j) = lo;
+        *reinterpret_cast<u32x2*>(tk + r * D + D / 2 + 4 * j) = hi;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tv[(8 * j + e) * kBlk + r] = (uint16_t)(vv[e / 2] >> (16 * (e & 1)));
+      }
+      if (lds) {
+        *reinterpret_cast<u32x2*>(sm.k + r * D + 4 * j) = lo;
+        *reinterpret_cast<u32x2*>(sm.k + r * D + D / 2 + 4 * j) = hi;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sm.v[(8 * j + e) * kVRow + r] = (uint16_t)(vv[e / 2] >> (16 * (e & 1)));
+      }
+    }
+  };
+
+  const bool assemble = complete || (have_old && !tag_ok);
+  if (!assemble) {  // most calls of one token: nothing but its rows
+    put(blk, row0, row1, true, false);
+    if (!have_old && tid == 0) a.tail_block[bh * 2 + slot] = blk;
+    return;
+  }
+  if (have_old) {
+    const float ksc = a.k_scale[at], vsc = a.v_scale[at];
+    for (int i = tid; i < row0 * (D / 8); i += 256) {
+      const int r = i / (D / 8), c = (i % (D / 8)) * 8;
+      *reinterpret_cast<u32x4*>(sm.k + r * D + c) =
+          tag_ok ? ld16(tail_k(slot) + r * D + c) : expand8(*reinterpret_cast<const u32x2*>(kc + r * D + c), ksc);
+    }
+    const int nc = (row0 + 7) / 8;
+    for (int i = tid; i < D * nc; i += 256) {
+      const int d = i / nc, c = (i % nc) * 8;
+      *reinterpret_cast<u32x4*>(sm.v + d * kVRow + c) =
+          tag_ok ? ld16(tail_v(slot) + d * kBlk + c) : expand8(*reinterpret_cast<const u32x2*>(vc + d * kBlk + c), vsc);
+    }
+  }
+  __syncthreads();  // the old rows' last chunk reaches into the new rows
+  put(blk, row0, row1, in_tail && !have_old && !(old_first && blk == after), true);
+  __syncthreads();
+  if (in_tail && have_old) {  // the whole block: its old rows may not be in the ring
+    for (int i = tid; i < row1 * (D / 8); i += 256)
+      reinterpret_cast<u32x4*>(tail_k(slot))[i] = reinterpret_cast<const u32x4*>(sm.k)[i];
+    const int nc = (row1 + 7) / 8;
+    for (int i = tid; i < D * nc; i += 256) {
+      const int d = i / nc, c = (i % nc) * 8;
+      *reinterpret_cast<u32x4*>(tail_v(slot) + d * kBlk + c) = *reinterpret_cast<const u32x4*>(sm.v + d * kVRow + c);
+    }
+  }
+  if (old_first && blk == fb) {
+    put(after, 0, after == lb ? s.end - lb * kBlk : kBlk, true, false);
+    if (tid == 0) a.tail_block[bh * 2 + slot] = after;
+  } else if (in_tail && !(old_first && blk == after) && tid == 0) {
+    a.tail_block[bh * 2 + slot] = blk;
+  }
+  if (!complete) return;
+
+  constexpr int NC = kBlk * D / 8 / 256;  // chunks of 8 per thread
+  u32x4 kx[NC], vx[NC];
+  float top[2] = {0.f, 0.f};
+  int bad[2] = {0, 0};
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int i = n * 256 + tid;
+    kx[n] = reinterpret_cast<const u32x4*>(sm.k)[i];
+    vx[n] = *reinterpret_cast<const u32x4*>(sm.v + (i / 8) * kVRow + (i % 8) * 8);
+    top8(kx[n], top[0], bad[0]);
+    top8(vx[n], top[1], bad[1]);
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top[w] = fmaxf(top[w], __shfl_xor(top[w], off));
+    bad[w] = __any(bad[w]);
+    if ((tid & 63) == 0) sm.top[w][tid >> 6] = top[w], sm.bad[w][tid >> 6] = bad[w];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    top[w] = fmaxf(fmaxf(sm.top[w][0], sm.top[w][1]), fmaxf(sm.top[w][2], sm.top[w][3]));
+    bad[w] = sm.bad[w][0] | sm.bad[w][1] | sm.bad[w][2] | sm.bad[w][3];
+  }
+  if (tid == 0) {
+    const float ks = top[0] / 127.f, vs = top[1] / 127.f;
+    a.k_scale[at] = bad[0] ? -ks : ks;  // -0 counts as negative
+    a.v_scale[at] = bad[1] ? -vs : vs;
+  }
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int i = n * 256 + tid;
+    reinterpret_cast<u32x2*>(kc)[i] = code8(kx[n], top[0]);
+    reinterpret_cast<u32x2*>(vc)[i] = code8(vx[n], top[1]);
+  }
+}
+
+// The values of positions pos .. pos + T - 1 of sequences that end there, in fp32:
+// a workgroup per 16 (D 128) or 32 tokens of a kv head.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Args a, float* ko, float* vo) {
+  constexpr int LPH = D / 8, RPP = 256 / LPH;
+  const int groups = (a.T + RPP - 1) / RPP;
+  const int bh = blockIdx.x / groups, b = bh / a.Hk, h = bh - b * a.Hk;
+  const int t = (int)(blockIdx.x - (int64_t)bh * groups) * RPP + threadIdx.x / LPH, j = threadIdx.x % LPH;
+  if (t >= a.T) return;
+  const Span s = span_of(a, b);
+  const int p = s.first + t;
+  float kv[8] = {}, vv[8] = {};
+  if (p >= s.beg && p < s.end) {
+    const int blk = p / kBlk, r = p % kBlk, slot = blk & 1;
+    const int64_t at = (int64_t)bh * a.NB + blk, tl = ((int64_t)bh * 2 + slot) * (kBlk * D);
+    if (blk == s.end / kBlk && a.tail_block[bh * 2 + slot] == blk) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        kv[e] = bf16_bits_to_f32(a.k_tail[tl + r * D + 8 * j + e]);
+        vv[e] = bf16_bits_to_f32(a.v_tail[tl + (8 * j + e) * kBlk + r]);
+      }
+    } else {
+      const float ks = fabsf(a.k_scale[at]), vs = fabsf(a.v_scale[at]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int kc = a.k_codes[at * (kBlk * D) + r * D + 8 * j + e];
+        const int vc = a.v_codes[at * (kBlk * D) + (8 * j + e) * kBlk + r];
+        kv[e] = kc == -128 ? __uint_as_float(0x7fc00000u) : (float)kc * ks;
+        vv[e] = vc == -128 ? __uint_as_float(0x7fc00000u) : (float)vc * vs;
+      }
+    }
+  }
+  const int64_t o = (((int64_t)b * a.T + t) * a.Hk + h) * D + 8 * j;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    reinterpret_cast<f32x4*>(ko + o)[e] = f32x4{kv[4 * e], kv[4 * e + 1], kv[4 * e + 2], kv[4 * e + 3]};
+    reinterpret_cast<f32x4*>(vo + o)[e] = f32x4{vv[4 * e], vv[4 * e + 1], vv[4 * e + 2], vv[4 * e + 3]};
+  }
+}
+
+// ---- attention --------------------------------------------------------------
+
+// Last key that query row rr (token rr / G) sees; -1: none (a token past the
+// sequence's own, or at a position outside the cache).
+__device__ __forceinline__ int last_key(const Span& s, int t) {
+  const int p = s.first + t;
+  return t < s.tokens && p >= s.beg && p < s.end ? p : -1;
+}
+
+// One softmax step over the 16 keys that a lane holds of each of its row columns:
+// scores x (in units of log 2) to probabilities, m and l updated; returns what the
+// row's earlier sums are multiplied by.
+__device__ __forceinline__ float softmax_step(f32x4 (&x)[4], float& mx, float& sum) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m = fmaxf(m, x[n][r]);
+  const float mn = fmaxf(mx, col_max(m));
+  const float base = mn == -INFINITY ? 0.f : mn;
+  const float al = exp2_fast(mx - base);
+  mx = mn;
+  float l = 0.f;
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[n][r] = exp2_fast(x[n][r] - base);
+      l += x[n][r];
+    }
+  sum = sum * al + l;
+  return al;
+}
+// Its probabilities as the two B operands of 32 keys.
+__device__ __forceinline__ void p_operands(const f32x4 (&x)[4], u32x4 (&pf)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    pf[i] = u32x4{pack_f16x2(x[2 * i][0], x[2 * i][1]), pack_f16x2(x[2 * i][2], x[2 * i][3]),
+                  pack_f16x2(x[2 * i + 1][0], x[2 * i + 1][1]), pack_f16x2(x[2 * i + 1][2], x[2 * i + 1][3])};
+}
+
+__device__ __forceinline__ int64_t part_row(const Kv8Args& a, int split, int bh, int64_t rr) {
+  return ((int64_t)split * a.B * a.Hk + bh) * ((int64_t)a.T * (a.Hq / a.Hk)) + rr;
+}
+
+// The ring's values of one block as fp16 operands at the scale 2^e that puts the largest
+// of them into [1, 2): keys from `rows` on as zeros (the ring holds anything there).
+// vb: 16 bytes of 8 keys for d block dt and half i of the lane group's 16 keys.
+template <int DT>
+__device__ __forceinline__ float tail_values(u32x4 (&v)[DT][2], int rows, int grp) {
+  float top = 0.f;
+  int bad = 0;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int key = 16 * grp + 8 * i + 2 * w;
+        if (key >= rows) v[dt][i][w] = 0u;
+        else if (key + 1 >= rows) v[dt][i][w] &= 0xffffu;
+      }
+      top8(v[dt][i], top, bad);
+    }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const uint32_t e = __float_as_uint(top) & 0x7f800000u;  // 2^floor(log2 top)
+  const float scale = e == 0u ? 1.17549435e-38f : __uint_as_float(e);
+  const float inv = 1.f / scale;  // 2^-126 .. 2^126: exact (2^127 gives a subnormal, exact too)
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        v[dt][i][w] = pack_f16x2(__uint_as_float(v[dt][i][w] << 16) * inv,
+                                 __uint_as_float(v[dt][i][w] & 0xffff0000u) * inv);
+  return scale;
+}
+
+// Decode and verify. A workgroup takes one kv head of one sequence, 16 * RT query
+// rows (token t, group head g at row t * G + g) and one contiguous range of blocks;
+// its four waves take blocks w, w + 4, ... of the range straight into registers, each
+// with the next one's loads in flight (buffers that end with the last whole block
+// return zeros past it, so loads are issued without a branch), and merge their softmax
+// states through LDS in wave order.
+template <int D, int RT>
+__global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
+  constexpr int NW = 4, DK = D / 32, DT = D / 16, KU = D / 64;
+  __shared__ __attribute__((aligned(16))) float sO[NW][16 * RT][D + 4];
+  __shared__ float sM[NW][16 * RT], sL[NW][16 * RT];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 15, grp = lane >> 4;
+  const int G = a.Hq / a.Hk, rows = a.T * G;
+  const int bh = blockIdx.y, b = bh / a.Hk, kh = bh - b * a.Hk;
+  const int row0 = blockIdx.z * 16 * RT;
+  const Span s = span_of(a, b);
+  const int end = s.beg < s.end ? s.end : 0;  // no live row: no keys
+  const int nc = (end + kBlk - 1) / kBlk, full = end / kBlk;
+  const int per = (nc + a.nsplit - 1) / a.nsplit;
+  const int c_lo = (int)blockIdx.x * per, c_hi = c_lo + per < nc ? c_lo + per : nc;
+  const int f_hi = c_hi < full ? c_hi : full;  // whole blocks of the range
+
+  // q of this lane's row columns, in the order of the keys' 16-byte loads: step
+  // 2u + h holds elements 64 u + 16 grp + 8 h ..
+  u32x4 qf[RT][DK];
+  int lim[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int rr = row0 + rt * 16 + li;
+    if (rr >= rows) rr = rows - 1;
+    const int t = rr / G, h = kh * G + (rr - t * G);
+    lim[rt] = last_key(s, t);
+    const uint16_t* qp = a.qsrc + ((int64_t)b * a.T + t) * a.ldqs + (int64_t)h * D + 16 * grp;
+#pragma unroll
+    for (int i = 0; i < DK; ++i) qf[rt][i] = ld16_any(qp + 64 * (i / 2) + 8 * (i & 1));
+  }
+
+  const int64_t at = (int64_t)bh * a.NB;
+  const __amdgpu_buffer_rsrc_t kr = make_rsrc(a.k_codes + at * (kBlk * D), (int64_t)full * (kBlk * D));
+  const __amdgpu_buffer_rsrc_t vr = make_rsrc(a.v_codes + at * (kBlk * D), (int64_t)full * (kBlk * D));
+  const __amdgpu_buffer_rsrc_t ksr = make_rsrc(a.k_scale + at, (int64_t)full * 4);
+  const __amdgpu_buffer_rsrc_t vsr = make_rsrc(a.v_scale + at, (int64_t)full * 4);
+  const uint32_t koff = (uint32_t)((16 * (li >> 2) + (li & 3)) * D + 16 * grp);
+  const uint32_t voff = (uint32_t)(li * kBlk + 16 * grp);
+
+  const float sc = kLog2e / sqrtf((float)D);
+  f32x4 o[DT][RT];
+  float mx[RT], sum[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    mx[rt] = -INFINITY;
+    sum[rt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  struct Block {
+    u32x4 k[4][KU], v[DT];
+    float ks, vs;
+  };
+  auto load = [&](Block& x, int c) {
+    const uint32_t base = c < f_hi ? (uint32_t)c * (kBlk * D) : 0x7fff0000u;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+        x.k[n][u] = __builtin_amdgcn_raw_buffer_load_b128(kr, base + koff + 4 * n * D + 64 * u, 0, 0);
+    const uint32_t sb = c < f_hi ? (uint32_t)c * 4 : 0x7fff0000u;
+    x.ks = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ksr, sb, 0, 0));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      x.v[dt] = __builtin_amdgcn_raw_buffer_load_b128(vr, base + voff + dt * 16 * kBlk, 0, 0);
+    x.vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsr, sb, 0, 0));
+  };
+  // scores of block c at factor f to probabilities; what o is multiplied by in al
+  auto softmax = [&](f32x4 (&x)[4][RT], int c, float f, u32x4 (&pf)[RT][2], float (&al)[RT]) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      f32x4 y[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          y[n][r] = c * kBlk + 16 * grp + 4 * n + r <= lim[rt] ? x[n][rt][r] * f : -INFINITY;
+      al[rt] = softmax_step(y, mx[rt], sum[rt]);
+      p_operands(y, pf[rt]);
+    }
+  };
+  auto compute = [&](const Block& x, int c, auto bad) {
+    constexpr bool BAD = decltype(bad)::value;
+    f32x4 y[4][RT];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) y[n][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 kf = codes8_bf16<BAD>(x.k[n][u][2 * h], x.k[n][u][2 * h + 1]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) y[n][rt] = mfma16(kf, qf[rt][2 * u + h], y[n][rt]);
+        }
+    }
+    u32x4 pf[RT][2];
+    float al[RT];
+    softmax(y, c, fabsf(x.ks) * sc, pf, al);
+    const float vs = fabsf(x.vs);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const u32x4 v0 = codes8_f16<BAD>(x.v[dt][0], x.v[dt][1]), v1 = codes8_f16<BAD>(x.v[dt][2], x.v[dt][3]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x4 pv = mfma16h(v0, pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        pv = mfma16h(v1, pf[rt][1], pv);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r] * al[rt]);
+      }
+    }
+  };
+  auto step = [&](const Block& x, int c) {
+    const uint32_t sign = (__float_as_uint(x.ks) | __float_as_uint(x.vs)) >> 31;
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(sign), 0)) compute(x, c, std::true_type{});
+    else compute(x, c, std::false_type{});
+  };
+
+  Block x0, x1;
+  int c = c_lo + wave;
+  load(x0, c);
+  while (c < f_hi) {
+    load(x1, c + NW);
+    step(x0, c);
+    c += NW;
+    if (c >= f_hi) break;
+    load(x0, c + NW);
+    step(x1, c);
+    c += NW;
+  }
+
+  // the unfinished block, from the ring: the wave whose turn it is
+  if (full < c_hi && c_lo <= full && ((full - c_lo) & (NW - 1)) == wave) {
+    const int64_t tl = ((int64_t)bh * 2 + (full & 1)) * (kBlk * D);
+    const uint16_t* kt = a.k_tail + tl;
+    const uint16_t* vt = a.v_tail + tl;
+    f32x4 y[4][RT];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) y[n][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DK; ++i) {
+        const u32x4 kf = ld16(kt + koff + 4 * n * D + 64 * (i / 2) + 8 * (i & 1));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) y[n][rt] = mfma16(kf, qf[rt][i], y[n][rt]);
+      }
+    }
+    u32x4 v[DT][2];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[dt][i] = ld16(vt + voff + dt * 16 * kBlk + 8 * i);
+    const float vs = tail_values<DT>(v, end - full * kBlk, grp);
+    u32x4 pf[RT][2];
+    float al[RT];
+    softmax(y, full, sc, pf, al);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x4 pv = mfma16h(v[dt][0], pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        pv = mfma16h(v[dt][1], pf[rt][1], pv);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r] * al[rt]);
+      }
+  }
+
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float l = col_sum(sum[rt]);
+    if (grp == 0) {
+      sM[wave][rt * 16 + li] = mx[rt];
+      sL[wave][rt * 16 + li] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<f32x4*>(&sO[wave][rt * 16 + li][dt * 16 + 4 * grp]) = o[dt][rt];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * RT * (D / 4); i += NW * 64) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4, rr = row0 + r;
+    if (rr >= rows) continue;
+    float m = sM[0][r];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, sM[w][r]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float e = exp2_fast(sM[w][r] - base);
+      l += e * sL[w][r];
+      v += *reinterpret_cast<const f32x4*>(&sO[w][r][d]) * e;
+    }
+    if (a.nsplit > 1) {
+      const int64_t pr = part_row(a, blockIdx.x, bh, rr);
+      *reinterpret_cast<f32x4*>(a.part + pr * D + d) = v;
+      if (d == 0) *reinterpret_cast<f32x2*>(a.stat + pr * 2) = f32x2{m, l};
+    } else {
+      const int t = rr / G, h = kh * G + (rr - t * G);
+      if (l == 0.f) v = f32x4{0.f, 0.f, 0.f, 0.f}, l = 1.f;  // a row that sees no key
+      *reinterpret_cast<u32x2*>(a.y + (((int64_t)b * a.T + t) * a.Hq + h) * D + d) =
+          u32x2{pack_bf16x2(v[0] / l, v[1] / l), pack_bf16x2(v[2] / l, v[3] / l)};
+    }
+  }
+}
+
+// Prompts. A workgroup takes one kv head of one sequence and 64 * RT query rows
+// (wave w rows 16 RT w ..), and walks its blocks: codes into registers one block ahead,
+// then converted once for the four waves into LDS (keys bf16, values fp16, both
+// double-buffered), one barrier per block. Row tiles with the most keys start first.
+template <int D, int RT>
+__global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) {
+  constexpr int DK = D / 32, DT = D / 16;
+  constexpr int NL = kBlk * D / 16 / 256;  // 16-code chunks per thread
+  constexpr int CH = D / 8;                // 16-byte chunks of a key row in LDS
+  __shared__ __attribute__((aligned(16))) char sK[2][kBlk * D * 2];
+  __shared__ __attribute__((aligned(16))) char sV[2][kBlk * D * 2];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int li = lane & 15, grp = lane >> 4;
+  const int G = a.Hq / a.Hk, rows = a.T * G;
+  const int bh = blockIdx.y, b = bh / a.Hk, kh = bh - b * a.Hk;
+  const int tile = n_rt - 1 - (int)blockIdx.x;
+  const int row0 = tile * 64 * RT + wave * 16 * RT;
+  const Span s = span_of(a, b);
+  const int end = s.beg < s.end ? s.end : 0;
+  const int full = end / kBlk;
+  // keys this workgroup's last row sees
+  int last = (tile + 1) * 64 * RT - 1;
+  if (last >= rows) last = rows - 1;
+  const int64_t seen = (int64_t)s.first + last / G + 1;
+  const int kend = seen < 0 ? 0 : seen < end ? (int)seen : end;
+  const int nt = (kend + kBlk - 1) / kBlk;
+  const int per = (nt + a.nsplit - 1) / a.nsplit;
+  const int t_lo = (int)blockIdx.z * per, t_hi = t_lo + per < nt ? t_lo + per : nt;
+
+  u32x4 qf[RT][DK];
+  int lim[RT];
+  int hi = -1;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int rr = row0 + rt * 16 + li;
+    if (rr >= rows) rr = rows - 1;
+    const int t = rr / G, h = kh * G + (rr - t * G);
+    lim[rt] = last_key(s, t);
+    hi = hi > lim[rt] ? hi : lim[rt];
+    const uint16_t* qp = a.qsrc + ((int64_t)b * a.T + t) * a.ldqs + (int64_t)h * D + 8 * grp;
+#pragma unroll
+    for (int i = 0; i < DK; ++i) qf[rt][i] = ld16_any(qp + 32 * i);
+  }
+  // the least and the largest last key of the wave's rows
+  int lo = lim[0];
+#pragma unroll
+  for (int rt = 1; rt < RT; ++rt) lo = lo < lim[rt] ? lo : lim[rt];
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) {
+    const int x = __shfl_xor(lo, off), y = __shfl_xor(hi, off);
+    lo = x < lo ? x : lo;
+    hi = y > hi ? y : hi;
+  }
+  const int lim_lo = __builtin_amdgcn_readfirstlane(lo), lim_hi = __builtin_amdgcn_readfirstlane(hi);
+
+  const int64_t at = (int64_t)bh * a.NB;
+  // LDS places: key row r's chunk c at c ^ (4 (r / 16) + r % 4) (16 rows that a read
+  // takes together differ there), value row d's chunk at c ^ (d % 8)
+  auto k_at = [](int r, int c) { return r * (D * 2) + ((c ^ (((r >> 4) * 4 + (r & 3)) & (CH - 1))) * 16); };
+  auto v_at = [](int d, int c) { return d * (kBlk * 2) + ((c ^ (d & 7)) * 16); };
+  u32x4 kx[NL], vx[NL];
+  float ksc = 0.f, vsc = 0.f;
+  auto load = [&](int kt) {
+    if (kt >= full) return;
+    const u32x4* kc = reinterpret_cast<const u32x4*>(a.k_codes + (at + kt) * (kBlk * D));
+    const u32x4* vc = reinterpret_cast<const u32x4*>(a.v_codes + (at + kt) * (kBlk * D));
+#pragma unroll
+    for (int n = 0; n < NL; ++n) kx[n] = kc[n * 256 + tid], vx[n] = vc[n * 256 + tid];
+  };
+  auto put = [&](char* k, char* v, auto bad) {
+    constexpr bool BAD = decltype(bad)::value;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int i = n * 256 + tid;
+      const int r = i / (D / 16), c = (i % (D / 16)) * 2, d = i / 4, e = (i % 4) * 2;
+      *reinterpret_cast<u32x4*>(k + k_at(r, c)) = codes8_bf16<BAD>(kx[n][0], kx[n][1]);
+      *reinterpret_cast<u32x4*>(k + k_at(r, c + 1)) = codes8_bf16<BAD>(kx[n][2], kx[n][3]);
+      *reinterpret_cast<u32x4*>(v + v_at(d, e)) = codes8_f16<BAD>(vx[n][0], vx[n][1]);
+      *reinterpret_cast<u32x4*>(v + v_at(d, e + 1)) = codes8_f16<BAD>(vx[n][2], vx[n][3]);
+    }
+  };
+  __shared__ float sTop[4];
+  // block kt (loaded before, if whole) into LDS; its scales into ks, vs
+  auto store = [&](char* k, char* v, int kt, float& ks, float& vs) {
+    if (kt < full) {
+      const float k0 = a.k_scale[at + kt], v0 = a.v_scale[at + kt];
+      if (__builtin_expect((__float_as_uint(k0) | __float_as_uint(v0)) >> 31, 0)) put(k, v, std::true_type{});
+      else put(k, v, std::false_type{});
+      ks = fabsf(k0), vs = fabsf(v0);
+      return;
+    }
+    const int64_t tl = ((int64_t)bh * 2 + (full & 1)) * (kBlk * D);
+    constexpr int NT = kBlk * D / 8 / 256;
+    const int n_rows = end - full * kBlk;
+    float top = 0.f;
+    int bad = 0;
+    u32x4 vv[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int i = n * 256 + tid;
+      *reinterpret_cast<u32x4*>(k + k_at(i / CH, i % CH)) = ld16(a.k_tail + tl + i * 8);
+      vv[n] = ld16(a.v_tail + tl + i * 8);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int key = (i % 8) * 8 + 2 * w;
+        if (key >= n_rows) vv[n][w] = 0u;
+        else if (key + 1 >= n_rows) vv[n][w] &= 0xffffu;
+      }
+      top8(vv[n], top, bad);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    __syncthreads();
+    if (lane == 0) sTop[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sTop[0], sTop[1]), fmaxf(sTop[2], sTop[3]));
+    const uint32_t e = __float_as_uint(top) & 0x7f800000u;
+    const float scale = e == 0u ? 1.17549435e-38f : __uint_as_float(e), inv = 1.f / scale;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int i = n * 256 + tid;
+      u32x4 o;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        o[w] = pack_f16x2(__uint_as_float(vv[n][w] << 16) * inv, __uint_as_float(vv[n][w] & 0xffff0000u) * inv);
+      *reinterpret_cast<u32x4*>(v + v_at(i / 8, i % 8)) = o;
+    }
+    ks = 1.f, vs = scale;
+  };
+
+  const float sc = kLog2e / sqrtf((float)D);
+  f32x4 o[DT][RT];
+  float mx[RT], sum[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    mx[rt] = -INFINITY;
+    sum[rt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto compute = [&](const char* k, const char* v, int kt, float ks, float vs) {
+    if (kt * kBlk > lim_hi) return;  // every key hidden from every row
+    f32x4 x[RT][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) x[rt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DK; ++i) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(k + k_at(16 * (li >> 2) + 4 * n + (li & 3), 4 * i + grp));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) x[rt][n] = mfma16(kf, qf[rt][i], x[rt][n]);
+      }
+    }
+    const bool mask = kt * kBlk + kBlk - 1 > lim_lo;  // uniform
+    const float f = ks * sc;
+    u32x4 pf[RT][2];
+    float al[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[rt][n][r] *= f;
+          if (mask && kt * kBlk + 16 * grp + 4 * n + r > lim[rt]) x[rt][n][r] = -INFINITY;
+        }
+      al[rt] = softmax_step(x[rt], mx[rt], sum[rt]);
+      p_operands(x[rt], pf[rt]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const u32x4 v0 = *reinterpret_cast<const u32x4*>(v + v_at(dt * 16 + li, 2 * grp));
+      const u32x4 v1 = *reinterpret_cast<const u32x4*>(v + v_at(dt * 16 + li, 2 * grp + 1));
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x4 pv = mfma16h(v0, pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        pv = mfma16h(v1, pf[rt][1], pv);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r] * al[rt]);
+      }
+    }
+  };
+
+  if (t_lo < t_hi) {
+    load(t_lo);
+    store(sK[0], sV[0], t_lo, ksc, vsc);
+    __syncthreads();
+    for (int kt = t_lo; kt < t_hi; ++kt) {
+      const int u = (kt - t_lo) & 1;
+      const bool more = kt + 1 < t_hi;
+      if (more) load(kt + 1);
+      compute(sK[u], sV[u], kt, ksc, vsc);
+      if (more) {
+        store(sK[u ^ 1], sV[u ^ 1], kt + 1, ksc, vsc);
+        __syncthreads();
+      }
+    }
+  }
+
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float l = col_sum(sum[rt]);
+    const int rr = row0 + rt * 16 + li;
+    if (rr >= rows) continue;
+    if (a.nsplit > 1) {
+      const int64_t pr = part_row(a, blockIdx.z, bh, rr);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<f32x4*>(a.part + pr * D + dt * 16 + 4 * grp) = o[dt][rt];
+      if (grp == 0) *reinterpret_cast<f32x2*>(a.stat + pr * 2) = f32x2{mx[rt], l};
+    } else {
+      const int t = rr / G, h = kh * G + (rr - t * G);
+      const bool none = l == 0.f;  // a row that sees no key
+      uint16_t* yp = a.y + (((int64_t)b * a.T + t) * a.Hq + h) * D + 4 * grp;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const f32x4 v = o[dt][rt];
+        *reinterpret_cast<u32x2*>(yp + dt * 16) =
+            none ? u32x2{0u, 0u} : u32x2{pack_bf16x2(v[0] / l, v[1] / l), pack_bf16x2(v[2] / l, v[3] / l)};
+      }
+    }
+  }
+}
+
+// One output row per workgroup: lane s of each wave holds split s's statistics; each
+// group of D / 4 threads sums every NG-th split's partials, then the groups in order.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
+  constexpr int LPR = D / 4, NG = 256 / LPR;
+  __shared__ __attribute__((aligned(16))) f32x4 part[NG][LPR];
+  const int rows = a.T * (a.Hq / a.Hk);
+  const int64_t total = (int64_t)a.B * a.Hk * rows, i = blockIdx.x;
+  const int lane = threadIdx.x & 63, grp = threadIdx.x / LPR, q = threadIdx.x % LPR;
+  const bool has = lane < a.nsplit;
+  f32x2 st = {-INFINITY, 0.f};
+  if (has) st = *reinterpret_cast<const f32x2*>(a.stat + (lane * total + i) * 2);
+  float m = st.x;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+  const float base = m == -INFINITY ? 0.f : m;
+  const float e = has ? exp2_fast(st.x - base) : 0.f;
+  float l = wave_sum(has ? e * st.y : 0.f);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < kKv8MaxSplit / NG; ++n) {
+    const int s = n * NG + grp;
+    const float w = __shfl(e, s);  // every lane takes part in the exchange
+    if (s < a.nsplit) v += *reinterpret_cast<const f32x4*>(a.part + (s * total + i) * D + q * 4) * w;
+  }
+  part[grp][q] = v;
+  __syncthreads();
+  if (grp != 0) return;
+#pragma unroll
+  for (int g = 1; g < NG; ++g) v += part[g][q];
+  if (l == 0.f) v = f32x4{0.f, 0.f, 0.f, 0.f}, l = 1.f;  // a row that sees no key
+  const int bh = (int)(i / rows), b = bh / a.Hk, kh = bh - b * a.Hk;
+  const int rr = (int)(i - (int64_t)bh * rows), G = a.Hq / a.Hk;
+  const int t = rr / G, h = kh * G + (rr - t * G);
+  *reinterpret_cast<u32x2*>(a.y + (((int64_t)b * a.T + t) * a.Hq + h) * D + q * 4) =
+      u32x2{pack_bf16x2(v[0] / l, v[1] / l), pack_bf16x2(v[2] / l, v[3] / l)};
+}
+
+// The attention kernel's shape for a call that may see `keys` keys.
+struct Kv8Plan {
+  bool rows;   // kv8_rows_kernel (else kv8_tiles_kernel)
+  int rt;      // 16-row blocks per wave
+  int n_rt;    // row groups (rows) or row tiles
+  int nsplit;  // key ranges
+};
+constexpr int kKv8RowsMax = 64;   // query rows per kv head of kv8_rows_kernel
+constexpr int kKv8Groups = 512;   // workgroups a call aims at (two per CU)
+
+Kv8Plan kv8_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t keys) {
+  Kv8Plan p;
+  const int64_t rows = T * (Hq / Hk);
+  p.rows = rows <= kKv8RowsMax;
+  if (p.rows) {
+    p.rt = rows <= 16 ? 1 : 2;
+    p.n_rt = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
+  } else {
+    p.rt = B * Hk * ((rows + 127) / 128) >= kKv8Groups ? 2 : 1;
+    p.n_rt = (int)((rows + 64 * p.rt - 1) / (64 * p.rt));
+  }
+  // no range shorter than a block for each wave, or four tiles
+  const int64_t groups = B * Hk * p.n_rt, most = (keys + 4 * kBlk - 1) / (4 * kBlk);
+  int64_t ns = kKv8Groups / groups;
+  ns = ns < most ? ns : most;
+  ns = ns < kKv8MaxSplit ? ns : kKv8MaxSplit;
+  p.nsplit = (int)(ns < 1 ? 1 : ns);
+  return p;
+}
+
+inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+
+template <int D>
+int launch_write_d(const Kv8Args& a, bool with_q, hipStream_t s) {
+  constexpr int RPP = 256 / (D / 8);
+  int64_t groups = (int64_t)a.B * a.Hk * a.touch;
+  if (with_q) groups += ((int64_t)a.B * a.T * a.Hq + RPP - 1) / RPP;
+  hipLaunchKernelGGL(kv8_write_kernel<D>, dim3((unsigned)groups), dim3(256), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+template <int D>
+int launch_kv8_d(Kv8Args a, int64_t keys, hipStream_t s) {
+  int e = launch_write_d<D>(a, a.cos != nullptr, s);
+  if (e) return e;
+  const Kv8Plan p = kv8_plan(a.B, a.T, a.Hq, a.Hk, keys);
+  const unsigned bh = (unsigned)(a.B * a.Hk);
+  if (p.rows) {
+    const dim3 grid((unsigned)p.nsplit, bh, (unsigned)p.n_rt);
+    if (p.rt == 1) hipLaunchKernelGGL((kv8_rows_kernel<D, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv8_rows_kernel<D, 2>), grid, dim3(256), 0, s, a);
+  } else {
+    const dim3 grid((unsigned)p.n_rt, bh, (unsigned)p.nsplit);
+    if (p.rt == 1) hipLaunchKernelGGL((kv8_tiles_kernel<D, 1>), grid, dim3(256), 0, s, a, p.n_rt);
+    else hipLaunchKernelGGL((kv8_tiles_kernel<D, 2>), grid, dim3(256), 0, s, a, p.n_rt);
+  }
+  e = (int)hipGetLastError();
+  if (e || p.nsplit == 1) return e;
+  hipLaunchKernelGGL(kv8_combine_kernel<D>, dim3((unsigned)((int64_t)a.B * a.T * a.Hq)), dim3(256), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+// Blocks that T new tokens can touch.
+inline int touched(int64_t T) { return (int)((T + 2 * kBlk - 2) / kBlk); }
+
+}  // namespace
+
+int64_t kv8_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys) {
+  const Kv8Plan p = kv8_plan(B, T, Hq, Hk, keys);
+  const int64_t rows = B * T * Hq;
+  int64_t b = up256(rows * D * 2);
+  if (p.nsplit > 1) b += up256(rows * p.nsplit * 8) + rows * p.nsplit * D * 4;
+  return b;
+}
+
+int launch_kv8_attention(Kv8Args a, int64_t D, int64_t keys, void* ws, hipStream_t s) {
+  const Kv8Plan p = kv8_plan(a.B, a.T, a.Hq, a.Hk, keys);
+  const int64_t rows = (int64_t)a.B * a.T * a.Hq;
+  char* w = (char*)ws;
+  a.qn = (uint16_t*)w;
+  w += up256(rows * D * 2);
+  a.stat = (float*)w;
+  if (p.nsplit > 1) w += up256(rows * p.nsplit * 8);
+  a.part = (float*)w;
+  a.nsplit = p.nsplit;
+  a.touch = touched(a.T);
+  a.qsrc = a.cos ? a.qn : a.q;
+  a.ldqs = a.cos ? (int64_t)a.Hq * D : a.ldq;
+  return D == 128 ? launch_kv8_d<128>(a, keys, s) : launch_kv8_d<64>(a, keys, s);
+}
+
+int launch_kv8_write(Kv8Args a, int64_t D, hipStream_t s) {
+  a.touch = touched(a.T);
+  return D == 128 ? launch_write_d<128>(a, false, s) : launch_write_d<64>(a, false, s);
+}
+
+int launch_kv8_read(Kv8Args a, int64_t D, float* k, float* v, hipStream_t s) {
+  const int rpp = D == 128 ? 16 : 32;
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hk * ((a.T + rpp - 1) / rpp)));
+  if (D == 128) hipLaunchKernelGGL(kv8_read_kernel<128>, grid, dim3(256), 0, s, a, k, v);
+  else hipLaunchKernelGGL(kv8_read_kernel<64>, grid, dim3(256), 0, s, a, k, v);
+  return (int)hipGetLastError();
+}
+
+}  // namespace fp

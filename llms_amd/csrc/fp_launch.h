@@ -194,6 +194,42 @@ struct AttnArgs {
 int64_t attn_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
 int launch_attention(AttnArgs a, int64_t D, int64_t keys, void* ws, hipStream_t s);
 
+// A layer's key/value cache in 8 bits and attention over it (fp_kv8.hip). q, k, v as
+// in AttnArgs; cos/sin NULL: q and k are normalised and rotated already. Codes
+// [B][Hk][NB][64][D] (keys) and [B][Hk][NB][D][64] (values), scales [B][Hk][NB], ring
+// [B][Hk][2][64][D] and [B][Hk][2][D][64] bf16 with the block in each slot, y [B T][Hq D].
+struct Kv8Args {
+  const uint16_t *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  const uint16_t *gq, *gk;
+  float epsq, epsk;
+  const uint16_t *cos, *sin;
+  int64_t ldc, lds;
+  int8_t *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  uint16_t *k_tail, *v_tail;
+  int32_t* tail_block;
+  uint16_t* y;
+  int B, T, Hq, Hk, S, NB;  // S: positions in the cache, NB: blocks
+  int64_t pos;
+  const int64_t* pos_dev;  // sequence b's first position at b * pos_stride; NULL: pos
+  int64_t pos_stride;
+  const int64_t* lengths;  // tokens of each sequence (NULL: T)
+  // set by the launchers: blocks that a call can touch; q as the attention kernels read
+  // it; workspace as in AttnArgs
+  int touch;
+  const uint16_t* qsrc;
+  int64_t ldqs;
+  uint16_t* qn;
+  float *part, *stat;
+  int nsplit;
+};
+int64_t kv8_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
+int launch_kv8_attention(Kv8Args a, int64_t D, int64_t keys, void* ws, hipStream_t s);
+int launch_kv8_write(Kv8Args a, int64_t D, hipStream_t s);
+// k, v [B][T][Hk][D] fp32.
+int launch_kv8_read(Kv8Args a, int64_t D, float* k, float* v, hipStream_t s);
+
 // Projections on 4-bit weights (fp_w4.hip). q: rows of ceil(K / 2) bytes, s: rows
 // of ceil(K / group) bf16 (strides in elements); gate-up has two of each.
 struct W4Args {

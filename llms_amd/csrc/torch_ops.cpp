@@ -381,6 +381,141 @@ std::tuple<at::Tensor, at::Tensor> quantize_w8(const at::Tensor& w) {
   return {q, s};
 }
 
+// ---- 8-bit cache ----
+
+// The seven buffers of a layer's cache: codes, scales and tails of keys and values, the
+// blocks in the tails. Fills the cache part of the call for its first B sequences.
+fp_kv8_args kv8_cache(const at::TensorList c, int64_t cache_len, int64_t B) {
+  TORCH_CHECK(c.size() == 7, "an 8-bit cache has 7 buffers, got ", c.size());
+  const at::ScalarType types[7] = {at::kChar,  at::kChar,     at::kFloat, at::kFloat,
+                                   at::kBFloat16, at::kBFloat16, at::kInt};
+  TORCH_CHECK(c[0].dim() == 5, "key codes must be 5-D, got ", c[0].dim(), "-D");
+  const int64_t mb = c[0].size(0), H = c[0].size(1), D = c[0].size(4), NB = (cache_len + 63) / 64;
+  const std::vector<int64_t> sizes[7] = {{mb, H, NB, 64, D}, {mb, H, NB, D, 64}, {mb, H, NB},
+                                         {mb, H, NB},        {mb, H, 2, 64, D},  {mb, H, 2, D, 64},
+                                         {mb, H, 2}};
+  for (int i = 0; i < 7; ++i) {
+    TORCH_CHECK(c[i].scalar_type() == types[i] && c[i].sizes() == at::IntArrayRef(sizes[i]) && c[i].is_contiguous(),
+                "buffer ", i, " of the 8-bit cache must be a contiguous ", c10::toString(types[i]),
+                " tensor of ", at::IntArrayRef(sizes[i]), ", got ", c10::toString(c[i].scalar_type()), " ",
+                c[i].sizes());
+    TORCH_CHECK(c[i].is_cuda() && c[i].device() == c[0].device(), "the 8-bit cache must be on one HIP device");
+  }
+  TORCH_CHECK(B >= 1 && B <= mb, "the 8-bit cache holds ", mb, " sequences, the call has ", B);
+  fp_kv8_args a{};
+  a.k_codes = c[0].data_ptr<int8_t>(), a.v_codes = c[1].data_ptr<int8_t>();
+  a.k_scale = c[2].data_ptr<float>(), a.v_scale = c[3].data_ptr<float>();
+  a.k_tail = c[4].data_ptr(), a.v_tail = c[5].data_ptr(), a.tail_block = c[6].data_ptr<int32_t>();
+  a.B = B, a.n_kv_heads = H, a.head_dim = D, a.cache_len = cache_len;
+  return a;
+}
+
+// Where the call's tokens go: pos (0-D or [B]) or start_pos, and lengths [B].
+void kv8_place(fp_kv8_args& a, const at::Tensor& on, int64_t start_pos,
+               const c10::optional<at::Tensor>& pos, const c10::optional<at::Tensor>& lengths) {
+  const auto check = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.scalar_type() == at::kLong && t.device() == on.device() && t.is_contiguous() &&
+                    t.dim() == 1 && t.size(0) == a.B,
+                name, " must be a contiguous int64 tensor of ", a.B, " elements on ", on.device());
+  };
+  a.pos = start_pos;
+  if (pos.has_value()) {
+    if (pos->dim() == 0) {
+      TORCH_CHECK(pos->scalar_type() == at::kLong && pos->device() == on.device(),
+                  "start_pos must be an int64 tensor on ", on.device());
+    } else {
+      check(*pos, "start_pos");
+      a.pos_stride = 1;
+    }
+    a.pos_dev = pos->data_ptr<int64_t>();
+  }
+  if (lengths.has_value()) {
+    check(*lengths, "lengths");
+    a.lengths = lengths->data_ptr<int64_t>();
+  }
+}
+
+// k, v [B, T, H * D] rows of the call (token_rows-shaped: the wrapper sees to it).
+void kv8_tokens(fp_kv8_args& a, const at::Tensor& k, const at::Tensor& v, const at::Tensor& on) {
+  const int64_t n = a.n_kv_heads * a.head_dim;
+  for (const at::Tensor* t : {&k, &v})
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->device() == on.device() && !t->is_neg(),
+                "keys and values must be bfloat16 on ", on.device());
+  a.ldk = token_rows(k, a.B, a.T, n);
+  a.ldv = token_rows(v, a.B, a.T, n);
+  TORCH_CHECK(a.ldk >= 0 && a.ldv >= 0, "keys ", k.sizes(), " ", k.strides(), " and values ", v.sizes(), " ",
+              v.strides(), " must be rows of ", n, " for ", a.B, " sequences of ", a.T, " tokens");
+  a.k = k.data_ptr(), a.v = v.data_ptr();
+}
+
+at::Tensor attention_kv8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                         const c10::optional<at::Tensor>& q_gamma,
+                         const c10::optional<at::Tensor>& k_gamma, double q_eps, double k_eps,
+                         const c10::optional<at::Tensor>& cos, const c10::optional<at::Tensor>& sin,
+                         at::TensorList cache, int64_t cache_len, int64_t start_pos,
+                         const c10::optional<at::Tensor>& pos,
+                         const c10::optional<at::Tensor>& lengths) {
+  TORCH_CHECK(q.dim() == 3 && q.is_cuda(), "q must be [B, T, heads * D] on a HIP device");
+  fp_kv8_args a = kv8_cache(cache, cache_len, q.size(0));
+  TORCH_CHECK(cache[0].device() == q.device(), "q and the cache must be on one device");
+  a.T = q.size(1);
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 && !q.is_neg() && q.size(2) % a.head_dim == 0,
+              "q must be bfloat16 rows of whole heads of ", a.head_dim);
+  a.n_heads = q.size(2) / a.head_dim;
+  a.ldq = token_rows(q, a.B, a.T, q.size(2));
+  TORCH_CHECK(a.ldq >= 0, "q ", q.sizes(), " ", q.strides(), " must be rows of whole heads");
+  a.q = q.data_ptr();
+  kv8_tokens(a, k, v, q);
+  kv8_place(a, q, start_pos, pos, lengths);
+  const auto row = [&](const c10::optional<at::Tensor>& t, int64_t rows, const char* name) -> const void* {
+    if (!t.has_value()) return nullptr;
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->device() == q.device() && !t->is_neg() &&
+                    (rows ? t->dim() == 2 && t->size(0) == rows && t->size(1) == a.head_dim
+                          : t->dim() == 1 && t->size(0) == a.head_dim) &&
+                    t->stride(-1) == 1,
+                name, " has the wrong type, device, shape or stride");
+    return t->data_ptr();
+  };
+  a.q_gamma = row(q_gamma, 0, "q_gamma"), a.k_gamma = row(k_gamma, 0, "k_gamma");
+  a.cos = row(cos, a.T, "cos"), a.sin = row(sin, a.T, "sin");
+  if (a.cos && a.sin && a.T > 1) a.ld_cos = cos->stride(0), a.ld_sin = sin->stride(0);
+  else a.ld_cos = a.ld_sin = a.head_dim;
+  a.q_eps = (float)q_eps, a.k_eps = (float)k_eps;
+  const c10::DeviceGuard guard(q.device());
+  const int64_t keys = a.pos_dev ? cache_len : start_pos + a.T;
+  const int64_t bytes = fp_kv8_workspace_bytes(a.B, a.T, a.n_heads, a.n_kv_heads, a.head_dim, keys);
+  at::Tensor y = at::empty({a.B, a.T, q.size(2)}, q.options());
+  at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  a.y = y.data_ptr();
+  check_status(fp_kv8_attention(&a, bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(q)), "fp_kv8_attention");
+  return y;
+}
+
+void write_kv8(const at::Tensor& k, const at::Tensor& v, at::TensorList cache, int64_t cache_len,
+               int64_t start_pos, const c10::optional<at::Tensor>& pos,
+               const c10::optional<at::Tensor>& lengths) {
+  TORCH_CHECK(k.dim() == 3 && k.is_cuda(), "k must be [B, T, heads * D] on a HIP device");
+  fp_kv8_args a = kv8_cache(cache, cache_len, k.size(0));
+  TORCH_CHECK(cache[0].device() == k.device(), "k and the cache must be on one device");
+  a.T = k.size(1);
+  kv8_tokens(a, k, v, k);
+  kv8_place(a, k, start_pos, pos, lengths);
+  const c10::DeviceGuard guard(k.device());
+  check_status(fp_kv8_write(&a, cur_stream(k)), "fp_kv8_write");
+}
+
+std::tuple<at::Tensor, at::Tensor> read_kv8(at::TensorList cache, int64_t cache_len, int64_t B,
+                                            int64_t T, int64_t start_pos,
+                                            const c10::optional<at::Tensor>& pos) {
+  fp_kv8_args a = kv8_cache(cache, cache_len, B);
+  a.T = T;
+  kv8_place(a, cache[0], start_pos, pos, c10::nullopt);
+  const c10::DeviceGuard guard(cache[0].device());
+  at::Tensor k = at::empty({B, T, a.n_kv_heads, a.head_dim}, cache[2].options()), v = at::empty_like(k);
+  check_status(fp_kv8_read(&a, k.data_ptr<float>(), v.data_ptr<float>(), cur_stream(cache[0])), "fp_kv8_read");
+  return {k, v};
+}
+
 // ---- 4-bit weights ----
 
 // Row stride of a matrix (a single row may carry any).
@@ -508,6 +643,13 @@ TORCH_LIBRARY(llms_amd, m) {
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_gamma, Tensor? k_gamma, float q_eps, "
         "float k_eps, Tensor cos, Tensor sin, Tensor(a!) cache_k, Tensor(b!) cache_v, "
         "int n_heads, int start_pos, Tensor? pos) -> Tensor");
+  m.def("attention_kv8(Tensor q, Tensor k, Tensor v, Tensor? q_gamma, Tensor? k_gamma, float q_eps, "
+        "float k_eps, Tensor? cos, Tensor? sin, Tensor(a!)[] cache, int cache_len, int start_pos, "
+        "Tensor? pos, Tensor? lengths) -> Tensor");
+  m.def("write_kv8(Tensor k, Tensor v, Tensor(a!)[] cache, int cache_len, int start_pos, Tensor? pos, "
+        "Tensor? lengths) -> ()");
+  m.def("read_kv8(Tensor[] cache, int cache_len, int B, int T, int start_pos, Tensor? pos) -> "
+        "(Tensor, Tensor)");
   m.def("linear_w4(Tensor x, Tensor? gamma, float eps, Tensor q, Tensor scale, int group) -> Tensor");
   m.def("gate_up_silu_w4(Tensor x, Tensor? gamma, float eps, Tensor qg, Tensor sg, Tensor qu, "
         "Tensor su, int group) -> Tensor");
@@ -529,6 +671,9 @@ TORCH_LIBRARY_IMPL(llms_amd, CUDA, m) {
   m.impl("rmsnorm_qkv_w8", rmsnorm_qkv_w8);
   m.impl("rmsnorm_gate_up_silu_w8", rmsnorm_gate_up_silu_w8);
   m.impl("attention", attention);
+  m.impl("attention_kv8", attention_kv8);
+  m.impl("write_kv8", write_kv8);
+  m.impl("read_kv8", read_kv8);
   m.impl("linear_w4", linear_w4);
   m.impl("gate_up_silu_w4", gate_up_silu_w4);
   m.impl("quantize_w4", quantize_w4);

@@ -38,6 +38,7 @@ from torch import nn
 
 from .kernels._eager import RMSNorm, apply_rope, attend, build_rope_tables, write_kv
 from .kernels.fused_norm import fused_rmsnorm_head
+from .kernels.kv8 import KVCache8
 from .kernels.logprobs import TokenLogprobs, token_logprobs
 
 
@@ -85,6 +86,8 @@ class Attention(nn.Module):
         self.k_norm = RMSNorm(c.head_dim, eps=c.rms_norm_eps)
 
     def forward(self, x, *, kv_cache, layer_idx, cos, sin, start_pos):
+        if isinstance(kv_cache, KVCache8):
+            raise TypeError("an 8-bit cache needs the fused attention: apply_triton_kernels(model) first")
         B, T, _ = x.shape
         q = self.q(x).view(B, T, self.num_heads, self.head_dim)
         k = self.k(x).view(B, T, self.num_kv_heads, self.head_dim)
@@ -142,9 +145,14 @@ class Qwen3Model(nn.Module):
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
 
-    def alloc_cache(self, max_seq_len: int, *, max_batch: int = 1) -> KVCache:
+    def alloc_cache(self, max_seq_len: int, *, max_batch: int = 1, kv8: bool = False) -> KVCache | KVCache8:
+        """A cache for up to ``max_batch`` sequences; ``kv8``: in 8 bits (a swapped
+        model on a HIP device)."""
         c = self.cfg
         w = self.embed.weight
+        if kv8:
+            return KVCache8.alloc(c.num_hidden_layers, max_seq_len, max_batch=max_batch,
+                                  n_kv_heads=c.num_key_value_heads, head_dim=c.head_dim, device=w.device)
         shape = (max_batch, c.num_key_value_heads, max_seq_len, c.head_dim)
         mk = lambda: [torch.zeros(shape, dtype=w.dtype, device=w.device)  # noqa: E731
                       for _ in range(c.num_hidden_layers)]
@@ -226,10 +234,11 @@ def random_model(c: Cfg, *, device="cuda", seed: int = 0, dtype=torch.bfloat16) 
     return m.to(device=device, dtype=dtype).eval()
 
 
-def greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device) -> list[int]:
+def greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device, *,
+                    kv8: bool = False) -> list[int]:
     """Prefill the prompt, then decode n_new tokens one at a time (argmax)."""
     ids = torch.tensor([prompt], dtype=torch.long, device=device)
-    cache = model.alloc_cache(len(prompt) + n_new + 4)
+    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8)
     out: list[int] = []
     with torch.inference_mode():
         logits = model(ids, cache, start_pos=0)
@@ -249,14 +258,15 @@ def teacher_forced_logits(model: Qwen3Model, tokens: list[int], device) -> torch
         return model(ids, model.alloc_cache(len(tokens) + 4), start_pos=0)[0].float()
 
 
-def teacher_forced_logprobs(model: Qwen3Model, tokens: list[int], device, *,
-                            top_k: int = 0) -> TokenLogprobs:
+def teacher_forced_logprobs(model: Qwen3Model, tokens: list[int], device, *, top_k: int = 0,
+                            kv8: bool = False) -> TokenLogprobs:
     """How likely the model finds ``tokens``, fed as one prefill: of each token but
     the first its log-probability after the ones before it, with the entropy there
-    and the ``top_k`` most likely tokens (``[len(tokens) - 1]`` each; a HIP device)."""
+    and the ``top_k`` most likely tokens (``[len(tokens) - 1]`` each; a HIP device).
+    With ``kv8`` over an 8-bit cache."""
     ids = torch.tensor([tokens], dtype=torch.long, device=device)
     with torch.inference_mode():
-        logits = model(ids, model.alloc_cache(len(tokens) + 4), start_pos=0)
+        logits = model(ids, model.alloc_cache(len(tokens) + 4, kv8=kv8), start_pos=0)
         return token_logprobs(logits[0, :-1], ids[0, 1:], top_k)
 
 
@@ -266,19 +276,27 @@ class StepGraph:
     position: ``step(ids, pos)`` copies the tokens and the position into the
     graph's static buffers, replays, and returns the static logits tensor
     (overwritten by the next replay). The warm-up runs before capture write
-    the last T positions of the cache, so callers keep those free."""
+    the last T positions of the cache, so callers keep those free. (In an 8-bit
+    cache they would displace the unfinished block, which is put back.)"""
 
     def __init__(self, model: Qwen3Model, cache: KVCache, T: int = 1, batch: int = 1):
         dev = model.embed.weight.device
         self.model, self.cache, self.T = model, cache, T
         self.ids = torch.zeros((batch, T), dtype=torch.long, device=dev)
-        self.pos = torch.full((), cache.k[0].shape[2] - T, dtype=torch.long, device=dev)
+        kv8 = isinstance(cache, KVCache8)
+        seq = cache.max_seq if kv8 else cache.k[0].shape[2]
+        self.pos = torch.full((), seq - T, dtype=torch.long, device=dev)
+        kept = cache.tails() if kv8 else []
+        saved = [t.clone() for t in kept]
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.inference_mode(), torch.cuda.stream(side):
             for _ in range(2):  # load code objects, settle the caching allocator
                 model(self.ids, cache, start_pos=self.pos)
         torch.cuda.current_stream(dev).wait_stream(side)
+        with torch.inference_mode():
+            for t, old in zip(kept, saved):
+                t.copy_(old)
         torch.cuda.synchronize(dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.inference_mode(), torch.cuda.graph(self.graph):
@@ -292,11 +310,12 @@ class StepGraph:
         return self.logits
 
 
-def graph_greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device) -> list[int]:
+def graph_greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device, *,
+                          kv8: bool = False) -> list[int]:
     """``greedy_generate`` with every decode step replayed from one captured
     ``StepGraph`` (the prefill runs eagerly)."""
     ids = torch.tensor([prompt], dtype=torch.long, device=device)
-    cache = model.alloc_cache(len(prompt) + n_new + 4)
+    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8)
     with torch.inference_mode():
         logits = model(ids, cache, start_pos=0)
     step = StepGraph(model, cache, T=1)

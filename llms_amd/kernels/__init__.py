@@ -10,6 +10,7 @@ from .fused_qkv import TritonAttention, fused_qkv, fused_qkv_w8, triton_fused_qk
 from .fused_norm import (fused_rmsnorm_gate_up_silu, fused_rmsnorm_gate_up_silu_w8,
                          fused_rmsnorm_qkv, fused_rmsnorm_qkv_w8)
 from .linear import FusedLinear, fused_linear, fused_linear_w8
+from .kv8 import KVCache8, attention_kv8
 from .logprobs import TokenLogprobs, token_logprobs
 from .quant import dequantize_w4, dequantize_w8, quantize_w4, quantize_w8_per_row
 from .swap import apply_triton_kernels, prewarm_triton_kernels
@@ -41,6 +42,8 @@ __all__ = [
     "fused_rmsnorm_gate_up_silu_w4",
     "quantize_w4",
     "dequantize_w4",
+    "KVCache8",
+    "attention_kv8",
     "TokenLogprobs",
     "token_logprobs",
     "quantize_w8_per_row",

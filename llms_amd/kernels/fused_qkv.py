@@ -18,6 +18,7 @@ from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
 from ._eager import RMSNorm, apply_rope, attend, write_kv
 from .fused_attention import attention_core
+from .kv8 import KVCache8, attention_core_kv8
 from .quant import pack_weight
 from .w4 import fused_qkv_w4, fused_rmsnorm_qkv_w4
 
@@ -133,7 +134,9 @@ class TritonAttention(nn.Module):
     QK-norm, RoPE, the KV-cache write and attention run on HIP kernels too
     (:func:`~llms_amd.kernels.fused_attention.attention_core`) in bf16
     inference, else eagerly (:func:`attend`, fp32 softmax attention with the
-    reference's causal semantics); ``o`` is the module's own Linear.
+    reference's causal semantics); ``o`` is the module's own Linear. With a
+    :class:`~llms_amd.kernels.kv8.KVCache8` as its cache it attends over that, on HIP
+    kernels only.
 
     With ``from_eager(..., int8=True)`` the stacked weight is kept as
     per-row int8 (``q_qkv``, ``s_qkv`` buffers) and the int8 kernel runs; with
@@ -242,6 +245,10 @@ class TritonAttention(nn.Module):
         # place of the reference's three SDPA branches.
         B, T, _ = x.shape
         q_flat, k_flat, v_flat = self.project(x)
+        if isinstance(kv_cache, KVCache8):
+            return self.o(attention_core_kv8(q_flat, k_flat, v_flat, q_norm=self.q_norm, k_norm=self.k_norm,
+                                             num_heads=self.num_heads, cache=kv_cache, layer=layer_idx,
+                                             cos=cos, sin=sin, start_pos=start_pos))
         attn = attention_core(q_flat, k_flat, v_flat, q_norm=self.q_norm, k_norm=self.k_norm,
                               num_heads=self.num_heads, cache_k=kv_cache.k[layer_idx],
                               cache_v=kv_cache.v[layer_idx], cos=cos, sin=sin, start_pos=start_pos)
