@@ -395,13 +395,14 @@ int fp_kv8_read(const fp_kv8_args* args, float* k_out, float* v_out, void* strea
  *      2j (low half) and 2j + 1, each code + 8; the last half byte of an odd K is unused
  *   s  [N, ceil(K/group)] bf16, row stride lds, of five significant bits, so that
  *      code * s is exact in bf16
- *   y = x W^T with W[n,k] = code[n,k] * s[n, k/group], in the bf16 contract above
+ *   y = bf16(x W^T) with W[n,k] = code[n,k] * s[n, k/group], summed in fp32; gate-up
+ *   y = bf16(silu(x Wg^T) * (x Wu^T)), rounded once
  * gamma [K], when not NULL, is an RMSNorm weight applied to x first (the contract of
- * fp_rmsnorm_qkv_bf16; eps finite and >= 0). Up to 64 rows the weights are read as they
- * are; above that their bf16 values go to the workspace and the bf16 tiles run.
+ * fp_rmsnorm_qkv_bf16; eps finite and >= 0). The weights are read in 4 bits at every
+ * row count; the workspace holds x as the tiles read it and the partial sums of a split k.
  * A row of x with an infinity has NaN outputs (also where its codes are zero).
  * workspace: at least fp_w4_workspace_bytes(M, N, K, gate_up), 16-byte aligned.
- * ldq < 2^26 and lds < 2^26.
+ * ldx, ldq and lds < 2^26.
  */
 int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up);
 

@@ -236,69 +236,35 @@ int check_norm(float eps, void* ws, int64_t ws_bytes) {
 
 // ---- 4-bit weights ----
 
-// Workspace of a 4-bit call: the normalised rows, the rows padded to whole 64-wide
-// steps, then, above kW4RowsMaxM rows, the weights as bf16 and the split-k partials.
-struct W4Room {
-  int64_t kp, xn, xp, w, split;  // padded K, bytes of each part
-};
-W4Room w4_room(int64_t M, int64_t N, int64_t K, bool gateup) {
-  W4Room r{round_up(K, 64), round_up(M * K * 2, 256), 0, 0, 0};
-  r.xp = round_up(M * r.kp * 2, 256);
-  if (M <= kW4RowsMaxM) return r;
-  r.w = round_up(N * r.kp * 2, 256) * (gateup ? 2 : 1);
-  r.split = 4 * gemm_split_ws_floats(gemm_split_plan_bf16(M, N, r.kp, gateup), M, N, r.kp, gateup);
-  return r;
-}
+// Workspace of a 4-bit call: the normalised rows, then what launch_w4 asks for.
+int64_t w4_norm_bytes(int64_t M, int64_t K) { return round_up(M * K * 2, 256); }
 
 template <bool GATEUP>
 int run_w4(W4Args a, const uint16_t* gamma, float eps, void* ws, hipStream_t s) {
-  const W4Room r = w4_room(a.M, a.N, a.K, GATEUP);
-  char* at = (char*)ws;
-  int rc = 0;
   if (gamma) {
     const bool vec = a.K % 8 == 0 && a.ldx % 8 == 0 && al16(a.x) && al16(gamma);
-    if ((rc = launch_rmsnorm(a.x, a.ldx, gamma, eps, (uint16_t*)at, a.M, a.K, vec, s))) return launch_status(rc);
-    a.x = (uint16_t*)at;
+    const int rc = launch_rmsnorm(a.x, a.ldx, gamma, eps, (uint16_t*)ws, a.M, a.K, vec, s);
+    if (rc) return launch_status(rc);
+    a.x = (uint16_t*)ws;
     a.ldx = a.K;
   }
-  at += r.xn;
-  const bool rows = a.M <= kW4RowsMaxM;
-  // rows that 16-byte loads do not divide (or, for the tiles, of no whole 64-wide
-  // steps), or too far apart for the row kernel's 32-bit offsets
-  if (a.K % (rows ? 8 : 64) != 0 || a.ldx % 8 != 0 || !al16(a.x) || a.ldx >= (int64_t)1 << 23) {
-    if ((rc = launch_w4_pad(a.x, a.ldx, (uint16_t*)at, a.M, a.K, r.kp, s))) return launch_status(rc);
-    a.x = (uint16_t*)at;
-    a.ldx = r.kp;
-  }
-  at += r.xp;
-  if (rows) {
-    const auto on16 = [](const void* p, int64_t ld) { return al16(p) && ld % 16 == 0; };
-    const bool aligned = on16(a.q0, a.ldq0) && (!GATEUP || on16(a.q1, a.ldq1));
-    return launch_status(launch_w4_rows(a, GATEUP, aligned, s));
-  }
-  uint16_t* w0 = (uint16_t*)at;
-  uint16_t* w1 = GATEUP ? (uint16_t*)(at + r.w / 2) : nullptr;
-  if ((rc = launch_w4_dequantize(a.q0, a.ldq0, a.s0, a.lds0, a.group, w0, a.N, a.K, r.kp, s)))
-    return launch_status(rc);
-  if (GATEUP && (rc = launch_w4_dequantize(a.q1, a.ldq1, a.s1, a.lds1, a.group, w1, a.N, a.K, r.kp, s)))
-    return launch_status(rc);
-  at += r.w;
-  StreamArgs g{a.x, a.ldx, w0, r.kp, w1, r.kp, nullptr, nullptr, a.y, a.ldy, a.M, a.N, r.kp,
-               r.split ? (float*)at : nullptr, r.split / 4, nullptr, 0.f};
-  return run<GATEUP, false>(g, true, s);
+  const auto on16 = [](const void* p, int64_t ld) { return al16(p) && ld % 16 == 0; };
+  const bool aligned = on16(a.q0, a.ldq0) && (!GATEUP || on16(a.q1, a.ldq1));
+  return launch_status(launch_w4(a, GATEUP, aligned, (char*)ws + w4_norm_bytes(a.M, a.K), s));
 }
 
 // Arguments of a 4-bit call but for its pointers.
 int check_w4(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t ldq, int64_t lds,
              int64_t group) {
   if (M < 0 || N < 1 || K < 1 || (group != 32 && group != 64 && group != 128)) return FP_ERR_SHAPE;
-  // the packing's, the dequantisation's and the padding's grids in threads within 2^32
+  // every grid in threads within 2^32, the column workgroups within a grid's 65535
   constexpr int64_t kLim = (int64_t)1 << 32;
-  if (N > (int64_t)1 << 31 || K > (int64_t)1 << 26 || M > (int64_t)1 << 31 || N * (round_up(K, 64) / 32) > kLim ||
-      M * (round_up(K, 64) / 8) > kLim)
+  if (N > 65535 * 64 || K > (int64_t)1 << 26 || M > (int64_t)1 << 24 || (M + 127) * (round_up(K, 128) / 8) > kLim ||
+      (M + 15) / 16 * ((N + 63) / 64) * 256 > kLim / 16 || M * N > kLim)
     return FP_ERR_SHAPE;
   if (ldx < K || ldy < N || ldq < (K + 1) / 2 || lds < (K + group - 1) / group) return FP_ERR_STRIDE;
-  if (ldq >= (int64_t)1 << 26 || lds >= (int64_t)1 << 26) return FP_ERR_STRIDE;
+  constexpr int64_t kFar = (int64_t)1 << 26;  // sixteen rows within the kernels' 32-bit offsets
+  if (ldx >= kFar || ldq >= kFar || lds >= kFar) return FP_ERR_STRIDE;
   return FP_OK;
 }
 bool off2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }
@@ -761,8 +727,7 @@ int fp_kv8_read(const fp_kv8_args* g, float* k_out, float* v_out, void* stream) 
 
 int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up) {
   if (M < 1 || fp::check_w4(M, N, K, K, N, (K + 1) / 2, (K + 31) / 32, 32)) return 0;
-  const fp::W4Room r = fp::w4_room(M, N, K, gate_up != 0);
-  return r.xn + r.xp + r.w + r.split;
+  return fp::w4_norm_bytes(M, K) + fp::w4_workspace_bytes(M, N, K, gate_up != 0);
 }
 
 int fp_linear_w4(const void* x, int64_t ldx, const void* gamma, float eps, const uint8_t* q,
@@ -778,7 +743,7 @@ int fp_linear_w4(const void* x, int64_t ldx, const void* gamma, float eps, const
   if (!workspace || !fp::al16(workspace) || workspace_bytes < fp_w4_workspace_bytes(M, N, K, 0))
     return FP_ERR_WORKSPACE;
   const fp::W4Args a{(const uint16_t*)x, ldx, q, nullptr, ldq, 0, (const uint16_t*)s, nullptr, lds, 0,
-                     (uint16_t*)y, ldy, M, N, K, (int)group};
+                     (uint16_t*)y, ldy, M, N, K, (int)group, nullptr, nullptr, 1};
   return fp::run_w4<false>(a, (const uint16_t*)gamma, eps, workspace, (hipStream_t)stream);
 }
 
@@ -796,7 +761,7 @@ int fp_gate_up_silu_w4(const void* x, int64_t ldx, const void* gamma, float eps,
   if (!workspace || !fp::al16(workspace) || workspace_bytes < fp_w4_workspace_bytes(M, N, K, 1))
     return FP_ERR_WORKSPACE;
   const fp::W4Args a{(const uint16_t*)x, ldx, qg, qu, ldqg, ldqu, (const uint16_t*)sg,
-                     (const uint16_t*)su, ldsg, ldsu, (uint16_t*)y, ldy, M, N, K, (int)group};
+                     (const uint16_t*)su, ldsg, ldsu, (uint16_t*)y, ldy, M, N, K, (int)group, nullptr, nullptr, 1};
   return fp::run_w4<true>(a, (const uint16_t*)gamma, eps, workspace, (hipStream_t)stream);
 }
 

@@ -243,17 +243,16 @@ struct W4Args {
   int64_t ldy;
   int64_t M, N, K;
   int group;  // 32, 64 or 128
+  // set by launch_w4: x laid out by panels, ranges of k and their partial sums
+  char* panels;
+  float* part;
+  int splits;
 };
-constexpr int64_t kW4RowsMaxM = 64;
-// M <= kW4RowsMaxM rows of x, 16-byte aligned, of K rounded up to 8 elements (zeros past
-// K), 128 ldx and 16 ldq bytes under 2^31. aligned: weight rows on 16 bytes.
-int launch_w4_rows(const W4Args& a, bool gateup, bool aligned, hipStream_t s);
-// The weights as bf16 [N][Kp], zero from K on (Kp a multiple of 32).
-int launch_w4_dequantize(const uint8_t* q, int64_t ldq, const uint16_t* sc, int64_t lds, int group,
-                         uint16_t* out, int64_t N, int64_t K, int64_t Kp, hipStream_t s);
-// x [M][K] as [M][Kp], zero from K on (Kp a multiple of 8).
-int launch_w4_pad(const uint16_t* x, int64_t ldx, uint16_t* out, int64_t M, int64_t K, int64_t Kp,
-                  hipStream_t s);
+// LDS that w4_row_kernel may take for x and the scales.
+constexpr int64_t kW4RowLds = 156 << 10;
+int64_t w4_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gateup);
+// 16 ldq bytes under 2^31. aligned: weight rows on 16 bytes.
+int launch_w4(const W4Args& a, bool gateup, bool aligned, void* ws, hipStream_t s);
 int launch_w4_quantize(const uint16_t* w, int64_t ldw, uint8_t* q, int64_t ldq, uint16_t* sc,
                        int64_t lds, int64_t N, int64_t K, int group, hipStream_t s);
 

@@ -4,9 +4,9 @@ of the bf16 bytes, with or without the RMSNorm before them.
 
 The reference has no such path (reference DESIGN.md:120 lists quantisation as future
 work). The format is :func:`~llms_amd.kernels.quant.quantize_w4`'s: the weight is
-exactly ``code * scale``, up to 64 rows read in 4 bits and multiplied in the matrix
-cores (``llms_amd/csrc/fp_w4.hip``), above that expanded to bf16 in a workspace for
-the bf16 tiles (the expansion is exact, so both compute the same sums).
+exactly ``code * scale``, read in 4 bits at every row count and multiplied in the
+matrix cores with fp32 sums (``llms_amd/csrc/fp_w4.hip``). Outputs are rounded once: the
+gate-up product is of the fp32 sums, where the bf16 form rounds each of its steps.
 
 Path: wrapper -> ``torch.ops.llms_amd.linear_w4`` / ``gate_up_silu_w4`` -> C ABI
 ``fp_linear_w4`` / ``fp_gate_up_silu_w4`` -> HIP kernels on torch's current stream.
@@ -97,8 +97,7 @@ def fused_qkv_w4(x: torch.Tensor, q_qkv: torch.Tensor, s_qkv: torch.Tensor, *, n
 
 def fused_gate_up_silu_w4(x: torch.Tensor, qg: torch.Tensor, sg: torch.Tensor, qu: torch.Tensor,
                           su: torch.Tensor, *, group: int = 128) -> torch.Tensor:
-    """``silu(x @ Wg.T) * (x @ Wu.T)`` with both weights in 4 bits, at the rounding
-    points of the bf16 form."""
+    """``silu(x @ Wg.T) * (x @ Wu.T)`` with both weights in 4 bits, rounded once."""
     return _gate_up("fused_gate_up_silu_w4", x, None, 0.0, qg, sg, qu, su, group)
 
 
