@@ -401,10 +401,11 @@ int fp_kv8_read(const fp_kv8_args* args, float* k_out, float* v_out, void* strea
  * fp_rmsnorm_qkv_bf16; eps finite and >= 0). The weights are read in 4 bits at every
  * row count; the workspace holds x as the tiles read it and the partial sums of a split k.
  * A row of x with an infinity has NaN outputs (also where its codes are zero).
- * workspace: at least fp_w4_workspace_bytes(M, N, K, gate_up), 16-byte aligned.
- * ldx, ldq and lds < 2^26.
+ * workspace: at least fp_w4_workspace_bytes(M, N, K, gate_up, norm) bytes, 16-byte
+ * aligned (norm: whether gamma is given; 0 for most calls of few rows without it: NULL
+ * will do). ldx, ldq and lds < 2^26.
  */
-int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up);
+int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up, int norm);
 
 int fp_linear_w4(const void* x, int64_t ldx, const void* gamma, float eps,
                  const uint8_t* q, int64_t ldq, const void* s, int64_t lds, int64_t group,

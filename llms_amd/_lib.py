@@ -61,7 +61,7 @@ CAPI_SIGNATURES: dict[str, list] = {
     "fp_kv8_attention": [_P, _P, _I64, _P],
     "fp_kv8_write": [_P, _P],
     "fp_kv8_read": [_P, _P, _P, _P],
-    "fp_w4_workspace_bytes": [_I64, _I64, _I64, ctypes.c_int],
+    "fp_w4_workspace_bytes": [_I64, _I64, _I64, ctypes.c_int, ctypes.c_int],
     "fp_linear_w4": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
     "fp_gate_up_silu_w4": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64,
                            _I64, _I64, _P, _I64, _P],

@@ -247,10 +247,11 @@ int run_w4(W4Args a, const uint16_t* gamma, float eps, void* ws, hipStream_t s) 
     if (rc) return launch_status(rc);
     a.x = (uint16_t*)ws;
     a.ldx = a.K;
+    ws = (char*)ws + w4_norm_bytes(a.M, a.K);
   }
   const auto on16 = [](const void* p, int64_t ld) { return al16(p) && ld % 16 == 0; };
   const bool aligned = on16(a.q0, a.ldq0) && (!GATEUP || on16(a.q1, a.ldq1));
-  return launch_status(launch_w4(a, GATEUP, aligned, (char*)ws + w4_norm_bytes(a.M, a.K), s));
+  return launch_status(launch_w4(a, GATEUP, aligned, ws, s));
 }
 
 // Arguments of a 4-bit call but for its pointers.
@@ -725,9 +726,9 @@ int fp_kv8_read(const fp_kv8_args* g, float* k_out, float* v_out, void* stream) 
   return fp::launch_status(fp::launch_kv8_read(a, g->head_dim, k_out, v_out, (hipStream_t)stream));
 }
 
-int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up) {
+int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up, int norm) {
   if (M < 1 || fp::check_w4(M, N, K, K, N, (K + 1) / 2, (K + 31) / 32, 32)) return 0;
-  return fp::w4_norm_bytes(M, K) + fp::w4_workspace_bytes(M, N, K, gate_up != 0);
+  return (norm ? fp::w4_norm_bytes(M, K) : 0) + fp::w4_workspace_bytes(M, N, K, gate_up != 0);
 }
 
 int fp_linear_w4(const void* x, int64_t ldx, const void* gamma, float eps, const uint8_t* q,
@@ -740,8 +741,8 @@ int fp_linear_w4(const void* x, int64_t ldx, const void* gamma, float eps, const
   if (M == 0) return FP_OK;
   if (!x || !q || !s || !y) return FP_ERR_NULL;
   if (fp::off2(x) || fp::off2(gamma) || fp::off2(s) || fp::off2(y)) return FP_ERR_STRIDE;
-  if (!workspace || !fp::al16(workspace) || workspace_bytes < fp_w4_workspace_bytes(M, N, K, 0))
-    return FP_ERR_WORKSPACE;
+  const int64_t need = fp_w4_workspace_bytes(M, N, K, 0, gamma != nullptr);
+  if (workspace_bytes < need || (need > 0 && !workspace) || !fp::al16(workspace)) return FP_ERR_WORKSPACE;
   const fp::W4Args a{(const uint16_t*)x, ldx, q, nullptr, ldq, 0, (const uint16_t*)s, nullptr, lds, 0,
                      (uint16_t*)y, ldy, M, N, K, (int)group, nullptr, nullptr, 1};
   return fp::run_w4<false>(a, (const uint16_t*)gamma, eps, workspace, (hipStream_t)stream);
@@ -758,8 +759,8 @@ int fp_gate_up_silu_w4(const void* x, int64_t ldx, const void* gamma, float eps,
   if (M == 0) return FP_OK;
   if (!x || !qg || !sg || !qu || !su || !y) return FP_ERR_NULL;
   if (fp::off2(x) || fp::off2(gamma) || fp::off2(sg) || fp::off2(su) || fp::off2(y)) return FP_ERR_STRIDE;
-  if (!workspace || !fp::al16(workspace) || workspace_bytes < fp_w4_workspace_bytes(M, N, K, 1))
-    return FP_ERR_WORKSPACE;
+  const int64_t need = fp_w4_workspace_bytes(M, N, K, 1, gamma != nullptr);
+  if (workspace_bytes < need || (need > 0 && !workspace) || !fp::al16(workspace)) return FP_ERR_WORKSPACE;
   const fp::W4Args a{(const uint16_t*)x, ldx, qg, qu, ldqg, ldqu, (const uint16_t*)sg,
                      (const uint16_t*)su, ldsg, ldsu, (uint16_t*)y, ldy, M, N, K, (int)group, nullptr, nullptr, 1};
   return fp::run_w4<true>(a, (const uint16_t*)gamma, eps, workspace, (hipStream_t)stream);

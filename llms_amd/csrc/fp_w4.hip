@@ -659,7 +659,8 @@ struct W4Plan {
   int nc, waves, rt, splits;
 };
 
-constexpr int64_t kW4Wide = 512;  // workspace of a weight of under 16 bytes
+// Workspace of a weight that may have under 16 bytes (rows apart only make it longer).
+int64_t wide_bytes(int64_t N, int64_t K) { return N * ((K + 1) / 2) < 16 ? 512 : 0; }
 
 int64_t row_lds(int64_t M, int64_t K, int nc, int group) {
   const int64_t slabs = (K + 127) / 128;
@@ -728,7 +729,7 @@ int launch_gs(W4Args a, const W4Plan& p, bool gateup, bool aligned, char* ws, hi
     if (gateup) a.q1 = wide + 256, a.ldq1 = 16;
     aligned = true;
   }
-  ws += kW4Wide;
+  ws += wide_bytes(a.N, a.K);
   if (p.row) {
     if (gateup) return aligned ? launch_row<GS, true, true>(a, p, s) : launch_row<GS, true, false>(a, p, s);
     return aligned ? launch_row<GS, false, true>(a, p, s) : launch_row<GS, false, false>(a, p, s);
@@ -756,7 +757,7 @@ int64_t w4_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gateup) {
     if (p.splits > 1) b += p.splits * M * N * (gateup ? 8 : 4);
     most = most > b ? most : b;
   }
-  return most + kW4Wide;
+  return most + wide_bytes(N, K);
 }
 
 int launch_w4(const W4Args& a, bool gateup, bool aligned, void* ws, hipStream_t s) {

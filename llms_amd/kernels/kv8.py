@@ -15,10 +15,12 @@ kernels (``llms_amd/csrc/fp_kv8.hip``) on torch's current stream.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .. import _lib
-from ._checks import autocast, plain_norm, refuse_grad, require_bf16_hip, transformed
+from ._checks import autocast, plain_norm, refuse_grad, transformed
 
 BLOCK = 64
 MAX_SEQ = 1 << 23
@@ -35,13 +37,11 @@ class KVCache8:
     (one stream, or streams that wait for each other).
     """
 
-    def __init__(self, layers: list, max_seq: int) -> None:
-        # per layer: codes, scales and bf16 tails of keys and of values, the blocks in the tails
-        self.layers = layers
-        self.max_seq = max_seq
+    def __init__(self, layers: list, max_batch: int, n_kv_heads: int, head_dim: int, max_seq: int) -> None:
+        self.layers = layers  # a buffer of bytes each (see parts)
+        self.max_batch, self.n_kv_heads, self.head_dim, self.max_seq = max_batch, n_kv_heads, head_dim, max_seq
+        self.size = (max_batch, n_kv_heads, head_dim, max_seq)
         self.cur_len = 0
-        c = layers[0][0]
-        self.max_batch, self.n_kv_heads, _, _, self.head_dim = c.shape
 
     @classmethod
     def alloc(cls, num_layers: int, max_seq: int, *, max_batch: int = 1, n_kv_heads: int, head_dim: int,
@@ -53,27 +53,36 @@ class KVCache8:
             raise ValueError(f"KVCache8: heads of 64 or 128 are taken, got {head_dim}")
         if not 1 <= max_seq <= MAX_SEQ:
             raise ValueError(f"KVCache8: max_seq must be 1 to {MAX_SEQ}, got {max_seq}")
-        lead, nb, D = (max_batch, n_kv_heads), -(-max_seq // BLOCK), head_dim
-        layers = []
-        for _ in range(num_layers):
-            z = lambda *s, t: torch.zeros(*lead, *s, dtype=t, device=device)  # noqa: E731
-            layers.append([z(nb, BLOCK, D, t=torch.int8), z(nb, D, BLOCK, t=torch.int8),
-                           z(nb, t=torch.float32), z(nb, t=torch.float32),
-                           z(2, BLOCK, D, t=torch.bfloat16), z(2, D, BLOCK, t=torch.bfloat16),
-                           torch.full((*lead, 2), -1, dtype=torch.int32, device=device)])
-        return cls(layers, max_seq)
+        size = max_batch, n_kv_heads, head_dim, max_seq
+        n = _lib.ops().kv8_layout(*size)[-1]
+        c = cls([torch.zeros(n, dtype=torch.uint8, device=device) for _ in range(num_layers)], *size)
+        for i in range(num_layers):
+            c.parts(i)[-1].fill_(-1)
+        return c
+
+    def parts(self, layer: int) -> list:
+        """A layer's codes of keys ``[max_batch, heads, blocks, 64, D]`` and values (``.., D, 64``),
+        their scales, the bf16 tails of keys ``[.., 2, 64, D]`` and values (``.., D, 64``) and the
+        blocks in the tails ``[.., 2]``: views of its buffer."""
+        lead, D, nb = (self.max_batch, self.n_kv_heads), self.head_dim, -(-self.max_seq // BLOCK)
+        shapes = [(nb, BLOCK, D), (nb, D, BLOCK), (nb,), (nb,), (2, BLOCK, D), (2, D, BLOCK), (2,)]
+        types = [torch.int8] * 2 + [torch.float32] * 2 + [torch.bfloat16] * 2 + [torch.int32]
+        out = []
+        for at, shape, t in zip(_lib.ops().kv8_layout(*self.size), shapes, types):
+            n = math.prod(lead + shape) * t.itemsize
+            out.append(self.layers[layer][at : at + n].view(t).view(*lead, *shape))
+        return out
 
     @property
     def device(self) -> torch.device:
-        return self.layers[0][0].device
+        return self.layers[0].device
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, start_pos, *, lengths=None) -> None:
         """Put ``k``, ``v`` ``[B, T, n_kv_heads, D]`` (bfloat16, normalised and rotated)
         at positions ``start_pos ..``; arguments as in :func:`attention_kv8`."""
-        B, T = _tokens("KVCache8.write", self, k, v)
-        start, pos = _place("KVCache8.write", self, B, T, start_pos, lengths)
-        if B and T:
-            _lib.ops().write_kv8(_flat(k), _flat(v), self.layers[layer], self.max_seq, start, pos, lengths)
+        start, pos = _place("KVCache8.write", start_pos, lengths)
+        refuse_grad("KVCache8.write", k, v)
+        _lib.ops().write_kv8(k, v, self.layers[layer], self.size, start, pos, lengths)  # which checks the rest
 
     def read(self, layer: int, start_pos, T: int, *, batch: int | None = None):
         """The keys and values ``[B, T, n_kv_heads, D]`` in float32 that attention sees at
@@ -84,61 +93,23 @@ class KVCache8:
             batch = start_pos.shape[0] if torch.is_tensor(start_pos) and start_pos.dim() == 1 else self.max_batch
         if not 1 <= batch <= self.max_batch or T < 1:
             raise ValueError(f"KVCache8.read: batch {batch} and T {T} must be 1 to {self.max_batch} and at least 1")
-        start, pos = _place("KVCache8.read", self, batch, T, start_pos, None)
-        if self.device.type != "cuda":
-            raise ValueError(f"KVCache8.read: the cache is on {self.device}; it runs only on a HIP (ROCm) device")
-        return _lib.ops().read_kv8(self.layers[layer], self.max_seq, batch, T, start, pos)
+        start, pos = _place("KVCache8.read", start_pos, None)
+        return _lib.ops().read_kv8(self.layers[layer], self.size, batch, T, start, pos)
 
     def tails(self) -> list:
         """The buffers of every layer that a write outside the sequence would lose."""
-        return [t for c in self.layers for t in c[4:]]
+        at = _lib.ops().kv8_layout(*self.size)[4]
+        return [c[at:] for c in self.layers]
 
 
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    """t [B, T, H, D] as rows [B, T, H * D] that the kernels take (a copy where a
-    head, a row or the batch is not laid out for them)."""
-    B, T, H, D = t.shape
-    s = t.stride()
-    ok = s[3] == 1 and (H == 1 or s[2] == D) and t.data_ptr() % 8 == 0
-    ld = s[1] if T > 1 else s[0] if B > 1 else H * D
-    if not ok or ld % 4 or ld < H * D or (B > 1 and s[0] != T * ld):
-        t = t.contiguous()
-    return t.reshape(B, T, H * D) if t.is_contiguous() else t.as_strided((B, T, H * D), (T * ld, ld, 1))
-
-
-def _tokens(fn: str, cache: KVCache8, k: torch.Tensor, v: torch.Tensor) -> tuple[int, int]:
-    if k.dim() != 4 or k.shape != v.shape or k.shape[2:] != (cache.n_kv_heads, cache.head_dim):
-        raise ValueError(f"{fn}: k {tuple(k.shape)} and v {tuple(v.shape)} must be "
-                         f"(B, T, {cache.n_kv_heads}, {cache.head_dim})")
-    if k.shape[0] > cache.max_batch:
-        raise ValueError(f"{fn}: {k.shape[0]} sequences, the cache holds {cache.max_batch}")
-    require_bf16_hip(fn, k=k, v=v)
-    if not (k.device == v.device == cache.device):
-        raise ValueError(f"{fn}: k ({k.device}), v ({v.device}) and the cache ({cache.device}) "
-                         "must be on the same device")
-    refuse_grad(fn, k, v)
-    return k.shape[0], k.shape[1]
-
-
-def _place(fn: str, cache: KVCache8, B: int, T: int, start_pos, lengths):
-    """(start_pos as an int, as a device tensor or None)."""
-    if lengths is not None:
-        if not torch.is_tensor(lengths) or lengths.dtype != torch.int64 or lengths.shape != (B,):
-            raise ValueError(f"{fn}: lengths must be an int64 tensor of {B} elements")
-        if lengths.device != cache.device or not lengths.is_contiguous():
-            raise ValueError(f"{fn}: lengths must be contiguous on {cache.device}")
+def _place(fn: str, start_pos, lengths):
+    """(start_pos as an int, as a tensor or None)."""
+    if lengths is not None and not torch.is_tensor(lengths):
+        raise ValueError(f"{fn}: lengths must be an int64 tensor, got {type(lengths).__name__}")
     if torch.is_tensor(start_pos):
-        if start_pos.dtype != torch.int64 or start_pos.shape not in ((), (B,)):
-            raise ValueError(f"{fn}: start_pos must be an int or an int64 tensor of shape () or ({B},), got "
-                             f"{start_pos.dtype} {tuple(start_pos.shape)}")
-        if start_pos.device != cache.device or not start_pos.is_contiguous():
-            raise ValueError(f"{fn}: start_pos must be contiguous on {cache.device}")
         return 0, start_pos
     if type(start_pos) is not int:
         raise TypeError(f"{fn}: start_pos must be an int or an int64 tensor, got {type(start_pos).__name__}")
-    if start_pos < 0 or start_pos + T > cache.max_seq:
-        raise ValueError(f"{fn}: positions {start_pos} .. {start_pos + T - 1} are outside the cache of "
-                         f"{cache.max_seq}")
     return start_pos, None
 
 
@@ -162,22 +133,12 @@ def attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCa
         positions outside the cache (whose tokens are not written), are zero.
     """
     fn = "attention_kv8"
-    B, T = _tokens(fn, cache, k, v)
-    if q.dim() != 4 or q.shape[:2] != (B, T) or q.shape[3] != cache.head_dim:
-        raise ValueError(f"{fn}: q {tuple(q.shape)} must be ({B}, {T}, heads, {cache.head_dim})")
-    H = q.shape[2]
-    if H < 1 or H % cache.n_kv_heads:
-        raise ValueError(f"{fn}: {H} query heads are no multiple of {cache.n_kv_heads} kv heads")
-    require_bf16_hip(fn, q=q)
-    if q.device != cache.device:
-        raise ValueError(f"{fn}: q ({q.device}) and the cache ({cache.device}) must be on the same device")
-    refuse_grad(fn, q)
-    start, pos = _place(fn, cache, B, T, start_pos, lengths)
-    if B == 0 or T == 0:
-        return torch.empty_like(q)
-    y = _lib.ops().attention_kv8(_flat(q), _flat(k), _flat(v), None, None, 0.0, 0.0, None, None,
-                                 cache.layers[layer], cache.max_seq, start, pos, lengths)
-    return y.view(B, T, H, cache.head_dim)
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"{fn}: q {tuple(q.shape)} and k {tuple(k.shape)} must be (B, T, heads, {cache.head_dim})")
+    start, pos = _place(fn, start_pos, lengths)
+    refuse_grad(fn, q, k, v)
+    return _lib.ops().attention_kv8(q, k, v, None, None, 0.0, 0.0, None, None, cache.layers[layer], cache.size,
+                                    start, pos, lengths)  # which checks the rest
 
 
 def attention_core_kv8(q, k, v, *, q_norm, k_norm, num_heads: int, cache: KVCache8, layer: int, cos, sin,
@@ -188,7 +149,6 @@ def attention_core_kv8(q, k, v, *, q_norm, k_norm, num_heads: int, cache: KVCach
     type is not bf16's), the cache write and attention. Returns ``[B, T, num_heads * D]``."""
     fn, D = "attention_kv8", cache.head_dim
     B, T, _ = q.shape
-    q4, k4, v4 = (t.view(B, T, -1, D) for t in (q, k, v))
     fused = (plain_norm(q_norm) and plain_norm(k_norm) and not autocast()
              and all(t.dtype == torch.bfloat16 and t.shape == (D,) and t.is_contiguous()
                      for t in (q_norm.weight, k_norm.weight))
@@ -198,11 +158,10 @@ def attention_core_kv8(q, k, v, *, q_norm, k_norm, num_heads: int, cache: KVCach
     if not fused:
         from ._eager import apply_rope
 
+        q4, k4, v4 = (t.view(B, T, -1, D) for t in (q, k, v))
         q4, k4 = apply_rope(q_norm(q4).transpose(1, 2), k_norm(k4).transpose(1, 2), cos, sin)
         return attention_kv8(q4.transpose(1, 2), k4.transpose(1, 2), v4, cache, layer, start_pos).view(B, T, -1)
-    _tokens(fn, cache, k4, v4)
-    require_bf16_hip(fn, q=q)
-    refuse_grad(fn, q)
-    start, pos = _place(fn, cache, B, T, start_pos, None)
-    return _lib.ops().attention_kv8(_flat(q4), _flat(k4), _flat(v4), q_norm.weight, k_norm.weight, q_norm.eps,
-                                    k_norm.eps, cos, sin, cache.layers[layer], cache.max_seq, start, pos, None)
+    start, pos = _place(fn, start_pos, None)
+    refuse_grad(fn, q, k, v)
+    return _lib.ops().attention_kv8(q, k, v, q_norm.weight, k_norm.weight, q_norm.eps, k_norm.eps, cos, sin,
+                                    cache.layers[layer], cache.size, start, pos, None)

@@ -67,8 +67,8 @@ def new(P, H, D, B=1, layers=1, garbage=True):
     """A cache whose buffers hold anything, as memory never written does."""
     c = fk.KVCache8.alloc(layers, P, max_batch=B, n_kv_heads=H, head_dim=D, device=DEV)
     if garbage:
-        for layer in c.layers:
-            for i, t in enumerate(layer[:6]):
+        for i in range(layers):
+            for t in c.parts(i)[:6]:
                 t.random_(-128, 128) if t.dtype == torch.int8 else t.fill_(math.nan)
     return c
 
@@ -78,7 +78,7 @@ def new(P, H, D, B=1, layers=1, garbage=True):
 
 def test_refusals_on_the_cpu():
     c = fk.KVCache8.alloc(2, 100, max_batch=2, n_kv_heads=2, head_dim=64, device="cpu")
-    assert c.layers[1][0].shape == (2, 2, 2, 64, 64) and c.max_seq == 100 and len(c.tails()) == 6
+    assert c.parts(1)[0].shape == (2, 2, 2, 64, 64) and c.max_seq == 100 and len(c.tails()) == 2
     q, k = torch.zeros(1, 3, 4, 64).bfloat16(), torch.zeros(1, 3, 2, 64).bfloat16()
     with pytest.raises(ValueError, match="HIP"):
         fk.attention_kv8(q, k, k, c, 0, 0)
@@ -252,9 +252,9 @@ def test_sequences_of_their_own_lengths(T, D):
     c.write(0, k.to(DEV), v.to(DEV), 0, lengths=before)
     idx = [[min(max(p + t, 0), S - 1) for t in range(T)] for p in starts]
     nk, nv = (torch.stack([t[b, idx[b]] for b in range(B)]) for t in (k, v))
-    kept = [t[5].clone() for t in c.layers[0]] + [t[2].clone() for t in c.layers[0]]
+    kept = [t[5].clone() for t in c.parts(0)] + [t[2].clone() for t in c.parts(0)]
     y = fk.attention_kv8(q.to(DEV), nk.to(DEV), nv.to(DEV), c, 0, place, lengths=torch.tensor(lens, device=DEV)).cpu()
-    for old, t in zip(kept, [t[5] for t in c.layers[0]] + [t[2] for t in c.layers[0]]):
+    for old, t in zip(kept, [t[5] for t in c.parts(0)] + [t[2] for t in c.parts(0)]):
         assert torch.equal(old.view(torch.uint8), t.view(torch.uint8))  # nothing of theirs was written
     for b in range(B):
         live = [t for t in range(lens[b]) if 0 <= starts[b] + t < S]

@@ -115,17 +115,20 @@ def test_refusals_on_the_cpu():
 def test_c_entry_refusals():
     lib = _lib.capi()
     P = 4096  # never dereferenced: every call below is refused before a launch
-    need = lib.fp_w4_workspace_bytes(4, 96, 256, 0)
-    assert need > 0 and lib.fp_w4_workspace_bytes(0, 96, 256, 0) == 0
-    assert lib.fp_w4_workspace_bytes(65, 96, 256, 1) >= 65 * 256 * 2  # x as the tiles read it
+    assert lib.fp_w4_workspace_bytes(4, 96, 256, 0, 0) == 0
+    need = lib.fp_w4_workspace_bytes(20, 96, 256, 0, 0)
+    assert need > 0 and lib.fp_w4_workspace_bytes(0, 96, 256, 0, 1) == 0
+    assert lib.fp_w4_workspace_bytes(65, 96, 256, 1, 0) >= 65 * 256 * 2  # x as the tiles read it
+    assert lib.fp_w4_workspace_bytes(65, 96, 256, 1, 1) >= 2 * 65 * 256 * 2  # and as the norm wrote it
+    assert lib.fp_w4_workspace_bytes(2, 2, 5, 1, 0) > 0  # weights of under 16 bytes
     ok = dict(x=P, ldx=256, gamma=None, eps=0.0, q=P, ldq=128, s=P, lds=2, group=128, y=P, ldy=96,
-              M=4, N=96, K=256, ws=P, nb=need)
+              M=20, N=96, K=256, ws=P, nb=need)
 
     def call(**kw):
         a = dict(ok, **kw)
         one = lib.fp_linear_w4(a["x"], a["ldx"], a["gamma"], a["eps"], a["q"], a["ldq"], a["s"], a["lds"],
                                a["group"], a["y"], a["ldy"], a["M"], a["N"], a["K"], a["ws"], a["nb"], None)
-        nb = a["nb"] if "nb" in kw else lib.fp_w4_workspace_bytes(4, 96, 256, 1)
+        nb = a["nb"] if "nb" in kw else lib.fp_w4_workspace_bytes(20, 96, 256, 1, 0)
         two = lib.fp_gate_up_silu_w4(a["x"], a["ldx"], a["gamma"], a["eps"], P, 128, P, 2, a["q"], a["ldq"],
                                      a["s"], a["lds"], a["group"], a["y"], a["ldy"], a["M"], a["N"], a["K"],
                                      a["ws"], nb, None)
