@@ -44,6 +44,7 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 constexpr int kBlk = 64;
 constexpr int kKv8MaxSplit = 64;  // one lane per split in kv8_combine_kernel
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRise = 8.f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ f32x4 mfma16h(u32x4 a, u32x4 b, f32x4 c) {
@@ -59,8 +60,10 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 // max / sum over the four lane groups that share a row column.
 __device__ __forceinline__ float col_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float col_sum(float v) {
   v += __shfl_xor(v, 16);
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
     u32x4 k[4][KU], v[DT];
     float ks, vs;
   };
-  auto load = [&](Block& x, int c) {
+  auto load = [&](Block& x, int c) __attribute__((always_inline)) {
     const uint32_t base = c < f_hi ? (uint32_t)c * (kBlk * D) : 0x7fff0000u;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
     x.vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsr, sb, 0, 0));
   };
   // scores of block c at factor f to probabilities; what o is multiplied by in al
-  auto softmax = [&](f32x4 (&x)[4][RT], int c, float f, u32x4 (&pf)[RT][2], float (&al)[RT]) {
+  auto softmax = [&](f32x4 (&x)[4][RT], int c, float f, u32x4 (&pf)[RT][2], float (&al)[RT]) __attribute__((always_inline)) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       f32x4 y[4];
@@ -548,7 +551,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
       p_operands(y, pf[rt]);
     }
   };
-  auto compute = [&](const Block& x, int c, auto bad) {
+  auto compute = [&](const Block& x, int c, auto bad) __attribute__((always_inline)) {
     constexpr bool BAD = decltype(bad)::value;
     f32x4 y[4][RT];
 #pragma unroll
@@ -580,7 +583,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
       }
     }
   };
-  auto step = [&](const Block& x, int c) {
+  auto step = [&](const Block& x, int c) __attribute__((always_inline)) {
     const uint32_t sign = (__float_as_uint(x.ks) | __float_as_uint(x.vs)) >> 31;
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(sign), 0)) compute(x, c, std::true_type{});
     else compute(x, c, std::false_type{});
@@ -739,15 +742,16 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
   auto k_at = [](int r, int c) { return r * (D * 2) + ((c ^ (((r >> 4) * 4 + (r & 3)) & (CH - 1))) * 16); };
   auto v_at = [](int d, int c) { return d * (kBlk * 2) + ((c ^ (d & 7)) * 16); };
   u32x4 kx[NL], vx[NL];
-  float ksc = 0.f, vsc = 0.f;
-  auto load = [&](int kt) {
+  float ksc = 0.f, vsc = 0.f, ks_next = 0.f, vs_next = 0.f;
+  auto load = [&](int kt) __attribute__((always_inline)) {
     if (kt >= full) return;
+    ks_next = a.k_scale[at + kt], vs_next = a.v_scale[at + kt];
     const u32x4* kc = reinterpret_cast<const u32x4*>(a.k_codes + (at + kt) * (kBlk * D));
     const u32x4* vc = reinterpret_cast<const u32x4*>(a.v_codes + (at + kt) * (kBlk * D));
 #pragma unroll
     for (int n = 0; n < NL; ++n) kx[n] = kc[n * 256 + tid], vx[n] = vc[n * 256 + tid];
   };
-  auto put = [&](char* k, char* v, auto bad) {
+  auto put = [&](char* k, char* v, auto bad) __attribute__((always_inline)) {
     constexpr bool BAD = decltype(bad)::value;
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
@@ -761,10 +765,15 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
   };
   __shared__ float sTop[4];
   // block kt (loaded before, if whole) into LDS; its scales into ks, vs
-  auto store = [&](char* k, char* v, int kt, float& ks, float& vs) {
+  auto store = [&](char* k, char* v, int kt, float& ks, float& vs) __attribute__((always_inline)) {
     if (kt < full) {
-      const float k0 = a.k_scale[at + kt], v0 = a.v_scale[at + kt];
-      if (__builtin_expect((__float_as_uint(k0) | __float_as_uint(v0)) >> 31, 0)) put(k, v, std::true_type{});
+      // not before here: the compiler would pull the conversions' shifts up to the loads
+      // and wait for them there
+#pragma unroll
+      for (int n = 0; n < NL; ++n) asm volatile("" : "+v"(kx[n]), "+v"(vx[n]));
+      const float k0 = ks_next, v0 = vs_next;
+      const uint32_t sign = (__float_as_uint(k0) | __float_as_uint(v0)) >> 31;
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(sign), 0)) put(k, v, std::true_type{});
       else put(k, v, std::false_type{});
       ks = fabsf(k0), vs = fabsf(v0);
       return;
@@ -810,16 +819,17 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
 
   const float sc = kLog2e / sqrtf((float)D);
   f32x4 o[DT][RT];
-  float mx[RT], sum[RT];
+  float mx[RT];
+  f32x4 sum[RT];  // four equal rows: the products of ones and p
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     mx[rt] = -INFINITY;
-    sum[rt] = 0.f;
+    sum[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  auto compute = [&](const char* k, const char* v, int kt, float ks, float vs) {
-    if (kt * kBlk > lim_hi) return;  // every key hidden from every row
+  auto compute = [&](const char* k, const char* v, int kt, float ks, float vs, auto masked) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(masked)::value;
     f32x4 x[RT][4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -832,22 +842,53 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
         for (int rt = 0; rt < RT; ++rt) x[rt][n] = mfma16(kf, qf[rt][i], x[rt][n]);
       }
     }
-    const bool mask = kt * kBlk + kBlk - 1 > lim_lo;  // uniform
     const float f = ks * sc;
-    u32x4 pf[RT][2];
-    float al[RT];
+    float top[RT];
+    bool rise = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+      if constexpr (MASK) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            x[rt][n][r] = kt * kBlk + 16 * grp + 4 * n + r <= lim[rt] ? x[rt][n][r] * f : -INFINITY;
+      }
+      float m = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[rt][n][r] *= f;
-          if (mask && kt * kBlk + 16 * grp + 4 * n + r > lim[rt]) x[rt][n][r] = -INFINITY;
-        }
-      al[rt] = softmax_step(x[rt], mx[rt], sum[rt]);
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, x[rt][n][r]);
+      top[rt] = col_max(MASK ? m : m * f);
+      rise |= top[rt] > mx[rt] + kRise;
+    }
+    if (__ballot(rise)) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float to = top[rt] > mx[rt] + kRise ? top[rt] : mx[rt];
+        const float al = exp2_fast(mx[rt] - (to == -INFINITY ? 0.f : to));
+        mx[rt] = to;
+        sum[rt] *= al;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt][rt] *= al;
+      }
+    }
+    u32x4 pf[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float base = mx[rt] == -INFINITY ? 0.f : mx[rt];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[rt][n][r] = exp2_fast(MASK ? x[rt][n][r] - base : fmaf(x[rt][n][r], f, -base));
       p_operands(x[rt], pf[rt]);
     }
+    constexpr u32x4 kOnes = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sum[rt] = mfma16h(kOnes, pf[rt][i], sum[rt]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const u32x4 v0 = *reinterpret_cast<const u32x4*>(v + v_at(dt * 16 + li, 2 * grp));
@@ -857,11 +898,22 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
         f32x4 pv = mfma16h(v0, pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
         pv = mfma16h(v1, pf[rt][1], pv);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r] * al[rt]);
+        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r]);
       }
     }
   };
+  auto step = [&](const char* k, const char* v, int kt, float ks, float vs) __attribute__((always_inline)) {
+    if (kt * kBlk > lim_hi) return;  // every key hidden from every row
+    if (kt * kBlk + kBlk - 1 > lim_lo) compute(k, v, kt, ks, vs, std::true_type{});
+    else compute(k, v, kt, ks, vs, std::false_type{});
+  };
 
+  // q has arrived: a load pending at the loop's entry would have the compiler wait, in
+  // every round, for the loads of the next block too (109 us against %s)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int i = 0; i < DK; ++i) asm volatile("" : "+v"(qf[rt][i]));
   if (t_lo < t_hi) {
     load(t_lo);
     store(sK[0], sV[0], t_lo, ksc, vsc);
@@ -870,7 +922,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
       const int u = (kt - t_lo) & 1;
       const bool more = kt + 1 < t_hi;
       if (more) load(kt + 1);
-      compute(sK[u], sV[u], kt, ksc, vsc);
+      step(sK[u], sV[u], kt, ksc, vsc);
       if (more) {
         store(sK[u ^ 1], sV[u ^ 1], kt + 1, ksc, vsc);
         __syncthreads();
@@ -880,7 +932,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    float l = col_sum(sum[rt]);
+    const float l = sum[rt][0];
     const int rr = row0 + rt * 16 + li;
     if (rr >= rows) continue;
     if (a.nsplit > 1) {
