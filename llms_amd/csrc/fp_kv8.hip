@@ -467,7 +467,7 @@ __device__ __forceinline__ float tail_values(u32x4 (&v)[DT][2], int rows, int gr
 // return zeros past it, so loads are issued without a branch), and merge their softmax
 // states through LDS in wave order.
 template <int D, int RT>
-__global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
+__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args a) {
   constexpr int NW = 4, DK = D / 32, DT = D / 16, KU = D / 64;
   __shared__ __attribute__((aligned(16))) float sO[NW][16 * RT][D + 4];
   __shared__ float sM[NW][16 * RT], sL[NW][16 * RT];
@@ -519,23 +519,28 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
     for (int dt = 0; dt < DT; ++dt) o[dt][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  struct Block {
-    u32x4 k[4][KU], v[DT];
-    float ks, vs;
+  // one block's codes: a block's keys come in behind the last one's values and its values
+  // behind its scores, each into the registers that have just been used, its scales before
+  u32x4 xk[4][KU], xv[DT];
+  float ks, vs, ks_next, vs_next;
+  auto load_s = [&](int c) __attribute__((always_inline)) {
+    const uint32_t sb = c < f_hi ? (uint32_t)c * 4 : 0x7fff0000u;
+    ks_next = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ksr, sb, 0, 0));
+    vs_next = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsr, sb, 0, 0));
   };
-  auto load = [&](Block& x, int c) __attribute__((always_inline)) {
+  auto load_k = [&](int c) __attribute__((always_inline)) {
     const uint32_t base = c < f_hi ? (uint32_t)c * (kBlk * D) : 0x7fff0000u;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
       for (int u = 0; u < KU; ++u)
-        x.k[n][u] = __builtin_amdgcn_raw_buffer_load_b128(kr, base + koff + 4 * n * D + 64 * u, 0, 0);
-    const uint32_t sb = c < f_hi ? (uint32_t)c * 4 : 0x7fff0000u;
-    x.ks = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ksr, sb, 0, 0));
+        xk[n][u] = __builtin_amdgcn_raw_buffer_load_b128(kr, base + koff + 4 * n * D + 64 * u, 0, 0);
+  };
+  auto load_v = [&](int c) __attribute__((always_inline)) {
+    const uint32_t base = c < f_hi ? (uint32_t)c * (kBlk * D) : 0x7fff0000u;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
-      x.v[dt] = __builtin_amdgcn_raw_buffer_load_b128(vr, base + voff + dt * 16 * kBlk, 0, 0);
-    x.vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsr, sb, 0, 0));
+      xv[dt] = __builtin_amdgcn_raw_buffer_load_b128(vr, base + voff + dt * 16 * kBlk, 0, 0);
   };
   // scores of block c at factor f to probabilities; what o is multiplied by in al
   auto softmax = [&](f32x4 (&x)[4][RT], int c, float f, u32x4 (&pf)[RT][2], float (&al)[RT]) __attribute__((always_inline)) {
@@ -551,7 +556,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
       p_operands(y, pf[rt]);
     }
   };
-  auto compute = [&](const Block& x, int c, auto bad) __attribute__((always_inline)) {
+  auto compute = [&](int c, auto bad) __attribute__((always_inline)) {
     constexpr bool BAD = decltype(bad)::value;
     f32x4 y[4][RT];
 #pragma unroll
@@ -562,44 +567,48 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Args a) {
       for (int u = 0; u < KU; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const u32x4 kf = codes8_bf16<BAD>(x.k[n][u][2 * h], x.k[n][u][2 * h + 1]);
+          const u32x4 kf = codes8_bf16<BAD>(xk[n][u][2 * h], xk[n][u][2 * h + 1]);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) y[n][rt] = mfma16(kf, qf[rt][2 * u + h], y[n][rt]);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(c + NW);
+    __builtin_amdgcn_sched_barrier(0);
     u32x4 pf[RT][2];
     float al[RT];
-    softmax(y, c, fabsf(x.ks) * sc, pf, al);
-    const float vs = fabsf(x.vs);
+    softmax(y, c, fabsf(ks) * sc, pf, al);
+    const float f = fabsf(vs);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const u32x4 v0 = codes8_f16<BAD>(x.v[dt][0], x.v[dt][1]), v1 = codes8_f16<BAD>(x.v[dt][2], x.v[dt][3]);
+      const u32x4 v0 = codes8_f16<BAD>(xv[dt][0], xv[dt][1]), v1 = codes8_f16<BAD>(xv[dt][2], xv[dt][3]);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         f32x4 pv = mfma16h(v0, pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
         pv = mfma16h(v1, pf[rt][1], pv);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r] * al[rt]);
+        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], f, o[dt][rt][r] * al[rt]);
       }
     }
-  };
-  auto step = [&](const Block& x, int c) __attribute__((always_inline)) {
-    const uint32_t sign = (__float_as_uint(x.ks) | __float_as_uint(x.vs)) >> 31;
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(sign), 0)) compute(x, c, std::true_type{});
-    else compute(x, c, std::false_type{});
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(c + NW);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  Block x0, x1;
-  int c = c_lo + wave;
-  load(x0, c);
-  while (c < f_hi) {
-    load(x1, c + NW);
-    step(x0, c);
-    c += NW;
-    if (c >= f_hi) break;
-    load(x0, c + NW);
-    step(x1, c);
-    c += NW;
+  load_s(c_lo + wave);
+  load_k(c_lo + wave);
+  load_v(c_lo + wave);
+  // q has arrived (a load pending at the loop's entry would be waited for in every round)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int i = 0; i < DK; ++i) asm volatile("" : "+v"(qf[rt][i]));
+  for (int c = c_lo + wave; c < f_hi; c += NW) {
+    ks = ks_next, vs = vs_next;
+    load_s(c + NW);
+    const uint32_t sign = (__float_as_uint(ks) | __float_as_uint(vs)) >> 31;
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(sign), 0)) compute(c, std::true_type{});
+    else compute(c, std::false_type{});
   }
 
   // the unfinished block, from the ring: the wave whose turn it is
@@ -1016,7 +1025,7 @@ Kv8Plan kv8_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t keys) {
   }
   // no range shorter than a block for each wave, or four tiles
   const int64_t groups = B * Hk * p.n_rt, most = (keys + 4 * kBlk - 1) / (4 * kBlk);
-  int64_t ns = kKv8Groups / groups;
+  int64_t ns = (p.rows && p.rt == 2 ? kKv8Groups / 2 : kKv8Groups) / groups;
   ns = ns < most ? ns : most;
   ns = ns < kKv8MaxSplit ? ns : kKv8MaxSplit;
   p.nsplit = (int)(ns < 1 ? 1 : ns);
