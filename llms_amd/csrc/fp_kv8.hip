@@ -264,6 +264,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
 
   const bool assemble = complete || (have_old && !tag_ok);
   if (!assemble) {  // most calls of one token: nothing but its rows
+    if (old_first && blk == after) return;
     put(blk, row0, row1, true, false);
     if (!have_old && tid == 0) a.tail_block[bh * 2 + slot] = blk;
     return;
