@@ -426,39 +426,17 @@ __device__ __forceinline__ int64_t part_row(const Kv8Args& a, int split, int bh,
   return ((int64_t)split * a.B * a.Hk + bh) * ((int64_t)a.T * (a.Hq / a.Hk)) + rr;
 }
 
-// The ring's values of one block as fp16 operands at the scale 2^e that puts the largest
-// of them into [1, 2): keys from `rows` on as zeros (the ring holds anything there).
-// vb: 16 bytes of 8 keys for d block dt and half i of the lane group's 16 keys.
-template <int DT>
-__device__ __forceinline__ float tail_values(u32x4 (&v)[DT][2], int rows, int grp) {
-  float top = 0.f;
-  int bad = 0;
+// ... and as those of their bf16 values and of what is left: p to 2^-17 of itself.
+__device__ __forceinline__ void p_operands_bf16(const f32x4 (&x)[4], u32x4 (&hi)[2], u32x4 (&lo)[2]) {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int key = 16 * grp + 8 * i + 2 * w;
-        if (key >= rows) v[dt][i][w] = 0u;
-        else if (key + 1 >= rows) v[dt][i][w] &= 0xffffu;
-      }
-      top8(v[dt][i], top, bad);
+    for (int w = 0; w < 4; ++w) {
+      const float a = x[2 * i + w / 2][2 * (w & 1)], b = x[2 * i + w / 2][2 * (w & 1) + 1];
+      const uint32_t h = pack_bf16x2(a, b);
+      hi[i][w] = h;
+      lo[i][w] = pack_bf16x2(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
     }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  const uint32_t e = __float_as_uint(top) & 0x7f800000u;  // 2^floor(log2 top)
-  const float scale = e == 0u ? 1.17549435e-38f : __uint_as_float(e);
-  const float inv = 1.f / scale;  // 2^-126 .. 2^126: exact (2^127 gives a subnormal, exact too)
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        v[dt][i][w] = pack_f16x2(__uint_as_float(v[dt][i][w] << 16) * inv,
-                                 __uint_as_float(v[dt][i][w] & 0xffff0000u) * inv);
-  return scale;
 }
 
 // Decode and verify. A workgroup takes one kv head of one sequence, 16 * RT query
@@ -543,19 +521,14 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
     for (int dt = 0; dt < DT; ++dt)
       xv[dt] = __builtin_amdgcn_raw_buffer_load_b128(vr, base + voff + dt * 16 * kBlk, 0, 0);
   };
-  // scores of block c at factor f to probabilities; what o is multiplied by in al
-  auto softmax = [&](f32x4 (&x)[4][RT], int c, float f, u32x4 (&pf)[RT][2], float (&al)[RT]) __attribute__((always_inline)) {
+  // scores of block c at factor f to probabilities of row column rt; what o is multiplied by
+  auto softmax = [&](const f32x4 (&x)[4][RT], int rt, int c, float f, f32x4 (&y)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      f32x4 y[4];
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          y[n][r] = c * kBlk + 16 * grp + 4 * n + r <= lim[rt] ? x[n][rt][r] * f : -INFINITY;
-      al[rt] = softmax_step(y, mx[rt], sum[rt]);
-      p_operands(y, pf[rt]);
-    }
+      for (int r = 0; r < 4; ++r)
+        y[n][r] = c * kBlk + 16 * grp + 4 * n + r <= lim[rt] ? x[n][rt][r] * f : -INFINITY;
+    return softmax_step(y, mx[rt], sum[rt]);
   };
   auto compute = [&](int c, auto bad) __attribute__((always_inline)) {
     constexpr bool BAD = decltype(bad)::value;
@@ -578,7 +551,12 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
     __builtin_amdgcn_sched_barrier(0);
     u32x4 pf[RT][2];
     float al[RT];
-    softmax(y, c, fabsf(ks) * sc, pf, al);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      f32x4 p[4];
+      al[rt] = softmax(y, rt, c, fabsf(ks) * sc, p);
+      p_operands(p, pf[rt]);
+    }
     const float f = fabsf(vs);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
@@ -617,36 +595,55 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
     const int64_t tl = ((int64_t)bh * 2 + (full & 1)) * (kBlk * D);
     const uint16_t* kt = a.k_tail + tl;
     const uint16_t* vt = a.v_tail + tl;
+    u32x4 k[4][DK], v[DT][2];
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < DK; ++i) k[n][i] = ld16(kt + koff + 4 * n * D + 64 * (i / 2) + 8 * (i & 1));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[dt][i] = ld16(vt + voff + dt * 16 * kBlk + 8 * i);
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 y[4][RT];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) y[n][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < DK; ++i) {
-        const u32x4 kf = ld16(kt + koff + 4 * n * D + 64 * (i / 2) + 8 * (i & 1));
+      for (int i = 0; i < DK; ++i)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) y[n][rt] = mfma16(kf, qf[rt][i], y[n][rt]);
-      }
+        for (int rt = 0; rt < RT; ++rt) y[n][rt] = mfma16(k[n][i], qf[rt][i], y[n][rt]);
     }
-    u32x4 v[DT][2];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) v[dt][i] = ld16(vt + voff + dt * 16 * kBlk + 8 * i);
-    const float vs = tail_values<DT>(v, end - full * kBlk, grp);
-    u32x4 pf[RT][2];
+    u32x4 hi[RT][2], lo[RT][2], live[2];
     float al[RT];
-    softmax(y, full, sc, pf, al);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int rt = 0; rt < RT; ++rt) {
+      f32x4 p[4];
+      al[rt] = softmax(y, rt, full, sc, p);
+      p_operands_bf16(p, hi[rt], lo[rt]);
+    }
+    const int left = end - full * kBlk - 16 * grp;  // of the lane group's 16 keys
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // the ring holds anything past the last key
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int key = 8 * i + 2 * w;
+        live[i][w] = key + 1 < left ? ~0u : key < left ? 0xffffu : 0u;
+      }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const u32x4 v0 = v[dt][0] & live[0], v1 = v[dt][1] & live[1];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        f32x4 pv = mfma16h(v[dt][0], pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
-        pv = mfma16h(v[dt][1], pf[rt][1], pv);
+        f32x4 pv = mfma16(v0, hi[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        pv = mfma16(v1, hi[rt][1], pv);
+        pv = mfma16(v0, lo[rt][0], pv);
+        pv = mfma16(v1, lo[rt][1], pv);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r] * al[rt]);
+        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(o[dt][rt][r], al[rt], pv[r]);
       }
+    }
   }
 
 #pragma unroll
@@ -1024,8 +1021,8 @@ Kv8Plan kv8_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t keys) {
     p.rt = B * Hk * ((rows + 127) / 128) >= kKv8Groups ? 2 : 1;
     p.n_rt = (int)((rows + 64 * p.rt - 1) / (64 * p.rt));
   }
-  // no range shorter than a block for each wave, or four tiles
-  const int64_t groups = B * Hk * p.n_rt, most = (keys + 4 * kBlk - 1) / (4 * kBlk);
+  // no range shorter than two blocks for each wave, or eight tiles
+  const int64_t groups = B * Hk * p.n_rt, most = (keys + 8 * kBlk - 1) / (8 * kBlk);
   int64_t ns = (p.rows && p.rt == 2 ? kKv8Groups / 2 : kKv8Groups) / groups;
   ns = ns < most ? ns : most;
   ns = ns < kKv8MaxSplit ? ns : kKv8MaxSplit;
