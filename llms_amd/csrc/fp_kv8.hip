@@ -44,7 +44,7 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 constexpr int kBlk = 64;
 constexpr int kKv8MaxSplit = 64;  // one lane per split in kv8_combine_kernel
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRise = 8.f;
+constexpr float kRise = 8.f;  // kv8_tiles_kernel: log2 of the largest p
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ f32x4 mfma16h(u32x4 a, u32x4 b, f32x4 c) {
@@ -234,28 +234,37 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
 
   // rows r0 .. r1-1 of block w: into the ring (tail) and into LDS (lds)
   auto put = [&](int w, int r0, int r1, bool tail, bool lds) {
+    constexpr int NP = kBlk / RPP;
     uint16_t* tk = tail_k(w & 1);
     uint16_t* tv = tail_v(w & 1);
-    for (int r = r0 + tid / LPH; r < r1; r += RPP) {
-      const int t = w * kBlk + r - s.first;
-      const int64_t m = (int64_t)b * a.T + t;
+    u32x2 lo[NP], hi[NP], v0[NP], v1[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {  // every row's loads before the first store
+      const int r = r0 + tid / LPH + p * RPP;
+      if (r >= r1) continue;
+      const int64_t m = (int64_t)b * a.T + (w * kBlk + r - s.first);
       const uint16_t* ks = a.k + m * a.ldk + (int64_t)h * D;
       const uint16_t* vs = a.v + m * a.ldv + (int64_t)h * D;
-      u32x2 lo = *reinterpret_cast<const u32x2*>(ks + 4 * j);
-      u32x2 hi = *reinterpret_cast<const u32x2*>(ks + D / 2 + 4 * j);
-      const u32x2 v0 = *reinterpret_cast<const u32x2*>(vs + 8 * j);
-      const u32x2 v1 = *reinterpret_cast<const u32x2*>(vs + 8 * j + 4);
-      if (a.cos) norm_rope_row<D>(lo, hi, a.gk, a.epsk, a.cos + t * a.ldc, a.sin + t * a.lds, j);
-      const uint32_t vv[4] = {v0.x, v0.y, v1.x, v1.y};
+      lo[p] = *reinterpret_cast<const u32x2*>(ks + 4 * j);
+      hi[p] = *reinterpret_cast<const u32x2*>(ks + D / 2 + 4 * j);
+      v0[p] = *reinterpret_cast<const u32x2*>(vs + 8 * j);
+      v1[p] = *reinterpret_cast<const u32x2*>(vs + 8 * j + 4);
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int r = r0 + tid / LPH + p * RPP, t = w * kBlk + r - s.first;
+      if (r >= r1) continue;
+      if (a.cos) norm_rope_row<D>(lo[p], hi[p], a.gk, a.epsk, a.cos + t * a.ldc, a.sin + t * a.lds, j);
+      const uint32_t vv[4] = {v0[p].x, v0[p].y, v1[p].x, v1[p].y};
       if (tail) {
-        *reinterpret_cast<u32x2*>(tk + r * D + 4 * j) = lo;
-        *reinterpret_cast<u32x2*>(tk + r * D + D / 2 + 4 * j) = hi;
+        *reinterpret_cast<u32x2*>(tk + r * D + 4 * j) = lo[p];
+        *reinterpret_cast<u32x2*>(tk + r * D + D / 2 + 4 * j) = hi[p];
 #pragma unroll
         for (int e = 0; e < 8; ++e) tv[(8 * j + e) * kBlk + r] = (uint16_t)(vv[e / 2] >> (16 * (e & 1)));
       }
       if (lds) {
-        *reinterpret_cast<u32x2*>(sm.k + r * D + 4 * j) = lo;
-        *reinterpret_cast<u32x2*>(sm.k + r * D + D / 2 + 4 * j) = hi;
+        *reinterpret_cast<u32x2*>(sm.k + r * D + 4 * j) = lo[p];
+        *reinterpret_cast<u32x2*>(sm.k + r * D + D / 2 + 4 * j) = hi[p];
 #pragma unroll
         for (int e = 0; e < 8; ++e) sm.v[(8 * j + e) * kVRow + r] = (uint16_t)(vv[e / 2] >> (16 * (e & 1)));
       }
@@ -686,30 +695,38 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
   }
 }
 
-// Prompts. A workgroup takes one kv head of one sequence and 64 * RT query rows
-// (wave w rows 16 RT w ..), and walks its blocks: codes into registers one block ahead,
-// then converted once for the four waves into LDS (keys bf16, values fp16, both
-// double-buffered), one barrier per block. Row tiles with the most keys start first.
-template <int D, int RT>
+// Prompts. A workgroup takes one kv head of one sequence and 64 query rows (wave w rows
+// 16 w ..), and walks its blocks: codes into registers one block ahead, then converted once
+// for the four waves into LDS (keys bf16, values fp16, both double-buffered), one
+// barrier per block. p is taken relative to a maximum that is moved only when the running
+// one has passed it by kRise (p up to 2^8: fp16 and the sums have room), so that a block
+// seldom rescales o. 128 rows to a workgroup halve the conversions and the LDS reads but
+// leave the registers no room: 8192 tokens of 16 heads 617 us against 580.
+// 1000 tokens at 1111, 32 heads: 65 us, 400 TFLOP/s; 2048 at 30000, 16 heads: 885 us with its
+// write, 590 TFLOP/s: bound by the vector unit (softmax and conversions) beside the matrix core.
+template <int D>
 __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) {
   constexpr int DK = D / 32, DT = D / 16;
   constexpr int NL = kBlk * D / 16 / 256;  // 16-code chunks per thread
   constexpr int CH = D / 8;                // 16-byte chunks of a key row in LDS
-  __shared__ __attribute__((aligned(16))) char sK[2][kBlk * D * 2];
-  __shared__ __attribute__((aligned(16))) char sV[2][kBlk * D * 2];
+  constexpr uint32_t SZ = kBlk * D * 2;
+  __shared__ __attribute__((aligned(16))) char sm[4 * SZ];  // keys, keys, values, values
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, grp = lane >> 4;
   const int G = a.Hq / a.Hk, rows = a.T * G;
   const int bh = blockIdx.y, b = bh / a.Hk, kh = bh - b * a.Hk;
-  const int tile = n_rt - 1 - (int)blockIdx.x;
-  const int row0 = tile * 64 * RT + wave * 16 * RT;
+  // the tiles with the most keys first; where the whole grid is resident at once (two
+  // workgroups per CU) its second half goes the other way, so that a CU's two make up for each other
+  const bool back = (int64_t)gridDim.x * gridDim.y * gridDim.z <= 512 && 2 * blockIdx.y >= gridDim.y;
+  const int tile = back ? (int)blockIdx.x : n_rt - 1 - (int)blockIdx.x;
+  const int row0 = tile * 64 + wave * 16;
   const Span s = span_of(a, b);
   const int end = s.beg < s.end ? s.end : 0;
   const int full = end / kBlk;
   // keys this workgroup's last row sees
-  int last = (tile + 1) * 64 * RT - 1;
+  int last = (tile + 1) * 64 - 1;
   if (last >= rows) last = rows - 1;
   const int64_t seen = (int64_t)s.first + last / G + 1;
   const int kend = seen < 0 ? 0 : seen < end ? (int)seen : end;
@@ -717,24 +734,14 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
   const int per = (nt + a.nsplit - 1) / a.nsplit;
   const int t_lo = (int)blockIdx.z * per, t_hi = t_lo + per < nt ? t_lo + per : nt;
 
-  u32x4 qf[RT][DK];
-  int lim[RT];
-  int hi = -1;
+  const int rr = row0 + li < rows ? row0 + li : rows - 1;
+  const int tq = rr / G, hq = kh * G + (rr - tq * G), lim = last_key(s, tq);
+  const uint16_t* qp = a.qsrc + ((int64_t)b * a.T + tq) * a.ldqs + (int64_t)hq * D + 8 * grp;
+  u32x4 qf[DK];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    int rr = row0 + rt * 16 + li;
-    if (rr >= rows) rr = rows - 1;
-    const int t = rr / G, h = kh * G + (rr - t * G);
-    lim[rt] = last_key(s, t);
-    hi = hi > lim[rt] ? hi : lim[rt];
-    const uint16_t* qp = a.qsrc + ((int64_t)b * a.T + t) * a.ldqs + (int64_t)h * D + 8 * grp;
-#pragma unroll
-    for (int i = 0; i < DK; ++i) qf[rt][i] = ld16_any(qp + 32 * i);
-  }
+  for (int i = 0; i < DK; ++i) qf[i] = ld16_any(qp + 32 * i);
   // the least and the largest last key of the wave's rows
-  int lo = lim[0];
-#pragma unroll
-  for (int rt = 1; rt < RT; ++rt) lo = lo < lim[rt] ? lo : lim[rt];
+  int lo = lim, hi = lim;
 #pragma unroll
   for (int off = 1; off < 16; off <<= 1) {
     const int x = __shfl_xor(lo, off), y = __shfl_xor(hi, off);
@@ -746,8 +753,18 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
   const int64_t at = (int64_t)bh * a.NB;
   // LDS places: key row r's chunk c at c ^ (4 (r / 16) + r % 4) (16 rows that a read
   // takes together differ there), value row d's chunk at c ^ (d % 8)
-  auto k_at = [](int r, int c) { return r * (D * 2) + ((c ^ (((r >> 4) * 4 + (r & 3)) & (CH - 1))) * 16); };
-  auto v_at = [](int d, int c) { return d * (kBlk * 2) + ((c ^ (d & 7)) * 16); };
+  auto k_at = [](int r, int c) { return (uint32_t)(r * (D * 2) + ((c ^ (((r >> 4) * 4 + (r & 3)) & (CH - 1))) * 16)); };
+  auto v_at = [](int d, int c) { return (uint32_t)(d * (kBlk * 2) + ((c ^ (d & 7)) * 16)); };
+  // where this lane reads (tile n of the keys 4 n rows on, value block dt 16 dt rows on) and
+  // puts its codes (the second half of 16 codes one chunk on: 16 off by an exclusive or)
+  uint32_t k_rd[DK], v_rd[2], k_wr[NL];
+#pragma unroll
+  for (int i = 0; i < DK; ++i) k_rd[i] = k_at(16 * (li >> 2) + (li & 3), 4 * i + grp);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v_rd[i] = v_at(li, 2 * grp + i);
+#pragma unroll
+  for (int n = 0; n < NL; ++n) k_wr[n] = k_at((n * 256 + tid) / (D / 16), (n * 256 + tid) % (D / 16) * 2);
+  const uint32_t v_wr = v_at(tid / 4, tid % 4 * 2);  // 64 n rows on
   u32x4 kx[NL], vx[NL];
   float ksc = 0.f, vsc = 0.f, ks_next = 0.f, vs_next = 0.f;
   auto load = [&](int kt) __attribute__((always_inline)) {
@@ -758,21 +775,20 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
 #pragma unroll
     for (int n = 0; n < NL; ++n) kx[n] = kc[n * 256 + tid], vx[n] = vc[n * 256 + tid];
   };
-  auto put = [&](char* k, char* v, auto bad) __attribute__((always_inline)) {
+  auto st = [&](uint32_t at, u32x4 x) { *reinterpret_cast<u32x4*>(sm + at) = x; };
+  auto put = [&](uint32_t k, uint32_t v, auto bad) __attribute__((always_inline)) {
     constexpr bool BAD = decltype(bad)::value;
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      const int i = n * 256 + tid;
-      const int r = i / (D / 16), c = (i % (D / 16)) * 2, d = i / 4, e = (i % 4) * 2;
-      *reinterpret_cast<u32x4*>(k + k_at(r, c)) = codes8_bf16<BAD>(kx[n][0], kx[n][1]);
-      *reinterpret_cast<u32x4*>(k + k_at(r, c + 1)) = codes8_bf16<BAD>(kx[n][2], kx[n][3]);
-      *reinterpret_cast<u32x4*>(v + v_at(d, e)) = codes8_f16<BAD>(vx[n][0], vx[n][1]);
-      *reinterpret_cast<u32x4*>(v + v_at(d, e + 1)) = codes8_f16<BAD>(vx[n][2], vx[n][3]);
+      st(k + k_wr[n], codes8_bf16<BAD>(kx[n][0], kx[n][1]));
+      st(k + (k_wr[n] ^ 16), codes8_bf16<BAD>(kx[n][2], kx[n][3]));
+      st(v + v_wr + n * (64 * kBlk * 2), codes8_f16<BAD>(vx[n][0], vx[n][1]));
+      st(v + (v_wr ^ 16) + n * (64 * kBlk * 2), codes8_f16<BAD>(vx[n][2], vx[n][3]));
     }
   };
   __shared__ float sTop[4];
   // block kt (loaded before, if whole) into LDS; its scales into ks, vs
-  auto store = [&](char* k, char* v, int kt, float& ks, float& vs) __attribute__((always_inline)) {
+  auto store = [&](uint32_t k, uint32_t v, int kt, float& ks, float& vs) __attribute__((always_inline)) {
     if (kt < full) {
       // not before here: the compiler would pull the conversions' shifts up to the loads
       // and wait for them there
@@ -794,7 +810,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int i = n * 256 + tid;
-      *reinterpret_cast<u32x4*>(k + k_at(i / CH, i % CH)) = ld16(a.k_tail + tl + i * 8);
+      st(k + k_at(i / CH, i % CH), ld16(a.k_tail + tl + i * 8));
       vv[n] = ld16(a.v_tail + tl + i * 8);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -819,147 +835,115 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
 #pragma unroll
       for (int w = 0; w < 4; ++w)
         o[w] = pack_f16x2(__uint_as_float(vv[n][w] << 16) * inv, __uint_as_float(vv[n][w] & 0xffff0000u) * inv);
-      *reinterpret_cast<u32x4*>(v + v_at(i / 8, i % 8)) = o;
+      st(v + v_at(i / 8, i % 8), o);
     }
     ks = 1.f, vs = scale;
   };
 
   const float sc = kLog2e / sqrtf((float)D);
-  f32x4 o[DT][RT];
-  float mx[RT];
-  f32x4 sum[RT];  // four equal rows: the products of ones and p
+  f32x4 o[DT], sum = {0.f, 0.f, 0.f, 0.f};  // sum: of p, four equal rows of ones times p
+  float mx = -INFINITY;  // what p is relative to: at most kRise under the running maximum
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    mx[rt] = -INFINITY;
-    sum[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  auto compute = [&](const char* k, const char* v, int kt, float ks, float vs, auto masked) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(masked)::value;
-    f32x4 x[RT][4];
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](uint32_t k, uint32_t v, int kt, float ks, float vs) __attribute__((always_inline)) {
+    if (kt * kBlk > lim_hi) return;  // every key hidden from every row
+    f32x4 x[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) x[rt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      x[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < DK; ++i) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(k + k_at(16 * (li >> 2) + 4 * n + (li & 3), 4 * i + grp));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) x[rt][n] = mfma16(kf, qf[rt][i], x[rt][n]);
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(sm + (k + k_rd[i]) + 4 * n * (D * 2));
+        x[n] = mfma16(kf, qf[i], x[n]);
       }
     }
+    // the values' reads go out behind the scores, ahead of the softmax
+    u32x4 vf[DT][2];
+    auto read_v = [&](int dt) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) vf[dt][i] = *reinterpret_cast<const u32x4*>(sm + (v + v_rd[i]) + dt * 16 * (kBlk * 2));
+    };
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) read_v(dt);
+    __builtin_amdgcn_sched_barrier(0);
     const float f = ks * sc;
-    float top[RT];
-    bool rise = false;
+    float top = -INFINITY;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if constexpr (MASK) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x[rt][n][r] = kt * kBlk + 16 * grp + 4 * n + r <= lim[rt] ? x[rt][n][r] * f : -INFINITY;
-      }
-      float m = -INFINITY;
+    for (int n = 0; n < 4; ++n) x[n] *= f;
+    if (kt * kBlk + kBlk - 1 > lim_lo) {
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m = fmaxf(m, x[rt][n][r]);
-      top[rt] = col_max(MASK ? m : m * f);
-      rise |= top[rt] > mx[rt] + kRise;
+        for (int r = 0; r < 4; ++r) x[n][r] = kt * kBlk + 16 * grp + 4 * n + r <= lim ? x[n][r] : -INFINITY;
     }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, x[n][r]);
+    top = col_max(top);
+    const bool rise = top > mx + kRise;
     if (__ballot(rise)) {
+      const float to = rise ? top : mx;
+      const float al = exp2_fast(mx - (to == -INFINITY ? 0.f : to));
+      mx = to;
+      sum *= al;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float to = top[rt] > mx[rt] + kRise ? top[rt] : mx[rt];
-        const float al = exp2_fast(mx[rt] - (to == -INFINITY ? 0.f : to));
-        mx[rt] = to;
-        sum[rt] *= al;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt][rt] *= al;
-      }
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= al;
     }
-    u32x4 pf[RT][2];
+    const float base = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float base = mx[rt] == -INFINITY ? 0.f : mx[rt];
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x[rt][n][r] = exp2_fast(MASK ? x[rt][n][r] - base : fmaf(x[rt][n][r], f, -base));
-      p_operands(x[rt], pf[rt]);
-    }
+      for (int r = 0; r < 4; ++r) x[n][r] = exp2_fast(x[n][r] - base);
+    u32x4 pf[2];
+    p_operands(x, pf);
     constexpr u32x4 kOnes = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sum[rt] = mfma16h(kOnes, pf[rt][i], sum[rt]);
+    for (int i = 0; i < 2; ++i) sum = mfma16h(kOnes, pf[i], sum);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const u32x4 v0 = *reinterpret_cast<const u32x4*>(v + v_at(dt * 16 + li, 2 * grp));
-      const u32x4 v1 = *reinterpret_cast<const u32x4*>(v + v_at(dt * 16 + li, 2 * grp + 1));
+      f32x4 pv = mfma16h(vf[dt][0], pf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      pv = mfma16h(vf[dt][1], pf[1], pv);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        f32x4 pv = mfma16h(v0, pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
-        pv = mfma16h(v1, pf[rt][1], pv);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[dt][rt][r] = fmaf(pv[r], vs, o[dt][rt][r]);
-      }
+      for (int r = 0; r < 4; ++r) o[dt][r] = fmaf(pv[r], vs, o[dt][r]);
     }
-  };
-  auto step = [&](const char* k, const char* v, int kt, float ks, float vs) __attribute__((always_inline)) {
-    if (kt * kBlk > lim_hi) return;  // every key hidden from every row
-    if (kt * kBlk + kBlk - 1 > lim_lo) compute(k, v, kt, ks, vs, std::true_type{});
-    else compute(k, v, kt, ks, vs, std::false_type{});
   };
 
   // q has arrived: a load pending at the loop's entry would have the compiler wait, in
-  // every round, for the loads of the next block too (109 us against %s)
+  // every round, for the loads of the next block too
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-    for (int i = 0; i < DK; ++i) asm volatile("" : "+v"(qf[rt][i]));
+  for (int i = 0; i < DK; ++i) asm volatile("" : "+v"(qf[i]));
   if (t_lo < t_hi) {
     load(t_lo);
-    store(sK[0], sV[0], t_lo, ksc, vsc);
+    store(0, 2 * SZ, t_lo, ksc, vsc);
     __syncthreads();
-    for (int kt = t_lo; kt < t_hi; ++kt) {
-      const int u = (kt - t_lo) & 1;
+    uint32_t u = 0;
+    for (int kt = t_lo; kt < t_hi; ++kt, u ^= SZ) {
       const bool more = kt + 1 < t_hi;
       if (more) load(kt + 1);
-      step(sK[u], sV[u], kt, ksc, vsc);
+      step(u, 2 * SZ + u, kt, ksc, vsc);
       if (more) {
-        store(sK[u ^ 1], sV[u ^ 1], kt + 1, ksc, vsc);
+        store(u ^ SZ, 2 * SZ + (u ^ SZ), kt + 1, ksc, vsc);
         __syncthreads();
       }
     }
   }
 
+  if (row0 + li >= rows) return;
+  const float l = sum[0];
+  if (a.nsplit > 1) {
+    const int64_t pr = part_row(a, blockIdx.z, bh, rr);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const float l = sum[rt][0];
-    const int rr = row0 + rt * 16 + li;
-    if (rr >= rows) continue;
-    if (a.nsplit > 1) {
-      const int64_t pr = part_row(a, blockIdx.z, bh, rr);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        *reinterpret_cast<f32x4*>(a.part + pr * D + dt * 16 + 4 * grp) = o[dt][rt];
-      if (grp == 0) *reinterpret_cast<f32x2*>(a.stat + pr * 2) = f32x2{mx[rt], l};
-    } else {
-      const int t = rr / G, h = kh * G + (rr - t * G);
-      const bool none = l == 0.f;  // a row that sees no key
-      uint16_t* yp = a.y + (((int64_t)b * a.T + t) * a.Hq + h) * D + 4 * grp;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const f32x4 v = o[dt][rt];
-        *reinterpret_cast<u32x2*>(yp + dt * 16) =
-            none ? u32x2{0u, 0u} : u32x2{pack_bf16x2(v[0] / l, v[1] / l), pack_bf16x2(v[2] / l, v[3] / l)};
-      }
-    }
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(a.part + pr * D + dt * 16 + 4 * grp) = o[dt];
+    if (grp == 0) *reinterpret_cast<f32x2*>(a.stat + pr * 2) = f32x2{mx, l};
+    return;
   }
+  const bool none = l == 0.f;  // a row that sees no key
+  uint16_t* yp = a.y + (((int64_t)b * a.T + tq) * a.Hq + hq) * D + 4 * grp;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    *reinterpret_cast<u32x2*>(yp + dt * 16) =
+        none ? u32x2{0u, 0u} : u32x2{pack_bf16x2(o[dt][0] / l, o[dt][1] / l), pack_bf16x2(o[dt][2] / l, o[dt][3] / l)};
 }
 
 // One output row per workgroup: lane s of each wave holds split s's statistics; each
@@ -1003,7 +987,7 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
 // The attention kernel's shape for a call that may see `keys` keys.
 struct Kv8Plan {
   bool rows;   // kv8_rows_kernel (else kv8_tiles_kernel)
-  int rt;      // 16-row blocks per wave
+  int rt;      // 16-row blocks per wave (rows)
   int n_rt;    // row groups (rows) or row tiles
   int nsplit;  // key ranges
 };
@@ -1018,8 +1002,8 @@ Kv8Plan kv8_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t keys) {
     p.rt = rows <= 16 ? 1 : 2;
     p.n_rt = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
   } else {
-    p.rt = B * Hk * ((rows + 127) / 128) >= kKv8Groups ? 2 : 1;
-    p.n_rt = (int)((rows + 64 * p.rt - 1) / (64 * p.rt));
+    p.rt = 1;
+    p.n_rt = (int)((rows + 63) / 64);
   }
   // no range shorter than two blocks for each wave, or eight tiles
   const int64_t groups = B * Hk * p.n_rt, most = (keys + 8 * kBlk - 1) / (8 * kBlk);
@@ -1053,8 +1037,7 @@ int launch_kv8_d(Kv8Args a, int64_t keys, hipStream_t s) {
     else hipLaunchKernelGGL((kv8_rows_kernel<D, 2>), grid, dim3(256), 0, s, a);
   } else {
     const dim3 grid((unsigned)p.n_rt, bh, (unsigned)p.nsplit);
-    if (p.rt == 1) hipLaunchKernelGGL((kv8_tiles_kernel<D, 1>), grid, dim3(256), 0, s, a, p.n_rt);
-    else hipLaunchKernelGGL((kv8_tiles_kernel<D, 2>), grid, dim3(256), 0, s, a, p.n_rt);
+    hipLaunchKernelGGL(kv8_tiles_kernel<D>, grid, dim3(256), 0, s, a, p.n_rt);
   }
   e = (int)hipGetLastError();
   if (e || p.nsplit == 1) return e;
