@@ -40,6 +40,13 @@ __device__ __forceinline__ float wave_max(float v) {
                      __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 48))));
 }
 
+// The largest of three that is a number (fmaxf would first quiet each operand).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float v;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(v) : "v"(a), "v"(b), "v"(c));
+  return v;
+}
+
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
   const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
@@ -95,6 +102,19 @@ struct Eight {
     if constexpr (DT == 1)
       return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[0][e / 2] >> (16 * (e & 1))));
     return __uint_as_float(w[e / 4][e & 3]);
+  }
+  // elements i .. i+7 of a row, all of them before `end` or none: -inf
+  __device__ __forceinline__ void load_whole(const void* row, int64_t i, int64_t end) {
+    constexpr int size = DT == 2 ? 4 : 2;
+    constexpr uint32_t none = DT == 0 ? 0xff80ff80u : DT == 1 ? 0xfc00fc00u : 0xff800000u;
+    const bool has = i < end;
+    const char* p = (const char*)row + (has ? i : end - 8) * size;
+#pragma unroll
+    for (int q = 0; q < (DT == 2 ? 2 : 1); ++q) {
+      w[q] = ld16_any(p + 16 * q);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[q][c] = has ? w[q][c] : none;
+    }
   }
   // elements i .. i+7 of a row, -inf from `end` on
   __device__ __forceinline__ void load(const void* row, int64_t i, int64_t end) {
@@ -154,8 +174,13 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a) {
   const void* x = (const char*)a.x + row * a.ld * (DT == 2 ? 4 : 2);
 
   Eight<DT> v[NV];
+  if ((end - i0) % 8 == 0) {  // whole chunks: no branch between the loads
 #pragma unroll
-  for (int j = 0; j < NV; ++j) v[j].load(x, i0 + (int64_t)(j * 256 + tid) * 8, end);
+    for (int j = 0; j < NV; ++j) v[j].load_whole(x, i0 + (int64_t)(j * 256 + tid) * 8, end);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j].load(x, i0 + (int64_t)(j * 256 + tid) * 8, end);
+  }
   if (TOP && tid == 0) sCount = 0;
 
   float vm[NV], tm = -INFINITY;
@@ -163,7 +188,7 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a) {
   for (int j = 0; j < NV; ++j) {
     vm[j] = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) vm[j] = fmaxf(vm[j], v[j].at(e));
+    for (int e = 0; e < 8; e += 2) vm[j] = max3(vm[j], v[j].at(e), v[j].at(e + 1));
     tm = fmaxf(tm, vm[j]);
   }
   tm = fmaxf(tm, dpp_f32<0xb1>(tm));
@@ -175,15 +200,34 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a) {
 
   float l = 0.f, u = 0.f;
   const float base = m == -INFINITY ? 0.f : m;
+  if (fabsf(base) < 0x1p120f) {
+    // exponents (x - base) log2 e by one operation each, about c = fl(base log2 e); what c is
+    // off by goes into the sums afterwards
+    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+    const float c = base * kLog2e, d = -fmaf(base, kLog2e, -c);
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float z = v[j].at(e) - base;
-      const float p = __builtin_amdgcn_exp2f(z * 1.4426950408889634f);
-      l += p;
-      u += fmaxf(z, -1e4f) * p;  // 0 where z is -inf
-    }
+      for (int e = 0; e < 8; ++e) {
+        const float z = fmaf(v[j].at(e), kLog2e, -c);
+        const float p = __builtin_amdgcn_exp2f(z);
+        l += p;
+        u = fmaf(fmaxf(z, -1e4f), p, u);  // 0 where z is -inf
+      }
+    const float r = __builtin_amdgcn_exp2f(d);
+    u = fmaf(d, l, u) * (r * kLn2);
+    l *= r;
+  } else {  // the product might be infinite (and a maximum of +inf gives NaN)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float z = v[j].at(e) - base;
+        const float p = __builtin_amdgcn_exp2f(z * 1.4426950408889634f);
+        l += p;
+        u += fmaxf(z, -1e4f) * p;
+      }
+  }
   l = wave_sum(l);
   u = wave_sum(u);
   if (lane == 0) sL[wave] = l, sU[wave] = u;
@@ -200,16 +244,28 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a) {
     // at or under -inf every element of the piece is a candidate
     const bool all = tau <= 0x7fu;
     const float cut = all ? -INFINITY : from_ordered(tau << 16);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (!(vm[j] >= cut)) continue;
-      const int64_t i = i0 + (int64_t)(j * 256 + tid) * 8;
+    auto offer = [&](const Eight<DT>& c, int64_t i) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float f = v[j].at(e);
+        const float f = c.at(e);
         if (!(f >= cut) || i + e >= end) continue;
         const int at = atomicAdd(&sCount, 1);
         if (at < kTopCap) sKey[at] = top_key(f, (uint32_t)(i + e));
+      }
+    };
+    if constexpr (E == 16) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (vm[j] >= cut) offer(v[j], i0 + (int64_t)(j * 256 + tid) * 8);
+    } else {  // read again: kept in registers, the logits would leave two waves per SIMD (206 us)
+      uint32_t some = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) some |= (uint32_t)(vm[j] >= cut) << j;
+      for (; some; some &= some - 1) {
+        const int64_t i = i0 + (int64_t)(__builtin_ctz(some) * 256 + tid) * 8;
+        Eight<DT> c;
+        c.load(x, i, end);
+        offer(c, i);
       }
     }
   }
@@ -242,14 +298,16 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a) {
   uint64_t last = ~0ull;
   for (int r = 0; r < a.k; ++r) {
     uint64_t best = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
+#pragma unroll 2
+    for (int64_t i = i0 + tid * 8; i < end; i += 2048) {
+      Eight<DT> c;
+      c.load(x, i, end);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int64_t i = i0 + (int64_t)(j * 256 + tid) * 8 + e;
-        const uint64_t key = i < end ? top_key(v[j].at(e), (uint32_t)i) : 0;
+        const uint64_t key = i + e < end ? top_key(c.at(e), (uint32_t)(i + e)) : 0;
         if (key < last && key > best) best = key;
       }
+    }
     best = wave_umax64(best);
     __syncthreads();  // sBest of the last round has been read
     if (lane == 0) sBest[wave] = best;
