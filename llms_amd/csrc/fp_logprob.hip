@@ -328,7 +328,21 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a) {
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x;
   const bool has = lane < a.pieces;
-  for (int i = lane; i < a.pieces * a.k; i += 64) list[i] = a.keys[row * a.pieces * a.k + i];
+  const int n_keys = a.pieces * a.k;
+  const uint64_t* keys = a.keys + row * n_keys;
+  for (int i0 = 0; i0 < n_keys; i0 += 512) {  // eight loads in flight (one at a time: 7.2 us for 760, against 5.6)
+    uint64_t key[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * 64 + lane;
+      key[j] = keys[i < n_keys ? i : 0];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * 64 + lane;
+      if (i < n_keys) list[i] = key[j];
+    }
+  }
   f32x4 st = {-INFINITY, 0.f, 0.f, 0.f};
   if (has) st = reinterpret_cast<const f32x4*>(a.stat)[row * a.pieces + lane];
   const float m = wave_max(st[0]);
