@@ -28,6 +28,8 @@
 #include "fp_common.h"
 #include "fp_launch.h"
 
+#include <type_traits>
+
 namespace fp {
 
 namespace {
@@ -143,11 +145,13 @@ struct Weights {
   }
 };
 
-// The scales of the same rows: a slab's in one load, moved back at the row's end and
-// shifted when they are used (past the last group: 0, where the codes meet zeros).
+// The scales of the same rows: a slab's in one load (without a branch, as the weights'),
+// moved back at the row's end and shifted when they are used (past the last group: 0, where the codes meet zeros).
 template <int NC, int GS, bool GATEUP>
 struct Scales {
   static constexpr int NG = 128 / GS;
+  // 32 bits where that is enough: a wider one is widened, and so waited for, at its load
+  using Raw = std::conditional_t<NG == 4, uint64_t, uint32_t>;
   const uint16_t* row[NC];
   int groups, last;
 
@@ -161,24 +165,19 @@ struct Scales {
       row[c] = (up ? a.s1 : a.s0) + (n < a.N ? n : a.N - 1) * (up ? a.lds1 : a.lds0);
     }
   }
-  __device__ __forceinline__ uint64_t load(int c, int slab) const {
+  __device__ __forceinline__ Raw load(int c, int slab) const {
     const int at = slab * NG < last ? slab * NG : last;
     if constexpr (NG == 1) return row[c][at];
     uint32_t v[2] = {0u, 0u};
-    if (groups >= NG) {
-      __builtin_memcpy(v, row[c] + at, 2 * NG);
-    } else {  // (the whole row: K of one slab)
-#pragma unroll
-      for (int g = 0; g < NG - 1; ++g)
-        if (g < groups) v[g / 2] |= (uint32_t)row[c][g] << (16 * (g & 1));
-    }
-    return v[0] | ((uint64_t)v[1] << 32);
+    __builtin_memcpy(v, row[c] + at, 2 * NG);  // rows of fewer have been widened
+    if constexpr (NG == 4) return v[0] | ((uint64_t)v[1] << 32);
+    else return v[0];
   }
-  __device__ __forceinline__ uint64_t fix(uint64_t s, int slab) const {
+  __device__ __forceinline__ Raw fix(Raw s, int slab) const {
     return NG > 1 && slab * NG > last ? s >> (16 * (slab * NG - last)) : s;
   }
-  static __device__ __forceinline__ float at(uint64_t s, int g) {
-    return bf16_bits_to_f32((uint32_t)(s >> (16 * g)) & 0xffffu);
+  static __device__ __forceinline__ float at(Raw s, int g) {
+    return __uint_as_float((uint32_t)(s >> (16 * g)) << 16);
   }
 };
 
@@ -464,7 +463,7 @@ __global__ __launch_bounds__(W * 64, 2) void w4_tiles_kernel(W4Args a) {
     }
   };
   u32x4 wq[PF][NC];
-  uint64_t sc[PF][NC];
+  typename Scales<NC, GS, GATEUP>::Raw sc[PF][NC];
   auto load_w = [&](int p, int slab) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -481,7 +480,7 @@ __global__ __launch_bounds__(W * 64, 2) void w4_tiles_kernel(W4Args a) {
     for (int c = 0; c < NC; ++c) acc[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto compute = [&](const char* x, int p, int slab) {
     u32x4 t[NC];
-    uint64_t s4[NC];
+    typename Scales<NC, GS, GATEUP>::Raw s4[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const u32x4 w = wt.fix(c, wq[p][c], slab);
@@ -543,9 +542,12 @@ __global__ __launch_bounds__(W * 64, 2) void w4_tiles_kernel(W4Args a) {
   if (lo < hi) {
     load_x(lo);
 #pragma unroll
-    for (int p = 0; p < PF; ++p) load_w(p, lo + p);
+    for (int p = 0; p < PF - 1; ++p) load_w(p, lo + p);
     store_x(sx[0]);
     load_x(lo + 1);
+    // in the loop's order: x with no weights behind it here would have the compiler wait for
+    // the weights in flight once in PF slabs
+    load_w(PF - 1, lo + PF - 1);
     __syncthreads();
     for (int i = lo; i < hi; i += PF) {
 #pragma unroll
@@ -581,10 +583,14 @@ __global__ __launch_bounds__(W * 64, 2) void w4_tiles_kernel(W4Args a) {
     }
 }
 
-// A weight of under 16 bytes as rows of 16 (the kernels load 16 bytes at a time).
-__global__ void w4_widen_kernel(const uint8_t* q, int64_t ldq, uint8_t* out, int64_t N, int64_t rowb) {
-  for (int64_t i = threadIdx.x; i < N * 16; i += blockDim.x)
-    out[i] = i % 16 < rowb ? q[i / 16 * ldq + i % 16] : 0;
+// Rows of rowb bytes as rows of `to`, zeros behind them: for a weight of under 16 bytes (the
+// kernels load 16 at a time) and for scales of less than a slab's groups.
+__global__ __launch_bounds__(256) void w4_widen_kernel(const uint8_t* q, int64_t ld, uint8_t* out, int64_t rows,
+                                                       int64_t rowb, int to) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * to) return;
+  const int64_t r = i / to, c = i - r * to;
+  out[i] = c < rowb ? q[r * ld + c] : 0;
 }
 
 template <bool GATEUP>
@@ -661,6 +667,8 @@ struct W4Plan {
 
 // Workspace of a weight that may have under 16 bytes (rows apart only make it longer).
 int64_t wide_bytes(int64_t N, int64_t K) { return N * ((K + 1) / 2) < 16 ? 512 : 0; }
+// ... and of the scales of two weights of at most three groups.
+int64_t scale_bytes(int64_t N, int64_t K) { return K <= 96 ? (N * 16 + 255) / 256 * 256 : 0; }
 
 int64_t row_lds(int64_t M, int64_t K, int nc, int group) {
   const int64_t slabs = (K + 127) / 128;
@@ -716,14 +724,19 @@ int launch_tiles(const W4Args& a, const W4Plan& p, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+int widen(const uint8_t* q, int64_t ld, uint8_t* out, int64_t rows, int64_t rowb, int to, hipStream_t s) {
+  hipLaunchKernelGGL(w4_widen_kernel, dim3((unsigned)((rows * to + 255) / 256)), dim3(256), 0, s, q, ld, out, rows,
+                     rowb, to);
+  return (int)hipGetLastError();
+}
+
 template <int GS>
 int launch_gs(W4Args a, const W4Plan& p, bool gateup, bool aligned, char* ws, hipStream_t s) {
   const int64_t rowb = (a.K + 1) / 2;
   if (!aligned && ((a.N - 1) * a.ldq0 + rowb < 16 || (gateup && (a.N - 1) * a.ldq1 + rowb < 16))) {
     uint8_t* wide = (uint8_t*)ws;  // N <= 15 rows, twice
-    hipLaunchKernelGGL(w4_widen_kernel, dim3(1), dim3(256), 0, s, a.q0, a.ldq0, wide, a.N, rowb);
-    if (gateup) hipLaunchKernelGGL(w4_widen_kernel, dim3(1), dim3(256), 0, s, a.q1, a.ldq1, wide + 256, a.N, rowb);
-    const int e = (int)hipGetLastError();
+    int e = widen(a.q0, a.ldq0, wide, a.N, rowb, 16, s);
+    if (!e && gateup) e = widen(a.q1, a.ldq1, wide + 256, a.N, rowb, 16, s);
     if (e) return e;
     a.q0 = wide, a.ldq0 = 16;
     if (gateup) a.q1 = wide + 256, a.ldq1 = 16;
@@ -735,6 +748,17 @@ int launch_gs(W4Args a, const W4Plan& p, bool gateup, bool aligned, char* ws, hi
     return aligned ? launch_row<GS, false, true>(a, p, s) : launch_row<GS, false, false>(a, p, s);
   }
   const int64_t slabs = (a.K + 127) / 128, rows = (a.M + 16 * p.rt - 1) / (16 * p.rt) * (16 * p.rt);
+  const int64_t groups = (a.K + GS - 1) / GS, most = 128 / GS;
+  if (groups < most) {
+    uint8_t* wide = (uint8_t*)ws;
+    const int64_t one = a.N * most * 2;
+    int e = widen((const uint8_t*)a.s0, a.lds0 * 2, wide, a.N, groups * 2, (int)most * 2, s);
+    if (!e && gateup) e = widen((const uint8_t*)a.s1, a.lds1 * 2, wide + one, a.N, groups * 2, (int)most * 2, s);
+    if (e) return e;
+    a.s0 = (const uint16_t*)wide, a.lds0 = most;
+    if (gateup) a.s1 = (const uint16_t*)(wide + one), a.lds1 = most;
+  }
+  ws += scale_bytes(a.N, a.K);
   a.panels = ws;
   a.part = (float*)(ws + rows / (16 * p.rt) * slabs * panel_bytes(p.rt));
   a.splits = p.splits;
@@ -753,7 +777,7 @@ int64_t w4_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gateup) {
   for (int group = 32; group <= 128; group *= 2) {
     const W4Plan p = w4_plan(M, N, K, group, gateup);
     if (p.row) continue;
-    int64_t b = (M + 16 * p.rt - 1) / (16 * p.rt) * ((K + 127) / 128) * panel_bytes(p.rt);
+    int64_t b = (M + 16 * p.rt - 1) / (16 * p.rt) * ((K + 127) / 128) * panel_bytes(p.rt) + scale_bytes(N, K);
     if (p.splits > 1) b += p.splits * M * N * (gateup ? 8 : 4);
     most = most > b ? most : b;
   }

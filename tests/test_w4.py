@@ -206,7 +206,7 @@ def test_packing_of_non_finite_and_tiny_groups():
 
 SHAPES = [(1, 1, 1), (1, 33, 17), (1, 128, 16), (2, 130, 5), (3, 1024, 64), (5, 2541, 50), (16, 512, 100),
           (17, 640, 33), (33, 384, 130), (64, 1000, 20), (65, 513, 70), (130, 256, 300), (1, 9728, 48),
-          (4, 12288, 32), (64, 4100, 97)]
+          (4, 12288, 32), (64, 4100, 97), (20, 40, 37), (70, 96, 20), (40, 3, 5)]
 
 
 @pytest.mark.gpu
