@@ -298,7 +298,7 @@ int kv8_args(const fp_kv8_args& g, bool tokens, bool queries, Kv8Args* out) {
   const int st = check_attention(g.B, g.T, queries ? g.n_heads : g.n_kv_heads, g.n_kv_heads, D);
   if (st) return st;
   if (S < 1 || S > (int64_t)1 << 23 || g.pos_stride < 0 || g.pos_stride > 1) return FP_ERR_SHAPE;
-  if (!g.pos_dev && (g.pos < 0 || g.pos + g.T > S)) return FP_ERR_SHAPE;
+  if (!g.pos_dev && (g.pos < 0 || g.pos > S - g.T)) return FP_ERR_SHAPE;
   // workgroups of the write and of the read, in threads within 2^32
   if (g.B * g.n_kv_heads * ((g.T + 126) / 64 + (g.T + 15) / 16) > (int64_t)1 << 23) return FP_ERR_SHAPE;
   if (tokens && (g.ldk < g.n_kv_heads * D || g.ldv < g.n_kv_heads * D || ((g.ldk | g.ldv) & 3)))

@@ -27,7 +27,9 @@
 // summed in fp32 and scaled after the sum, softmax and its sum in fp32. p enters the
 // matrix core in fp16 (2^-12 of itself, an eighth of the output's rounding): the codes
 // carry no more than 8 bits, so the parts that fp_attn.hip adds would be lost on
-// them. A block's product is scaled by s_v in fp32.
+// them. A block's product is scaled by s_v in fp32. The unfinished block's values are bf16:
+// kv8_rows_kernel takes p in two bf16 parts there, kv8_tiles_kernel brings the values to
+// fp16 at a power of two that puts the largest into [1, 2).
 #include "fp_common.h"
 #include "fp_launch.h"
 #include "fp_rope.h"
@@ -150,6 +152,9 @@ __device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
 
 // ---- write ------------------------------------------------------------------
 
+// 17 blocks of 8 heads take 16 us, 16 sequences of 4000 tokens (8000 blocks) 132 us, 3 TB/s: the
+// exact division of each entry and the turning of the values bound a block; one token of
+// 16 sequences, without a block to pack, 3-5 us.
 constexpr int kVRow = kBlk + 8;  // LDS row of a value column, padded against bank conflicts
 
 template <int D>
@@ -450,10 +455,13 @@ __device__ __forceinline__ void p_operands_bf16(const f32x4 (&x)[4], u32x4 (&hi)
 
 // Decode and verify. A workgroup takes one kv head of one sequence, 16 * RT query
 // rows (token t, group head g at row t * G + g) and one contiguous range of blocks;
-// its four waves take blocks w, w + 4, ... of the range straight into registers, each
-// with the next one's loads in flight (buffers that end with the last whole block
-// return zeros past it, so loads are issued without a branch), and merge their softmax
-// states through LDS in wave order.
+// its four waves take blocks w, w + 4, ... of the range straight into registers (buffers
+// that end with the last whole block return zeros past it, so loads are issued without a
+// branch) and merge their softmax
+// states through LDS in wave order. 16 sequences of 4000 tokens, 32 heads over 8: 23.5 us
+// and 4 us to combine, 4.3 TB/s of codes (RT 1: two workgroups per CU); five tokens at 65001:
+// 36 us, 3.7 TB/s (RT 2: one workgroup per CU, 109 registers would spill at two); one token
+// at 333: 7.5 us, of which most is the way to the first scores and through the merge.
 template <int D, int RT>
 __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args a) {
   constexpr int NW = 4, DK = D / 32, DT = D / 16, KU = D / 64;
@@ -1005,7 +1013,8 @@ Kv8Plan kv8_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t keys) {
     p.rt = 1;
     p.n_rt = (int)((rows + 63) / 64);
   }
-  // no range shorter than two blocks for each wave, or eight tiles
+  // no range shorter than two blocks for each wave, or eight tiles: one token at 333 keys
+  // 7.5 us in one range against 10.8 and 3.8 to combine in two
   const int64_t groups = B * Hk * p.n_rt, most = (keys + 8 * kBlk - 1) / (8 * kBlk);
   int64_t ns = (p.rows && p.rt == 2 ? kKv8Groups / 2 : kKv8Groups) / groups;
   ns = ns < most ? ns : most;

@@ -444,21 +444,23 @@ void check_w4(const char* fn, const at::Tensor& x, const at::Tensor& q, const at
   value_device(x, fn, "x");
 }
 
-const void* w4_gamma(const char* fn, const at::Tensor& x, const c10::optional<at::Tensor>& gamma, double eps) {
-  if (!gamma.has_value()) return nullptr;
+// The norm weight as the kernels read it, or an undefined tensor.
+at::Tensor w4_gamma(const char* fn, const at::Tensor& x, const c10::optional<at::Tensor>& gamma, double eps) {
+  if (!gamma.has_value()) return {};
+  TORCH_CHECK_VALUE(x.dim() >= 1, fn, ": x must have a last dimension of at least 1, got ", x.sizes());
   TORCH_CHECK_VALUE(gamma->dim() == 1 && gamma->size(0) == x.size(-1), fn, ": norm weight shape ", gamma->sizes(),
                     " != (", x.size(-1), ",)");
   TORCH_CHECK_VALUE(eps >= 0.0 && eps < 3.0e38, fn, ": eps must be finite and >= 0, got ", eps);
   type_is(*gamma, at::kBFloat16, fn, "norm weight");
   value_same(x, *gamma, fn, "x", "norm weight");
-  TORCH_CHECK_VALUE(gamma->is_contiguous(), fn, ": norm weight must be contiguous");
-  return gamma->data_ptr();
+  return as_rows(*gamma, gamma->size(0));
 }
 
 at::Tensor linear_w4(const at::Tensor& x, const c10::optional<at::Tensor>& gamma, double eps,
                      const at::Tensor& q_, const at::Tensor& s_, int64_t group) {
   const char* fn = "fused_linear_w4";
-  const void* g = w4_gamma(fn, x, gamma, eps);
+  const at::Tensor gm = w4_gamma(fn, x, gamma, eps);
+  const void* g = gm.defined() ? gm.data_ptr() : nullptr;
   check_w4(fn, x, q_, s_, group);
   const int64_t K = x.size(-1), N = q_.size(0);
   const c10::DeviceGuard guard(x.device());
@@ -480,7 +482,8 @@ at::Tensor gate_up_silu_w4(const at::Tensor& x, const c10::optional<at::Tensor>&
                            const at::Tensor& su_, int64_t group) {
   const char* fn = "fused_gate_up_silu_w4";
   TORCH_CHECK_VALUE(qg_.sizes() == qu_.sizes(), fn, ": qg shape ", qg_.sizes(), " != qu shape ", qu_.sizes());
-  const void* g = w4_gamma(fn, x, gamma, eps);
+  const at::Tensor gm = w4_gamma(fn, x, gamma, eps);
+  const void* g = gm.defined() ? gm.data_ptr() : nullptr;
   check_w4(fn, x, qg_, sg_, group);
   check_w4(fn, x, qu_, su_, group);
   const int64_t K = x.size(-1), N = qg_.size(0);
@@ -558,7 +561,7 @@ fp_kv8_args kv8_call(const char* fn, const at::Tensor& cache, at::IntArrayRef si
     a.pos_dev = pos->data_ptr<int64_t>();
     a.pos_stride = pos->dim();
   } else {
-    TORCH_CHECK_VALUE(start_pos >= 0 && start_pos + T <= size[3], fn, ": positions ", start_pos, " .. ",
+    TORCH_CHECK_VALUE(start_pos >= 0 && start_pos <= size[3] - T, fn, ": positions ", start_pos, " .. ",
                       start_pos + T - 1, " are outside the cache of ", size[3]);
     a.pos = start_pos;
   }

@@ -150,7 +150,7 @@ def attention_core_kv8(q, k, v, *, q_norm, k_norm, num_heads: int, cache: KVCach
     fn, D = "attention_kv8", cache.head_dim
     B, T, _ = q.shape
     fused = (plain_norm(q_norm) and plain_norm(k_norm) and not autocast()
-             and all(t.dtype == torch.bfloat16 and t.shape == (D,) and t.is_contiguous()
+             and all(t.dtype == torch.bfloat16 and t.shape == (D,) and t.is_contiguous() and t.data_ptr() % 8 == 0
                      for t in (q_norm.weight, k_norm.weight))
              and all(t.dtype == torch.bfloat16 and t.shape == (T, D) and t.stride(1) == 1 and t.device == q.device
                      for t in (cos, sin))

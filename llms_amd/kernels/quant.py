@@ -46,18 +46,7 @@ def quantize_w4(W: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, torch.
 
     Returns ``(q, s)``: uint8 ``[N, ceil(K/2)]`` and bfloat16 ``[N, ceil(K/group)]``.
     """
-    if W.dim() != 2:
-        raise ValueError(f"W must be 2D (N, K), got shape {tuple(W.shape)}")
-    if W.shape[1] < 1:
-        raise ValueError(f"quantize_w4: rows of at least one input are taken, got shape {tuple(W.shape)}")
-    if group not in (32, 64, 128):
-        raise ValueError(f"quantize_w4: group must be 32, 64 or 128, got {group}")
-    require_bf16_hip("quantize_w4", W=W)
-    W = inner_contiguous(W.detach())
-    if W.shape[0] > 1 and W.stride(0) < W.shape[1]:
-        W = W.contiguous()
-    q, s = _lib.ops().quantize_w4(W, group)
-    return q, s
+    return _lib.ops().quantize_w4(W.detach(), group)  # which checks them
 
 
 def dequantize_w4(q: torch.Tensor, s: torch.Tensor, K: int, *, group: int = 128) -> torch.Tensor:

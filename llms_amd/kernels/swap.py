@@ -50,6 +50,8 @@ def apply_triton_kernels(
     """
     if int8 and int4:
         raise ValueError("apply_triton_kernels: int8 and int4 exclude each other")
+    if int4 and w4_group not in (32, 64, 128):
+        raise ValueError(f"apply_triton_kernels: w4_group must be 32, 64 or 128, got {w4_group}")
     low = dict(int8=int8, w4_group=w4_group if int4 else 0)
     if linear_down_o and getattr(model, "fused_head", None) is False:
         model.fused_head = True

@@ -101,8 +101,9 @@ def test_refusals_on_the_cpu():
             fk.KVCache8.alloc(**a)
     with pytest.raises(ValueError, match="batch"):
         c.read(0, 0, 5, batch=3)
-    with pytest.raises(ValueError, match="outside"):
-        c.read(0, 98, 3)
+    for p in (98, -1, (1 << 63) - 1):
+        with pytest.raises(ValueError, match="outside"):
+            c.read(0, p, 3)
     from llms_amd import harness as h
 
     m = h.tiny_model(h.Cfg(head_dim=64))
@@ -142,7 +143,8 @@ def test_c_entry_refusals():
     NULL, SHAPE, STRIDE, WORKSPACE = 1, 2, 3, 6
     for fn in ("attention", "write", "read"):
         for kw in (dict(B=0), dict(T=0), dict(n_kv_heads=0), dict(head_dim=96), dict(cache_len=0), dict(pos=-1),
-                   dict(pos=198), dict(cache_len=(1 << 23) + 1), dict(pos_stride=2), dict(T=1 << 30)):
+                   dict(pos=198), dict(pos=(1 << 63) - 1), dict(cache_len=(1 << 23) + 1), dict(pos_stride=2),
+                   dict(T=1 << 30)):
             assert call(fn, **kw) == SHAPE, (fn, kw)
         for n in ("k_codes", "v_codes", "k_scale", "v_scale", "k_tail", "v_tail", "tail_block"):
             assert call(fn, **{n: None}) == NULL, (fn, n)

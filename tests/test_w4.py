@@ -110,6 +110,9 @@ def test_refusals_on_the_cpu():
         fk.quantize_w4(x)
     with pytest.raises(ValueError, match="exclude"):
         fk.apply_triton_kernels(torch.nn.Module(), int8=True, int4=True)
+    for group in (0, 48):
+        with pytest.raises(ValueError, match="w4_group"):
+            fk.apply_triton_kernels(torch.nn.Module(), int4=True, w4_group=group)
 
 
 def test_c_entry_refusals():
@@ -257,6 +260,9 @@ def test_qkv_norm_and_views(M):
         xn = norm(xd)
     a = fk.fused_rmsnorm_qkv_w4(xd, gamma.to(DEV), norm.eps, *wd, n_q=n_q, n_k=n_k)
     check_linear(torch.cat(a, -1), xn.cpu(), w, 128)
+    spread = gamma.repeat_interleave(2).to(DEV)[::2]
+    b = fk.fused_rmsnorm_qkv_w4(xd, spread, norm.eps, *wd, n_q=n_q, n_k=n_k)
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
     g = fk.fused_rmsnorm_gate_up_silu_w4(xd, gamma.to(DEV), norm.eps, *wd, *wd)
     check_gate_up(g, xn.cpu(), w, w, 128)
 
