@@ -152,7 +152,7 @@ __device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
 
 // ---- write ------------------------------------------------------------------
 
-// 17 blocks of 8 heads take 16 us, 16 sequences of 4000 tokens (8000 blocks) 132 us, 3 TB/s: the
+// 17 blocks of 8 heads take 15 us, 16 sequences of 4000 tokens (8000 blocks) 132 us, 3 TB/s: the
 // exact division of each entry and the turning of the values bound a block; one token of
 // 16 sequences, without a block to pack, 3-5 us.
 constexpr int kVRow = kBlk + 8;  // LDS row of a value column, padded against bank conflicts
@@ -237,8 +237,8 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
   auto tail_k = [&](int sl) { return a.k_tail + ((int64_t)bh * 2 + sl) * (kBlk * D); };
   auto tail_v = [&](int sl) { return a.v_tail + ((int64_t)bh * 2 + sl) * (kBlk * D); };
 
-  // rows r0 .. r1-1 of block w: into the ring (tail) and into LDS (lds)
-  auto put = [&](int w, int r0, int r1, bool tail, bool lds) {
+  // rows r0 .. r1-1 of block w: into the ring, or into LDS
+  auto put = [&](int w, int r0, int r1, bool ring) {
     constexpr int NP = kBlk / RPP;
     uint16_t* tk = tail_k(w & 1);
     uint16_t* tv = tail_v(w & 1);
@@ -261,13 +261,12 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
       if (r >= r1) continue;
       if (a.cos) norm_rope_row<D>(lo[p], hi[p], a.gk, a.epsk, a.cos + t * a.ldc, a.sin + t * a.lds, j);
       const uint32_t vv[4] = {v0[p].x, v0[p].y, v1[p].x, v1[p].y};
-      if (tail) {
+      if (ring) {
         *reinterpret_cast<u32x2*>(tk + r * D + 4 * j) = lo[p];
         *reinterpret_cast<u32x2*>(tk + r * D + D / 2 + 4 * j) = hi[p];
 #pragma unroll
         for (int e = 0; e < 8; ++e) tv[(8 * j + e) * kBlk + r] = (uint16_t)(vv[e / 2] >> (16 * (e & 1)));
-      }
-      if (lds) {
+      } else {
         *reinterpret_cast<u32x2*>(sm.k + r * D + 4 * j) = lo[p];
         *reinterpret_cast<u32x2*>(sm.k + r * D + D / 2 + 4 * j) = hi[p];
 #pragma unroll
@@ -276,10 +275,25 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
     }
   };
 
+  // LDS rows 0 .. n-1 into a slot of the ring (of a value column's last eight, anything
+  // behind them)
+  auto keep = [&](int sl, int n) {
+    for (int i = tid; i < n * (D / 8); i += 256)
+      reinterpret_cast<u32x4*>(tail_k(sl))[i] = reinterpret_cast<const u32x4*>(sm.k)[i];
+    const int nc = (n + 7) / 8;
+    for (int i = tid; i < D * nc; i += 256) {
+      const int d = i / nc, c = (i % nc) * 8;
+      *reinterpret_cast<u32x4*>(tail_v(sl) + d * kBlk + c) = *reinterpret_cast<const u32x4*>(sm.v + d * kVRow + c);
+    }
+  };
+
+  const bool mine = !(old_first && blk == after);  // whether this workgroup stores its block's ring
+  if (!complete && !mine) return;
   const bool assemble = complete || (have_old && !tag_ok);
-  if (!assemble) {  // most calls of one token: nothing but its rows
-    if (old_first && blk == after) return;
-    put(blk, row0, row1, true, false);
+  // most calls of one token: nothing but its rows; more than a few of them as single
+  // elements of the value columns cost more than the way through LDS
+  if (!assemble && (have_old || row1 < 8)) {
+    put(blk, row0, row1, true);
     if (!have_old && tid == 0) a.tail_block[bh * 2 + slot] = blk;
     return;
   }
@@ -298,22 +312,11 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
     }
   }
   __syncthreads();  // the old rows' last chunk reaches into the new rows
-  put(blk, row0, row1, in_tail && !have_old && !(old_first && blk == after), true);
+  put(blk, row0, row1, false);
   __syncthreads();
-  if (in_tail && have_old) {  // the whole block: its old rows may not be in the ring
-    for (int i = tid; i < row1 * (D / 8); i += 256)
-      reinterpret_cast<u32x4*>(tail_k(slot))[i] = reinterpret_cast<const u32x4*>(sm.k)[i];
-    const int nc = (row1 + 7) / 8;
-    for (int i = tid; i < D * nc; i += 256) {
-      const int d = i / nc, c = (i % nc) * 8;
-      *reinterpret_cast<u32x4*>(tail_v(slot) + d * kBlk + c) = *reinterpret_cast<const u32x4*>(sm.v + d * kVRow + c);
-    }
-  }
-  if (old_first && blk == fb) {
-    put(after, 0, after == lb ? s.end - lb * kBlk : kBlk, true, false);
-    if (tid == 0) a.tail_block[bh * 2 + slot] = after;
-  } else if (in_tail && !(old_first && blk == after) && tid == 0) {
-    a.tail_block[bh * 2 + slot] = blk;
+  if (in_tail && mine) {  // the whole block: its old rows may not be in the ring
+    keep(slot, row1);
+    if (tid == 0) a.tail_block[bh * 2 + slot] = blk;
   }
   if (!complete) return;
 
@@ -352,6 +355,13 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
     const int i = n * 256 + tid;
     reinterpret_cast<u32x2*>(kc)[i] = code8(kx[n], top[0]);
     reinterpret_cast<u32x2*>(vc)[i] = code8(vx[n], top[1]);
+  }
+  if (old_first && blk == fb) {  // `after`, behind the old rows and the packed block
+    const int n = after == lb ? s.end - lb * kBlk : kBlk;
+    put(after, 0, n, false);
+    __syncthreads();
+    keep(slot, n);
+    if (tid == 0) a.tail_block[bh * 2 + slot] = after;
   }
 }
 
