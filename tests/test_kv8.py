@@ -196,6 +196,24 @@ def test_what_the_cache_holds(P, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("first,then", [(37, 91), (37, 100), (63, 65), (63, 66), (1, 191), (5, 250), (70, 129), (64, 130)])
+def test_a_write_from_inside_a_block_over_the_next_ones(first, then, D):
+    """Old rows are read from the ring slot that a later block of the same call goes to."""
+    B, H, P = 8, 4, first + then + 70
+    k, v = tokens(first, B, P, H, D), tokens(then, B, P, H, D)
+    kd, vd = k.to(DEV), v.to(DEV)
+    c = new(P, H, D, B)
+    at = 0
+    for n in (first, then, 1, 69):
+        c.write(0, kd[:, at : at + n], vd[:, at : at + n], at)
+        at += n
+        rk, rv = (t.cpu() for t in c.read(0, 0, at))
+        for b in range(B):
+            assert torch.equal(rk[b], held(k[b], at)) and torch.equal(rv[b], held(v[b], at)), (b, at)
+
+
+@pytest.mark.gpu
 def test_packing_ties_zeros_and_sizes():
     x = torch.zeros(1, 256, 1, 64)
     x[0, 0, 0, 0], x[0, 1, 0] = 3.0, 1.5              # half of the largest: 63.5 is a tie
@@ -325,6 +343,23 @@ def test_non_finite_entries(T):
     c.write(0, k.to(DEV), v.to(DEV), 0)
     y = fk.attention_kv8(q.to(DEV), k2.to(DEV), v2.to(DEV), c, 0, P).cpu()
     assert y[0, :, :2, 7].isnan().all() and y[0, :, :2].isnan().sum() == 2 * T  # the bad value's column
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rise", [1.0, 5.0, 7.9, 40.0, -5.0])
+@pytest.mark.parametrize("T,D", [(100, 64), (70, 128), (3, 128)])
+def test_a_maximum_that_rises_by_blocks(T, D, rise):
+    """Scores that grow (or fall) by 2^rise from block to block: what p is relative to
+    follows in steps or at once, and every row comes out the same."""
+    P = 1300
+    u = torch.ones(D) * D**-0.25
+    at = (torch.arange(P) // BLOCK).float() * rise * math.log(2)
+    k = (at[:, None, None] * u + 0.1 * tokens(1, 1, P, 1, D)[0].float()).bfloat16()[None]
+    v, q = tokens(2, 1, P, 1, D), (u + 0.02 * tokens(3, 1, T, 2, D).float()).bfloat16()
+    c = new(P, 1, D)
+    c.write(0, k[:, : P - T].to(DEV), v[:, : P - T].to(DEV), 0)
+    y = fk.attention_kv8(q.to(DEV), k[:, P - T :].to(DEV), v[:, P - T :].to(DEV), c, 0, P - T)
+    check(y[0], q[0], held(k[0], P), held(v[0], P), P - T)
 
 
 @pytest.mark.gpu
