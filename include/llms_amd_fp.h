@@ -360,8 +360,9 @@ int fp_attention_bf16(const fp_attention_args* args, void* workspace, int64_t wo
  * positions pos .. pos+T-1 of sequences that end there (0 outside the cache).
  * head_dim is 64 or 128; cache_len at most 2^23; codes, scales and tails 16-byte
  * aligned. With pos, [pos, pos+T) has to lie in the cache (FP_ERR_SHAPE). Calls on one
- * cache must not overlap. workspace: at least fp_kv8_workspace_bytes(..., keys) with keys
- * = pos + T, or cache_len with pos_dev; 16-byte aligned; written before it is read.
+ * cache must not overlap. workspace: at least fp_kv8_workspace_bytes(..., keys, rope) with
+ * keys = pos + T, or cache_len with pos_dev, and rope whether cos is given; 16-byte aligned;
+ * written before it is read (0 bytes for short caches without cos: NULL will do).
  */
 typedef struct fp_kv8_args {
   const void *q, *k, *v;
@@ -382,7 +383,7 @@ typedef struct fp_kv8_args {
 } fp_kv8_args;
 
 int64_t fp_kv8_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int64_t n_kv_heads,
-                               int64_t head_dim, int64_t keys);
+                               int64_t head_dim, int64_t keys, int rope);
 int fp_kv8_attention(const fp_kv8_args* args, void* workspace, int64_t workspace_bytes,
                      void* stream);
 int fp_kv8_write(const fp_kv8_args* args, void* stream);

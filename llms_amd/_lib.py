@@ -57,7 +57,7 @@ CAPI_SIGNATURES: dict[str, list] = {
                                    _I64, _P, _I64, _P],
     "fp_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64],
     "fp_attention_bf16": [_P, _P, _I64, _P],
-    "fp_kv8_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64],
+    "fp_kv8_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64, ctypes.c_int],
     "fp_kv8_attention": [_P, _P, _I64, _P],
     "fp_kv8_write": [_P, _P],
     "fp_kv8_read": [_P, _P, _P, _P],

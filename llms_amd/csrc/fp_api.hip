@@ -691,9 +691,9 @@ int fp_attention_bf16(const fp_attention_args* g, void* workspace, int64_t works
 }
 
 int64_t fp_kv8_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int64_t n_kv_heads,
-                               int64_t head_dim, int64_t keys) {
+                               int64_t head_dim, int64_t keys, int rope) {
   if (fp::check_attention(B, T, n_heads, n_kv_heads, head_dim) || keys < 1) return 0;
-  return fp::kv8_workspace_bytes(B, T, n_heads, n_kv_heads, head_dim, keys);
+  return fp::kv8_workspace_bytes(B, T, n_heads, n_kv_heads, head_dim, keys, rope != 0);
 }
 
 int fp_kv8_attention(const fp_kv8_args* g, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -702,9 +702,9 @@ int fp_kv8_attention(const fp_kv8_args* g, void* workspace, int64_t workspace_by
   const int st = fp::kv8_args(*g, true, true, &a);
   if (st) return st;
   const int64_t keys = g->pos_dev ? g->cache_len : g->pos + g->T;
-  if (!workspace || !fp::al16(workspace) ||
-      workspace_bytes < fp::kv8_workspace_bytes(g->B, g->T, g->n_heads, g->n_kv_heads, g->head_dim, keys))
-    return FP_ERR_WORKSPACE;
+  const int64_t need =
+      fp::kv8_workspace_bytes(g->B, g->T, g->n_heads, g->n_kv_heads, g->head_dim, keys, g->cos != nullptr);
+  if (workspace_bytes < need || (need > 0 && !workspace) || !fp::al16(workspace)) return FP_ERR_WORKSPACE;
   return fp::launch_status(fp::launch_kv8_attention(a, g->head_dim, keys, workspace, (hipStream_t)stream));
 }
 

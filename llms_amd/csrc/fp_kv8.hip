@@ -1069,10 +1069,10 @@ inline int touched(int64_t T) { return (int)((T + 2 * kBlk - 2) / kBlk); }
 
 }  // namespace
 
-int64_t kv8_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys) {
+int64_t kv8_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys, bool rope) {
   const Kv8Plan p = kv8_plan(B, T, Hq, Hk, keys);
   const int64_t rows = B * T * Hq;
-  int64_t b = up256(rows * D * 2);
+  int64_t b = rope ? up256(rows * D * 2) : 0;
   if (p.nsplit > 1) b += up256(rows * p.nsplit * 8) + rows * p.nsplit * D * 4;
   return b;
 }
@@ -1081,8 +1081,8 @@ int launch_kv8_attention(Kv8Args a, int64_t D, int64_t keys, void* ws, hipStream
   const Kv8Plan p = kv8_plan(a.B, a.T, a.Hq, a.Hk, keys);
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
   char* w = (char*)ws;
-  a.qn = (uint16_t*)w;
-  w += up256(rows * D * 2);
+  a.qn = (uint16_t*)w;  // q normalised and rotated
+  if (a.cos) w += up256(rows * D * 2);
   a.stat = (float*)w;
   if (p.nsplit > 1) w += up256(rows * p.nsplit * 8);
   a.part = (float*)w;

@@ -224,7 +224,7 @@ struct Kv8Args {
   float *part, *stat;
   int nsplit;
 };
-int64_t kv8_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
+int64_t kv8_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t keys, bool rope);
 int launch_kv8_attention(Kv8Args a, int64_t D, int64_t keys, void* ws, hipStream_t s);
 int launch_kv8_write(Kv8Args a, int64_t D, hipStream_t s);
 // k, v [B][T][Hk][D] fp32.

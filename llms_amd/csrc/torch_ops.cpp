@@ -647,8 +647,9 @@ at::Tensor attention_kv8(const at::Tensor& q_, const at::Tensor& k_, const at::T
     a.q_eps = (float)q_eps, a.k_eps = (float)k_eps;
   }
   const int64_t keys = a.pos_dev ? a.cache_len : start_pos + T;
-  const int64_t bytes = fp_kv8_workspace_bytes(B, T, H, size[1], D, keys);
-  at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const int64_t bytes = fp_kv8_workspace_bytes(B, T, H, size[1], D, keys, a.cos != nullptr);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({bytes}, q.options().dtype(at::kByte));
   a.y = y.data_ptr();
   check_status(fp_kv8_attention(&a, bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(q)), "fp_kv8_attention");
   return y;

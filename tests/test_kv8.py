@@ -126,8 +126,10 @@ class Args(ctypes.Structure):
 def test_c_entry_refusals():
     lib = _lib.capi()
     P = 4096  # never dereferenced: every call below is refused before a launch
-    need = lib.fp_kv8_workspace_bytes(2, 3, 4, 2, 128, 103)
-    assert need > 0 and lib.fp_kv8_workspace_bytes(2, 3, 4, 2, 96, 103) == 0
+    need = lib.fp_kv8_workspace_bytes(2, 3, 4, 2, 128, 103, 1)
+    assert need > 0 and lib.fp_kv8_workspace_bytes(2, 3, 4, 2, 96, 103, 1) == 0
+    assert lib.fp_kv8_workspace_bytes(2, 3, 4, 2, 128, 103, 0) == 0
+    assert lib.fp_kv8_workspace_bytes(2, 3, 4, 2, 128, 8000, 0) > 0
 
     def call(fn="attention", ws=P, nb=need, ko=P, **kw):
         a = dict(q=P, k=P, v=P, ldq=512, ldk=256, ldv=256, k_codes=P, v_codes=P, k_scale=P, v_scale=P, k_tail=P,
@@ -162,7 +164,7 @@ def test_c_entry_refusals():
                dict(q_gamma=P, k_gamma=P)):
         assert call(**kw) == NULL, kw
     for kw in (dict(ws=None), dict(nb=need - 1), dict(ws=P + 8)):
-        assert call(**kw) == WORKSPACE, kw
+        assert call(**kw, cos=P, sin=P, ld_cos=128, ld_sin=128) == WORKSPACE, kw
     assert call("read", ko=None) == NULL and call("read", ko=P + 4) == STRIDE
 
 
