@@ -204,9 +204,10 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a) {
 
   float l = 0.f, u = 0.f;
   const float base = m == -INFINITY ? 0.f : m;
-  if (fabsf(base) < 0x1p120f) {
+  if (fabsf(base) < 0x1p20f) {
     // exponents (x - base) log2 e by one operation each, about c = fl(base log2 e); what c is
-    // off by goes into the sums afterwards
+    // off by (d, up to half a step of c: 2^-4 here, far beyond exp2's range for a mask of
+    // -1e10) goes into the sums afterwards
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     const float c = base * kLog2e, d = -fmaf(base, kLog2e, -c);
 #pragma unroll
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(256) void logprob_part_kernel(LogprobArgs a) {
     const float r = __builtin_amdgcn_exp2f(d);
     u = fmaf(d, l, u) * (r * kLn2);
     l *= r;
-  } else {  // the product might be infinite (and a maximum of +inf gives NaN)
+  } else {  // (a maximum of +inf gives NaN)
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll

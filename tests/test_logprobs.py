@@ -244,3 +244,33 @@ def test_scoring_a_text_with_a_model():
     got = h.teacher_forced_logprobs(m, tokens, DEV, top_k=4)
     logits = h.teacher_forced_logits(m, tokens, DEV)[:-1]
     check(logits, torch.tensor(tokens[1:], device=DEV), 4, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [60, 5000, 151936])
+@pytest.mark.parametrize("mask", [-1e5, -1e9, -1e10, -1e20, -1e30, "lowest"])
+def test_finite_masks(mask, V, dtype):
+    """Forbidden tokens at a large finite value instead of -inf: whole pieces of a row, all
+    but one token, the whole row, all but a token as far above zero. What is not masked
+    spreads over less than 32 (check's tolerance there); a masked token's distance is a
+    difference of fp32 values, and a second one with log l (2^-23 of it)."""
+    low = torch.finfo(dtype).min if mask == "lowest" else mask
+    x, _ = make(5, V, torch.float32, seed=9)
+    x[0, : V // 2] = low
+    x[1] = low
+    x[1, V - 1] = 1.0
+    x[2] = low
+    x[3] = low
+    x[3, 0] = -low
+    x[4, V // 3 :] = low
+    x, t = x.to(dtype), torch.tensor([V - 1, V - 1, 3, 0, 0], device=DEV)
+    got = fk.token_logprobs(x, t, 5)
+    at, h, ids, top = reference(x, t, 5)
+    tol = 2.0**-24 * (160 + 8 * 32)
+    assert ((got.logprob.cpu().double() - at).abs() <= tol).all()
+    assert ((got.entropy.cpu().double() - h).abs() <= tol * (2 + 2 * math.log(V))).all()
+    top = top.float().double()  # (twice the largest number is -inf in 32 bits)
+    g = got.top_logprobs.cpu().double()
+    assert ((g == top) | ((g - top).abs() <= tol + top.abs() * 2.0**-23)).all()
+    assert torch.equal(got.top_ids.cpu(), ids)
