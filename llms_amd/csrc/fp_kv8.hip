@@ -27,9 +27,14 @@
 // summed in fp32 and scaled after the sum, softmax and its sum in fp32. p enters the
 // matrix core in fp16 (2^-12 of itself, an eighth of the output's rounding): the codes
 // carry no more than 8 bits, so the parts that fp_attn.hip adds would be lost on
-// them. A block's product is scaled by s_v in fp32. The unfinished block's values are bf16:
-// kv8_rows_kernel takes p in two bf16 parts there, kv8_tiles_kernel brings the values to
-// fp16 at a power of two that puts the largest into [1, 2).
+// them. fp16 has its full 11 bits from 2^-14 on only, and a row of one large p and many
+// tiny ones is common (a first token that most heads look at): so p goes in times
+// 2^kLift, up to 2^15 with what kRise leaves it, and the value codes times 2^-kLift, both
+// exact. p keeps 2^-12 of itself down to 2^-28 of a row's largest in kv8_rows_kernel, 2^-24
+// in kv8_tiles_kernel; below, what is lost is 2^-39 and 2^-35 of that largest. A block's
+// product is scaled by s_v in fp32. The unfinished block's values are bf16: kv8_rows_kernel
+// takes p in two bf16 parts there, kv8_tiles_kernel brings the values to fp16 at a power of
+// two that puts the largest into [1, 2).
 #include "fp_common.h"
 #include "fp_launch.h"
 #include "fp_rope.h"
@@ -46,7 +51,10 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 constexpr int kBlk = 64;
 constexpr int kKv8MaxSplit = 64;  // one lane per split in kv8_combine_kernel
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRise = 8.f;  // kv8_tiles_kernel: log2 of the largest p
+constexpr float kRise = 5.f;  // kv8_tiles_kernel: log2 of the largest p
+// p's factor in fp16, as a power of two, and so that of the codes: the largest p times it
+// is 2^14 and 2^15 (fp16 ends at 65504), a code of 1 by it no less than 2^-14
+constexpr int kLiftRows = 14, kLiftTiles = 10;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ f32x4 mfma16h(u32x4 a, u32x4 b, f32x4 c) {
@@ -90,27 +98,30 @@ __device__ __forceinline__ u32x4 codes8_bf16(uint32_t a, uint32_t b) {
   const u32x2 lo = codes4_bf16<BAD>(a), hi = codes4_bf16<BAD>(b);
   return u32x4{lo.x, lo.y, hi.x, hi.y};
 }
-// Four codes as fp16: 1024 + (code + 128) is exact, and so is 1152 less.
-template <bool BAD>
+// Four codes times 2^-LIFT as fp16: 1024 + (code + 128) is exact, and so is 1152 less.
+template <bool BAD, int LIFT>
 __device__ __forceinline__ u32x2 codes4_f16(uint32_t w) {
+  constexpr float kDown = 1.f / (1 << LIFT);
+  constexpr uint32_t kBad = 0xd800u - (LIFT << 10);  // -128 times 2^-LIFT
   const uint32_t u = w ^ 0x80808080u;
   u32x2 v;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t biased = __builtin_amdgcn_perm(0x64646464u, u, i ? 0x04030402u : 0x04010400u);
-    const f16x2 h = __builtin_bit_cast(f16x2, biased) + f16x2{(_Float16)-1152.f, (_Float16)-1152.f};
+    const f16x2 h = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, biased), f16x2{(_Float16)kDown, (_Float16)kDown},
+                                              f16x2{(_Float16)(-1152.f * kDown), (_Float16)(-1152.f * kDown)});
     uint32_t w2 = __builtin_bit_cast(uint32_t, h);
     if constexpr (BAD) {
-      if ((w2 & 0xffffu) == 0xd800u) w2 = (w2 & 0xffff0000u) | 0x7e00u;  // -128
-      if ((w2 >> 16) == 0xd800u) w2 = (w2 & 0xffffu) | 0x7e000000u;
+      if ((w2 & 0xffffu) == kBad) w2 = (w2 & 0xffff0000u) | 0x7e00u;
+      if ((w2 >> 16) == kBad) w2 = (w2 & 0xffffu) | 0x7e000000u;
     }
     v[i] = w2;
   }
   return v;
 }
-template <bool BAD>
+template <bool BAD, int LIFT>
 __device__ __forceinline__ u32x4 codes8_f16(uint32_t a, uint32_t b) {
-  const u32x2 lo = codes4_f16<BAD>(a), hi = codes4_f16<BAD>(b);
+  const u32x2 lo = codes4_f16<BAD, LIFT>(a), hi = codes4_f16<BAD, LIFT>(b);
   return u32x4{lo.x, lo.y, hi.x, hi.y};
 }
 // Eight codes at scale s as bf16 values (what a block going back into the ring holds).
@@ -415,8 +426,8 @@ __device__ __forceinline__ int last_key(const Span& s, int t) {
 }
 
 // One softmax step over the 16 keys that a lane holds of each of its row columns:
-// scores x (in units of log 2) to probabilities, m and l updated; returns what the
-// row's earlier sums are multiplied by.
+// scores x (in units of log 2) to probabilities times 2^kLiftRows, m and l (of such
+// probabilities) updated; returns what the row's earlier sums are multiplied by.
 __device__ __forceinline__ float softmax_step(f32x4 (&x)[4], float& mx, float& sum) {
   float m = -INFINITY;
 #pragma unroll
@@ -425,14 +436,14 @@ __device__ __forceinline__ float softmax_step(f32x4 (&x)[4], float& mx, float& s
     for (int r = 0; r < 4; ++r) m = fmaxf(m, x[n][r]);
   const float mn = fmaxf(mx, col_max(m));
   const float base = mn == -INFINITY ? 0.f : mn;
-  const float al = exp2_fast(mx - base);
+  const float al = exp2_fast(mx - base), lift = base - kLiftRows;
   mx = mn;
   float l = 0.f;
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      x[n][r] = exp2_fast(x[n][r] - base);
+      x[n][r] = exp2_fast(x[n][r] - lift);
       l += x[n][r];
     }
   sum = sum * al + l;
@@ -450,13 +461,15 @@ __device__ __forceinline__ int64_t part_row(const Kv8Args& a, int split, int bh,
   return ((int64_t)split * a.B * a.Hk + bh) * ((int64_t)a.T * (a.Hq / a.Hk)) + rr;
 }
 
-// ... and as those of their bf16 values and of what is left: p to 2^-17 of itself.
+// ... and as those of their bf16 values (times 2^-LIFT) and of what is left: p to 2^-17 of itself.
+template <int LIFT>
 __device__ __forceinline__ void p_operands_bf16(const f32x4 (&x)[4], u32x4 (&hi)[2], u32x4 (&lo)[2]) {
+  constexpr float kDown = 1.f / (1 << LIFT);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float a = x[2 * i + w / 2][2 * (w & 1)], b = x[2 * i + w / 2][2 * (w & 1) + 1];
+      const float a = x[2 * i + w / 2][2 * (w & 1)] * kDown, b = x[2 * i + w / 2][2 * (w & 1) + 1] * kDown;
       const uint32_t h = pack_bf16x2(a, b);
       hi[i][w] = h;
       lo[i][w] = pack_bf16x2(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
@@ -587,7 +600,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
     const float f = fabsf(vs);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const u32x4 v0 = codes8_f16<BAD>(xv[dt][0], xv[dt][1]), v1 = codes8_f16<BAD>(xv[dt][2], xv[dt][3]);
+      const u32x4 v0 = codes8_f16<BAD, kLiftRows>(xv[dt][0], xv[dt][1]);
+      const u32x4 v1 = codes8_f16<BAD, kLiftRows>(xv[dt][2], xv[dt][3]);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         f32x4 pv = mfma16h(v0, pf[rt][0], f32x4{0.f, 0.f, 0.f, 0.f});
@@ -648,7 +662,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
     for (int rt = 0; rt < RT; ++rt) {
       f32x4 p[4];
       al[rt] = softmax(y, rt, full, sc, p);
-      p_operands_bf16(p, hi[rt], lo[rt]);
+      p_operands_bf16<kLiftRows>(p, hi[rt], lo[rt]);
     }
     const int left = end - full * kBlk - 16 * grp;  // of the lane group's 16 keys
 #pragma unroll
@@ -675,7 +689,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const float l = col_sum(sum[rt]);
+    const float l = col_sum(sum[rt]) * (1.f / (1 << kLiftRows));
     if (grp == 0) {
       sM[wave][rt * 16 + li] = mx[rt];
       sL[wave][rt * 16 + li] = l;
@@ -717,8 +731,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
 // 16 w ..), and walks its blocks: codes into registers one block ahead, then converted once
 // for the four waves into LDS (keys bf16, values fp16, both double-buffered), one
 // barrier per block. p is taken relative to a maximum that is moved only when the running
-// one has passed it by kRise (p up to 2^8: fp16 and the sums have room), so that a block
-// seldom rescales o. 128 rows to a workgroup halve the conversions and the LDS reads but
+// one has passed it by kRise (fp16 and the sums have room), so that a block seldom rescales o. 128 rows to a workgroup halve the conversions and the LDS reads but
 // leave the registers no room: 8192 tokens of 16 heads 617 us against 580.
 // 1000 tokens at 1111, 32 heads: 65 us, 400 TFLOP/s; 2048 at 30000, 16 heads: 885 us with its
 // write, 590 TFLOP/s: bound by the vector unit (softmax and conversions) beside the matrix core.
@@ -800,8 +813,8 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
     for (int n = 0; n < NL; ++n) {
       st(k + k_wr[n], codes8_bf16<BAD>(kx[n][0], kx[n][1]));
       st(k + (k_wr[n] ^ 16), codes8_bf16<BAD>(kx[n][2], kx[n][3]));
-      st(v + v_wr + n * (64 * kBlk * 2), codes8_f16<BAD>(vx[n][0], vx[n][1]));
-      st(v + (v_wr ^ 16) + n * (64 * kBlk * 2), codes8_f16<BAD>(vx[n][2], vx[n][3]));
+      st(v + v_wr + n * (64 * kBlk * 2), codes8_f16<BAD, kLiftTiles>(vx[n][0], vx[n][1]));
+      st(v + (v_wr ^ 16) + n * (64 * kBlk * 2), codes8_f16<BAD, kLiftTiles>(vx[n][2], vx[n][3]));
     }
   };
   __shared__ float sTop[4];
@@ -855,11 +868,11 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
         o[w] = pack_f16x2(__uint_as_float(vv[n][w] << 16) * inv, __uint_as_float(vv[n][w] & 0xffff0000u) * inv);
       st(v + v_at(i / 8, i % 8), o);
     }
-    ks = 1.f, vs = scale;
+    ks = 1.f, vs = scale * (1.f / (1 << kLiftTiles));
   };
 
   const float sc = kLog2e / sqrtf((float)D);
-  f32x4 o[DT], sum = {0.f, 0.f, 0.f, 0.f};  // sum: of p, four equal rows of ones times p
+  f32x4 o[DT], sum = {0.f, 0.f, 0.f, 0.f};  // sum: of p, four equal rows of ones (by 2^kLift) times p
   float mx = -INFINITY;  // what p is relative to: at most kRise under the running maximum
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -908,14 +921,15 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= al;
     }
-    const float base = mx == -INFINITY ? 0.f : mx;
+    const float lift = (mx == -INFINITY ? 0.f : mx) - kLiftTiles;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[n][r] = exp2_fast(x[n][r] - base);
+      for (int r = 0; r < 4; ++r) x[n][r] = exp2_fast(x[n][r] - lift);
     u32x4 pf[2];
     p_operands(x, pf);
-    constexpr u32x4 kOnes = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+    constexpr uint32_t kOne = (0x3c00u - (kLiftTiles << 10)) * 0x10001u;  // 2^-kLiftTiles, as the codes have it
+    constexpr u32x4 kOnes = {kOne, kOne, kOne, kOne};
 #pragma unroll
     for (int i = 0; i < 2; ++i) sum = mfma16h(kOnes, pf[i], sum);
 #pragma unroll

@@ -553,3 +553,32 @@ def over_held_values(m, ids, cuts):
         out.append(torch.nn.functional.linear(m.final_norm(x), m.embed.weight))
         at += T
     return torch.cat(out, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,D", [(1, 64), (6, 64), (6, 128), (80, 64), (80, 128)])
+@pytest.mark.parametrize("gap", [12.0, 18.0, 21.0])
+def test_one_key_far_above_the_rest(T, D, gap):
+    """A first token of small values whose score is `gap` above every other one's: the others'
+    probabilities, e^-gap of the largest, still make up the output. Each p is off by
+    2^-12 of itself (fp16) down to 2^-24 of the row's largest, and by 2^-35 of that below.
+    256 heads, so that no range of keys is so short that the sink is in another one."""
+    B, Hk, G, P = 32, 8, 4, 12000
+    u = torch.ones(D) * D**-0.5
+    k = 0.05 * tokens(1, 1, P, 1, D, 0.0).float()
+    k -= (k @ u)[..., None] * u              # scores of about zero ...
+    k[0, 0, 0] = 4 * u                       # ... but for the first
+    v = 1 + 0.5 * tokens(2, 1, P, 1, D, 0.0).float()
+    v[0, 0] *= 1e-3
+    k, v = k.bfloat16(), v.bfloat16()
+    q = (u * gap * D**0.5 / 4).bfloat16().expand(1, T, G, D)
+    c = new(P, Hk, D, B)
+    kd, vd = (t.to(DEV).expand(B, P, Hk, D) for t in (k, v))
+    c.write(0, kd[:, : P - T], vd[:, : P - T], 0)
+    y = fk.attention_kv8(q.to(DEV).repeat(B, 1, Hk, 1), kd[:, P - T :], vd[:, P - T :], c, 0, P - T).cpu()
+    assert torch.equal(y, y[:1, :, :1].expand_as(y))
+    ek, ev = held(k[0], P), held(v[0], P)
+    e, pv, size, vmax, top = attend(q[0, :, :1], ek, ev, P - T)
+    tol = e.abs() * 2.0**-8 + pv * (2.0**-11 + size * 2.0**-19) + P * 2.0**-35 * vmax * top
+    err = (y[0, :, :1].double() - e).abs()
+    assert (err <= tol).all(), (err / tol).max()
