@@ -32,9 +32,9 @@
 // 2^kLift, up to 2^15 with what kRise leaves it, and the value codes times 2^-kLift, both
 // exact. p keeps 2^-12 of itself down to 2^-28 of a row's largest in kv8_rows_kernel, 2^-24
 // in kv8_tiles_kernel; below, what is lost is 2^-39 and 2^-35 of that largest. A block's
-// product is scaled by s_v in fp32. The unfinished block's values are bf16: kv8_rows_kernel
-// takes p in two bf16 parts there, kv8_tiles_kernel brings the values to fp16 at a power of
-// two that puts the largest into [1, 2).
+// product is scaled by s_v in fp32. The unfinished block's values are bf16, and stay it (in
+// fp16 a large value would take the bits of the small ones beside it): p is taken in two
+// bf16 parts there.
 #include "fp_common.h"
 #include "fp_launch.h"
 #include "fp_rope.h"
@@ -817,7 +817,6 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
       st(v + (v_wr ^ 16) + n * (64 * kBlk * 2), codes8_f16<BAD, kLiftTiles>(vx[n][2], vx[n][3]));
     }
   };
-  __shared__ float sTop[4];
   // block kt (loaded before, if whole) into LDS; its scales into ks, vs
   auto store = [&](uint32_t k, uint32_t v, int kt, float& ks, float& vs) __attribute__((always_inline)) {
     if (kt < full) {
@@ -835,40 +834,20 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
     const int64_t tl = ((int64_t)bh * 2 + (full & 1)) * (kBlk * D);
     constexpr int NT = kBlk * D / 8 / 256;
     const int n_rows = end - full * kBlk;
-    float top = 0.f;
-    int bad = 0;
-    u32x4 vv[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int i = n * 256 + tid;
       st(k + k_at(i / CH, i % CH), ld16(a.k_tail + tl + i * 8));
-      vv[n] = ld16(a.v_tail + tl + i * 8);
+      u32x4 vv = ld16(a.v_tail + tl + i * 8);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 4; ++w) {  // the ring holds anything past the last key
         const int key = (i % 8) * 8 + 2 * w;
-        if (key >= n_rows) vv[n][w] = 0u;
-        else if (key + 1 >= n_rows) vv[n][w] &= 0xffffu;
+        if (key >= n_rows) vv[w] = 0u;
+        else if (key + 1 >= n_rows) vv[w] &= 0xffffu;
       }
-      top8(vv[n], top, bad);
+      st(v + v_at(i / 8, i % 8), vv);
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-    __syncthreads();
-    if (lane == 0) sTop[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(sTop[0], sTop[1]), fmaxf(sTop[2], sTop[3]));
-    const uint32_t e = __float_as_uint(top) & 0x7f800000u;
-    const float scale = e == 0u ? 1.17549435e-38f : __uint_as_float(e), inv = 1.f / scale;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int i = n * 256 + tid;
-      u32x4 o;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        o[w] = pack_f16x2(__uint_as_float(vv[n][w] << 16) * inv, __uint_as_float(vv[n][w] & 0xffff0000u) * inv);
-      st(v + v_at(i / 8, i % 8), o);
-    }
-    ks = 1.f, vs = scale * (1.f / (1 << kLiftTiles));
+    ks = 1.f, vs = 1.f;
   };
 
   const float sc = kLog2e / sqrtf((float)D);
@@ -876,7 +855,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
   float mx = -INFINITY;  // what p is relative to: at most kRise under the running maximum
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto step = [&](uint32_t k, uint32_t v, int kt, float ks, float vs) __attribute__((always_inline)) {
+  auto step = [&](uint32_t k, uint32_t v, int kt, float ks, float vs, auto tail) __attribute__((always_inline)) {
     if (kt * kBlk > lim_hi) return;  // every key hidden from every row
     f32x4 x[4];
 #pragma unroll
@@ -926,6 +905,18 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
     for (int n = 0; n < 4; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[n][r] = exp2_fast(x[n][r] - lift);
+    if constexpr (decltype(tail)::value) {  // bf16 values
+      u32x4 ph[2], pl[2];
+      p_operands_bf16<kLiftTiles>(x, ph, pl);
+      constexpr u32x4 kOnes = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sum = mfma16(kOnes, pl[i], mfma16(kOnes, ph[i], sum));
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) o[dt] = mfma16(vf[dt][i], pl[i], mfma16(vf[dt][i], ph[i], o[dt]));
+      return;
+    }
     u32x4 pf[2];
     p_operands(x, pf);
     constexpr uint32_t kOne = (0x3c00u - (kLiftTiles << 10)) * 0x10001u;  // 2^-kLiftTiles, as the codes have it
@@ -949,16 +940,18 @@ __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) 
     load(t_lo);
     store(0, 2 * SZ, t_lo, ksc, vsc);
     __syncthreads();
+    const int f_hi = t_hi < full ? t_hi : full;
     uint32_t u = 0;
-    for (int kt = t_lo; kt < t_hi; ++kt, u ^= SZ) {
+    for (int kt = t_lo; kt < f_hi; ++kt, u ^= SZ) {
       const bool more = kt + 1 < t_hi;
       if (more) load(kt + 1);
-      step(u, 2 * SZ + u, kt, ksc, vsc);
+      step(u, 2 * SZ + u, kt, ksc, vsc, std::false_type{});
       if (more) {
         store(u ^ SZ, 2 * SZ + (u ^ SZ), kt + 1, ksc, vsc);
         __syncthreads();
       }
     }
+    if (f_hi < t_hi) step(u, 2 * SZ + u, full, 1.f, 1.f, std::true_type{});
   }
 
   if (row0 + li >= rows) return;

@@ -582,3 +582,44 @@ def test_one_key_far_above_the_rest(T, D, gap):
     tol = e.abs() * 2.0**-8 + pv * (2.0**-11 + size * 2.0**-19) + P * 2.0**-35 * vmax * top
     err = (y[0, :, :1].double() - e).abs()
     assert (err <= tol).all(), (err / tol).max()
+
+
+def check_sizes(y, q, k, v, first):
+    """check's bound without its absolute term: outputs down to the subnormal numbers, of
+    which the smallest bf16 is 2^-133, and fp32 sums of them off by a few of 2^-149."""
+    e, pv, size, vmax, top = attend(q, k, v, first)
+    tol = e.abs() * 2.0**-8 + pv * (2.0**-11 + size * 2.0**-19) + k.shape[0] * 2.0**-25 * vmax * top + 2.0**-134 + 2.0**-142
+    err = (y.cpu().double() - e).abs()
+    assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("P", [40, 64, 100, 190])
+@pytest.mark.parametrize("size", [1e30, 1e8, 1e-12, 1e-30, 2.0**-126, 2.0**-130, 0.0])
+def test_a_cache_of_values_of_one_size(size, P, T):
+    """Whole blocks and unfinished ones of values far from 1, at few and at many rows."""
+    D = 128
+    k, q = tokens(1, 1, P, 1, D), tokens(7, 1, T, 2, D)
+    v = (tokens(2, 1, P, 1, D).double() * size).bfloat16()
+    c = new(256, 1, D)
+    if P > T:
+        c.write(0, k[:, : P - T].to(DEV), v[:, : P - T].to(DEV), 0)
+    y = fk.attention_kv8(q.to(DEV), k[:, P - T :].to(DEV), v[:, P - T :].to(DEV), c, 0, P - T)
+    check_sizes(y[0], q[0], held(k[0], P), held(v[0], P), P - T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("size", [2.0**14, 2.0**24, 2.0**60])
+def test_a_large_channel_of_the_unfinished_block(size, T):
+    """The unfinished block is held in bf16: a value channel far larger than the others takes
+    nothing from them (as it would in a packed block)."""
+    P, D = 60, 128
+    k, q = tokens(1, 1, P, 1, D), tokens(7, 1, T, 2, D)
+    v = tokens(2, 1, P, 1, D)
+    v[..., 5] *= size
+    c = new(128, 1, D)
+    c.write(0, k[:, : P - T].to(DEV), v[:, : P - T].to(DEV), 0)
+    y = fk.attention_kv8(q.to(DEV), k[:, P - T :].to(DEV), v[:, P - T :].to(DEV), c, 0, P - T)
+    check_sizes(y[0], q[0], k[0].float(), v[0].float(), P - T)
