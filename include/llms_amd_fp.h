@@ -338,8 +338,8 @@ int fp_attention_bf16(const fp_attention_args* args, void* workspace, int64_t wo
  * of its 64 x head_dim entries, the scale is top / 127 and a code rne(127 x / top), the
  * division correctly rounded; its values are code * scale. An entry that is not finite
  * has the code -128 (a NaN) and makes the scale negative (values use its magnitude).
- * Positions of the unfinished block are in bf16 in slot (block & 1) of the tail, which
- * tail_block names; the last two blocks written stay there.
+ * Positions of the unfinished block are in bf16 (infinities as NaN) in slot (block & 1) of
+ * the tail, which tail_block names; the last two blocks written stay there.
  *   q, k, v    rows m = b*T + t of n_heads / n_kv_heads heads of head_dim, bf16, 8-byte
  *              aligned, row strides ld* multiples of 4
  *   cos, sin   [T, head_dim] bf16 (the two halves share frequencies), or both NULL: q and

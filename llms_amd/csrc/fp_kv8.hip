@@ -12,7 +12,7 @@
 // expanded into the ring first. Keys are held [64][D], values [D][64] (codes and
 // ring): a value column then is 16 contiguous bytes per lane of a V^T operand.
 // Code -128 stands for an entry that was not finite; a block with one has its scale
-// negated, so that only such blocks pay for the check.
+// negated, so that only such blocks pay for the check. The ring holds such entries as NaN too.
 //
 //   - kv8_write_kernel: a workgroup per touched block and kv head; QK-norm and RoPE of
 //     the new keys on the way where the caller asks (and of q, in more workgroups).
@@ -203,6 +203,12 @@ __device__ __forceinline__ u32x2 code8(u32x4 v, float top) {
   return o;
 }
 
+// Two bf16 with an infinity as a NaN: an exponent of ones gets a bit in its fraction.
+__device__ __forceinline__ uint32_t inf_to_nan(uint32_t w) {
+  return w | ((((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 9);
+}
+__device__ __forceinline__ u32x2 inf_to_nan(u32x2 w) { return u32x2{inf_to_nan(w.x), inf_to_nan(w.y)}; }
+
 template <int D>
 __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
   constexpr int LPH = D / 8, RPP = 256 / LPH;  // lanes per row, rows per pass
@@ -271,6 +277,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
       const int r = r0 + tid / LPH + p * RPP, t = w * kBlk + r - s.first;
       if (r >= r1) continue;
       if (a.cos) norm_rope_row<D>(lo[p], hi[p], a.gk, a.epsk, a.cos + t * a.ldc, a.sin + t * a.lds, j);
+      lo[p] = inf_to_nan(lo[p]), hi[p] = inf_to_nan(hi[p]), v0[p] = inf_to_nan(v0[p]), v1[p] = inf_to_nan(v1[p]);
       const uint32_t vv[4] = {v0[p].x, v0[p].y, v1[p].x, v1[p].y};
       if (ring) {
         *reinterpret_cast<u32x2*>(tk + r * D + 4 * j) = lo[p];

@@ -623,3 +623,30 @@ def test_a_large_channel_of_the_unfinished_block(size, T):
     c.write(0, k[:, : P - T].to(DEV), v[:, : P - T].to(DEV), 0)
     y = fk.attention_kv8(q.to(DEV), k[:, P - T :].to(DEV), v[:, P - T :].to(DEV), c, 0, P - T)
     check_sizes(y[0], q[0], k[0].float(), v[0].float(), P - T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_infinities_of_the_unfinished_block(T):
+    """They are NaN from the call that writes them on, not from the one that packs their
+    block: a key's rows are NaN and do not lose that key, a value's column is."""
+    P, H, D = 64, 2, 64
+    k, v, q = tokens(1, 1, P, H, D), tokens(2, 1, P, H, D), tokens(3, 1, P, 4, D)
+    k[0, 2, 0, 3], v[0, 4, 1, 7], v[0, 5, 1, 9] = -math.inf, math.inf, math.nan
+    q[0, :, :2, 3] = 1.0  # the bad key's score would be -inf
+    c = new(P, H, D)
+    n = 20 + T
+    for at in (0, 20):
+        m = 20 if at == 0 else T
+        y = fk.attention_kv8(q[:, at : at + m].to(DEV), k[:, at : at + m].to(DEV), v[:, at : at + m].to(DEV), c, 0, at)
+    def spoilt(y):
+        assert y[0, :, :2].isnan().all()
+        assert y[0, :, 2:, [7, 9]].isnan().all() and y[0, :, 2:].isnan().sum() == y.shape[1] * 4
+    spoilt(y.cpu())
+    rk, rv = (t[0].cpu() for t in c.read(0, 0, n))
+    assert rk[2, 0, 3].isnan() and rk.isnan().sum() == 1
+    assert rv[4, 1, 7].isnan() and rv[5, 1, 9].isnan() and rv.isnan().sum() == 2
+    y = fk.attention_kv8(q[:, n:].to(DEV), k[:, n:].to(DEV), v[:, n:].to(DEV), c, 0, n)  # packs the block
+    spoilt(y.cpu())
+    rk, rv = (t[0].cpu() for t in c.read(0, 0, P))
+    assert rk[2, 0, 3].isnan() and rk.isnan().sum() == 1 and rv.isnan().sum() == 2
