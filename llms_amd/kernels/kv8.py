@@ -145,15 +145,15 @@ def attention_core_kv8(q, k, v, *, q_norm, k_norm, num_heads: int, cache: KVCach
                        start_pos) -> torch.Tensor:
     """What ``TritonAttention.forward`` does between its projections with an 8-bit
     cache: QK-norm and RoPE of the flat projections ``[B, T, heads * D]`` in the
-    kernel that writes the keys (in torch where a norm is not the plain one or a
-    type is not bf16's), the cache write and attention. Returns ``[B, T, num_heads * D]``."""
+    kernel that writes the keys (in torch where a norm is not the plain one, a type is not
+    bf16's or rows of cos and sin share memory), the cache write and attention. Returns ``[B, T, num_heads * D]``."""
     fn, D = "attention_kv8", cache.head_dim
     B, T, _ = q.shape
     fused = (plain_norm(q_norm) and plain_norm(k_norm) and not autocast()
              and all(t.dtype == torch.bfloat16 and t.shape == (D,) and t.is_contiguous() and t.data_ptr() % 8 == 0
                      for t in (q_norm.weight, k_norm.weight))
-             and all(t.dtype == torch.bfloat16 and t.shape == (T, D) and t.stride(1) == 1 and t.device == q.device
-                     for t in (cos, sin))
+             and all(t.dtype == torch.bfloat16 and t.shape == (T, D) and t.stride(1) == 1 and (T == 1 or t.stride(0) >= D)
+                     and t.device == q.device for t in (cos, sin))
              and not transformed(q_norm.weight, k_norm.weight, cos, sin))
     if not fused:
         from ._eager import apply_rope

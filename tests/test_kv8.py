@@ -650,3 +650,17 @@ def test_infinities_of_the_unfinished_block(T):
     spoilt(y.cpu())
     rk, rv = (t[0].cpu() for t in c.read(0, 0, P))
     assert rk[2, 0, 3].isnan() and rk.isnan().sum() == 1 and rv.isnan().sum() == 2
+
+
+@pytest.mark.gpu
+def test_rope_rows_that_share_memory():
+    """cos and sin of tokens at one position, as an expanded row."""
+    h, m = model()
+    attn = m.layers[0].attn
+    x = tokens(1, 1, 3, 1, 192).view(1, 3, 192).to(DEV)
+    a, b = (m.alloc_cache(64, kv8=True) for _ in range(2))
+    cos, sin = (t[5:6].expand(3, -1) for t in (m.rope_cos, m.rope_sin))
+    with torch.inference_mode():
+        y = attn(x, kv_cache=a, layer_idx=0, cos=cos, sin=sin, start_pos=0)
+        z = attn(x, kv_cache=b, layer_idx=0, cos=cos.contiguous(), sin=sin.contiguous(), start_pos=0)
+    assert torch.equal(y, z)
