@@ -401,7 +401,8 @@ int fp_kv8_read(const fp_kv8_args* args, float* k_out, float* v_out, void* strea
  * gamma [K], when not NULL, is an RMSNorm weight applied to x first (the contract of
  * fp_rmsnorm_qkv_bf16; eps finite and >= 0). The weights are read in 4 bits at every
  * row count; the workspace holds x as the tiles read it and the partial sums of a split k.
- * A row of x with an infinity has NaN outputs (also where its codes are zero).
+ * A row of x with an infinity has NaN outputs (also where its codes are zero); outputs are
+ * finite while the magnitudes of a group's inputs stay under 2^123 together.
  * workspace: at least fp_w4_workspace_bytes(M, N, K, gate_up, norm) bytes, 16-byte
  * aligned (norm: whether gamma is given; 0 for most calls of few rows without it: NULL
  * will do). ldx, ldq and lds < 2^26.

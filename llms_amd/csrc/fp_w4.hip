@@ -10,9 +10,13 @@
 //
 // x is the A operand of v_mfma_f32_16x16x32_bf16, the codes the B operand: a lane's
 // accumulators belong to one weight row (column lane % 16), so its group's scale is one
-// register. Codes become bf16 without a conversion: (w & 0x000f000f) | 0x43004300
-// holds two codes as 128 + (q + 8) exactly. The 136 too much times the group's sum
-// of x is what the group's sum starts from. The nibbles of a dword come out as k 0 4 1 5
+// register. Codes become bf16 without a conversion: (w >> s & 0x00780078) | 0x41804180
+// holds two codes as 16 + (q + 8) exactly. The 24 too much times the group's sum
+// of x is what the group's sum starts from: sums of up to 31 |x|, where products of codes alone
+// have 7 |x|, so fp32 rounds a group's sum at up to four times their size (with the codes
+// in the low bits, as 128 + (q + 8), twenty times: an input of 1e5 then cost outputs that
+// do not use it as much as their rounding), and a group's inputs have to stay under 2^123
+// together. The nibbles of a dword come out as k 0 4 1 5
 // 2 6 3 7: x is put into that order on its way into LDS. A lane's 16 bytes are 32
 // consecutive k of its row, so with groups of 128 the four operands of a slab of 128
 // k are its dwords as they come; with groups of 64 or 32 a 4 x 4 transpose of dwords between
@@ -34,6 +38,8 @@ namespace fp {
 
 namespace {
 
+constexpr float kOff = -24.f;  // what codes_bf16 has too much, taken off
+
 constexpr uint32_t kOut = 0x7ffffff0u;  // a buffer offset past every buffer: reads 0
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, int64_t bytes) {
@@ -47,18 +53,18 @@ __device__ __forceinline__ u32x4 nibble_order(u32x4 v) {
                __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
 }
 
-// Eight codes as bf16 128 + (q + 8), in that order; high is 0x43004300 in a vector
+// Eight codes as bf16 16 + (q + 8), in that order; high is 0x41804180 in a vector
 // register that the compiler cannot see through: it then masks and sets a pair in one
 // instruction, which may read one scalar register only (with two constants it takes two).
 __device__ __forceinline__ u32x4 codes_bf16(uint32_t w, uint32_t high) {
   u32x4 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = ((w >> (4 * i)) & 0x000f000fu) | high;
+  for (int i = 0; i < 4; ++i) v[i] = ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) | high;
   return v;
 }
 __device__ __forceinline__ uint32_t code_high() {
   uint32_t v;
-  asm("v_mov_b32 %0, 0x43004300" : "=v"(v));
+  asm("v_mov_b32 %0, 0x41804180" : "=v"(v));
   return v;
 }
 
@@ -235,7 +241,7 @@ __global__ __launch_bounds__(W * 64) void w4_row_kernel(W4Args a) {
   const int64_t n0 = (int64_t)blockIdx.x * (16 * NB);
   const int M = (int)a.M, slabs = (int)((a.K + 127) / 128);
   const int kp = slabs * 128, ldx = kp * 2 + 16;  // LDS row of x, off the banks of the next
-  // LDS: x rows, -136 sum x [group][16], scales [group][16 NC]; the waves' sums at the end
+  // LDS: x rows, kOff sum x [group][16], scales [group][16 NC]; the waves' sums at the end
   char* sx = lds;
   float* sb = reinterpret_cast<float*>(lds + M * ldx);
   float* ss = sb + slabs * NG * 16;
@@ -264,7 +270,7 @@ __global__ __launch_bounds__(W * 64) void w4_row_kernel(W4Args a) {
     const float s = group_sum<GS>(sum8(v));
     if (i >= chunks) return;
     *reinterpret_cast<u32x4*>(sx + r * ldx + c * 16) = nibble_order(v);
-    if (c % (GS / 8) == 0) sb[c / (GS / 8) * 16 + r] = -136.f * s;
+    if (c % (GS / 8) == 0) sb[c / (GS / 8) * 16 + r] = kOff * s;
   };
   // scales: along a row's groups from lane to lane (loaded where they are used, each of the
   // 16 rows of a wave's load would cost as much as 64 bytes of weights)
@@ -403,7 +409,7 @@ __global__ __launch_bounds__(W * 64) void w4_row_kernel(W4Args a) {
 // ---- more rows --------------------------------------------------------------
 //
 // A panel of 16 RT rows of x is laid out slab by slab as it lies in LDS: for each block of
-// 16 rows and each of the slab's four operands the 64 lanes' 16 bytes, then -136
+// 16 rows and each of the slab's four operands the 64 lanes' 16 bytes, then kOff
 // sum x as [group of the slab][row].
 //
 // 64 rows of 4096 x 2 x 12288 take 30 us here, 5 us in prep and 5 in the reduction (350
@@ -428,7 +434,7 @@ __global__ __launch_bounds__(256) void w4_prep_kernel(const uint16_t* x, int64_t
   char* p = out + (panel * slabs + slab) * panel_bytes(rt);
   *reinterpret_cast<u32x4*>(p + ((r / 16) * 4 + frag_of<GS>(cc)) * 1024 + (grp_of<GS>(cc) * 16 + r % 16) * 16) =
       nibble_order(v);
-  if (cc % (GS / 8) == 0) reinterpret_cast<float*>(p + rt * 4096)[cc / (GS / 8) * (16 * rt) + r] = -136.f * s;
+  if (cc % (GS / 8) == 0) reinterpret_cast<float*>(p + rt * 4096)[cc / (GS / 8) * (16 * rt) + r] = kOff * s;
 }
 
 template <int RT, int NC, int GS, bool GATEUP, bool ALIGNED, int W>

@@ -356,3 +356,39 @@ def test_swapped_model(group, fuse_norm, linear):
         # both round at the same points: they differ by bf16 steps in few places
         assert (a - b).norm() <= 2e-2 * b.norm()
     assert h.greedy_generate(m, [1, 2, 3], 6, DEV) == h.graph_greedy_generate(m, [1, 2, 3], 6, DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("M", [1, 5, 16, 30, 64, 100])
+def test_outliers_of_x(M, group):
+    """An input far above the others, as the inputs of a down projection have: outputs whose
+    code there is zero lose nothing. Whole numbers and scales of 1, and what a code
+    carries in the sums (16 + code + 8, at most 31) keeps every partial sum under 2^24: all of
+    them are exact, and so is the output but for its rounding."""
+    K, N = 1000, 48
+    g = torch.Generator().manual_seed(M)
+    x = torch.randint(-3, 4, (M, K), generator=g).float()
+    x[:, 77], x[:, 801] = 2.0**18, -(2.0**18)
+    q = torch.randint(1, 16, (N, K), generator=g)
+    q[::2, 77], q[::2, 801] = 8, 8
+    packed = (q[:, 0::2] | q[:, 1::2] << 4).to(torch.uint8)
+    s = torch.ones(N, -(-K // group), dtype=torch.bfloat16)
+    e = x.double() @ (q.double() - 8).T
+    y = fk.fused_linear_w4(x.bfloat16().to(DEV), packed.to(DEV), s.to(DEV), group=group)
+    assert torch.equal(y.cpu(), e.bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("M", [1, 5, 30, 100])
+def test_very_large_x(M, group):
+    """Finite as long as a group's inputs stay under 2^123 together (31 times that is finite)."""
+    K, N = 512, 32
+    x, (w,) = make(M, M, K, N, group)
+    x = (x.float() * 2.0**100).bfloat16()
+    x[:, 7] = 2.0**122
+    x[:, 300] = -(2.0**122)
+    y = fk.fused_linear_w4(x.to(DEV), w[0].to(DEV), w[1].to(DEV), group=group)
+    assert y.isfinite().all()
+    check_linear(y, x, w, group)
