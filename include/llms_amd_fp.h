@@ -405,7 +405,8 @@ int fp_kv8_read(const fp_kv8_args* args, float* k_out, float* v_out, void* strea
  * finite while the magnitudes of a group's inputs stay under 2^123 together.
  * workspace: at least fp_w4_workspace_bytes(M, N, K, gate_up, norm) bytes, 16-byte
  * aligned (norm: whether gamma is given; 0 for most calls of few rows without it: NULL
- * will do). ldx, ldq and lds < 2^26.
+ * will do). ldx, ldq and lds < 2^26; M <= 2^24, N <= 2^22 - 64, K <= 2^26, ceil(M / 128) *
+ * ceil(N / 64) <= 2^24, (M + 127) * K <= 2^35 (K in whole 128).
  */
 int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up, int norm);
 

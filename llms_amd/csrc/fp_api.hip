@@ -258,10 +258,12 @@ int run_w4(W4Args a, const uint16_t* gamma, float eps, void* ws, hipStream_t s) 
 int check_w4(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t ldq, int64_t lds,
              int64_t group) {
   if (M < 0 || N < 1 || K < 1 || (group != 32 && group != 64 && group != 128)) return FP_ERR_SHAPE;
-  // every grid in threads within 2^32, the column workgroups within a grid's 65535
+  // Every grid in threads within 2^32, the column workgroups within a grid's 65535. The
+  // tiles take 128 rows and at least 64 columns to a workgroup of 256 from 65 rows on (below, a
+  // panel is the whole of x), and k is split, with a reduction, in grids of at most 512 only.
   constexpr int64_t kLim = (int64_t)1 << 32;
   if (N > 65535 * 64 || K > (int64_t)1 << 26 || M > (int64_t)1 << 24 || (M + 127) * (round_up(K, 128) / 8) > kLim ||
-      (M + 15) / 16 * ((N + 63) / 64) * 256 > kLim / 16 || M * N > kLim)
+      (M + 127) / 128 * ((N + 63) / 64) * 256 > kLim)
     return FP_ERR_SHAPE;
   if (ldx < K || ldy < N || ldq < (K + 1) / 2 || lds < (K + group - 1) / group) return FP_ERR_STRIDE;
   constexpr int64_t kFar = (int64_t)1 << 26;  // sixteen rows within the kernels' 32-bit offsets

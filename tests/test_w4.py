@@ -392,3 +392,24 @@ def test_very_large_x(M, group):
     y = fk.fused_linear_w4(x.to(DEV), w[0].to(DEV), w[1].to(DEV), group=group)
     assert y.isfinite().all()
     check_linear(y, x, w, group)
+
+
+def test_large_calls_are_taken():
+    """Row counts and widths that the bf16 and int8 projections take, too: the grids of the
+    larger tiles that such calls run on are far from 2^32 threads."""
+    lib = _lib.capi()
+    for M, N, K, gate_up in ((90000, 12288, 4096, 1), (8192, 151936, 4096, 0), (1 << 17, 4096, 2560, 0),
+                             (349000, 12288, 64, 1)):
+        assert lib.fp_w4_workspace_bytes(M, N, K, gate_up, 0) >= M * K * 2, (M, N, K)
+    for M, N, K in ((1 << 25, 16, 64), (1 << 24, 1 << 22, 64), (16, 65535 * 64 + 1, 64), (1 << 24, 64, 1 << 20)):
+        assert lib.fp_w4_workspace_bytes(M, N, K, 0, 0) == 0, (M, N, K)
+
+
+@pytest.mark.gpu
+def test_a_large_output():
+    """More than 2^30 outputs in one call (2.2 GB)."""
+    M, K, N = 33000, 64, 33000
+    x, (w,) = make(1, M, K, N, 64)
+    y = fk.fused_linear_w4(x.to(DEV), w[0].to(DEV), w[1].to(DEV), group=64)
+    rows = [0, 63, 64, 16387, 32639, 32999]
+    check_linear(y[rows], x[rows], w, 64)
