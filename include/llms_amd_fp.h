@@ -352,7 +352,9 @@ int fp_attention_bf16(const fp_attention_args* args, void* workspace, int64_t wo
  *              into 0 .. T; the rows behind them are neither written nor attended
  * fp_kv8_attention writes the new keys and values, then attends (scale head_dim^-0.5, key
  * position <= query position, grouped-query heads sharing their kv head), over the
- * cache as it then is. Rows that see no key (behind a sequence's length, at a position outside
+ * cache as it then is: a block that this call completes is read in its codes, also for the
+ * rows before its end, whose values later positions then touch through the scale (a call of
+ * which no row but the last ends a block has none). Rows that see no key (behind a sequence's length, at a position outside
  * the cache) are zero. fp_kv8_write only writes. Both may start anywhere up to the
  * number of positions written so far: what is behind is dropped. (A call that starts
  * later than that leaves a gap: the unfinished block before it is lost.)

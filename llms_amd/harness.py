@@ -38,7 +38,7 @@ from torch import nn
 
 from .kernels._eager import RMSNorm, apply_rope, attend, build_rope_tables, write_kv
 from .kernels.fused_norm import fused_rmsnorm_head
-from .kernels.kv8 import KVCache8
+from .kernels.kv8 import BLOCK as KV8_BLOCK, KVCache8
 from .kernels.logprobs import TokenLogprobs, token_logprobs
 
 
@@ -259,14 +259,23 @@ def teacher_forced_logits(model: Qwen3Model, tokens: list[int], device) -> torch
 
 
 def teacher_forced_logprobs(model: Qwen3Model, tokens: list[int], device, *, top_k: int = 0,
-                            kv8: bool = False) -> TokenLogprobs:
+                            kv8: bool = False, causal: bool = False) -> TokenLogprobs:
     """How likely the model finds ``tokens``, fed as one prefill: of each token but
     the first its log-probability after the ones before it, with the entropy there
     and the ``top_k`` most likely tokens (``[len(tokens) - 1]`` each; a HIP device).
-    With ``kv8`` over an 8-bit cache."""
+    With ``kv8`` over an 8-bit cache, whose blocks of 64 tokens a prefill reads in 8
+    bits at scales that all of a block's tokens set: a score then also depends, within that
+    rounding, on the rest of its block. ``causal`` feeds the text in pieces of 63 tokens
+    and 1, so that none does (the scores of a decode loop, at two steps per block)."""
     ids = torch.tensor([tokens], dtype=torch.long, device=device)
+    cuts = [len(tokens)]
+    if kv8 and causal:
+        blocks, rest = divmod(len(tokens), KV8_BLOCK)
+        cuts = [KV8_BLOCK - 1, 1] * blocks + [rest] * (rest > 0)
     with torch.inference_mode():
-        logits = model(ids, model.alloc_cache(len(tokens) + 4, kv8=kv8), start_pos=0)
+        cache = model.alloc_cache(len(tokens) + 4, kv8=kv8)
+        steps = [model(piece, cache) for piece in ids.split(cuts, 1)]
+        logits = steps[0] if len(steps) == 1 else torch.cat(steps, 1)
         return token_logprobs(logits[0, :-1], ids[0, 1:], top_k)
 
 
@@ -277,7 +286,9 @@ class StepGraph:
     graph's static buffers, replays, and returns the static logits tensor
     (overwritten by the next replay). The warm-up runs before capture write
     the last T positions of the cache, so callers keep those free. (In an 8-bit
-    cache they would displace the unfinished block, which is put back.)"""
+    cache they would displace the unfinished block, which is put back. A verify step over
+    one whose tokens end a block answers for those before its end from the 8-bit block, with the
+    later drafts in its scale.)"""
 
     def __init__(self, model: Qwen3Model, cache: KVCache, T: int = 1, batch: int = 1):
         dev = model.embed.weight.device

@@ -8,6 +8,14 @@ therefore does not depend on how its tokens were cut into calls, and a
 verify step that takes back a few tokens finds them unpacked. Going further back,
 to any position, works too: the block it lands in goes on from its packed values.
 
+What a call answers does depend on the cut. Attention reads the cache as it is after
+the call's write, so a block that the call completes is read in 8 bits by all of the
+call's rows, those before its end included, and its scale is the largest entry of all 64
+tokens: such a row depends, within the rounding of 8 bits, on up to 63 tokens behind it.
+Where a row must not (scoring a text, drafts that may be rejected), no token but a call's
+last may end a block: calls of one token, or calls cut before and behind each block's last
+token (``teacher_forced_logprobs(kv8=True, causal=True)`` does that).
+
 Path: wrapper -> ``torch.ops.llms_amd.attention_kv8`` / ``write_kv8`` /
 ``read_kv8`` -> C ABI ``fp_kv8_attention`` / ``fp_kv8_write`` / ``fp_kv8_read`` -> HIP
 kernels (``llms_amd/csrc/fp_kv8.hip``) on torch's current stream.
@@ -33,7 +41,9 @@ class KVCache8:
     ``cur_len`` is the model's count of tokens, as in ``KVCache``. Tokens are
     written in order: a call may start anywhere up to the tokens written so far (what
     is behind it is dropped), not later (the unfinished block would be lost).
-    A key or value that is not finite is held as NaN. Calls on one cache must be ordered
+    A key or value that is not finite is held as NaN: it spoils the rows that see the key,
+    and the value's column in the rows that its block is read for (0 * NaN, as torch's
+    product would, before its position too). Calls on one cache must be ordered
     (one stream, or streams that wait for each other).
     """
 
@@ -129,7 +139,9 @@ def attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCa
 
     Returns:
         ``[B, T, heads, D]`` bfloat16: softmax attention with scale ``D ** -0.5`` of the token
-        at position p over positions 0 .. p. Rows past a sequence's length, and at device
+        at position p over positions 0 .. p, as the cache holds them after the write: in
+        8 bits where this call's tokens end their block, whose scale later tokens of the
+        block take part in (see the module's head for calls where that must not be). Rows past a sequence's length, and at device
         positions outside the cache (whose tokens are not written), are zero.
     """
     fn = "attention_kv8"

@@ -664,3 +664,47 @@ def test_rope_rows_that_share_memory():
         y = attn(x, kv_cache=a, layer_idx=0, cos=cos, sin=sin, start_pos=0)
         z = attn(x, kv_cache=b, layer_idx=0, cos=cos.contiguous(), sin=sin.contiguous(), start_pos=0)
     assert torch.equal(y, z)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pos,T,D", [(0, 63, 64), (64, 63, 128), (100, 27, 128), (63, 1, 64), (126, 1, 128), (127, 1, 64),
+                                     (1000, 23, 64), (1, 62, 128)])
+def test_calls_that_end_no_block_before_their_last_token_are_causal(pos, T, D):
+    """Tokens after a row leave it bit for bit as it was."""
+    P, Hk = pos + T, 2
+    k, v, q = tokens(1, 1, P, Hk, D), tokens(2, 1, P, Hk, D), tokens(3, 1, T, 4, D)
+    outs = []
+    for t in sorted({0, T // 2, T - 1}):
+        k2, v2 = k.clone(), v.clone()
+        k2[:, pos + t + 1 :] *= 30
+        v2[:, pos + t + 1 :] *= -30
+        c = new(P, Hk, D)
+        if pos:
+            c.write(0, k[:, :pos].to(DEV), v[:, :pos].to(DEV), 0)
+        y = fk.attention_kv8(q.to(DEV), k2[:, pos:].to(DEV), v2[:, pos:].to(DEV), c, 0, pos)
+        outs.append((t, y))
+    for t, y in outs:
+        assert torch.equal(y[:, : t + 1], outs[-1][1][:, : t + 1]), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [2, 63, 64, 65, 128, 200])
+def test_causal_scores(n):
+    """A text's scores up to a token do not depend on what follows it, and are a decode loop's
+    but for the row counts of the projections (two layers' roundings, as in test_model_over_the_cache)."""
+    h, m = model(fuse_norm=True, linear_down_o=True)
+    g = torch.Generator().manual_seed(2)
+    a = torch.randint(0, 32, (n,), generator=g).tolist()
+    at = n // 2
+    b = a[: at + 1] + [(t + 7) % 32 for t in a[at + 1 :]]
+    x, y = (h.teacher_forced_logprobs(m, t, DEV, top_k=3, kv8=True, causal=True) for t in (a, b))
+    for s, t in zip(x, y):
+        assert s.shape[0] == n - 1 and torch.equal(s[:at], t[:at])
+    with torch.inference_mode():
+        cache, ids = m.alloc_cache(256, kv8=True), torch.tensor([a], device=DEV)
+        step = torch.cat([m(i, cache) for i in ids.split(1, 1)], 1)[0, :-1].float()
+        one = torch.cat([m(i, c) for c in [m.alloc_cache(256, kv8=True)]
+                         for i in ids.split([63, 1] * (n // 64) + [n % 64] * (n % 64 > 0), 1)], 1)[0, :-1]
+    assert (one.float() - step).norm() <= 2e-2 * step.norm()
+    direct = fk.token_logprobs(one, ids[0, 1:], 3)
+    assert all(torch.equal(s, t) for s, t in zip(x, direct))
