@@ -277,7 +277,8 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Args a) {
       const int r = r0 + tid / LPH + p * RPP, t = w * kBlk + r - s.first;
       if (r >= r1) continue;
       if (a.cos) norm_rope_row<D>(lo[p], hi[p], a.gk, a.epsk, a.cos + t * a.ldc, a.sin + t * a.lds, j);
-      lo[p] = inf_to_nan(lo[p]), hi[p] = inf_to_nan(hi[p]), v0[p] = inf_to_nan(v0[p]), v1[p] = inf_to_nan(v1[p]);
+      if (w >= lb - 1)  // a block that goes into the ring
+        lo[p] = inf_to_nan(lo[p]), hi[p] = inf_to_nan(hi[p]), v0[p] = inf_to_nan(v0[p]), v1[p] = inf_to_nan(v1[p]);
       const uint32_t vv[4] = {v0[p].x, v0[p].y, v1[p].x, v1[p].y};
       if (ring) {
         *reinterpret_cast<u32x2*>(tk + r * D + 4 * j) = lo[p];
