@@ -739,9 +739,10 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv8_rows_kernel(Kv8Args 
 // 16 w ..), and walks its blocks: codes into registers one block ahead, then converted once
 // for the four waves into LDS (keys bf16, values fp16, both double-buffered), one
 // barrier per block. p is taken relative to a maximum that is moved only when the running
-// one has passed it by kRise (fp16 and the sums have room), so that a block seldom rescales o. 128 rows to a workgroup halve the conversions and the LDS reads but
+// one has passed it by kRise (fp16 and the sums have room), so that a block seldom
+// rescales o. 128 rows to a workgroup of four waves halve the conversions and the LDS reads but
 // leave the registers no room: 8192 tokens of 16 heads 617 us against 580.
-// 1000 tokens at 1111, 32 heads: 65 us, 400 TFLOP/s; 2048 at 30000, 16 heads: 885 us with its
+// 1000 tokens at 1037, 32 heads: 65 us, 390 TFLOP/s; 2048 at 30000, 16 heads: 877 us with its
 // write, 590 TFLOP/s: bound by the vector unit (softmax and conversions) beside the matrix core.
 template <int D>
 __global__ __launch_bounds__(256, 2) void kv8_tiles_kernel(Kv8Args a, int n_rt) {

@@ -225,8 +225,8 @@ __device__ __forceinline__ void store_block(const W4Args& a, f32x4 v, f32x4 u, i
 // multiplies the other half's. (Larger batches and a staging loop unrolled further are
 // slower: a launch runs the code once, so its instructions come from memory.) Scales go
 // through LDS too: two bytes a row and slab read where they are needed cost as many
-// lines as the weights do. One row of 2560 x 2 x 9728 (groups of 128) 9.5 us, 2.7 TB/s of
-// packed weights, 10240 x 2 x 9728 29.6 us, 3.5 TB/s; below a few us of work the launch and x's
+// lines as the weights do. One row of 2560 x 2 x 9728 (groups of 128) 10 us, 2.6 TB/s of
+// packed weights from HBM, 10240 x 2 x 9728 30 us, 3.4 TB/s; below a few us of work the launch and x's
 // way into LDS bound it, above the loads that two workgroups of a CU keep in flight.
 template <int NC, int GS, bool GATEUP, bool ALIGNED, int W>
 __global__ __launch_bounds__(W * 64) void w4_row_kernel(W4Args a) {
@@ -412,9 +412,9 @@ __global__ __launch_bounds__(W * 64) void w4_row_kernel(W4Args a) {
 // 16 rows and each of the slab's four operands the 64 lanes' 16 bytes, then kOff
 // sum x as [group of the slab][row].
 //
-// 64 rows of 4096 x 2 x 12288 take 30 us here, 5 us in prep and 5 in the reduction (350
+// 64 rows of 4096 x 2 x 12288 take 31 us here, 4 us in prep and 5 in the reduction (350
 // TFLOP/s; 384 workgroups of sixteen slabs each, whose barrier a slab is what is left);
-// 1024 rows of 2560 x 2 x 9728 127 us, 2048 231 (880 TFLOP/s; 770 with groups of 32, whose codes are
+// 1024 rows of 2560 x 2 x 9728 125 us, 2048 235 (870 TFLOP/s; 770 with groups of 32, whose codes are
 // scaled before the product). The weights are expanded by each panel of rows anew, eight
 // blocks of 16 rows to a wave at most: the vector unit beside the matrix core bounds it.
 constexpr int panel_bytes(int rt) { return rt * 4096 + 4 * rt * 64; }
