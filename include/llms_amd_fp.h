@@ -354,10 +354,10 @@ int fp_attention_bf16(const fp_attention_args* args, void* workspace, int64_t wo
  * position <= query position, grouped-query heads sharing their kv head), over the
  * cache as it then is: a block that this call completes is read in its codes, also for the
  * rows before its end, whose values later positions then touch through the scale (a call of
- * which no row but the last ends a block has none). Rows that see no key (behind a sequence's length, at a position outside
- * the cache) are zero. fp_kv8_write only writes. Both may start anywhere up to the
- * number of positions written so far: what is behind is dropped. (A call that starts
- * later than that leaves a gap: the unfinished block before it is lost.)
+ * which no row but the last ends a block has none). Rows that see no key (behind a
+ * sequence's length, at a position outside the cache) are zero. fp_kv8_write only writes. Both
+ * may start anywhere up to the number of positions written so far: what is behind is dropped.
+ * (A call that starts later than that leaves a gap: the unfinished block before it is lost.)
  * fp_kv8_read gives k_out, v_out [B][T][n_kv_heads][head_dim] fp32, the values at
  * positions pos .. pos+T-1 of sequences that end there (0 outside the cache).
  * head_dim is 64 or 128; cache_len at most 2^23; codes, scales and tails 16-byte

@@ -16,8 +16,8 @@
 //   - logprob_join_kernel: one wave per row merges the pieces' sums and sorted lists.
 // A row of one piece needs no second launch. Everything is summed in a fixed order.
 // 2048 rows of 151936 bf16 logits take 131 us in a graph of such calls (a piece of 64 elements
-// per thread, five waves per SIMD), 6 of them to join, 4.8 TB/s: about nine vector operations per element keep
-// pace with the loads. One row with its top 20 takes 6 and 5.6 us: launches and the serial
+// per thread, five waves per SIMD), 6 of them to join, 4.8 TB/s: about nine vector operations
+// per element keep pace with the loads. One row with its top 20 takes 6 and 5.6 us: launches and the serial
 // search, not the 0.3 MB.
 //
 // A key is (order-preserving bits of the value, ~token): unique, larger is better.

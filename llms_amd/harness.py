@@ -271,7 +271,7 @@ def teacher_forced_logprobs(model: Qwen3Model, tokens: list[int], device, *, top
     cuts = [len(tokens)]
     if kv8 and causal:
         blocks, rest = divmod(len(tokens), KV8_BLOCK)
-        cuts = [KV8_BLOCK - 1, 1] * blocks + [rest] * (rest > 0)
+        cuts = [KV8_BLOCK - 1, 1] * blocks + [rest] * (rest > 0 or not blocks)
     with torch.inference_mode():
         cache = model.alloc_cache(len(tokens) + 4, kv8=kv8)
         steps = [model(piece, cache) for piece in ids.split(cuts, 1)]

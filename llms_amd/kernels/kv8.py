@@ -141,8 +141,9 @@ def attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCa
         ``[B, T, heads, D]`` bfloat16: softmax attention with scale ``D ** -0.5`` of the token
         at position p over positions 0 .. p, as the cache holds them after the write: in
         8 bits where this call's tokens end their block, whose scale later tokens of the
-        block take part in (see the module's head for calls where that must not be). Rows past a sequence's length, and at device
-        positions outside the cache (whose tokens are not written), are zero.
+        block take part in (see the module's head for calls where that must not be). Rows
+        past a sequence's length, and at device positions outside the cache (whose tokens
+        are not written), are zero.
     """
     fn = "attention_kv8"
     if q.dim() != 4 or k.dim() != 4:
@@ -158,14 +159,15 @@ def attention_core_kv8(q, k, v, *, q_norm, k_norm, num_heads: int, cache: KVCach
     """What ``TritonAttention.forward`` does between its projections with an 8-bit
     cache: QK-norm and RoPE of the flat projections ``[B, T, heads * D]`` in the
     kernel that writes the keys (in torch where a norm is not the plain one, a type is not
-    bf16's or rows of cos and sin share memory), the cache write and attention. Returns ``[B, T, num_heads * D]``."""
+    bf16's or rows of cos and sin share memory), the cache write and attention. Returns
+    ``[B, T, num_heads * D]``."""
     fn, D = "attention_kv8", cache.head_dim
     B, T, _ = q.shape
     fused = (plain_norm(q_norm) and plain_norm(k_norm) and not autocast()
              and all(t.dtype == torch.bfloat16 and t.shape == (D,) and t.is_contiguous() and t.data_ptr() % 8 == 0
                      for t in (q_norm.weight, k_norm.weight))
-             and all(t.dtype == torch.bfloat16 and t.shape == (T, D) and t.stride(1) == 1 and (T == 1 or t.stride(0) >= D)
-                     and t.device == q.device for t in (cos, sin))
+             and all(t.dtype == torch.bfloat16 and t.shape == (T, D) and t.stride(1) == 1 and t.device == q.device
+                     and (T == 1 or t.stride(0) >= D) for t in (cos, sin))
              and not transformed(q_norm.weight, k_norm.weight, cos, sin))
     if not fused:
         from ._eager import apply_rope

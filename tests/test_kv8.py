@@ -708,3 +708,12 @@ def test_causal_scores(n):
     assert (one.float() - step).norm() <= 2e-2 * step.norm()
     direct = fk.token_logprobs(one, ids[0, 1:], 3)
     assert all(torch.equal(s, t) for s, t in zip(x, direct))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_scores_of_the_shortest_texts(causal):
+    h, m = model()
+    for n in (0, 1):
+        s = h.teacher_forced_logprobs(m, list(range(n)), DEV, top_k=2, kv8=True, causal=causal)
+        assert s.logprob.shape == (0,) and s.top_ids.shape == (0, 2)
