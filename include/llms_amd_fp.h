@@ -439,6 +439,35 @@ int fp_quantize_w4(const void* w, int64_t ldw,
                    void* stream);
 
 /*
+ * Projections in 8-bit integers (no reference counterpart): int8 weights with a scale per
+ * row (fp_quantize_w8_per_row) and tokens quantised in the call with a scale each.
+ *   top = max |x| of a token, c = rne(127 x / top), sx = top / 127 in fp32 (0 with codes of 0
+ *   for a token of zeros)
+ *   y[m][n] = bf16(sx[m] * s[n] * sum_k c[m][k] q[n][k]), the sum exact in int32; gate-up
+ *   y = bf16(silu(g) * u) of the fp32 values, rounded once
+ * gamma [K], when not NULL, is an RMSNorm weight applied to x first (the contract of
+ * fp_rmsnorm_qkv_bf16; eps finite and >= 0). A token with an infinity or a NaN (after the
+ * norm) has NaN outputs. A token's outputs do not depend on the others of the call.
+ * workspace: at least fp_w8a8_workspace_bytes(M, N, K, gate_up) bytes, 16-byte aligned
+ * (0 for most calls of few tokens: NULL will do). M < 2^24, N <= 2^22 - 64, K <= 2^17,
+ * ceil(M / 128) * ceil(N / 64) < 2^24; ldx < 2^40, ldq < 2^31.
+ */
+int64_t fp_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up);
+
+int fp_linear_w8a8(const void* x, int64_t ldx, const void* gamma, float eps,
+                   const int8_t* q, int64_t ldq, const float* s,
+                   void* y, int64_t ldy,
+                   int64_t M, int64_t N, int64_t K,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+int fp_gate_up_silu_w8a8(const void* x, int64_t ldx, const void* gamma, float eps,
+                         const int8_t* qg, int64_t ldqg, const float* sg,
+                         const int8_t* qu, int64_t ldqu, const float* su,
+                         void* y, int64_t ldy,
+                         int64_t M, int64_t N, int64_t K,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Log-probabilities of given tokens, entropy and top alternatives of every row
  * of logits (no reference counterpart: the reference scores with torch's
  * log_softmax), in one pass over the logits.

@@ -66,6 +66,10 @@ CAPI_SIGNATURES: dict[str, list] = {
     "fp_gate_up_silu_w4": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64,
                            _I64, _I64, _P, _I64, _P],
     "fp_quantize_w4": [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P],
+    "fp_w8a8_workspace_bytes": [_I64, _I64, _I64, ctypes.c_int],
+    "fp_linear_w8a8": [_P, _I64, _P, _F, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "fp_gate_up_silu_w8a8": [_P, _I64, _P, _F, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P,
+                             _I64, _P],
     "fp_logprob_workspace_bytes": [_I64, _I64, _I64],
     "fp_token_logprobs": [_P, ctypes.c_int, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P],
     "fp_rmsnorm_qkv_bf16_noalloc": [_P, _I64, _P, _F, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P],
@@ -112,6 +116,7 @@ def capi() -> ctypes.CDLL:
                               "fp_attention_workspace_bytes": ctypes.c_int64,
                               "fp_kv8_workspace_bytes": ctypes.c_int64,
                               "fp_w4_workspace_bytes": ctypes.c_int64,
+                              "fp_w8a8_workspace_bytes": ctypes.c_int64,
                               "fp_logprob_workspace_bytes": ctypes.c_int64}.get(name, ctypes.c_int)
             _capi = lib
         return _capi

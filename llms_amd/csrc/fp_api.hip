@@ -271,6 +271,18 @@ int check_w4(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t 
   return FP_OK;
 }
 bool off2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }
+bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) != 0; }
+
+// Arguments of an 8-bit integer call but for its pointers. Sums stay within int32 (127^2 K), the
+// grids' column workgroups (64 columns at least) within 65535 and their threads under 2^32.
+int check_w8a8(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t ldq) {
+  if (M < 0 || N < 1 || K < 1) return FP_ERR_SHAPE;
+  if (N > 65535 * 64 || K > (int64_t)1 << 17 || M >= (int64_t)1 << 24 ||
+      (M + 127) / 128 * ((N + 63) / 64) >= (int64_t)1 << 24)
+    return FP_ERR_SHAPE;
+  if (ldx < K || ldx >= (int64_t)1 << 40 || ldy < N || ldq < K || ldq >= (int64_t)1 << 31) return FP_ERR_STRIDE;
+  return FP_OK;
+}
 
 int check_common(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy) {
   if (M < 0 || N < 1 || K < 1) return FP_ERR_SHAPE;
@@ -779,6 +791,49 @@ int fp_quantize_w4(const void* w, int64_t ldw, uint8_t* q, int64_t ldq, void* s,
   if (fp::off2(w) || fp::off2(s)) return FP_ERR_STRIDE;
   return fp::launch_status(fp::launch_w4_quantize((const uint16_t*)w, ldw, q, ldq, (uint16_t*)s, lds,
                                                   N, K, (int)group, (hipStream_t)stream));
+}
+
+int64_t fp_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up) {
+  if (M < 1 || fp::check_w8a8(M, N, K, K, N, K)) return 0;
+  return fp::w8a8_workspace_bytes(M, N, K, gate_up != 0);
+}
+
+int fp_linear_w8a8(const void* x, int64_t ldx, const void* gamma, float eps, const int8_t* q, int64_t ldq,
+                   const float* s, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+  int st = fp::check_w8a8(M, N, K, ldx, ldy, ldq);
+  if (!st && gamma) st = fp::check_norm(eps, nullptr, 0);
+  if (st) return st;
+  if (M == 0) return FP_OK;
+  if (!x || !q || !s || !y) return FP_ERR_NULL;
+  if (fp::off2(x) || fp::off2(gamma) || fp::off4(s) || fp::off2(y)) return FP_ERR_STRIDE;
+  const int64_t need = fp::w8a8_workspace_bytes(M, N, K, false);
+  if (workspace_bytes < need || (need > 0 && !workspace) || !fp::al16(workspace)) return FP_ERR_WORKSPACE;
+  fp::W8A8Args a{};
+  a.x = (const uint16_t*)x, a.ldx = ldx, a.gamma = (const uint16_t*)gamma, a.eps = eps;
+  a.q0 = q, a.ldq0 = ldq, a.s0 = s, a.y = (uint16_t*)y, a.ldy = ldy, a.M = M, a.N = N, a.K = K;
+  const bool aligned = fp::al16(q) && ldq % 16 == 0;
+  return fp::launch_status(fp::launch_w8a8(a, false, aligned, workspace, (hipStream_t)stream));
+}
+
+int fp_gate_up_silu_w8a8(const void* x, int64_t ldx, const void* gamma, float eps, const int8_t* qg, int64_t ldqg,
+                         const float* sg, const int8_t* qu, int64_t ldqu, const float* su, void* y, int64_t ldy,
+                         int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+  int st = fp::check_w8a8(M, N, K, ldx, ldy, ldqg);
+  if (!st) st = fp::check_w8a8(M, N, K, ldx, ldy, ldqu);
+  if (!st && gamma) st = fp::check_norm(eps, nullptr, 0);
+  if (st) return st;
+  if (M == 0) return FP_OK;
+  if (!x || !qg || !sg || !qu || !su || !y) return FP_ERR_NULL;
+  if (fp::off2(x) || fp::off2(gamma) || fp::off4(sg) || fp::off4(su) || fp::off2(y)) return FP_ERR_STRIDE;
+  const int64_t need = fp::w8a8_workspace_bytes(M, N, K, true);
+  if (workspace_bytes < need || (need > 0 && !workspace) || !fp::al16(workspace)) return FP_ERR_WORKSPACE;
+  fp::W8A8Args a{};
+  a.x = (const uint16_t*)x, a.ldx = ldx, a.gamma = (const uint16_t*)gamma, a.eps = eps;
+  a.q0 = qg, a.ldq0 = ldqg, a.s0 = sg, a.q1 = qu, a.ldq1 = ldqu, a.s1 = su;
+  a.y = (uint16_t*)y, a.ldy = ldy, a.M = M, a.N = N, a.K = K;
+  const bool aligned = fp::al16(qg) && ldqg % 16 == 0 && fp::al16(qu) && ldqu % 16 == 0;
+  return fp::launch_status(fp::launch_w8a8(a, true, aligned, workspace, (hipStream_t)stream));
 }
 
 int64_t fp_logprob_workspace_bytes(int64_t M, int64_t V, int64_t top_k) {

@@ -256,6 +256,28 @@ int launch_w4(const W4Args& a, bool gateup, bool aligned, void* ws, hipStream_t 
 int launch_w4_quantize(const uint16_t* w, int64_t ldw, uint8_t* q, int64_t ldq, uint16_t* sc,
                        int64_t lds, int64_t N, int64_t K, int group, hipStream_t s);
 
+// Projections in 8-bit integers (fp_w8a8.hip). q: [N][K] int8 at a row stride, s: [N] fp32;
+// gate-up has two of each. gamma: an RMSNorm weight [K] for x, or NULL.
+struct W8A8Args {
+  const uint16_t* x;
+  int64_t ldx;
+  const uint16_t* gamma;
+  float eps;
+  const int8_t *q0, *q1;
+  int64_t ldq0, ldq1;
+  const float *s0, *s1;
+  uint16_t* y;
+  int64_t ldy;
+  int64_t M, N, K;
+  // set by launch_w8a8: x in codes [M][Kp] (Kp: K in whole 128) and the tokens' scales
+  int64_t Kp;
+  int8_t* xq;
+  float* sx;
+};
+int64_t w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gateup);
+// aligned: weight rows on 16 bytes.
+int launch_w8a8(W8A8Args a, bool gateup, bool aligned, void* ws, hipStream_t s);
+
 // Log-probabilities of the rows of logits x [M][V] (fp_logprob.hip).
 struct LogprobArgs {
   const void* x;

@@ -398,7 +398,7 @@ void value_same(const at::Tensor& x, const at::Tensor& t, const char* fn, const 
 }
 // A type's name in Python.
 const char* py_name(at::ScalarType t) {
-  return t == at::kByte ? "uint8" : t == at::kBFloat16 ? "bfloat16" : t == at::kHalf ? "float16" :
+  return t == at::kByte ? "uint8" : t == at::kChar ? "int8" : t == at::kBFloat16 ? "bfloat16" : t == at::kHalf ? "float16" :
          t == at::kFloat ? "float32" : t == at::kLong ? "int64" : c10::toString(t);
 }
 void type_is(const at::Tensor& t, at::ScalarType dt, const char* fn, const char* name) {
@@ -521,6 +521,69 @@ std::tuple<at::Tensor, at::Tensor> quantize_w4(const at::Tensor& w_, int64_t gro
                               group, cur_stream(w)),
                "fp_quantize_w4");
   return {q, s};
+}
+
+// ---- 8-bit integer products ----
+
+// Codes q [N, K] and scales s [N] of one weight of x's K inputs.
+void check_w8a8(const char* fn, const at::Tensor& x, const at::Tensor& q, const at::Tensor& s) {
+  const int64_t K = x.dim() ? x.size(-1) : 0;
+  TORCH_CHECK_VALUE(K >= 1, fn, ": x must have a last dimension of at least 1, got ", x.sizes());
+  TORCH_CHECK_VALUE(q.dim() == 2 && q.size(1) == K, fn, ": q shape ", q.sizes(), " != (N, ", K, ")");
+  TORCH_CHECK_VALUE(s.dim() == 1 && s.size(0) == q.size(0), fn, ": s shape ", s.sizes(), " != (", q.size(0), ",)");
+  type_is(q, at::kChar, fn, "q");
+  type_is(s, at::kFloat, fn, "s");
+  type_is(x, at::kBFloat16, fn, "x");
+  value_same(x, q, fn, "x", "q");
+  value_same(x, s, fn, "x", "s");
+  value_device(x, fn, "x");
+}
+
+at::Tensor linear_w8a8(const at::Tensor& x, const c10::optional<at::Tensor>& gamma, double eps,
+                       const at::Tensor& q_, const at::Tensor& s_) {
+  const char* fn = "fused_linear_w8a8";
+  const at::Tensor gm = w4_gamma(fn, x, gamma, eps);
+  check_w8a8(fn, x, q_, s_);
+  const int64_t K = x.size(-1), N = q_.size(0);
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor x2 = as_rows(x, K), q = as_rows(q_, K), s = as_rows(s_, N);
+  at::Tensor y = at::empty(with_last(x, N), x.options());
+  const int64_t M = x2.size(0);
+  if (M == 0 || N == 0) return y;
+  const int64_t bytes = fp_w8a8_workspace_bytes(M, N, K, 0);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check_status(fp_linear_w8a8(x2.data_ptr(), ld(x2), gm.defined() ? gm.data_ptr() : nullptr, (float)eps,
+                              q.data_ptr<int8_t>(), ld(q), s.data_ptr<float>(), y.data_ptr(), N, M, N, K,
+                              bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(x)),
+               "fp_linear_w8a8");
+  return y;
+}
+
+at::Tensor gate_up_silu_w8a8(const at::Tensor& x, const c10::optional<at::Tensor>& gamma, double eps,
+                             const at::Tensor& qg_, const at::Tensor& sg_, const at::Tensor& qu_,
+                             const at::Tensor& su_) {
+  const char* fn = "fused_gate_up_silu_w8a8";
+  TORCH_CHECK_VALUE(qg_.sizes() == qu_.sizes(), fn, ": qg shape ", qg_.sizes(), " != qu shape ", qu_.sizes());
+  const at::Tensor gm = w4_gamma(fn, x, gamma, eps);
+  check_w8a8(fn, x, qg_, sg_);
+  check_w8a8(fn, x, qu_, su_);
+  const int64_t K = x.size(-1), N = qg_.size(0);
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor x2 = as_rows(x, K), qg = as_rows(qg_, K), sg = as_rows(sg_, N), qu = as_rows(qu_, K),
+                   su = as_rows(su_, N);
+  at::Tensor y = at::empty(with_last(x, N), x.options());
+  const int64_t M = x2.size(0);
+  if (M == 0 || N == 0) return y;
+  const int64_t bytes = fp_w8a8_workspace_bytes(M, N, K, 1);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check_status(fp_gate_up_silu_w8a8(x2.data_ptr(), ld(x2), gm.defined() ? gm.data_ptr() : nullptr, (float)eps,
+                                    qg.data_ptr<int8_t>(), ld(qg), sg.data_ptr<float>(), qu.data_ptr<int8_t>(),
+                                    ld(qu), su.data_ptr<float>(), y.data_ptr(), N, M, N, K,
+                                    bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(x)),
+               "fp_gate_up_silu_w8a8");
+  return y;
 }
 
 // ---- 8-bit cache ----
@@ -727,6 +790,8 @@ void low_bit(torch::Library& m) {
   m.impl("linear_w4", linear_w4);
   m.impl("gate_up_silu_w4", gate_up_silu_w4);
   m.impl("quantize_w4", quantize_w4);
+  m.impl("linear_w8a8", linear_w8a8);
+  m.impl("gate_up_silu_w8a8", gate_up_silu_w8a8);
   m.impl("attention_kv8", attention_kv8);
   m.impl("write_kv8", write_kv8);
   m.impl("read_kv8", read_kv8);
@@ -763,6 +828,9 @@ TORCH_LIBRARY(llms_amd, m) {
   m.def("gate_up_silu_w4(Tensor x, Tensor? gamma, float eps, Tensor qg, Tensor sg, Tensor qu, "
         "Tensor su, int group) -> Tensor");
   m.def("quantize_w4(Tensor w, int group) -> (Tensor, Tensor)");
+  m.def("linear_w8a8(Tensor x, Tensor? gamma, float eps, Tensor q, Tensor scale) -> Tensor");
+  m.def("gate_up_silu_w8a8(Tensor x, Tensor? gamma, float eps, Tensor qg, Tensor sg, Tensor qu, "
+        "Tensor su) -> Tensor");
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k) -> (Tensor, Tensor, Tensor, "
         "Tensor)");
   m.def("quantize_w8(Tensor w) -> (Tensor, Tensor)");

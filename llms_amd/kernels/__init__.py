@@ -16,6 +16,8 @@ from .quant import dequantize_w4, dequantize_w8, quantize_w4, quantize_w8_per_ro
 from .swap import apply_triton_kernels, prewarm_triton_kernels
 from .w4 import (fused_gate_up_silu_w4, fused_linear_w4, fused_qkv_w4, fused_rmsnorm_gate_up_silu_w4,
                  fused_rmsnorm_qkv_w4)
+from .w8a8 import (fused_gate_up_silu_w8a8, fused_linear_w8a8, fused_qkv_w8a8, fused_rmsnorm_gate_up_silu_w8a8,
+                   fused_rmsnorm_qkv_w8a8)
 
 __all__ = [
     "FusedLinear",
@@ -35,6 +37,11 @@ __all__ = [
     "fused_gate_up_silu",
     "fused_qkv_w8",
     "fused_gate_up_silu_w8",
+    "fused_linear_w8a8",
+    "fused_qkv_w8a8",
+    "fused_gate_up_silu_w8a8",
+    "fused_rmsnorm_qkv_w8a8",
+    "fused_rmsnorm_gate_up_silu_w8a8",
     "fused_linear_w4",
     "fused_qkv_w4",
     "fused_gate_up_silu_w4",

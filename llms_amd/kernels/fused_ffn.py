@@ -22,6 +22,7 @@ from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
 from .quant import pack_weight
 from .w4 import fused_gate_up_silu_w4, fused_rmsnorm_gate_up_silu_w4
+from .w8a8 import fused_gate_up_silu_w8a8, fused_rmsnorm_gate_up_silu_w8a8
 
 
 def triton_fused_gate_up_silu(
@@ -107,7 +108,8 @@ class TritonFFN(nn.Module):
 
     ``from_eager(..., int8=True)`` keeps per-row int8 gate/up weights
     (``qg``, ``sg``, ``qu``, ``su`` buffers) and runs the int8 kernel, with
-    ``w4_group=32, 64 or 128`` 4-bit ones with their group scales.
+    ``w4_group=32, 64 or 128`` 4-bit ones with their group scales. ``a8=True`` with
+    ``int8=True`` multiplies in integers (tokens in 8 bits).
     ``prenorm`` (set by ``apply_triton_kernels(..., fuse_norm=True)``) is the
     block's pre-FFN RMSNorm, run inside the projection call.
     """
@@ -115,6 +117,8 @@ class TritonFFN(nn.Module):
     # The group size of 4-bit weights, 0 for the other forms; on the class, so that a
     # module saved whole without it loads and runs as it did.
     w4_group = 0
+    # Whether int8 modules take their tokens in 8 bits too (on the class for the same reason).
+    a8 = False
 
     def __init__(self, hidden_size: int, intermediate_size: int) -> None:
         super().__init__()
@@ -133,6 +137,11 @@ class TritonFFN(nn.Module):
             if pn is not None:
                 return fused_rmsnorm_gate_up_silu_w4(x, pn.weight, pn.eps, *w, group=self.w4_group)
             return fused_gate_up_silu_w4(x, *w, group=self.w4_group)
+        if self.a8:
+            w = (self.qg, self.sg, self.qu, self.su)
+            if pn is not None:
+                return fused_rmsnorm_gate_up_silu_w8a8(x, pn.weight, pn.eps, *w)
+            return fused_gate_up_silu_w8a8(x, *w)
         if pn is not None:
             from .fused_norm import fused_rmsnorm_gate_up_silu, fused_rmsnorm_gate_up_silu_w8
 
@@ -149,14 +158,18 @@ class TritonFFN(nn.Module):
         return self.down(self.gate_up(x))
 
     @classmethod
-    def from_eager(cls, eager: nn.Module, *, int8: bool = False, w4_group: int = 0) -> "TritonFFN":
+    def from_eager(cls, eager: nn.Module, *, int8: bool = False, w4_group: int = 0,
+                   a8: bool = False) -> "TritonFFN":
         """Wrap a module with ``gate``/``up``/``down`` Linears, sharing their
         parameters (no copy). int8=True quantises gate and up per output row
-        and drops the bf16 gate/up modules; w4_group does so in 4 bits."""
+        and drops the bf16 gate/up modules; w4_group does so in 4 bits. a8 (with
+        int8) has the call's tokens in 8 bits as well."""
         out = cls.__new__(cls)
         nn.Module.__init__(out)
         out.down = eager.down
         out.int8 = bool(int8)
+        if a8:
+            out.a8 = True
         out.prenorm = None
         if w4_group:
             out.w4_group, out.in_features = w4_group, eager.gate.in_features

@@ -21,6 +21,7 @@ from .fused_attention import attention_core
 from .kv8 import KVCache8, attention_core_kv8
 from .quant import pack_weight
 from .w4 import fused_qkv_w4, fused_rmsnorm_qkv_w4
+from .w8a8 import fused_qkv_w8a8, fused_rmsnorm_qkv_w8a8
 
 
 def triton_fused_qkv(
@@ -140,7 +141,8 @@ class TritonAttention(nn.Module):
 
     With ``from_eager(..., int8=True)`` the stacked weight is kept as
     per-row int8 (``q_qkv``, ``s_qkv`` buffers) and the int8 kernel runs; with
-    ``w4_group=32, 64 or 128`` in 4 bits with group scales.
+    ``w4_group=32, 64 or 128`` in 4 bits with group scales, with ``int8=True`` and
+    ``a8=True`` multiplied in integers (tokens in 8 bits).
     ``prenorm`` (set by ``apply_triton_kernels(..., fuse_norm=True)``) is the
     block's pre-attention RMSNorm, run inside the projection call.
     """
@@ -148,6 +150,8 @@ class TritonAttention(nn.Module):
     # The group size of 4-bit weights, 0 for the other forms; on the class, so that a
     # module saved whole without it loads and runs as it did.
     w4_group = 0
+    # Whether int8 modules take their tokens in 8 bits too (on the class for the same reason).
+    a8 = False
 
     def __init__(
         self,
@@ -174,13 +178,14 @@ class TritonAttention(nn.Module):
         self.prenorm = None
 
     @classmethod
-    def from_eager(cls, eager: nn.Module, *, int8: bool = False, w4_group: int = 0) -> "TritonAttention":
+    def from_eager(cls, eager: nn.Module, *, int8: bool = False, w4_group: int = 0,
+                   a8: bool = False) -> "TritonAttention":
         """Build from an eager ``Attention`` with loaded weights: row-stack
         ``[Wq; Wk; Wv]`` once, reuse ``o``, ``q_norm`` and ``k_norm`` (no copy).
 
         int8=True quantises the stacked weight per output row on the device
         and keeps only the int8 weight and its scales; w4_group does so in 4
-        bits.
+        bits. a8 (with int8) has the call's tokens in 8 bits as well.
         """
         out = cls.__new__(cls)
         nn.Module.__init__(out)
@@ -192,6 +197,8 @@ class TritonAttention(nn.Module):
         out.n_k = eager.num_kv_heads * eager.head_dim
         W_qkv = torch.cat([eager.q.weight, eager.k.weight, eager.v.weight], dim=0)
         out.int8 = bool(int8)
+        if a8:
+            out.a8 = True
         if w4_group:
             out.w4_group, out.in_features = w4_group, eager.q.in_features
         if out.int8 or w4_group:
@@ -216,6 +223,11 @@ class TritonAttention(nn.Module):
             if pn is not None:
                 return fused_rmsnorm_qkv_w4(x, pn.weight, pn.eps, self.q_qkv, self.s_qkv, **n)
             return fused_qkv_w4(x, self.q_qkv, self.s_qkv, **n)
+        if self.a8:
+            n = dict(n_q=self.n_q, n_k=self.n_k)
+            if pn is not None:
+                return fused_rmsnorm_qkv_w8a8(x, pn.weight, pn.eps, self.q_qkv, self.s_qkv, **n)
+            return fused_qkv_w8a8(x, self.q_qkv, self.s_qkv, **n)
         if pn is not None:
             from .fused_norm import fused_rmsnorm_qkv, fused_rmsnorm_qkv_w8
 

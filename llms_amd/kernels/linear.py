@@ -20,6 +20,7 @@ from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
 from .quant import pack_weight
 from .w4 import fused_linear_w4
+from .w8a8 import fused_linear_w8a8
 
 
 def fused_linear(x: torch.Tensor, W: torch.Tensor) -> torch.Tensor:
@@ -83,6 +84,8 @@ class FusedLinear(nn.Module):
     # The group size of 4-bit weights, 0 for the other forms; on the class, so that a
     # module saved whole without it loads and runs as it did.
     w4_group = 0
+    # Whether int8 modules take their tokens in 8 bits too (on the class for the same reason).
+    a8 = False
 
     def __init__(self, in_features: int, out_features: int) -> None:
         super().__init__()
@@ -94,15 +97,19 @@ class FusedLinear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.w4_group:
             return fused_linear_w4(x, self.q, self.s, group=self.w4_group)
+        if self.a8:
+            return fused_linear_w8a8(x, self.q, self.s)
         if self.int8:
             return fused_linear_w8(x, self.q, self.s)
         return fused_linear(x, self.weight)
 
     @classmethod
-    def from_linear(cls, lin: nn.Linear, *, int8: bool = False, w4_group: int = 0) -> "FusedLinear":
+    def from_linear(cls, lin: nn.Linear, *, int8: bool = False, w4_group: int = 0,
+                    a8: bool = False) -> "FusedLinear":
         """Wrap a bias-free ``nn.Linear`` (its weight is shared, not copied);
         ``int8=True`` quantises it per output row on its device instead,
-        ``w4_group`` in 4 bits in groups of that many inputs."""
+        ``w4_group`` in 4 bits in groups of that many inputs. ``a8`` (with int8) has the
+        call's tokens in 8 bits as well."""
         if getattr(lin, "bias", None) is not None:
             raise ValueError("FusedLinear wraps bias-free Linears only")
         out = cls.__new__(cls)
@@ -110,6 +117,8 @@ class FusedLinear(nn.Module):
         out.in_features = lin.in_features
         out.out_features = lin.out_features
         out.int8 = bool(int8)
+        if a8:
+            out.a8 = True
         if w4_group:
             out.w4_group = w4_group
         if out.int8 or w4_group:
@@ -122,4 +131,4 @@ class FusedLinear(nn.Module):
         return out
 
     def extra_repr(self) -> str:
-        return f"in_features={self.in_features}, out_features={self.out_features}, int8={self.int8}, w4_group={self.w4_group}"
+        return f"in_features={self.in_features}, out_features={self.out_features}, int8={self.int8}, w4_group={self.w4_group}, a8={self.a8}"

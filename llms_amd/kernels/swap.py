@@ -30,6 +30,7 @@ def apply_triton_kernels(
     fuse_norm: bool = False,
     int4: bool = False,
     w4_group: int = 128,
+    a8: bool = False,
 ) -> nn.Module:
     """Replace ``block.ffn`` / ``block.attn`` of every ``model.layers`` block
     with ``TritonFFN`` / ``TritonAttention`` (reference ``swap.py:22-46``).
@@ -37,7 +38,8 @@ def apply_triton_kernels(
     Idempotent: blocks already swapped are left as they are. ``int8=True``
     (not in the reference) builds the int8 weight-only modules instead,
     ``int4=True`` those with 4-bit weights in groups of ``w4_group`` inputs (32, 64
-    or 128).
+    or 128). ``a8=True`` with ``int8=True`` has the int8 modules take their tokens in 8
+    bits too (products in integers, :mod:`~llms_amd.kernels.w8a8`).
     ``linear_down_o=True`` (not in the reference) also replaces each block's
     ``ffn.down`` and ``attn.o`` Linears with :class:`FusedLinear`, int8 when
     ``int8`` is set. ``fuse_norm=True`` (not in the reference) moves each
@@ -52,7 +54,9 @@ def apply_triton_kernels(
         raise ValueError("apply_triton_kernels: int8 and int4 exclude each other")
     if int4 and w4_group not in (32, 64, 128):
         raise ValueError(f"apply_triton_kernels: w4_group must be 32, 64 or 128, got {w4_group}")
-    low = dict(int8=int8, w4_group=w4_group if int4 else 0)
+    if a8 and not int8:
+        raise ValueError("apply_triton_kernels: a8 takes the tokens of int8 modules in 8 bits: int8=True too")
+    low = dict(int8=int8, w4_group=w4_group if int4 else 0, a8=a8)
     if linear_down_o and getattr(model, "fused_head", None) is False:
         model.fused_head = True
     for block in model.layers:
@@ -105,17 +109,17 @@ def prewarm_triton_kernels(
     for m in model.modules():
         if isinstance(m, TritonFFN):
             w = m.qg if m.int8 or m.w4_group else m.gate.weight
-            ffn_by_shape.setdefault((m.int8, m.w4_group, w.shape[0], _inputs(w, m)), m)
+            ffn_by_shape.setdefault((m.int8, m.a8, m.w4_group, w.shape[0], _inputs(w, m)), m)
     attn_by_shape: dict[tuple, TritonAttention] = {}
     for m in model.modules():
         if isinstance(m, TritonAttention):
             w = m.q_qkv if m.int8 or m.w4_group else m.W_qkv
-            attn_by_shape.setdefault((m.int8, m.w4_group, w.shape[0], _inputs(w, m)), m)
+            attn_by_shape.setdefault((m.int8, m.a8, m.w4_group, w.shape[0], _inputs(w, m)), m)
     lin_by_shape: dict[tuple, FusedLinear] = {}
     for m in model.modules():
         if isinstance(m, FusedLinear):
             w = m.q if m.int8 or m.w4_group else m.weight
-            lin_by_shape.setdefault((m.int8, m.w4_group, w.shape[0], _inputs(w, m)), m)
+            lin_by_shape.setdefault((m.int8, m.a8, m.w4_group, w.shape[0], _inputs(w, m)), m)
     if not ffn_by_shape and not attn_by_shape and not lin_by_shape:
         return
 
