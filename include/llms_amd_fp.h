@@ -450,7 +450,7 @@ int fp_quantize_w4(const void* w, int64_t ldw,
  * norm) has NaN outputs. A token's outputs do not depend on the others of the call.
  * workspace: at least fp_w8a8_workspace_bytes(M, N, K, gate_up) bytes, 16-byte aligned
  * (0 for most calls of few tokens: NULL will do). M < 2^24, N <= 2^22 - 64, K <= 2^17,
- * ceil(M / 128) * ceil(N / 64) < 2^24; ldx < 2^40, ldq < 2^31.
+ * ceil(M / 128) * ceil(N / 64) < 2^24; ldx < 2^40, ldq < 2^23.
  */
 int64_t fp_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up);
 

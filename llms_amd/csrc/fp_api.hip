@@ -273,14 +273,15 @@ int check_w4(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t 
 bool off2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }
 bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) != 0; }
 
-// Arguments of an 8-bit integer call but for its pointers. Sums stay within int32 (127^2 K), the
+// Arguments of an 8-bit integer call but for its pointers. Sums stay within int32 (127^2 K), 128 weight
+// rows within 32-bit offsets, the
 // grids' column workgroups (64 columns at least) within 65535 and their threads under 2^32.
 int check_w8a8(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t ldq) {
   if (M < 0 || N < 1 || K < 1) return FP_ERR_SHAPE;
   if (N > 65535 * 64 || K > (int64_t)1 << 17 || M >= (int64_t)1 << 24 ||
       (M + 127) / 128 * ((N + 63) / 64) >= (int64_t)1 << 24)
     return FP_ERR_SHAPE;
-  if (ldx < K || ldx >= (int64_t)1 << 40 || ldy < N || ldq < K || ldq >= (int64_t)1 << 31) return FP_ERR_STRIDE;
+  if (ldx < K || ldx >= (int64_t)1 << 40 || ldy < N || ldq < K || ldq >= (int64_t)1 << 23) return FP_ERR_STRIDE;
   return FP_OK;
 }
 
@@ -832,7 +833,7 @@ int fp_gate_up_silu_w8a8(const void* x, int64_t ldx, const void* gamma, float ep
   a.x = (const uint16_t*)x, a.ldx = ldx, a.gamma = (const uint16_t*)gamma, a.eps = eps;
   a.q0 = qg, a.ldq0 = ldqg, a.s0 = sg, a.q1 = qu, a.ldq1 = ldqu, a.s1 = su;
   a.y = (uint16_t*)y, a.ldy = ldy, a.M = M, a.N = N, a.K = K;
-  const bool aligned = fp::al16(qg) && ldqg % 16 == 0 && fp::al16(qu) && ldqu % 16 == 0;
+  const bool aligned = fp::al16(qg) && fp::al16(qu) && (ldqg | ldqu) % 16 == 0;
   return fp::launch_status(fp::launch_w8a8(a, true, aligned, workspace, (hipStream_t)stream));
 }
 

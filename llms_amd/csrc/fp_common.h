@@ -105,6 +105,11 @@ __device__ __forceinline__ uint32_t gate_up_silu_bits(float acc_g, float acc_u) 
   return f32_to_bf16_bits(s * u);
 }
 
+// silu(g) * u without roundings between (the epilogue of products that are rounded once).
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  return __fdividef(g, 1.f + __expf(-g)) * u;
+}
+
 // Two outputs of the same epilogue, packed as two bf16 (lo: (g0, u0), hi:
 // (g1, u1)); bit-identical to gate_up_silu_bits on each. The conversions of
 // the two outputs share each v_cvt_pk_bf16_f32 (one for g and u of an

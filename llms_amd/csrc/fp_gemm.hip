@@ -414,10 +414,16 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_kernel(StreamArgs a, int
 // 44.5 -> 39.9. Spreading alone, two stages each: 8B gate-up 577-585 (with the
 // loads in one burst 643), 4B QKV 57; a load every second or every MFMA 605, 631;
 // three stages of both operands with all loads in the second half: 4B o 43.5.
+// I8 (four waves): both operands are int8, a 16-bit element of the tile being two of them (a.x holds
+// codes, a.K, a.ldx and a.ldw* count pairs; a.wbytes is a weight row's true length, what lies behind
+// it meets codes of zero). v_mfma_i32_16x16x64_i8 reads the same bytes per lane as the bf16
+// instruction, so everything up to the accumulators (int32 bits) is the same, and so is its time:
+// twice the operations. The epilogue multiplies by the scales of weight row (s0, s1) and token (sx).
+// 8B gate-up at 4096 rows (256 x 256): 319 us, 2.59 POP/s (bf16 575 and 1.43 PFLOP/s).
 template <int BN, int BM, int WN, int WM, bool GATEUP, bool W8, int BK = kBK, int NS = 2,
-          bool SPLIT = false, bool W3 = false>
-__global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs a, int n_mt,
-                                                                    int n_nt, int nsplit,
+          bool SPLIT = false, bool W3 = false, bool I8 = false>
+__global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(std::conditional_t<I8, I8Args, StreamArgs> a,
+                                                                    int n_mt, int n_nt, int nsplit,
                                                                     int per, float* ws) {
   constexpr int NW = WN * WM;
   constexpr int CPR = BK / 8;
@@ -442,6 +448,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs 
   static_assert(!W3 || (NS == 2 && BK == 64 && WN * WM == 4 && !W8),
                 "three weight stages: 64-wide steps, four bf16 waves");
   static_assert(!SPLIT || NS > 2 || W3, "k split across workgroups: the staged four-wave loop");
+  static_assert(!I8 || (WN * WM == 4 && !W8), "int8 operands: four waves");
   static_assert(BN % WRPI == 0 && BM % (RPI * NW) == 0, "tile/waves");
   static_assert(W8 || NWI % NW == 0, "bf16 weight loads spread evenly over the waves");
   static_assert(NQC % kWave == 0, "int8 chunks: whole waves");
@@ -476,8 +483,10 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs 
   int b = (int)((int64_t)T * xcd / 8) + (int)blockIdx.x / 8;
   if (b >= t_end) return;  // uniform per workgroup
 
-  const int wbytes0 = (int)((a.N - 1) * a.ldw0 * WB + a.K * WB);
-  const int wbytes1 = GATEUP ? (int)((a.N - 1) * a.ldw1 * WB + a.K * WB) : wbytes0;
+  int64_t wrow = a.K * WB;  // bytes of a weight row
+  if constexpr (I8) wrow = a.wbytes;
+  const int wbytes0 = (int)((a.N - 1) * a.ldw0 * WB + wrow);
+  const int wbytes1 = GATEUP ? (int)((a.N - 1) * a.ldw1 * WB + wrow) : wbytes0;
   const int xbytes = (int)((a.M - 1) * a.ldx * 2 + a.K * 2);
   void* const wptr1 = (void*)(GATEUP ? a.w1 : a.w0);
   const int lrow = lane / CPR, lchunk = lane % CPR;
@@ -537,6 +546,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs 
   auto soff = [&](int64_t k0, int bytes, bool live) {
     return live ? (uint32_t)((kb * BK + k0) * bytes) : 0u;
   };
+  // (I8: the last step may pass a weight row's end, and so the buffer's: the step is in the lanes' offset)
   auto issue_w = [&](void* dst, int64_t k0, bool live = true) {
 #pragma unroll
     for (int j = 0; j < IW; ++j) {
@@ -544,15 +554,16 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs 
       if (NWI % NW != 0 && q >= NWI) break;  // uniform per wave
       const bool up = wrow_up(q * WRPI);
       load_lds16(up ? wptr1 : a.w0, live ? (up ? wbytes1 : wbytes0) : 0,
-                 (lds_ptr_t)((char*)dst + q * WRPI * BK * WB), woff[j],
-                 soff(k0, WB, live));
+                 (lds_ptr_t)((char*)dst + q * WRPI * BK * WB), I8 ? woff[j] + soff(k0, WB, live) : woff[j],
+                 I8 ? 0 : soff(k0, WB, live));
     }
   };
   auto issue_w1 = [&](void* dst, int j, int64_t k0, bool live) {
     const int q = wave + NW * j;
     const bool up = wrow_up(q * WRPI);
     load_lds16(up ? wptr1 : a.w0, live ? (up ? wbytes1 : wbytes0) : 0,
-               (lds_ptr_t)((char*)dst + q * WRPI * BK * WB), woff[j], soff(k0, WB, live));
+               (lds_ptr_t)((char*)dst + q * WRPI * BK * WB), I8 ? woff[j] + soff(k0, WB, live) : woff[j],
+               I8 ? 0 : soff(k0, WB, live));
   };
   auto issue_x1 = [&](uint16_t (*tx)[BK], int j, int64_t k0, bool live) {
     load_lds16(a.x, live ? xbytes : 0, (lds_ptr_t)&tx[(wave + NW * j) * RPI][0], xoff[j],
@@ -640,7 +651,11 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs 
     for (int i = 0; i < FN; ++i) {
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
-        if constexpr (NW == 4)
+        if constexpr (I8)
+          asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0"
+                       : "+a"(acc[i][j])
+                       : "v"(f.a[i]), "v"(f.b[j]));
+        else if constexpr (NW == 4)
           asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
                        : "+a"(acc[i][j])
                        : "v"(f.a[i]), "v"(f.b[j]));
@@ -947,13 +962,43 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs 
     // ---- epilogue: per wave, 16 x rows at a time through its strip ----
     uint16_t* strip = &sX1[0][0] + wave * 16 * SROW;
     const int64_t nw0 = ec0 + wn * TNO;  // first output column of this wave
+    // int8: the scales of this lane's weight rows (block i's from its first output column on)
+    const auto scales = [&](int i) -> f32x4 {
+      const float* sc = GATEUP && (i & 1) ? a.s1 : a.s0;
+      const int64_t n = nw0 + (GATEUP ? i / 2 : i) * 16 + 4 * grp;
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = sc[n + r < a.N ? n + r : a.N - 1];
+      return v;
+    };
+    f32x4 sw[I8 ? FN : 1];
+    if constexpr (I8) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i) sw[i] = scales(i);
+    }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
+      float sxj = 0.f;
+      if constexpr (I8) {
+        const int64_t m = em0 + wm * TM + j * 16 + li;
+        sxj = a.sx[m < a.M ? m : a.M - 1];
+      }
 #pragma unroll
       for (int i = 0; i < FN; i += (GATEUP ? 2 : 1)) {
         uint32_t p0, p1;
         int lc;
-        if constexpr (GATEUP) {
+        if constexpr (I8) {
+          float y[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            y[r] = (float)__float_as_int(acc[i][j][r]) * sw[i][r] * sxj;
+            if constexpr (GATEUP)
+              y[r] = silu_mul(y[r], (float)__float_as_int(acc[i + 1][j][r]) * sw[i + 1][r] * sxj);
+          }
+          p0 = pack_bf16x2(y[0], y[1]);
+          p1 = pack_bf16x2(y[2], y[3]);
+          lc = (GATEUP ? i / 2 : i) * 16 + 4 * grp;
+        } else if constexpr (GATEUP) {
           p0 = gate_up_silu_pair(acc[i][j][0], acc[i + 1][j][0], acc[i][j][1], acc[i + 1][j][1]);
           p1 = gate_up_silu_pair(acc[i][j][2], acc[i + 1][j][2], acc[i][j][3], acc[i + 1][j][3]);
           lc = (i / 2) * 16 + 4 * grp;
@@ -992,6 +1037,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(StreamArgs 
 // Sums the nsplit partial accumulators of each output in split order 0, 1,
 // ... (a fixed order: results do not depend on scheduling) and applies the
 // epilogue at the torch rounding points. One thread per 4 columns of a row.
+// (int8 partials have a reduction of their own, below.)
 template <bool GATEUP>
 __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* ws, int nsplit,
                                                             StreamArgs a) {
@@ -1163,7 +1209,8 @@ bool gemm_supported(const StreamArgs& a, bool aligned, bool w8) {
 // 128 KB).
 enum GemmTile { kT64x32, kT128x64, kT64x128, kT128x128, kT256x256, kT192x256,
                 kK64x64, kK96x128, kK128x128, kT320x256, kT192x128, kT160x128,
-                kT128x160, kT96x64, kT64x128w, kT96x128, kT160x256, kT256x128 };
+                kT128x160, kT96x64, kT64x128w, kT96x128, kT160x256, kT256x128,
+                kT64x64w, kT32x64 };
 struct TileInfo {
   int bn, bm, per_cu;
 };
@@ -1172,7 +1219,7 @@ constexpr TileInfo kTiles[] = {{64, 32, 4},   {128, 64, 3},  {64, 128, 2},
                                {64, 64, 2},   {96, 128, 1},  {128, 128, 1},
                                {320, 256, 1}, {192, 128, 1}, {160, 128, 1},
                                {128, 160, 1}, {96, 64, 1},   {64, 128, 1},  {96, 128, 1},
-                               {160, 256, 1}, {256, 128, 1}};
+                               {160, 256, 1}, {256, 128, 1}, {64, 64, 1}, {32, 64, 1}};
 constexpr int kCUs = 256;
 
 int64_t tile_count(int tile, int64_t M, int64_t N, bool gateup) {
@@ -1721,5 +1768,137 @@ template int launch_gemm<false, false>(const StreamArgs&, hipStream_t);
 template int launch_gemm<true, false>(const StreamArgs&, hipStream_t);
 template int launch_gemm<false, true>(const StreamArgs&, hipStream_t);
 template int launch_gemm<true, true>(const StreamArgs&, hipStream_t);
+
+// ---- int8 x int8 ----------------------------------------------------------------
+
+namespace {
+
+// The sum of the nsplit int32 partials of each output (exact, so in any order) and the
+// epilogue. One thread per 4 columns of a row.
+template <bool GATEUP>
+__global__ __launch_bounds__(256) void i8_reduce_kernel(const int* ws, int nsplit, I8Args a) {
+  const int64_t nq = (a.N + 3) / 4;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= a.M * nq) return;
+  const int64_t m = t / nq, n = (t - m * nq) * 4;
+  const int64_t wc = GATEUP ? 2 * a.N : a.N;
+  const int64_t plane = a.M * wc;
+  const int* p = ws + m * wc + n;
+  const float sx = a.sx[m];
+  int g[4] = {}, u[4] = {};
+  if ((a.N & 3) == 0) {  // 16-byte partials (u at N + n)
+    for (int s = 0; s < nsplit; ++s) {
+      const u32x4 v = ld16(p + s * plane);
+      const u32x4 w = GATEUP ? ld16(p + s * plane + a.N) : u32x4{};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) g[r] += (int)v[r], u[r] += (int)w[r];
+    }
+  } else {
+    for (int s = 0; s < nsplit; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < a.N) {
+          g[r] += p[s * plane + r];
+          if constexpr (GATEUP) u[r] += p[s * plane + r + a.N];
+        }
+  }
+  uint16_t* yrow = a.y + m * a.ldy;
+  uint32_t h[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int64_t c = n + r < a.N ? n + r : a.N - 1;
+    float y = (float)g[r] * a.s0[c] * sx;
+    if constexpr (GATEUP) y = silu_mul(y, (float)u[r] * a.s1[c] * sx);
+    h[r] = f32_to_bf16_bits(y);
+  }
+  if (((a.ldy & 3) == 0) && ((reinterpret_cast<uintptr_t>(a.y) & 7) == 0) && n + 3 < a.N) {
+    *reinterpret_cast<u32x2*>(yrow + n) = u32x2{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < a.N) yrow[n + r] = (uint16_t)h[r];
+  }
+}
+
+// BK, NS, W3 as in gemm_tiles_kernel; nsplit > 1: k in ranges of `per` steps of BK.
+template <int BN, int BM, int WN, int WM, bool GATEUP, int BK, int NS, bool W3, bool SPLIT>
+int launch_i8_cfg(const I8Args& a, int nsplit, int per, hipStream_t s) {
+  const int64_t cols = GATEUP ? BN / 2 : BN;
+  const int n_nt = (int)((a.N + cols - 1) / cols);
+  const int n_mt = (int)((a.M + BM - 1) / BM);
+  const int64_t items = (int64_t)n_nt * n_mt * nsplit;
+  const int grid = items < kTilesGrid ? (int)((items + 7) / 8 * 8) : kTilesGrid;
+  hipLaunchKernelGGL((gemm_tiles_kernel<BN, BM, WN, WM, GATEUP, false, BK, NS, SPLIT, W3, true>),
+                     dim3((unsigned)grid), dim3(WN * WM * kWave), 0, s, a, n_mt, n_nt, nsplit, per, a.ws);
+  const int e = (int)hipGetLastError();
+  if (e || !SPLIT) return e;
+  const int64_t threads = a.M * ((a.N + 3) / 4);
+  hipLaunchKernelGGL(i8_reduce_kernel<GATEUP>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s,
+                     (const int*)a.ws, nsplit, a);
+  return (int)hipGetLastError();
+}
+
+template <bool GATEUP, bool SPLIT>
+int launch_i8_tile(const I8Args& a, const I8Plan& p, hipStream_t s) {
+  switch (p.tile) {
+    case kT256x256: return launch_i8_cfg<256, 256, 2, 2, GATEUP, kBK, 2, true, SPLIT>(a, p.nsplit, p.per, s);
+    case kT192x256: return launch_i8_cfg<192, 256, 2, 2, GATEUP, kBK, 2, true, SPLIT>(a, p.nsplit, p.per, s);
+    case kT256x128: return launch_i8_cfg<256, 128, 4, 1, GATEUP, kBK, 2, true, SPLIT>(a, p.nsplit, p.per, s);
+    case kT192x128: return launch_i8_cfg<192, 128, 2, 2, GATEUP, kBK, 2, true, SPLIT>(a, p.nsplit, p.per, s);
+    case kT160x128:
+      return launch_i8_cfg<160, 128, GATEUP ? 1 : 2, GATEUP ? 4 : 2, GATEUP, kBK, 2, true, SPLIT>(a, p.nsplit, p.per, s);
+    case kT64x128w:
+      return launch_i8_cfg<64, 128, GATEUP ? 1 : 2, GATEUP ? 4 : 2, GATEUP, 2 * kBK, 3, false, SPLIT>(a, p.nsplit, p.per, s);
+    case kT64x64w:
+      return launch_i8_cfg<64, 64, GATEUP ? 1 : 2, GATEUP ? 4 : 2, GATEUP, 2 * kBK, 4, false, SPLIT>(a, p.nsplit, p.per, s);
+    case kT32x64:
+      return launch_i8_cfg<32, 64, GATEUP ? 1 : 2, GATEUP ? 4 : 2, GATEUP, 2 * kBK, 4, false, SPLIT>(a, p.nsplit, p.per, s);
+    case kT96x64:
+      return launch_i8_cfg<96, 64, GATEUP ? 1 : 2, GATEUP ? 4 : 2, GATEUP, 2 * kBK, 4, false, SPLIT>(a, p.nsplit, p.per, s);
+    default: return (int)hipErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+// The cheapest tile and split of k: rounds of at most one work item per CU, each costing its
+// k-steps and a fixed part (us). The larger tiles cost what they do on bf16 (tile_cost: the same
+// bytes per step, of 128 k here); 96 x 64 and 64 x 128 run steps of 256 (8B down, 12288 -> 4096, at 300
+// tokens in 48 steps 41.5 and 46.5 us with what makes the codes, 4B o, 4096 -> 2560, in 16 17.9 and
+// 21.0). A split writes and reads its partials (from the Infinity Cache, measured at about 6 TB/s) in one
+// launch more. Ranges of at least 4 steps. Over 0.6B, 4B and 8B shapes at 24-4096 tokens within 4% of the
+// best of nine tiles and four splits but for a few up to 16% off.
+I8Plan i8_plan(int64_t M, int64_t N, int64_t Kp, bool gateup) {
+  I8Plan best{-1, 1, 0};
+  double least = 0.0;
+  for (int t : {kT256x256, kT192x256, kT256x128, kT192x128, kT160x128, kT64x128w, kT96x64, kT64x64w, kT32x64}) {
+    const bool small = t == kT64x128w || t == kT96x64 || t == kT64x64w || t == kT32x64;
+    const TileCost c = t == kT96x64      ? TileCost{0.74, 0.0, 6.0}
+                       : t == kT64x128w ? TileCost{0.80, 0.0, 8.0}
+                       : t == kT64x64w  ? TileCost{0.48, 0.0, 4.4}
+                       : t == kT32x64   ? TileCost{0.47, 0.0, 4.0}
+                                        : tile_cost(t, kShortSteps, gateup, true);
+    const int64_t steps = Kp / (small ? 4 * kBK : 2 * kBK), tiles = tile_count(t, M, N, gateup);
+    for (int64_t ns = 1; ns <= 16 && (ns == 1 || (ns * 4 <= steps && tiles * ns <= 2 * kCUs)); ++ns) {
+      const int64_t per = (steps + ns - 1) / ns;
+      if ((steps + per - 1) / per != ns) continue;  // every range holds a step
+      double cost = (double)((tiles * ns + kCUs - 1) / kCUs) * ((double)per * c.single + c.tile);
+      if (ns > 1) cost += 3.0 + (double)(8 * ns * M * (gateup ? 2 * N : N)) / 6e6;
+      if (best.tile < 0 || cost < least) best = I8Plan{t, (int)ns, (int)per}, least = cost;
+    }
+  }
+  return best;
+}
+
+int64_t i8_workspace_bytes(int64_t M, int64_t N, int64_t Kp, bool gateup) {
+  const I8Plan p = i8_plan(M, N, Kp, gateup);
+  return p.nsplit > 1 ? (int64_t)p.nsplit * M * (gateup ? 2 * N : N) * 4 : 0;
+}
+
+int launch_i8(const I8Args& a, bool gateup, hipStream_t s) {
+  const I8Plan p = i8_plan(a.M, a.N, 2 * a.K, gateup);
+  if (gateup) return p.nsplit > 1 ? launch_i8_tile<true, true>(a, p, s) : launch_i8_tile<true, false>(a, p, s);
+  return p.nsplit > 1 ? launch_i8_tile<false, true>(a, p, s) : launch_i8_tile<false, false>(a, p, s);
+}
 
 }  // namespace fp

@@ -269,11 +269,27 @@ struct W8A8Args {
   uint16_t* y;
   int64_t ldy;
   int64_t M, N, K;
-  // set by launch_w8a8: x in codes [M][Kp] (Kp: K in whole 128) and the tokens' scales
+  // set by launch_w8a8: x in codes [M][Kp] (Kp: K in whole 512) and the tokens' scales
   int64_t Kp;
   int8_t* xq;
   float* sx;
 };
+// The int8 x int8 form of the prefill tiles (fp_gemm.hip): codes and weights as pairs of int8 in
+// StreamArgs' 16-bit elements (x: rows of Kp = 2 a.K codes, a multiple of 256; weight rows on 16
+// bytes, a.wbytes long), scales in s0, s1, sx; a.ws holds i8_workspace_bytes. Every operand's byte
+// size is below 2^31.
+struct I8Args : StreamArgs {
+  const float* sx;
+  int64_t wbytes;
+};
+struct I8Plan {
+  int tile;         // a GemmTile
+  int nsplit, per;  // ranges of k and their steps
+};
+I8Plan i8_plan(int64_t M, int64_t N, int64_t Kp, bool gateup);
+int64_t i8_workspace_bytes(int64_t M, int64_t N, int64_t Kp, bool gateup);
+int launch_i8(const I8Args& a, bool gateup, hipStream_t s);
+
 int64_t w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gateup);
 // aligned: weight rows on 16 bytes.
 int launch_w8a8(W8A8Args a, bool gateup, bool aligned, void* ws, hipStream_t s);

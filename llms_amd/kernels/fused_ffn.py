@@ -174,8 +174,8 @@ class TritonFFN(nn.Module):
         if w4_group:
             out.w4_group, out.in_features = w4_group, eager.gate.in_features
         if out.int8 or w4_group:
-            qg, sg = pack_weight(eager.gate.weight.detach(), w4_group)
-            qu, su = pack_weight(eager.up.weight.detach(), w4_group)
+            qg, sg = pack_weight(eager.gate.weight.detach(), w4_group, a8)
+            qu, su = pack_weight(eager.up.weight.detach(), w4_group, a8)
             for name, t in (("qg", qg), ("sg", sg), ("qu", qu), ("su", su)):
                 out.register_buffer(name, t)
             out.gate = None

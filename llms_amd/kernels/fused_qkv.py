@@ -202,7 +202,7 @@ class TritonAttention(nn.Module):
         if w4_group:
             out.w4_group, out.in_features = w4_group, eager.q.in_features
         if out.int8 or w4_group:
-            q, s = pack_weight(W_qkv.detach(), w4_group)
+            q, s = pack_weight(W_qkv.detach(), w4_group, a8)
             out.register_buffer("q_qkv", q)
             out.register_buffer("s_qkv", s)
             out.W_qkv = None

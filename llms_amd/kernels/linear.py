@@ -122,7 +122,7 @@ class FusedLinear(nn.Module):
         if w4_group:
             out.w4_group = w4_group
         if out.int8 or w4_group:
-            q, s = pack_weight(lin.weight.detach(), w4_group)
+            q, s = pack_weight(lin.weight.detach(), w4_group, a8)
             out.register_buffer("q", q)
             out.register_buffer("s", s)
             out.weight = None

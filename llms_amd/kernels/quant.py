@@ -56,7 +56,14 @@ def dequantize_w4(q: torch.Tensor, s: torch.Tensor, K: int, *, group: int = 128)
     return (code * s.float().repeat_interleave(group, dim=1)[:, :K]).to(torch.bfloat16)
 
 
-def pack_weight(W: torch.Tensor, w4_group: int) -> tuple[torch.Tensor, torch.Tensor]:
+def pack_weight(W: torch.Tensor, w4_group: int, a8: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, s)`` of a module's weight: 4 bits in groups of ``w4_group``, or int8
-    per row with 0."""
-    return quantize_w4(W, w4_group) if w4_group else quantize_w8_per_row(W)
+    per row with 0. ``a8``: int8 rows at a stride of whole 16 bytes, which the integer
+    products read in their fastest form at any length."""
+    if w4_group:
+        return quantize_w4(W, w4_group)
+    q, s = quantize_w8_per_row(W)
+    K = q.shape[1]
+    if a8 and K % 16:
+        q = torch.nn.functional.pad(q, (0, -K % 16))[:, :K]
+    return q, s

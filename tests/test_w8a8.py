@@ -119,7 +119,7 @@ def test_c_arguments():
     for kw in (dict(M=-1), dict(N=0), dict(K=0), dict(K=(1 << 17) + 1, ldx=1 << 18, ldq=1 << 18),
                dict(N=1 << 23, ldy=1 << 23), dict(M=1 << 24), dict(g=P, eps=-1.0), dict(g=P, eps=float("nan"))):
         assert lin(**kw) == SHAPE, kw
-    for kw in (dict(ldx=63), dict(ldq=63), dict(ldy=95), dict(x=P + 1), dict(s=P + 2), dict(y=P + 1), dict(ldq=1 << 31)):
+    for kw in (dict(ldx=63), dict(ldq=63), dict(ldy=95), dict(x=P + 1), dict(s=P + 2), dict(y=P + 1), dict(ldq=1 << 23)):
         assert lin(**kw) == STRIDE, kw
     for kw in (dict(x=None), dict(q=None), dict(s=None), dict(y=None)):
         assert lin(**kw) == NULL, kw
@@ -138,7 +138,7 @@ SHAPES = [  # M, K, N
     (1, 2541, 970), (5, 2560, 1000), (5, 2541, 97), (8, 128, 64), (9, 129, 65), (16, 9728, 40), (16, 300, 2560),
     (17, 1000, 17), (33, 1024, 129), (64, 4096, 600), (65, 2541, 200), (100, 64, 1000), (128, 256, 256),
     (129, 512, 513), (300, 2541, 970), (300, 2560, 1024), (257, 12288, 96), (1000, 1024, 700), (520, 4096, 3000),
-    (2100, 640, 2600), (7, 20000, 33), (40, 20001, 64), (3, 131072, 10),
+    (2100, 640, 2600), (7, 20000, 33), (40, 20001, 64), (3, 131072, 10), (2, 4360, 40), (1, 12296, 20), (4, 4104, 50), (6, 4264, 30),
 ]
 
 
