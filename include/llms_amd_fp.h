@@ -392,6 +392,53 @@ int fp_kv8_write(const fp_kv8_args* args, void* stream);
 int fp_kv8_read(const fp_kv8_args* args, float* k_out, float* v_out, void* stream);
 
 /*
+ * Attention over a bf16 cache of two parts: a fixed part, positions 0 .. n_fixed - 1, and an own
+ * part, the positions from n_fixed on (no reference counterpart; the reference's cache has one part).
+ *   one fixed part for all sequences (fix_s_b 0, no ring): sequences that continue one text
+ *   ring != 0: the own part holds position p >= n_fixed at (p - n_fixed) % own_len, own_len a
+ *     multiple of 64, and a token at p sees its last `window` positions, p - window + 1 .. p, and the
+ *     fixed ones up to p (T + window - 1 <= own_len). ring 0: position p at p - n_fixed, all seen.
+ *   q, k, v     rows of heads [n_heads or n_kv_heads][head_dim], strides (elements) of a sequence and
+ *               of a token; cos, sin as well ([head_dim] rows; NULL: q and k are normalised and rotated)
+ *   gamma       RMSNorm weights [head_dim] applied before RoPE, or NULL (with cos only)
+ *   fix_*, own_* strides of a sequence, a head and a position; keys and values alike
+ *   y           [B][T][n_heads][head_dim] at y_s_b per sequence
+ *   pos, pos_dev, pos_stride, lengths as in fp_kv8_args
+ * fp_seg_attention writes the new keys and values (of the tokens that there are), then attends with scale
+ * head_dim^-0.5, softmax in fp32. Rows past a sequence's length, or at a position outside the cache (a
+ * ring takes 0 .. 2^30 - 1), are zero and write nothing; an entry that a row does not see has no part
+ * in it, a value that is not finite makes the rows that see it NaN in its column. fp_seg_write only writes
+ * (q, y unused). A text shared by all is not written to: its positions are outside the cache.
+ * head_dim 64 or 128; rows, strides and pointers on 16 bytes (cos, sin: 2); each head's part under 2^31
+ * bytes. workspace: at least fp_seg_workspace_bytes(..., keys, shared, rope), 16-byte aligned, with
+ * keys the positions of the own part that a token may see (own_len; pos + T - n_fixed does where pos is
+ * given and no ring) and shared whether fix_s_b is 0 and there is no ring.
+ */
+typedef struct fp_seg_args {
+  const void *q, *k, *v;
+  int64_t q_s_b, q_s_t, k_s_b, k_s_t, v_s_b, v_s_t;
+  const void *q_gamma, *k_gamma;
+  const void *cos, *sin;
+  int64_t cos_s_b, cos_s_t, sin_s_b, sin_s_t;
+  void *fix_k, *fix_v;
+  int64_t fix_s_b, fix_s_h, fix_s_p;
+  void *own_k, *own_v;
+  int64_t own_s_b, own_s_h, own_s_p;
+  void* y;
+  int64_t y_s_b;
+  int64_t B, T, n_heads, n_kv_heads, head_dim, n_fixed, own_len, ring, window, pos;
+  const int64_t* pos_dev;
+  int64_t pos_stride;
+  const int64_t* lengths;
+  float q_eps, k_eps;
+} fp_seg_args;
+
+int64_t fp_seg_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                               int64_t n_fixed, int64_t keys, int shared, int rope);
+int fp_seg_attention(const fp_seg_args* args, int64_t keys, void* workspace, int64_t workspace_bytes, void* stream);
+int fp_seg_write(const fp_seg_args* args, void* stream);
+
+/*
  * Projections on 4-bit weights with a scale for each group of `group` (32, 64 or
  * 128) inputs (no reference counterpart).
  *   q  [N, ceil(K/2)] bytes, row stride ldq (bytes): byte j holds the codes of inputs

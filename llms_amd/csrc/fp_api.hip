@@ -304,6 +304,51 @@ int check_attention(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
   return FP_OK;
 }
 
+// ---- a cache of two parts ----
+
+// The checks and the kernels' form of such a call: queries (q, y) or only new tokens (k, v).
+int seg_args(const fp_seg_args& g, bool queries, SegArgs* out) {
+  const int64_t D = g.head_dim, F = g.n_fixed, S = g.own_len, Hk = g.n_kv_heads;
+  const int st = check_attention(g.B, g.T, queries ? g.n_heads : Hk, Hk, D);
+  if (st) return st;
+  constexpr int64_t kMost = (int64_t)1 << 28, kLim = (int64_t)1 << 31;
+  if (F < 0 || F > kMost || S < 1 || S > kMost) return FP_ERR_SHAPE;
+  if (g.ring ? g.window < 1 || S % 64 != 0 || g.T + g.window - 1 > S : g.window != 0) return FP_ERR_SHAPE;
+  const int64_t end = g.ring ? (int64_t)1 << 30 : F + S, first = g.ring ? 0 : F;
+  if (!g.pos_dev && (g.pos < first || g.pos > end - g.T)) return FP_ERR_SHAPE;
+  if (g.pos_dev && g.pos_stride != 0 && g.pos_stride != 1) return FP_ERR_STRIDE;
+  if (!(g.q_eps >= 0.f) || !(g.k_eps >= 0.f)) return FP_ERR_SHAPE;
+  if (!g.own_k || !g.own_v || !g.k || !g.v || (F > 0 && (!g.fix_k || !g.fix_v)) || (queries && (!g.q || !g.y)) ||
+      !g.cos != !g.sin || (g.cos && !g.q_gamma != !g.k_gamma))
+    return FP_ERR_NULL;
+  if (g.own_s_p < D || (F > 0 && g.fix_s_p < D) || g.k_s_t < Hk * D || g.v_s_t < Hk * D ||
+      (queries && g.q_s_t < g.n_heads * D) || (g.cos && (g.cos_s_t < D || g.sin_s_t < D)))
+    return FP_ERR_STRIDE;
+  int64_t any = g.own_s_b | g.own_s_h | g.own_s_p | g.k_s_b | g.k_s_t | g.v_s_b | g.v_s_t;
+  if (F > 0) any |= g.fix_s_b | g.fix_s_h | g.fix_s_p;
+  if (queries) any |= g.q_s_b | g.q_s_t | g.y_s_b;
+  if (any < 0 || (any & 7) != 0 || (g.cos && (g.cos_s_b < 0 || g.sin_s_b < 0))) return FP_ERR_STRIDE;
+  if ((S + 64) * g.own_s_p * 2 >= kLim || (F > 0 && (F + 64) * g.fix_s_p * 2 >= kLim)) return FP_ERR_SHAPE;
+  for (const void* p : {g.q, g.k, g.v, (const void*)g.fix_k, (const void*)g.fix_v, (const void*)g.own_k,
+                        (const void*)g.own_v, (const void*)g.y, g.q_gamma, g.k_gamma})
+    if (!al16(p)) return FP_ERR_STRIDE;
+  if (off2(g.cos) || off2(g.sin)) return FP_ERR_STRIDE;
+  SegArgs a{};
+  a.q = (const uint16_t*)g.q, a.k = (const uint16_t*)g.k, a.v = (const uint16_t*)g.v;
+  a.sqb = g.q_s_b, a.sqt = g.q_s_t, a.skb = g.k_s_b, a.skt = g.k_s_t, a.svb = g.v_s_b, a.svt = g.v_s_t;
+  a.gq = (const uint16_t*)g.q_gamma, a.gk = (const uint16_t*)g.k_gamma, a.epsq = g.q_eps, a.epsk = g.k_eps;
+  a.cos = (const uint16_t*)g.cos, a.sin = (const uint16_t*)g.sin;
+  a.scb = g.cos_s_b, a.sct = g.cos_s_t, a.ssb = g.sin_s_b, a.sst = g.sin_s_t;
+  a.fk = (uint16_t*)g.fix_k, a.fv = (uint16_t*)g.fix_v, a.sfb = g.fix_s_b, a.sfh = g.fix_s_h, a.sfs = g.fix_s_p;
+  a.ok = (uint16_t*)g.own_k, a.ov = (uint16_t*)g.own_v, a.sob = g.own_s_b, a.soh = g.own_s_h, a.sos = g.own_s_p;
+  a.y = (uint16_t*)g.y, a.syb = g.y_s_b;
+  a.B = (int)g.B, a.T = (int)g.T, a.Hq = (int)g.n_heads, a.Hk = (int)Hk;
+  a.F = (int)F, a.S = (int)S, a.ring = g.ring != 0, a.W = (int)(g.window < kMost ? g.window : kMost);
+  a.pos = g.pos, a.pos_dev = g.pos_dev, a.pos_stride = g.pos_stride, a.lengths = g.lengths;
+  *out = a;
+  return FP_OK;
+}
+
 // ---- 8-bit cache ----
 
 // The checks and the kernels' form of an 8-bit cache call: new tokens (k, v), queries
@@ -739,6 +784,34 @@ int fp_kv8_read(const fp_kv8_args* g, float* k_out, float* v_out, void* stream) 
   if (!k_out || !v_out) return FP_ERR_NULL;
   if (!fp::al16(k_out) || !fp::al16(v_out)) return FP_ERR_STRIDE;
   return fp::launch_status(fp::launch_kv8_read(a, g->head_dim, k_out, v_out, (hipStream_t)stream));
+}
+
+int64_t fp_seg_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                               int64_t n_fixed, int64_t keys, int shared, int rope) {
+  if (fp::check_attention(B, T, n_heads, n_kv_heads, head_dim) || n_fixed < 0 || keys < 1) return 0;
+  return fp::seg_workspace_bytes(B, T, n_heads, n_kv_heads, head_dim, n_fixed, keys, shared != 0, rope != 0);
+}
+
+int fp_seg_attention(const fp_seg_args* g, int64_t keys, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!g) return FP_ERR_NULL;
+  fp::SegArgs a;
+  const int st = fp::seg_args(*g, true, &a);
+  if (st) return st;
+  if (keys < 1) return FP_ERR_SHAPE;
+  const bool shared = !g->ring && g->n_fixed > 0 && g->fix_s_b == 0;
+  const int64_t need = fp::seg_workspace_bytes(g->B, g->T, g->n_heads, g->n_kv_heads, g->head_dim, g->n_fixed, keys,
+                                               shared, g->cos != nullptr);
+  if (workspace_bytes < need || (need > 0 && !workspace) || !fp::al16(workspace)) return FP_ERR_WORKSPACE;
+  return fp::launch_status(fp::launch_seg_attention(a, g->head_dim, keys, shared, workspace, (hipStream_t)stream));
+}
+
+int fp_seg_write(const fp_seg_args* g, void* stream) {
+  if (!g) return FP_ERR_NULL;
+  fp::SegArgs a;
+  const int st = fp::seg_args(*g, false, &a);
+  if (st) return st;
+  a.cos = a.sin = nullptr;
+  return fp::launch_status(fp::launch_seg_write(a, g->head_dim, (hipStream_t)stream));
 }
 
 int64_t fp_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int gate_up, int norm) {

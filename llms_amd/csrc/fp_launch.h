@@ -294,6 +294,47 @@ int64_t w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gateup);
 // aligned: weight rows on 16 bytes.
 int launch_w8a8(W8A8Args a, bool gateup, bool aligned, void* ws, hipStream_t s);
 
+// Attention over a cache of a fixed part (positions 0 .. F - 1) and an own part (fp_seg.hip).
+// Strides in elements; heads of a row of q, k, v and y lie one behind the other.
+struct SegArgs {
+  const uint16_t *q, *k, *v;
+  int64_t sqb, sqt, skb, skt, svb, svt;  // of a sequence and of a token
+  const uint16_t *gq, *gk;
+  float epsq, epsk;
+  const uint16_t *cos, *sin;  // [T][D], or of each sequence; NULL: q and k come normalised and rotated
+  int64_t scb, sct, ssb, sst;
+  uint16_t *fk, *fv;  // fixed part: of a sequence (0: one for all), of a head, of a position
+  int64_t sfb, sfh, sfs;
+  uint16_t *ok, *ov;  // own part
+  int64_t sob, soh, sos;
+  uint16_t* y;
+  int64_t syb;
+  int B, T, Hq, Hk;
+  int F, S;  // positions in the two parts
+  int ring;  // the own part holds the last S positions, S a multiple of 64
+  int W;     // positions of the own part that a token sees (0: all)
+  int64_t pos;
+  const int64_t* pos_dev;  // sequence b's first position at b * pos_stride; NULL: pos
+  int64_t pos_stride;
+  const int64_t* lengths;  // tokens of each sequence (NULL: T)
+  // set by the launchers: q as the attention kernels read it, and the workspace
+  const uint16_t* qsrc;
+  int64_t sqsb, sqst;
+  uint16_t* qn;
+  float *part, *stat;  // partial sums [planes][Hk][B T G][D] and their {max, sum}
+};
+// How a call's work is cut: items of the fixed part for all sequences together (shared), then of each
+// sequence; planes of partial sums (1: none); row blocks per wave of seg_rows_kernel (rt) and of
+// seg_tiles_kernel where it takes the fixed part (tiles1) or all (tiles2).
+struct SegPlan {
+  int items1, split1, tiles1, items2, split2, tiles2, rt, planes, shared;
+};
+// keys: how many positions of the own part a token may see.
+int64_t seg_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t F, int64_t keys, bool shared,
+                            bool rope);
+int launch_seg_write(const SegArgs& a, int64_t D, hipStream_t s);
+int launch_seg_attention(SegArgs a, int64_t D, int64_t keys, bool shared, void* ws, hipStream_t s);
+
 // Log-probabilities of the rows of logits x [M][V] (fp_logprob.hip).
 struct LogprobArgs {
   const void* x;

@@ -749,6 +749,158 @@ std::vector<int64_t> kv8_layout(int64_t batch, int64_t H, int64_t D, int64_t cac
   return v;
 }
 
+// ---- a cache of two parts ----
+
+// t [B, T, H, D] (or [B, T, H * D]) whose heads lie one behind the other, with strides of a sequence
+// and of a token that the kernels take: a view, or a copy.
+at::Tensor seg_rows(const at::Tensor& t, int64_t n, int64_t* sb, int64_t* st) {
+  const int64_t B = t.size(0), T = t.size(1);
+  const bool heads = t.dim() == 4;
+  const bool inner = t.stride(-1) == 1 && (!heads || t.size(2) == 1 || t.stride(2) == t.size(3));
+  const int64_t lt = T > 1 ? t.stride(1) : n, lb = B > 1 ? t.stride(0) : T * lt;
+  if (!inner || t.is_neg() || lt < n || lt % 8 != 0 || lb < 0 || lb % 8 != 0 || (uintptr_t)t.data_ptr() % 16 != 0) {
+    *st = n, *sb = T * n;
+    // (clone: contiguous() leaves a tensor that is so already, at any address)
+    return (t.is_neg() ? t.resolve_neg() : t).clone(at::MemoryFormat::Contiguous);
+  }
+  *st = lt, *sb = lb;
+  return t;
+}
+
+// One part of a layer's cache, keys and values alike: [B, H, len, D] (or [H, len, D], for all).
+void seg_part(const char* fn, const char* name, const at::Tensor& k, const at::Tensor& v, int64_t B, int64_t* H,
+              int64_t* D, int64_t* len, int64_t* sb, int64_t* sh, int64_t* sp) {
+  TORCH_CHECK(k.sizes() == v.sizes() && k.strides() == v.strides() && k.dim() >= 3 && k.dim() <= 4 &&
+                  k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.device() == v.device() &&
+                  !k.is_neg() && !v.is_neg() && (k.size(-1) == 1 || k.stride(-1) == 1),
+              fn, ": the ", name, " keys and values must be alike, bfloat16, (.., heads, positions, D)");
+  if (k.dim() == 4) TORCH_CHECK_VALUE(B <= k.size(0), fn, ": ", B, " sequences, the cache holds ", k.size(0));
+  *H = k.size(-3), *len = k.size(-2), *D = k.size(-1);
+  *sb = k.dim() == 4 && k.size(0) > 1 ? k.stride(0) : 0;
+  *sh = k.stride(-3), *sp = k.size(-2) > 1 ? k.stride(-2) : k.size(-1);
+}
+
+struct SegCall {
+  fp_seg_args a;
+  at::Tensor k, v;  // held until the launch
+};
+
+// What a write and an attention over such a cache have in common.
+SegCall seg_call(const char* fn, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& fix_k,
+                 const at::Tensor& fix_v, const at::Tensor& own_k, const at::Tensor& own_v, int64_t window,
+                 int64_t start_pos, const c10::optional<at::Tensor>& pos, const c10::optional<at::Tensor>& lengths) {
+  SegCall c{};
+  fp_seg_args& a = c.a;
+  TORCH_CHECK_VALUE(k_.dim() >= 3 && k_.sizes() == v_.sizes(), fn, ": k ", k_.sizes(), " and v ", v_.sizes(),
+                    " must be (B, T, n_kv_heads, D)");
+  const int64_t B = k_.size(0), T = k_.size(1);
+  int64_t H = 0, D = 0, fh = 0, fd = 0;
+  seg_part(fn, "own", own_k, own_v, B, &H, &D, &a.own_len, &a.own_s_b, &a.own_s_h, &a.own_s_p);
+  seg_part(fn, "fixed", fix_k, fix_v, B, &fh, &fd, &a.n_fixed, &a.fix_s_b, &a.fix_s_h, &a.fix_s_p);
+  TORCH_CHECK(fh == H && fd == D && own_k.dim() == 4 && own_k.device() == fix_k.device(), fn,
+              ": the cache's parts do not fit together");
+  TORCH_CHECK_VALUE(k_.numel() == B * T * H * D && (k_.dim() == 3 || (k_.dim() == 4 && k_.size(2) == H)), fn, ": k ",
+                    k_.sizes(), " and v ", v_.sizes(), " must be (B, T, ", H, ", ", D, ")");
+  type_is(k_, at::kBFloat16, fn, "k");
+  type_is(v_, at::kBFloat16, fn, "v");
+  value_same(k_, v_, fn, "k", "v");
+  value_same(k_, own_k, fn, "k", "the cache");
+  const auto place = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && (t.dim() == 0 || (t.dim() == 1 && t.size(0) == B)), fn, ": ",
+                      name, " must be an int64 tensor of ", B, " elements, got ", py_name(t.scalar_type()), " ",
+                      t.sizes());
+    TORCH_CHECK_VALUE(t.device() == own_k.device() && t.is_contiguous(), fn, ": ", name, " must be contiguous on ",
+                      own_k.device());
+  };
+  if (pos.has_value()) {
+    place(*pos, "start_pos");
+    a.pos_dev = pos->data_ptr<int64_t>();
+    a.pos_stride = pos->dim();
+  } else {
+    const int64_t first = window ? 0 : a.n_fixed, end = window ? (int64_t)1 << 30 : a.n_fixed + a.own_len;
+    TORCH_CHECK_VALUE(start_pos >= first && start_pos <= end - T, fn, ": positions ", start_pos, " .. ",
+                      start_pos + T - 1, " are outside ", first, " .. ", end - 1);
+    a.pos = start_pos;
+  }
+  if (lengths.has_value()) {
+    place(*lengths, "lengths");
+    TORCH_CHECK_VALUE(lengths->dim() == 1, fn, ": lengths must be an int64 tensor of ", B, " elements");
+    a.lengths = lengths->data_ptr<int64_t>();
+  }
+  value_device(own_k, fn, "the cache");
+  c.k = seg_rows(k_, H * D, &a.k_s_b, &a.k_s_t), c.v = seg_rows(v_, H * D, &a.v_s_b, &a.v_s_t);
+  a.k = c.k.data_ptr(), a.v = c.v.data_ptr();
+  a.fix_k = fix_k.data_ptr(), a.fix_v = fix_v.data_ptr(), a.own_k = own_k.data_ptr(), a.own_v = own_v.data_ptr();
+  a.B = B, a.T = T, a.n_heads = H, a.n_kv_heads = H, a.head_dim = D, a.ring = window > 0, a.window = window;
+  return c;
+}
+
+at::Tensor attention_seg(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+                         const c10::optional<at::Tensor>& q_gamma, const c10::optional<at::Tensor>& k_gamma,
+                         double q_eps, double k_eps, const c10::optional<at::Tensor>& cos,
+                         const c10::optional<at::Tensor>& sin, at::Tensor fix_k, at::Tensor fix_v, at::Tensor own_k,
+                         at::Tensor own_v, int64_t window, int64_t start_pos, const c10::optional<at::Tensor>& pos,
+                         const c10::optional<at::Tensor>& lengths) {
+  const char* fn = window ? "attention_window" : "attention_shared";
+  const c10::DeviceGuard guard(k_.device());
+  SegCall c = seg_call(fn, k_, v_, fix_k, fix_v, own_k, own_v, window, start_pos, pos, lengths);
+  fp_seg_args& a = c.a;
+  const int64_t B = a.B, T = a.T, D = a.head_dim;
+  TORCH_CHECK_VALUE(q_.dim() == k_.dim() && q_.size(0) == B && q_.size(1) == T &&
+                        (q_.dim() == 3 ? q_.size(2) % D == 0 : q_.size(3) == D),
+                    fn, ": q ", q_.sizes(), " must be (", B, ", ", T, ", heads, ", D, ")");
+  const int64_t n = q_.dim() == 3 ? q_.size(2) : q_.size(2) * D, H = n / D;
+  TORCH_CHECK_VALUE(H >= 1 && H % a.n_kv_heads == 0, fn, ": ", H, " query heads are no multiple of ", a.n_kv_heads,
+                    " kv heads");
+  type_is(q_, at::kBFloat16, fn, "q");
+  value_same(k_, q_, fn, "k", "q");
+  at::Tensor y = at::empty(q_.sizes(), q_.options());
+  if (B == 0 || T == 0) return y;
+  const at::Tensor q = seg_rows(q_, n, &a.q_s_b, &a.q_s_t);
+  a.q = q.data_ptr(), a.n_heads = H, a.y = y.data_ptr(), a.y_s_b = T * n;
+  if (cos.has_value()) {
+    const auto row = [&](const c10::optional<at::Tensor>& t, const char* name) -> const void* {
+      if (!t.has_value()) return nullptr;
+      TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->device() == q.device() && !t->is_neg() && t->dim() == 1 &&
+                      t->size(0) == D && t->stride(0) == 1,
+                  name, " has the wrong type, device, shape or stride");
+      return t->data_ptr();
+    };
+    const auto table = [&](const c10::optional<at::Tensor>& t, int64_t* sb, int64_t* st, const char* name) -> const void* {
+      TORCH_CHECK(t.has_value() && t->scalar_type() == at::kBFloat16 && t->device() == q.device() && !t->is_neg() &&
+                      (t->dim() == 2 || (t->dim() == 3 && t->size(0) == B)) && t->size(-2) == T && t->size(-1) == D &&
+                      t->stride(-1) == 1,
+                  name, " has the wrong type, device, shape or stride");
+      *sb = t->dim() == 3 && B > 1 ? t->stride(0) : 0;
+      *st = T > 1 ? t->stride(-2) : D;
+      return t->data_ptr();
+    };
+    a.q_gamma = row(q_gamma, "q_gamma"), a.k_gamma = row(k_gamma, "k_gamma");
+    a.cos = table(cos, &a.cos_s_b, &a.cos_s_t, "cos"), a.sin = table(sin, &a.sin_s_b, &a.sin_s_t, "sin");
+    a.q_eps = (float)q_eps, a.k_eps = (float)k_eps;
+  }
+  // what a token may see of the own part (at a device position: as much as there may be)
+  int64_t keys = window ? (window < a.own_len ? window : a.own_len) : a.own_len;
+  if (!a.pos_dev && start_pos + T - a.n_fixed < keys) keys = start_pos + T - a.n_fixed;
+  if (keys < 1) keys = 1;
+  const int shared = !window && a.n_fixed > 0 && a.fix_s_b == 0;
+  const int64_t bytes = fp_seg_workspace_bytes(B, T, H, a.n_kv_heads, D, a.n_fixed, keys, shared, a.cos != nullptr);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  check_status(fp_seg_attention(&a, keys, bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(q)), "fp_seg_attention");
+  return y;
+}
+
+void write_seg(const at::Tensor& k_, const at::Tensor& v_, at::Tensor fix_k, at::Tensor fix_v, at::Tensor own_k,
+               at::Tensor own_v, int64_t window, int64_t start_pos, const c10::optional<at::Tensor>& pos,
+               const c10::optional<at::Tensor>& lengths) {
+  const char* fn = window ? "KVCacheWindow.write" : "KVCacheShared.write";
+  const c10::DeviceGuard guard(k_.device());
+  const SegCall c = seg_call(fn, k_, v_, fix_k, fix_v, own_k, own_v, window, start_pos, pos, lengths);
+  if (c.a.B == 0 || c.a.T == 0) return;
+  check_status(fp_seg_write(&c.a, cur_stream(c.k)), fn);
+}
+
 // ---- log-probabilities of tokens ----
 
 // x [.., V], tokens [..]: {logprob [..], entropy [..], top_ids [.., k], top_logprobs [.., k]}.
@@ -795,6 +947,8 @@ void low_bit(torch::Library& m) {
   m.impl("attention_kv8", attention_kv8);
   m.impl("write_kv8", write_kv8);
   m.impl("read_kv8", read_kv8);
+  m.impl("attention_seg", attention_seg);
+  m.impl("write_seg", write_seg);
   m.impl("token_logprobs", token_logprobs);
 }
 
@@ -823,6 +977,11 @@ TORCH_LIBRARY(llms_amd, m) {
         "Tensor? lengths) -> ()");
   m.def("read_kv8(Tensor cache, int[] size, int B, int T, int start_pos, Tensor? pos) -> "
         "(Tensor, Tensor)");
+  m.def("attention_seg(Tensor q, Tensor k, Tensor v, Tensor? q_gamma, Tensor? k_gamma, float q_eps, "
+        "float k_eps, Tensor? cos, Tensor? sin, Tensor(a!) fix_k, Tensor(b!) fix_v, Tensor(c!) own_k, "
+        "Tensor(d!) own_v, int window, int start_pos, Tensor? pos, Tensor? lengths) -> Tensor");
+  m.def("write_seg(Tensor k, Tensor v, Tensor(a!) fix_k, Tensor(b!) fix_v, Tensor(c!) own_k, Tensor(d!) own_v, "
+        "int window, int start_pos, Tensor? pos, Tensor? lengths) -> ()");
   m.def("kv8_layout(int batch, int heads, int D, int cache_len) -> int[]", kv8_layout);
   m.def("linear_w4(Tensor x, Tensor? gamma, float eps, Tensor q, Tensor scale, int group) -> Tensor");
   m.def("gate_up_silu_w4(Tensor x, Tensor? gamma, float eps, Tensor qg, Tensor sg, Tensor qu, "

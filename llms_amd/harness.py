@@ -40,6 +40,7 @@ from .kernels._eager import RMSNorm, apply_rope, attend, build_rope_tables, writ
 from .kernels.fused_norm import fused_rmsnorm_head
 from .kernels.kv8 import BLOCK as KV8_BLOCK, KVCache8
 from .kernels.logprobs import TokenLogprobs, token_logprobs
+from .kernels.seg import KVCacheShared, KVCacheWindow
 
 
 @dataclass(frozen=True)
@@ -86,8 +87,8 @@ class Attention(nn.Module):
         self.k_norm = RMSNorm(c.head_dim, eps=c.rms_norm_eps)
 
     def forward(self, x, *, kv_cache, layer_idx, cos, sin, start_pos):
-        if isinstance(kv_cache, KVCache8):
-            raise TypeError("an 8-bit cache needs the fused attention: apply_triton_kernels(model) first")
+        if isinstance(kv_cache, (KVCache8, KVCacheShared, KVCacheWindow)):
+            raise TypeError(f"a {type(kv_cache).__name__} needs the fused attention: apply_triton_kernels(model) first")
         B, T, _ = x.shape
         q = self.q(x).view(B, T, self.num_heads, self.head_dim)
         k = self.k(x).view(B, T, self.num_kv_heads, self.head_dim)
@@ -145,11 +146,18 @@ class Qwen3Model(nn.Module):
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
 
-    def alloc_cache(self, max_seq_len: int, *, max_batch: int = 1, kv8: bool = False) -> KVCache | KVCache8:
-        """A cache for up to ``max_batch`` sequences; ``kv8``: in 8 bits (a swapped
-        model on a HIP device)."""
+    def alloc_cache(self, max_seq_len: int, *, max_batch: int = 1, kv8: bool = False, window: int = 0,
+                    sinks: int = 4) -> KVCache | KVCache8 | KVCacheWindow:
+        """A cache for up to ``max_batch`` sequences; ``kv8``: in 8 bits, ``window``: of the last
+        ``window`` tokens and the first ``sinks``, whatever ``max_seq_len`` (both: a swapped model
+        on a HIP device)."""
         c = self.cfg
         w = self.embed.weight
+        if window:
+            if kv8:
+                raise ValueError("alloc_cache: window and kv8 exclude each other")
+            return KVCacheWindow.alloc(c.num_hidden_layers, window, sinks=sinks, max_batch=max_batch,
+                                       n_kv_heads=c.num_key_value_heads, head_dim=c.head_dim, device=w.device)
         if kv8:
             return KVCache8.alloc(c.num_hidden_layers, max_seq_len, max_batch=max_batch,
                                   n_kv_heads=c.num_key_value_heads, head_dim=c.head_dim, device=w.device)
@@ -161,15 +169,17 @@ class Qwen3Model(nn.Module):
     def forward(self, input_ids, kv_cache, start_pos=None):
         """Logits for ``input_ids`` [B, T] at positions start_pos ..; an int
         start_pos (default ``kv_cache.cur_len``) advances ``cur_len``, a 0-dim
-        device tensor (graph mode) leaves it to the caller."""
+        device tensor (graph mode) leaves it to the caller, as one of [B] positions
+        does (sequences of different lengths; a ``KVCacheShared`` or ``KVCacheWindow``)."""
         if start_pos is None:
             start_pos = kv_cache.cur_len
         T = input_ids.shape[1]
         h = self.embed(input_ids)
         if torch.is_tensor(start_pos):
-            rows = start_pos + torch.arange(T, device=input_ids.device)
-            cos = self.rope_cos.index_select(0, rows)
-            sin = self.rope_sin.index_select(0, rows)
+            if start_pos.dim() and not isinstance(kv_cache, (KVCacheShared, KVCacheWindow)):
+                raise TypeError(f"positions of each sequence over a {type(kv_cache).__name__}: one is taken for all")
+            rows = start_pos[..., None] + torch.arange(T, device=input_ids.device)
+            cos, sin = (t.index_select(0, rows.flatten()).view(*rows.shape, -1) for t in (self.rope_cos, self.rope_sin))
         else:
             cos = self.rope_cos[start_pos:start_pos + T]
             sin = self.rope_sin[start_pos:start_pos + T]
@@ -235,10 +245,10 @@ def random_model(c: Cfg, *, device="cuda", seed: int = 0, dtype=torch.bfloat16) 
 
 
 def greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device, *,
-                    kv8: bool = False) -> list[int]:
+                    kv8: bool = False, window: int = 0) -> list[int]:
     """Prefill the prompt, then decode n_new tokens one at a time (argmax)."""
     ids = torch.tensor([prompt], dtype=torch.long, device=device)
-    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8)
+    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8, window=window)
     out: list[int] = []
     with torch.inference_mode():
         logits = model(ids, cache, start_pos=0)
@@ -288,16 +298,21 @@ class StepGraph:
     the last T positions of the cache, so callers keep those free. (In an 8-bit
     cache they would displace the unfinished block, which is put back. A verify step over
     one whose tokens end a block answers for those before its end from the 8-bit block, with the
-    later drafts in its scale.)"""
+    later drafts in its scale. In a ``KVCacheShared`` or ``KVCacheWindow`` what they write is put back;
+    with ``per_sequence`` ``pos`` is then a tensor of a position for each sequence.)"""
 
-    def __init__(self, model: Qwen3Model, cache: KVCache, T: int = 1, batch: int = 1):
+    def __init__(self, model: Qwen3Model, cache: KVCache, T: int = 1, batch: int = 1, per_sequence: bool = False):
         dev = model.embed.weight.device
         self.model, self.cache, self.T = model, cache, T
         self.ids = torch.zeros((batch, T), dtype=torch.long, device=dev)
-        kv8 = isinstance(cache, KVCache8)
-        seq = cache.max_seq if kv8 else cache.k[0].shape[2]
-        self.pos = torch.full((), seq - T, dtype=torch.long, device=dev)
-        kept = cache.tails() if kv8 else []
+        kept = []
+        if isinstance(cache, (KVCacheShared, KVCacheWindow)):
+            at, kept = cache.step_slots(T)
+        elif isinstance(cache, KVCache8):
+            at, kept = cache.max_seq - T, cache.tails()
+        else:
+            at = cache.k[0].shape[2] - T
+        self.pos = torch.full((batch,) if per_sequence else (), at, dtype=torch.long, device=dev)
         saved = [t.clone() for t in kept]
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
@@ -314,19 +329,21 @@ class StepGraph:
             self.logits = model(self.ids, cache, start_pos=self.pos)
         torch.cuda.synchronize(dev)
 
-    def __call__(self, ids: torch.Tensor, pos: int) -> torch.Tensor:
+    def __call__(self, ids: torch.Tensor, pos) -> torch.Tensor:
         self.ids.copy_(ids)
-        self.pos.fill_(pos)
+        self.pos.copy_(pos) if torch.is_tensor(pos) else self.pos.fill_(pos)
         self.graph.replay()
         return self.logits
 
 
 def graph_greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device, *,
-                          kv8: bool = False) -> list[int]:
+                          kv8: bool = False, window: int = 0) -> list[int]:
     """``greedy_generate`` with every decode step replayed from one captured
     ``StepGraph`` (the prefill runs eagerly)."""
     ids = torch.tensor([prompt], dtype=torch.long, device=device)
-    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8)
+    if window and len(prompt) + n_new > model.cfg.max_position_embeddings:
+        raise ValueError(f"{len(prompt) + n_new} positions, the model has {model.cfg.max_position_embeddings}")
+    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8, window=window)
     with torch.inference_mode():
         logits = model(ids, cache, start_pos=0)
     step = StepGraph(model, cache, T=1)
@@ -338,3 +355,34 @@ def graph_greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, devi
         out.append(int(nt.item()))
         pos += 1
     return out
+
+
+def batch_generate(model: Qwen3Model, text: list[int], continuations: list[list[int]], n_new: int, device, *,
+                   graph: bool = False) -> list[list[int]]:
+    """Greedy decoding of several continuations of one text (questions about a document, chats under one system
+    text): the text is fed once and its keys and values are shared, the continuations (of one token at
+    least, any lengths) are fed together, then ``n_new`` tokens of each decoded in steps of the batch, replayed
+    from one ``StepGraph`` with ``graph``. A swapped model on a HIP device. Returns the new tokens of each."""
+    if not text or not continuations or not all(continuations) or n_new < 1:
+        raise ValueError("batch_generate: a text, continuations of at least one token each and n_new >= 1 are needed")
+    B, P, longest = len(continuations), len(text), max(map(len, continuations))
+    if P + longest + n_new > model.cfg.max_position_embeddings:
+        raise ValueError(f"batch_generate: {P + longest + n_new} positions, the model has "
+                         f"{model.cfg.max_position_embeddings}")
+    count = torch.tensor([len(c) for c in continuations], device=device)
+    ids = torch.tensor([c + [0] * (longest - len(c)) for c in continuations], dtype=torch.long, device=device)
+    with torch.inference_mode():
+        plain = model.alloc_cache(P)
+        model(torch.tensor([text], dtype=torch.long, device=device), plain, start_pos=0)
+        cache = KVCacheShared.of(plain, P, max_batch=B, max_new=longest + n_new)
+        # (what the padding leaves behind a sequence is overwritten before any token sees it)
+        logits = model(ids, cache)
+        nt = logits[torch.arange(B, device=device), count - 1].argmax(-1, keepdim=True)
+        out, pos = [nt], P + count
+        step = StepGraph(model, cache, batch=B, per_sequence=True) if graph and n_new > 1 else None
+        for _ in range(n_new - 1):
+            logits = step(nt, pos) if step else model(nt, cache, start_pos=pos)
+            nt = logits[:, -1].argmax(-1, keepdim=True)
+            out.append(nt)
+            pos = pos + 1
+    return torch.cat(out, 1).tolist()

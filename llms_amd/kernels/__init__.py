@@ -13,6 +13,7 @@ from .linear import FusedLinear, fused_linear, fused_linear_w8
 from .kv8 import KVCache8, attention_kv8
 from .logprobs import TokenLogprobs, token_logprobs
 from .quant import dequantize_w4, dequantize_w8, quantize_w4, quantize_w8_per_row
+from .seg import KVCacheShared, KVCacheWindow, attention_shared, attention_window
 from .swap import apply_triton_kernels, prewarm_triton_kernels
 from .w4 import (fused_gate_up_silu_w4, fused_linear_w4, fused_qkv_w4, fused_rmsnorm_gate_up_silu_w4,
                  fused_rmsnorm_qkv_w4)
@@ -37,6 +38,10 @@ __all__ = [
     "fused_gate_up_silu",
     "fused_qkv_w8",
     "fused_gate_up_silu_w8",
+    "KVCacheShared",
+    "KVCacheWindow",
+    "attention_shared",
+    "attention_window",
     "fused_linear_w8a8",
     "fused_qkv_w8a8",
     "fused_gate_up_silu_w8a8",

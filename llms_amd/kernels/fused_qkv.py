@@ -20,6 +20,7 @@ from ._eager import RMSNorm, apply_rope, attend, write_kv
 from .fused_attention import attention_core
 from .kv8 import KVCache8, attention_core_kv8
 from .quant import pack_weight
+from .seg import KVCacheShared, KVCacheWindow, attention_core_seg
 from .w4 import fused_qkv_w4, fused_rmsnorm_qkv_w4
 from .w8a8 import fused_qkv_w8a8, fused_rmsnorm_qkv_w8a8
 
@@ -136,7 +137,9 @@ class TritonAttention(nn.Module):
     (:func:`~llms_amd.kernels.fused_attention.attention_core`) in bf16
     inference, else eagerly (:func:`attend`, fp32 softmax attention with the
     reference's causal semantics); ``o`` is the module's own Linear. With a
-    :class:`~llms_amd.kernels.kv8.KVCache8` as its cache it attends over that, on HIP
+    :class:`~llms_amd.kernels.kv8.KVCache8`,
+    :class:`~llms_amd.kernels.seg.KVCacheShared` or
+    :class:`~llms_amd.kernels.seg.KVCacheWindow` as its cache it attends over that, on HIP
     kernels only.
 
     With ``from_eager(..., int8=True)`` the stacked weight is kept as
@@ -259,6 +262,10 @@ class TritonAttention(nn.Module):
         q_flat, k_flat, v_flat = self.project(x)
         if isinstance(kv_cache, KVCache8):
             return self.o(attention_core_kv8(q_flat, k_flat, v_flat, q_norm=self.q_norm, k_norm=self.k_norm,
+                                             num_heads=self.num_heads, cache=kv_cache, layer=layer_idx,
+                                             cos=cos, sin=sin, start_pos=start_pos))
+        if isinstance(kv_cache, (KVCacheShared, KVCacheWindow)):
+            return self.o(attention_core_seg(q_flat, k_flat, v_flat, q_norm=self.q_norm, k_norm=self.k_norm,
                                              num_heads=self.num_heads, cache=kv_cache, layer=layer_idx,
                                              cos=cos, sin=sin, start_pos=start_pos))
         attn = attention_core(q_flat, k_flat, v_flat, q_norm=self.q_norm, k_norm=self.k_norm,
