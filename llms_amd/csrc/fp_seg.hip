@@ -30,9 +30,20 @@
 #include "fp_launch.h"
 #include "fp_rope.h"
 
+#include <type_traits>
+
 namespace fp {
 
 namespace {
+
+// f(0), f(1), .. f(N - 1) with constants, so that what they index stays in registers.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
+}
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -127,17 +138,27 @@ __device__ __forceinline__ void take_nonfinite8(u32x4& v, u32x4& bad) {
   }
 }
 
-// A operand of V^T for d block dt and keys {4g .. 4g+3, 16 + 4g ..} of 32 V rows in LDS (row
-// stride D * 2 bytes, 16-byte chunk c of row r at c ^ (r & (D / 8 - 1))).
+// Where 16-byte chunk c of key (value) row r lies in the row's D * 2 bytes of LDS: at c ^ swk (swv). Half a
+// wave's lanes of one read then meet every bank once: 16 rows of a chunk of the keys, 8 rows of a pair of
+// chunks of the values. (With c ^ r for both, two rows of each pair met: half of the LDS cycles were conflicts.)
+template <int D>
+__device__ __forceinline__ int swk(int r) {
+  return D == 128 ? r & 15 : (r >> 1) & 7;
+}
+template <int D>
+__device__ __forceinline__ int swv(int r) {
+  return D == 128 ? (r & 7) * 2 : ((r >> 1) & 3) * 2;
+}
+
+// A operand of V^T for d block dt and keys {4g .. 4g+3, 16 + 4g ..} of 32 V rows in LDS.
 template <int D>
 __device__ __forceinline__ u32x4 read_vt(const char* rows, int dt, int li, int grp) {
-  constexpr int CM = D / 8 - 1;
   const int key = 4 * grp + (li >> 2), c = 2 * dt + ((li & 3) >> 1), half = (li & 1) * 8;
   u32x4 out;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const int r = key + 16 * s;
-    const char* p = rows + r * (D * 2) + ((c ^ (r & CM)) * 16) + half;
+    const char* p = rows + r * (D * 2) + ((c ^ swv<D>(r)) * 16) + half;
     const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)p));
     out[2 * s] = w.x;
     out[2 * s + 1] = w.y;
@@ -188,6 +209,7 @@ __device__ __forceinline__ RowKeys row_keys(const SegArgs& a, int p) {
 struct Item {
   int b, kh, row0, rows;  // rows: of the kv head in all
   int nf, c0, lo, hi;
+  int ring, at;           // blocks of the ring (or more than there are), and the place of block c0 in it
   int plane;              // of the partial sums
   bool packed;
 };
@@ -221,9 +243,18 @@ __device__ __forceinline__ void item_keys(const SegArgs& a, Item& it, int n, boo
       }
     }
   }
+  it.ring = a.ring ? a.S / KB : 1 << 30;
+  it.at = it.c0 % it.ring;
   const int per = (total + nsplit - 1) / nsplit;
   it.lo = s * per;
   it.hi = it.lo + per < total ? it.lo + per : total;
+}
+
+// Where block c lies in its part. (An item's own blocks span the ring at most, and one more.)
+__device__ __forceinline__ int place(const Item& it, int c) {
+  if (c < it.nf) return c;
+  const int x = it.at + c - it.nf;
+  return x < it.ring ? x : x - it.ring;
 }
 
 // q row r of an item (clamped; rows past the last are not stored).
@@ -270,31 +301,37 @@ struct State {
       for (int dt = 0; dt < D / 16; ++dt) o[dt][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
-  // Scores s (NB blocks of 16 keys) of row block rt into probabilities about the reference.
+  // Raises the references where the scores s (NB blocks of 16 keys) pass them.
   template <int NB>
-  __device__ __forceinline__ void softmax(f32x4 (&s)[NB], int rt, float sc) {
-    float m = -INFINITY;
+  __device__ __forceinline__ void follow(const f32x4 (&s)[RT][NB], float sc) {
+    float m[RT];
+    bool up = false;
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) m = fmaxf(m, s[n][r]);
-    if (__any(m * sc > mx[rt] + kLift)) {
-      const float mn = fmaxf(mx[rt], col_max(m) * sc);
-      const float al = mn == -INFINITY ? 1.f : exp2_fast(mx[rt] - mn);
-      mx[rt] = mn;
-      sum[rt] *= al;
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) o[dt][rt] *= al;
+        for (int r = 0; r < 4; ++r) m[rt] = fmaxf(m[rt], s[rt][n][r]);
+      up |= m[rt] * sc > mx[rt] + kLift;
     }
-    const float base = mx[rt] == -INFINITY ? 0.f : mx[rt];
+    if (__any(up)) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+      for (int rt = 0; rt < RT; ++rt) {
+        const float mn = fmaxf(mx[rt], col_max(m[rt]) * sc);
+        const float al = mn == -INFINITY ? 1.f : exp2_fast(mx[rt] - mn);
+        mx[rt] = mn;
+        sum[rt] *= al;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[n][r] = exp2_fast(fmaf(s[n][r], sc, -base));
+        for (int dt = 0; dt < D / 16; ++dt) o[dt][rt] *= al;
+      }
+    }
   }
-  // Whether an infinity or a NaN is in any sum (of values: rows' own scores leave theirs in sum as well).
+  // Whether an infinity or a NaN is in any sum.
   __device__ __forceinline__ bool nonfinite() const {
     float t = 0.f;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) t = fmaf(sum[rt][0], 0.f, t);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -370,16 +407,16 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
   const int bytes[2] = {a.F > 0 ? (int)(((int64_t)(a.F - 1) * a.sfs + D) * 2) : 0,
                         (int)(((int64_t)(a.S - 1) * a.sos + D) * 2)};
   const uint32_t step[2] = {(uint32_t)(a.sfs * 2), (uint32_t)(a.sos * 2)};
-  const int vr = lane / CH, ring = a.ring ? a.S / KB : 1 << 30;
+  const int vr = lane / CH;
   auto issue = [&](u32x4 (&kf)[2][DK], char* sv, int c) {
     const int own = c < it.nf ? 0 : 1;
-    const int blk = own ? (it.c0 + c - it.nf) % ring : c;
+    const int blk = place(it, c);
     const uint32_t st = step[own];
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int r = n * RPI + vr;
       load_lds16(vb[own], bytes[own], (lds_ptr_t)(sv + n * 1024),
-                 (uint32_t)(blk * KB + r) * st + (uint32_t)(((lane % CH) ^ (r & (CH - 1))) * 16));
+                 (uint32_t)(blk * KB + r) * st + (uint32_t)(((lane % CH) ^ swv<D>(r)) * 16));
     }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -427,7 +464,15 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
         split_p<1>(t[0], t[1], f);
         seen[rt] = f[0];
       }
-      S.softmax(s[rt], rt, sc);
+    }
+    S.follow(s, sc);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float base = S.mx[rt] == -INFINITY ? 0.f : S.mx[rt];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[rt][kt][r] = exp2_fast(fmaf(s[rt][kt][r], sc, -base));
       split_p<PARTS>(s[rt][0], s[rt][1], pf[rt]);
 #pragma unroll
       for (int c2 = 0; c2 < PARTS; ++c2) S.sum[rt] = mfma16(ones8(), pf[rt][c2], S.sum[rt]);
@@ -530,9 +575,9 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
 // loads in flight while one is computed.
 // Items: ranges x row tiles (of one sequence, or of all where only a shared fixed part is read) with the kv
 // head fastest, so that one XCD runs a head's tiles.
-template <int D, int RT, int PARTS>
-__global__ __launch_bounds__(256, 2) void seg_tiles_kernel(SegArgs a, SegPlan pl) {
-  constexpr int NW = 4, KB = 64;
+template <int D, int RT, int PARTS, int NW>
+__global__ __launch_bounds__(NW * kWave, NW == 4 ? 2 : 1) void seg_tiles_kernel(SegArgs a, SegPlan pl) {
+  constexpr int KB = 64;
   constexpr int DK = D / 32, DT = D / 16;
   constexpr int RPI = 1024 / (D * 2);          // rows per load instruction
   constexpr int NL = KB / RPI / NW;            // load instructions per wave of a tile's keys
@@ -558,11 +603,12 @@ __global__ __launch_bounds__(256, 2) void seg_tiles_kernel(SegArgs a, SegPlan pl
     id /= a.B;
   }
   it.rows = (it.packed ? a.B : 1) * a.T * G;
-  const int n_rt = (it.rows + 64 * RT - 1) / (64 * RT);
-  const int tile = n_rt - 1 - id % n_rt;  // (the later tokens of a prompt see more)
+  constexpr int ROWS = NW * 16 * RT;
+  const int n_rt = (it.rows + ROWS - 1) / ROWS;
+  const int rtile = n_rt - 1 - id % n_rt;  // (the later tokens of a prompt see more)
   it.plane = id / n_rt;
-  it.row0 = tile * 64 * RT;
-  item_keys<KB>(a, it, 64 * RT, true, !it.packed, it.plane, it.packed ? pl.split1 : pl.split2);
+  it.row0 = rtile * ROWS;
+  item_keys<KB>(a, it, ROWS, true, !it.packed, it.plane, it.packed ? pl.split1 : pl.split2);
   const int row0 = it.row0 + wave * 16 * RT;  // this wave's first row
 
   u32x4 qf[RT][DK];
@@ -581,97 +627,155 @@ __global__ __launch_bounds__(256, 2) void seg_tiles_kernel(SegArgs a, SegPlan pl
   const int row1 = row0 + 16 * RT - 1;
   const RowKeys last = row_keys(a, row_pos(a, it, row1 < it.rows ? row1 : it.rows - 1, p0));
 
-  const uint16_t* const kb[2] = {a.fk + it.b * a.sfb + it.kh * a.sfh, a.ok + it.b * a.sob + it.kh * a.soh};
-  const uint16_t* const vb[2] = {a.fv + it.b * a.sfb + it.kh * a.sfh, a.ov + it.b * a.sob + it.kh * a.soh};
+  const uint16_t *const fk = a.fk + it.b * a.sfb + it.kh * a.sfh, *const ok = a.ok + it.b * a.sob + it.kh * a.soh;
+  const uint16_t *const fv = a.fv + it.b * a.sfb + it.kh * a.sfh, *const ov = a.ov + it.b * a.sob + it.kh * a.soh;
   const int bytes[2] = {a.F > 0 ? (int)(((int64_t)(a.F - 1) * a.sfs + D) * 2) : 0,
                         (int)(((int64_t)(a.S - 1) * a.sos + D) * 2)};
-  const int ring = a.ring ? a.S / KB : 1 << 30;
-  uint32_t off[2][NL];
+  const uint32_t step[2] = {(uint32_t)(a.sfs * 2), (uint32_t)(a.sos * 2)};
+  // this lane's row of a tile's first load instruction, and its chunks of keys and of values in each
+  const uint32_t row = (uint32_t)(wave * NL * RPI + lane / CH);
+  uint32_t chk[NL], chv[NL];
 #pragma unroll
   for (int n = 0; n < NL; ++n) {
-    const int r = (wave * NL + n) * RPI + lane / CH;
-    const uint32_t ch = (uint32_t)(((lane % CH) ^ (r & (CH - 1))) * 16);
-    off[0][n] = (uint32_t)r * (uint32_t)(a.sfs * 2) + ch;
-    off[1][n] = (uint32_t)r * (uint32_t)(a.sos * 2) + ch;
+    const int r = (int)row + n * RPI;
+    chk[n] = (uint32_t)(((lane % CH) ^ swk<D>(r)) * 16);
+    chv[n] = (uint32_t)(((lane % CH) ^ swv<D>(r)) * 16);
   }
   // each tile's rows through a buffer that starts at the tile and ends with the part's last row, so
   // that the lane offset alone tells whether a row is past it
-  auto issue = [&](char* sk, char* sv, int c) {
-    const int own = c < it.nf ? 0 : 1;
-    const int blk = own ? (it.c0 + c - it.nf) % ring : c;
-    const int skip = (int)((uint32_t)(blk * KB) * (uint32_t)((own ? a.sos : a.sfs) * 2));
-#pragma unroll
-    for (int n = 0; n < NL; ++n) {
-      const uint32_t o = own ? off[1][n] : off[0][n];
-      load_lds16((const char*)kb[own] + skip, bytes[own] - skip, (lds_ptr_t)(sk + (wave * NL + n) * 1024), o);
-      load_lds16((const char*)vb[own] + skip, bytes[own] - skip, (lds_ptr_t)(sv + (wave * NL + n) * 1024), o);
-    }
+  struct Tile {
+    const char* p;
+    int bytes;
+    uint32_t step;  // a row's bytes
+  };
+  auto tile_of = [&](const uint16_t* fix, const uint16_t* own, int c) __attribute__((always_inline)) -> Tile {
+    const bool o = c >= it.nf;
+    const uint32_t st = o ? step[1] : step[0];
+    const int skip = (int)((uint32_t)(place(it, c) * KB) * st);
+    return {(const char*)(o ? own : fix) + skip, c < it.hi ? (o ? bytes[1] : bytes[0]) - skip : 0, st};  // past the item's: nothing
+  };
+  auto issue = [&](const Tile& t, char* dst, int n, uint32_t ch) __attribute__((always_inline)) {
+    load_lds16(t.p, t.bytes, (lds_ptr_t)(dst + (wave * NL + n) * 1024), row * t.step + (uint32_t)(n * RPI) * t.step + ch);
   };
 
   const float sc = kLog2e / sqrtf((float)D);
   State<D, RT> S;
-  auto compute = [&](const char* sk, const char* sv, int c, bool careful) {
-    const int own = c < it.nf ? 0 : 1;
-    const int at = own ? (it.c0 + c - it.nf) * KB : c * KB;
-    // every key hidden from every row of this wave, or none from any (uniform)
-    if (at > (own ? last.hi_o : last.hi_f) || (own && at + KB - 1 < first.lo_o)) return;
-    const bool mask = at + KB - 1 > (own ? first.hi_o : first.hi_f) || (own && at < last.lo_o);
-    f32x4 s[RT][4];
+  bool ready = false;
+  // A bare barrier (__syncthreads' fence would wait for every load in flight); what was read from LDS before
+  // it has been used.
+  auto barrier = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // The operands of 16 keys (block n of a tile), and of the values for four d blocks of 32 keys: each lot
+  // is read from LDS while the products of the one before run.
+  auto read_k = [&](u32x4 (&f)[DK], const char* sk, int n) __attribute__((always_inline)) {
+    const int r = n * 16 + li;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int i = 0; i < DK; ++i)
+      f[i] = *reinterpret_cast<const u32x4*>(sk + r * (D * 2) + (((4 * i + grp) ^ swk<D>(r)) * 16));
+  };
+  constexpr int VB = DT / 4;  // lots of a half tile's values
+  auto read_v = [&](u32x4 (&f)[4], const char* sv, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = read_vt<D>(sv + b / VB * 32 * D * 2, b % VB * 4 + i, li, grp);
+  };
+  // Tile c of keys sk and values sv. Loads go out one at a time between the products (in one burst they
+  // would hold the wave's other instructions back): the next values (into nv) with the scores, as the values
+  // before these are done with then, and the keys after the next (into sk) with the values' products. So each
+  // has more than a tile's time to land in two stages; every step issues the same loads (past the item's
+  // end of nothing), so that the count in flight is known.
+  auto tile = [&](char* sk, const char* sv, char* nv, int c, bool careful) __attribute__((always_inline)) {
+    // these keys have landed (behind them: the values, the next keys), and every wave is done with the
+    // values before these
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * NL));
+    barrier();
+    const Tile tk = tile_of(fk, ok, c + 2), tv = tile_of(fv, ov, c + 1);
+    f32x4 s[RT][4];
+    u32x4 kf[2][DK];
+    read_k(kf[0], sk, 0);
+    each<4>([&](auto N) __attribute__((always_inline)) {
+      constexpr int n = decltype(N)::value;
+      if constexpr (n < 3) read_k(kf[(n + 1) & 1], sk, n + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) s[rt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < DK; ++i) {
-        const int r = n * 16 + li;
-        const u32x4 kf =
-            *reinterpret_cast<const u32x4*>(sk + r * (D * 2) + (((4 * i + grp) ^ (r & (CH - 1))) * 16));
+      for (int i = 0; i < DK; ++i)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][n] = mfma16(kf, qf[rt][i], s[rt][n]);
+        for (int rt = 0; rt < RT; ++rt) s[rt][n] = mfma16(kf[n & 1][i], qf[rt][i], s[rt][n]);
+#pragma unroll
+      for (int i = n * NL / 4; i < (n + 1) * NL / 4; ++i) {
+        issue(tv, nv, i, chv[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    const int own = c < it.nf ? 0 : 1;
+    const int at = own ? (it.c0 + c - it.nf) * KB : c * KB;
+    // whether a row of this wave does not see some key (uniform)
+    const bool mask = at + KB - 1 > (own ? first.hi_o : first.hi_f) || (own && at < last.lo_o);
+    u32x4 seen[RT][2];
+    if (mask || careful) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int lo = own ? rk[rt].lo_o : 0, hi = own ? rk[rt].hi_o : rk[rt].hi_f;
+        f32x4 one[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = at + n * 16 + 4 * grp + r;
+            const bool hidden = i < lo || i > hi;
+            if (hidden) s[rt][n][r] = -INFINITY;
+            one[n][r] = hidden ? 0.f : 1.f;
+          }
+        if (careful)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            u32x4 f[1];
+            split_p<1>(one[2 * n], one[2 * n + 1], f);
+            seen[rt][n] = f[0];
+          }
       }
     }
-    u32x4 pf[RT][2][PARTS], seen[RT][2];
+    // A row's reference comes from the first tiles that it sees keys of. After one that all of the wave's rows
+    // see whole, only the careful pass follows it: exponents then may reach 2^127 (floating point, so p
+    // is no less exact for that), and past it the sums are infinite and the item is done again.
+    if (mask || careful || !ready) S.follow(s, sc);
+    if (!mask) ready = true;
+    u32x4 pf[RT][2][PARTS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int lo = own ? rk[rt].lo_o : 0, hi = own ? rk[rt].hi_o : rk[rt].hi_f;
-      if (mask) {
+      const float base = S.mx[rt] == -INFINITY ? 0.f : S.mx[rt];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 4; ++n) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = at + n * 16 + 4 * grp + r;
-            if (i < lo || i > hi) s[rt][n][r] = -INFINITY;
-          }
-      }
-      if (careful) {
-        f32x4 t[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = at + n * 16 + 4 * grp + r;
-            t[n][r] = i < lo || i > hi ? 0.f : 1.f;
-          }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          u32x4 f[1];
-          split_p<1>(t[2 * n], t[2 * n + 1], f);
-          seen[rt][n] = f[0];
-        }
-      }
-      S.softmax(s[rt], rt, sc);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        split_p<PARTS>(s[rt][2 * n], s[rt][2 * n + 1], pf[rt][n]);
-#pragma unroll
-        for (int c2 = 0; c2 < PARTS; ++c2) S.sum[rt] = mfma16(ones8(), pf[rt][n][c2], S.sum[rt]);
+        for (int r = 0; r < 4; ++r) s[rt][n][r] = exp2_fast(fmaf(s[rt][n][r], sc, -base));
+        if (n & 1) split_p<PARTS>(s[rt][n - 1], s[rt][n], pf[rt][n / 2]);
       }
     }
+    // these values have landed (behind them: the next keys and values), and every wave is done with the keys
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * NL));
+    barrier();
+    u32x4 vf[2][4];
+    read_v(vf[0], sv, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    each<2 * VB>([&](auto B) __attribute__((always_inline)) {
+      constexpr int b = decltype(B)::value, n = b / VB;
+      if constexpr (b + 1 < 2 * VB) read_v(vf[(b + 1) & 1], sv, b + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (b % VB == 0) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        u32x4 vt = read_vt<D>(sv + n * 32 * D * 2, dt, li, grp);
+          for (int c2 = 0; c2 < PARTS; ++c2) S.sum[rt] = mfma16(ones8(), pf[rt][n][c2], S.sum[rt]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int dt = b % VB * 4 + i;
+        u32x4 vt = vf[b & 1][i];
         if (careful) {
           u32x4 bad;
           take_nonfinite8(vt, bad);
@@ -688,30 +792,46 @@ __global__ __launch_bounds__(256, 2) void seg_tiles_kernel(SegArgs a, SegPlan pl
 #pragma unroll
           for (int c2 = 0; c2 < PARTS; ++c2) S.o[dt][rt] = mfma16(vt, pf[rt][n][c2], S.o[dt][rt]);
       }
-  };
-  auto pass = [&](bool careful) {
-    S.clear();
-    if (it.lo >= it.hi) return;
-    issue(sK0, sV0, it.lo);
-    for (int c = it.lo; c < it.hi; c += 2) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int i = b * NL / (2 * VB); i < (b + 1) * NL / (2 * VB); ++i) issue(tk, sk, i, chk[i]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // (The compiler waits for every load at the top of a loop with some in flight: so four tiles a round.)
+  auto pass = [&](auto CAREFUL) __attribute__((always_inline)) {
+    constexpr bool careful = decltype(CAREFUL)::value;
+    constexpr int U = careful ? 2 : 4;
+    S.clear();
+    ready = false;
+    if (it.lo >= it.hi) return;
+    const Tile k0 = tile_of(fk, ok, it.lo), v0 = tile_of(fv, ov, it.lo), k1 = tile_of(fk, ok, it.lo + 1);
+#pragma unroll
+    for (int n = 0; n < NL; ++n) issue(k0, sK0, n, chk[n]);
+#pragma unroll
+    for (int n = 0; n < NL; ++n) issue(v0, sV0, n, chv[n]);
+#pragma unroll
+    for (int n = 0; n < NL; ++n) issue(k1, sK1, n, chk[n]);
+    for (int c = it.lo; c < it.hi; c += U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
         const int k = c + u;
         if (k >= it.hi) break;
-        // tile k has landed, and every wave is done with the one before
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-        __syncthreads();
-        if (k + 1 < it.hi) issue(u ? sK0 : sK1, u ? sV0 : sV1, k + 1);
-        compute(u ? sK1 : sK0, u ? sV1 : sV0, k, careful);
+        if (u & 1) tile(sK1, sV1, sV0, k, careful);
+        else tile(sK0, sV0, sV1, k, careful);
       }
     }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    __syncthreads();  // (a second pass writes the first stages)
   };
-  pass(false);
+  pass(std::false_type{});
   const int any = __any(S.nonfinite()) ? 1 : 0;
   if (lane == 0) sBad[wave] = any;
   __syncthreads();
-  if (sBad[0] | sBad[1] | sBad[2] | sBad[3]) {  // (the tiles are shared: all waves or none)
-    pass(true);
+  int bad = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) bad |= sBad[w];
+  if (bad) {  // (the tiles are shared: all waves or none)
+    pass(std::true_type{});
   }
 
 #pragma unroll
@@ -775,6 +895,7 @@ __global__ __launch_bounds__(256) void seg_combine_kernel(SegArgs a, int planes)
 
 // ---- plan ---------------------------------------------------------------------------
 
+constexpr int NWT = 4;
 constexpr int kGroups = 512;    // workgroups that a call aims at (two per CU)
 constexpr int64_t kRowsMax = 64;  // query rows per kv head of seg_rows_kernel
 
@@ -789,7 +910,7 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
     const int64_t all = B * rows;
     p.tiles1 = all > 32 ? (all > 64 ? 2 : 1) : 0;  // row blocks per wave; 0: seg_rows_kernel
     p.rt = rows > 16 || (!p.tiles1 && all > 16) ? 2 : 1;
-    const int64_t unit1 = p.tiles1 ? 64 * p.tiles1 : 16 * p.rt, n1 = (all + unit1 - 1) / unit1 * Hk;
+    const int64_t unit1 = p.tiles1 ? (p.tiles1 == 2 ? NWT * 32 : 64) : 16 * p.rt, n1 = (all + unit1 - 1) / unit1 * Hk;
     const int64_t least = p.tiles1 ? 256 : 128;
     p.split1 = (int)clamp(kGroups / n1, (F + least - 1) / least);
     const int64_t n2 = B * Hk * ((rows + 16 * p.rt - 1) / (16 * p.rt));
@@ -809,7 +930,7 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
     p.items2 = (int)(n * p.split2);
   } else {
     p.tiles2 = B * Hk * ((rows + 127) / 128) >= kGroups ? 2 : 1;
-    const int64_t n = B * Hk * ((rows + 64 * p.tiles2 - 1) / (64 * p.tiles2));
+    const int64_t u = p.tiles2 == 2 ? NWT * 32 : 64, n = B * Hk * ((rows + u - 1) / u);
     p.split2 = (int)clamp(clamp(kGroups / n, (all + 255) / 256), kMaxPlanes);
     p.items2 = (int)(n * p.split2);
   }
@@ -832,10 +953,10 @@ int launch_attend(const SegArgs& a, const SegPlan& p, hipStream_t s) {
   SegPlan r = p;
   if (p.tiles1 || p.tiles2) {
     const dim3 grid((unsigned)(p.tiles1 ? p.items1 : p.items2));
-    if (p.tiles1 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 2>), grid, dim3(256), 0, s, a, p);
-    else if (p.tiles1 == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 2>), grid, dim3(256), 0, s, a, p);
-    else if (p.tiles2 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 1>), grid, dim3(256), 0, s, a, p);
-    else hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1>), grid, dim3(256), 0, s, a, p);
+    if (p.tiles1 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 2, 4>), grid, dim3(256), 0, s, a, p);
+    else if (p.tiles1 == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1, NWT>), grid, dim3(NWT * 64), 0, s, a, p);
+    else if (p.tiles2 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 1, 4>), grid, dim3(256), 0, s, a, p);
+    else hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1, NWT>), grid, dim3(NWT * 64), 0, s, a, p);
     e = (int)hipGetLastError();
     if (e) return e;
     r.items1 = 0;

@@ -57,8 +57,10 @@ def check(y, e, parts, rows=None):
     assert (ok | bad).all(), float((err / tol)[~bad].max())
 
 
-def parts(T, Hq, Hk):
-    return 2 if T * Hq // Hk <= 64 else 1
+def parts(T, Hq, Hk, B=1):
+    """Query rows per kv head that one kernel takes: over 64 of them p enters in one part. (A shared text is read
+    for all sequences' rows together.)"""
+    return 2 if B * T * Hq // Hk <= 64 else 1
 
 
 # ------------------------------------------------------------- refusals (CPU)
@@ -190,7 +192,7 @@ def step_shared(g, c, hist, starts, counts, T, Hq, device_pos, lengths):
             hist[b][name] = torch.cat([hist[b][name][: P + starts[b]], x[b, :n]])
         if n:
             e = exact(q[b, :n], hist[b]["k"], hist[b]["v"], P + starts[b] + torch.arange(n), torch.arange(P + starts[b] + n))
-            check(y[b, :n], e, parts(T, Hq, Hk))
+            check(y[b, :n], e, parts(T, Hq, Hk, B))
         assert (y[b, n:] == 0).all()
         own = c.k[0][b, :, : starts[b] + n].transpose(0, 1).cpu()
         assert torch.equal(own, hist[b]["k"][P:])
