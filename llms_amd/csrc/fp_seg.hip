@@ -575,9 +575,9 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
 // loads in flight while one is computed.
 // Items: ranges x row tiles (of one sequence, or of all where only a shared fixed part is read) with the kv
 // head fastest, so that one XCD runs a head's tiles.
-template <int D, int RT, int PARTS, int NW>
-__global__ __launch_bounds__(NW * kWave, NW == 4 ? 2 : 1) void seg_tiles_kernel(SegArgs a, SegPlan pl) {
-  constexpr int KB = 64;
+template <int D, int RT, int PARTS>
+__global__ __launch_bounds__(256, RT > 2 ? 1 : 2) void seg_tiles_kernel(SegArgs a, SegPlan pl) {
+  constexpr int NW = 4, KB = 64;
   constexpr int DK = D / 32, DT = D / 16;
   constexpr int RPI = 1024 / (D * 2);          // rows per load instruction
   constexpr int NL = KB / RPI / NW;            // load instructions per wave of a tile's keys
@@ -593,23 +593,35 @@ __global__ __launch_bounds__(NW * kWave, NW == 4 ? 2 : 1) void seg_tiles_kernel(
   const int li = lane & 15, grp = lane >> 4;
   const int G = a.Hq / a.Hk;
   Item it;
-  int id = blockIdx.x;
-  it.kh = id % a.Hk;
-  id /= a.Hk;
-  it.packed = pl.items1 > 0;
+  it.kh = blockIdx.x % a.Hk;
+  const int64_t g = blockIdx.x / a.Hk, n1 = pl.items1 / a.Hk, n = n1 + pl.items2 / a.Hk;
+  int id = (int)(g * n1 / n);
+  it.packed = (g + 1) * n1 / n > id;
   it.b = 0;
   if (!it.packed) {
+    id = (int)g - id;
     it.b = id % a.B;
     id /= a.B;
   }
   it.rows = (it.packed ? a.B : 1) * a.T * G;
   constexpr int ROWS = NW * 16 * RT;
   const int n_rt = (it.rows + ROWS - 1) / ROWS;
-  const int rtile = n_rt - 1 - id % n_rt;  // (the later tokens of a prompt see more)
-  it.plane = id / n_rt;
+  int rtile, range;
+  if (it.packed) {
+    // (ranges fastest: the workgroups of a CU are then of several row tiles, and a last one with few rows
+    // leaves the matrix cores to the others; 160 rows of 50001 keys: 61 -> 57 us)
+    range = it.plane = id % pl.split1;
+    rtile = id / pl.split1;
+  } else {
+    rtile = n_rt - 1 - id % n_rt;  // the later tokens of a prompt see more
+    range = id / n_rt;
+    it.plane = pl.split1 + range;
+  }
   it.row0 = rtile * ROWS;
-  item_keys<KB>(a, it, ROWS, true, !it.packed, it.plane, it.packed ? pl.split1 : pl.split2);
+  item_keys<KB>(a, it, ROWS, it.packed || !pl.shared, !it.packed, range, it.packed ? pl.split1 : pl.split2);
   const int row0 = it.row0 + wave * 16 * RT;  // this wave's first row
+  // A wave without a row of a token loads its share of the tiles only.
+  const bool idle = row0 >= (it.packed ? it.rows : count(a, it.b) * G);
 
   u32x4 qf[RT][DK];
   RowKeys rk[RT];
@@ -811,7 +823,20 @@ __global__ __launch_bounds__(NW * kWave, NW == 4 ? 2 : 1) void seg_tiles_kernel(
     for (int n = 0; n < NL; ++n) issue(v0, sV0, n, chv[n]);
 #pragma unroll
     for (int n = 0; n < NL; ++n) issue(k1, sK1, n, chk[n]);
-    for (int c = it.lo; c < it.hi; c += U) {
+    if (idle) {
+      for (int c = it.lo; c < it.hi; ++c) {
+        const bool odd = (c - it.lo) & 1;
+        const Tile tk = tile_of(fk, ok, c + 2), tv = tile_of(fv, ov, c + 1);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * NL));
+        barrier();
+#pragma unroll
+        for (int n = 0; n < NL; ++n) issue(tv, odd ? sV0 : sV1, n, chv[n]);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * NL));
+        barrier();
+#pragma unroll
+        for (int n = 0; n < NL; ++n) issue(tk, odd ? sK1 : sK0, n, chk[n]);
+      }
+    } else for (int c = it.lo; c < it.hi; c += U) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int k = c + u;
@@ -854,48 +879,53 @@ __global__ __launch_bounds__(NW * kWave, NW == 4 ? 2 : 1) void seg_tiles_kernel(
 }
 
 // One output row per workgroup: lane s of each wave holds plane s's statistics (at most 64), so the
-// weights take one load and a few lane exchanges; then each group of D / 4 threads sums every NG-th
-// plane's partials and the groups' sums are added in group order.
-template <int D>
+// weights take one load and a few lane exchanges; each group of D / 4 threads sums every NG-th plane's
+// partials (loaded before the weights are known: one trip to memory) and the groups' sums are added in
+// group order. MP: a bound of the planes.
+template <int D, int MP>
 __global__ __launch_bounds__(256) void seg_combine_kernel(SegArgs a, int planes) {
-  constexpr int LPR = D / 4, NG = 256 / LPR;
+  constexpr int LPR = D / 4, NG = 256 / LPR, N = (MP + NG - 1) / NG;
   __shared__ __attribute__((aligned(16))) f32x4 part[NG][LPR];
   const int G = a.Hq / a.Hk;
   const int64_t rows = (int64_t)a.B * a.T * G, total = rows * a.Hk, i = blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1), grp = threadIdx.x / LPR, q = threadIdx.x % LPR;
-  const bool has = lane < planes;
-  f32x2 st = {-INFINITY, 0.f};
-  if (has) st = *reinterpret_cast<const f32x2*>(a.stat + (lane * total + i) * 2);
-  float m = st.x;
+  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stat + ((lane < planes ? lane : 0) * total + i) * 2);
+  f32x4 p[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int s = n * NG + grp;
+    p[n] = *reinterpret_cast<const f32x4*>(a.part + ((s < planes ? s : 0) * total + i) * D + q * 4);
+  }
+  const int kh = (int)(i / rows);
+  const int64_t r = i - (int64_t)kh * rows, t = r / G;
+  Item it;
+  it.kh = kh;
+  it.b = (int)(t / a.T);
+  const int rr = (int)(r - (int64_t)it.b * a.T * G);
+  const bool live = row_live(a, it, rr);
+  float m = lane < planes ? st.x : -INFINITY;
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
   const float base = m == -INFINITY ? 0.f : m;
-  const float e = has ? exp2_fast(st.x - base) : 0.f;
-  const float l = wave_sum(has ? e * st.y : 0.f);
+  const float e = lane < planes ? exp2_fast(st.x - base) : 0.f;
+  const float l = wave_sum(lane < planes ? e * st.y : 0.f);
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int n = 0; n < kMaxPlanes / NG; ++n) {
+  for (int n = 0; n < N; ++n) {
     const int s = n * NG + grp;
-    const float w = __shfl(e, s);  // every lane takes part in the exchange
-    if (s < planes) v += *reinterpret_cast<const f32x4*>(a.part + (s * total + i) * D + q * 4) * w;
+    const float w = __shfl(e, s < kWave ? s : 0);  // every lane takes part in the exchange
+    if (s < planes) v += p[n] * w;
   }
   part[grp][q] = v;
   __syncthreads();
   if (grp != 0) return;
 #pragma unroll
   for (int g = 1; g < NG; ++g) v += part[g][q];
-  const int kh = (int)(i / rows);
-  const int64_t r = i - (int64_t)kh * rows, n = r / G;
-  Item it;
-  it.kh = kh;
-  it.b = (int)(n / a.T);
-  const int rr = (int)(r - (int64_t)it.b * a.T * G);
-  store_row(a, it, rr, q * 4, D, v, l, row_live(a, it, rr));
+  store_row(a, it, rr, q * 4, D, v, l, live);
 }
 
 // ---- plan ---------------------------------------------------------------------------
 
-constexpr int NWT = 4;
 constexpr int kGroups = 512;    // workgroups that a call aims at (two per CU)
 constexpr int64_t kRowsMax = 64;  // query rows per kv head of seg_rows_kernel
 
@@ -909,12 +939,12 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
     // the fixed part's rows are all sequences', in ranges of at least 128 keys (rows) or four tiles
     const int64_t all = B * rows;
     p.tiles1 = all > 32 ? (all > 64 ? 2 : 1) : 0;  // row blocks per wave; 0: seg_rows_kernel
-    p.rt = rows > 16 || (!p.tiles1 && all > 16) ? 2 : 1;
-    const int64_t unit1 = p.tiles1 ? (p.tiles1 == 2 ? NWT * 32 : 64) : 16 * p.rt, n1 = (all + unit1 - 1) / unit1 * Hk;
+    p.rt = all > 16 ? 2 : 1;
+    const int64_t unit = p.tiles1 ? 64 * p.tiles1 : 16 * p.rt, n1 = (all + unit - 1) / unit * Hk;
     const int64_t least = p.tiles1 ? 256 : 128;
     p.split1 = (int)clamp(kGroups / n1, (F + least - 1) / least);
-    const int64_t n2 = B * Hk * ((rows + 16 * p.rt - 1) / (16 * p.rt));
-    p.split2 = (int)clamp(kGroups / n2, (keys + 127) / 128);
+    const int64_t n2 = B * Hk * ((rows + unit - 1) / unit);
+    p.split2 = (int)clamp(kGroups / n2, (keys + least - 1) / least);
     if (p.split1 > kMaxPlanes - 8) p.split1 = kMaxPlanes - 8;
     if (p.split2 > 8) p.split2 = 8;
     p.items1 = (int)(n1 * p.split1);
@@ -930,7 +960,7 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
     p.items2 = (int)(n * p.split2);
   } else {
     p.tiles2 = B * Hk * ((rows + 127) / 128) >= kGroups ? 2 : 1;
-    const int64_t u = p.tiles2 == 2 ? NWT * 32 : 64, n = B * Hk * ((rows + u - 1) / u);
+    const int64_t u = p.tiles2 == 2 ? 128 : 64, n = B * Hk * ((rows + u - 1) / u);
     p.split2 = (int)clamp(clamp(kGroups / n, (all + 255) / 256), kMaxPlanes);
     p.items2 = (int)(n * p.split2);
   }
@@ -950,26 +980,25 @@ int launch_prep(const SegArgs& a, hipStream_t s) {
 template <int D>
 int launch_attend(const SegArgs& a, const SegPlan& p, hipStream_t s) {
   int e = 0;
-  SegPlan r = p;
   if (p.tiles1 || p.tiles2) {
-    const dim3 grid((unsigned)(p.tiles1 ? p.items1 : p.items2));
-    if (p.tiles1 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 2, 4>), grid, dim3(256), 0, s, a, p);
-    else if (p.tiles1 == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1, NWT>), grid, dim3(NWT * 64), 0, s, a, p);
-    else if (p.tiles2 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 1, 4>), grid, dim3(256), 0, s, a, p);
-    else hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1, NWT>), grid, dim3(NWT * 64), 0, s, a, p);
+    const dim3 grid((unsigned)(p.items1 + p.items2));
+    if (p.tiles1 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 2>), grid, dim3(256), 0, s, a, p);
+    else if (p.tiles1 == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1>), grid, dim3(256), 0, s, a, p);
+    else if (p.tiles2 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 1>), grid, dim3(256), 0, s, a, p);
+    else hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1>), grid, dim3(256), 0, s, a, p);
     e = (int)hipGetLastError();
     if (e) return e;
-    r.items1 = 0;
-  }
-  if (!p.tiles2) {
-    const dim3 grid((unsigned)(r.items1 + r.items2));
-    if (p.rt == 1) hipLaunchKernelGGL((seg_rows_kernel<D, 1>), grid, dim3(256), 0, s, a, r);
-    else hipLaunchKernelGGL((seg_rows_kernel<D, 2>), grid, dim3(256), 0, s, a, r);
+  } else {
+    const dim3 grid((unsigned)(p.items1 + p.items2));
+    if (p.rt == 1) hipLaunchKernelGGL((seg_rows_kernel<D, 1>), grid, dim3(256), 0, s, a, p);
+    else hipLaunchKernelGGL((seg_rows_kernel<D, 2>), grid, dim3(256), 0, s, a, p);
     e = (int)hipGetLastError();
     if (e) return e;
   }
   if (p.planes > 1) {
-    hipLaunchKernelGGL(seg_combine_kernel<D>, dim3((unsigned)((int64_t)a.B * a.T * a.Hq)), dim3(256), 0, s, a, p.planes);
+    const dim3 grid((unsigned)((int64_t)a.B * a.T * a.Hq));
+    if (p.planes <= 16) hipLaunchKernelGGL((seg_combine_kernel<D, 16>), grid, dim3(256), 0, s, a, p.planes);
+    else hipLaunchKernelGGL((seg_combine_kernel<D, kMaxPlanes>), grid, dim3(256), 0, s, a, p.planes);
     e = (int)hipGetLastError();
   }
   return e;
