@@ -83,38 +83,43 @@ __device__ __forceinline__ bool in_cache(const SegArgs& a, int p) {
 
 // ---- new tokens -------------------------------------------------------------------
 
-// One head row per LPH = D / 8 lanes (fp_rope.h). Without cos: k and v only, as they are.
+// A new token's key or value of one head to its place, by LPH = D / 8 lanes (lane j; fp_rope.h).
+template <int D>
+__device__ __forceinline__ void put_new(const SegArgs& a, int b, int kh, int t, int p, bool value, int j) {
+  const uint16_t* src = value ? a.v + b * a.svb + t * a.svt + (int64_t)kh * D : a.k + b * a.skb + t * a.skt + (int64_t)kh * D;
+  u32x2 lo = *reinterpret_cast<const u32x2*>(src + 4 * j);
+  u32x2 hi = *reinterpret_cast<const u32x2*>(src + D / 2 + 4 * j);
+  if (a.cos && !value)
+    norm_rope_row<D>(lo, hi, a.gk, a.epsk, a.cos + b * a.scb + t * a.sct, a.sin + b * a.ssb + t * a.sst, j);
+  const int u = p - a.F;
+  uint16_t* dst;
+  if (u < 0) dst = (value ? a.fv : a.fk) + b * a.sfb + kh * a.sfh + (int64_t)p * a.sfs;
+  else dst = (value ? a.ov : a.ok) + b * a.sob + kh * a.soh + (int64_t)(a.ring ? u % a.S : u) * a.sos;
+  *reinterpret_cast<u32x2*>(dst + 4 * j) = lo;
+  *reinterpret_cast<u32x2*>(dst + D / 2 + 4 * j) = hi;
+}
+
+// Every new token's, and with queries the rotated q. (Lanes past the last row leave together with the others of
+// their row.)
 template <int D>
 __global__ __launch_bounds__(256) void seg_prep_kernel(SegArgs a) {
   constexpr int LPH = D / 8;
-  const int qh = a.cos ? a.Hq : 0, heads = qh + 2 * a.Hk;
-  const int64_t items = (int64_t)a.B * a.T * heads;
-  int64_t item = (int64_t)blockIdx.x * (256 / LPH) + threadIdx.x / LPH;
-  const bool live = item < items;  // dead lanes stay for the cross-lane sums
-  if (!live) item = items - 1;
+  const int qh = a.qn ? a.Hq : 0, heads = qh + 2 * a.Hk;
+  const int64_t item = (int64_t)blockIdx.x * (256 / LPH) + threadIdx.x / LPH;
+  if (item >= (int64_t)a.B * a.T * heads) return;
   const int j = threadIdx.x % LPH;
   const int64_t m = item / heads;
   const int h = (int)(item - m * heads), b = (int)(m / a.T), t = (int)(m - (int64_t)b * a.T);
-  const bool isq = h < qh, isk = !isq && h < qh + a.Hk;
-  const int hk = isk ? h - qh : h - qh - a.Hk;
-  const uint16_t* src = isq   ? a.q + b * a.sqb + t * a.sqt + (int64_t)h * D
-                        : isk ? a.k + b * a.skb + t * a.skt + (int64_t)hk * D
-                              : a.v + b * a.svb + t * a.svt + (int64_t)hk * D;
+  if (h >= qh) {
+    const int p = first_pos(a, b) + t, hk = h - qh;
+    if (t < count(a, b) && in_cache(a, p)) put_new<D>(a, b, hk < a.Hk ? hk : hk - a.Hk, t, p, hk >= a.Hk, j);
+    return;
+  }
+  const uint16_t* src = a.q + b * a.sqb + t * a.sqt + (int64_t)h * D;
+  uint16_t* dst = a.qn + (m * a.Hq + h) * D;
   u32x2 lo = *reinterpret_cast<const u32x2*>(src + 4 * j);
   u32x2 hi = *reinterpret_cast<const u32x2*>(src + D / 2 + 4 * j);
-  if (a.cos && (isq || isk))
-    norm_rope_row<D>(lo, hi, isq ? a.gq : a.gk, isq ? a.epsq : a.epsk, a.cos + b * a.scb + t * a.sct,
-                     a.sin + b * a.ssb + t * a.sst, j);
-  uint16_t* dst;
-  if (isq) {
-    dst = a.qn + (m * a.Hq + h) * D;
-  } else {
-    const int p = first_pos(a, b) + t, u = p - a.F;
-    if (t >= count(a, b) || !in_cache(a, p)) return;
-    if (u < 0) dst = (isk ? a.fk : a.fv) + b * a.sfb + hk * a.sfh + (int64_t)p * a.sfs;
-    else dst = (isk ? a.ok : a.ov) + b * a.sob + hk * a.soh + (int64_t)(a.ring ? u % a.S : u) * a.sos;
-  }
-  if (!live) return;
+  norm_rope_row<D>(lo, hi, a.gq, a.epsq, a.cos + b * a.scb + t * a.sct, a.sin + b * a.ssb + t * a.sst, j);
   *reinterpret_cast<u32x2*>(dst + 4 * j) = lo;
   *reinterpret_cast<u32x2*>(dst + D / 2 + 4 * j) = hi;
 }
@@ -257,6 +262,14 @@ __device__ __forceinline__ int place(const Item& it, int c) {
   return x < it.ring ? x : x - it.ring;
 }
 
+// The block of an item's own sequence that position p is in (-1: before those that it has).
+template <int KB>
+__device__ __forceinline__ int new_block(const SegArgs& a, const Item& it, int p) {
+  const int u = p - a.F;
+  if (u < 0) return p < 0 || it.nf == 0 ? -1 : p / KB;
+  return u / KB < it.c0 ? -1 : it.nf + u / KB - it.c0;
+}
+
 // q row r of an item (clamped; rows past the last are not stored).
 __device__ __forceinline__ const uint16_t* q_row(const SegArgs& a, const Item& it, int r, int D) {
   if (r >= it.rows) r = it.rows - 1;
@@ -350,7 +363,9 @@ __device__ __forceinline__ u32x4 ones8() { return u32x4{0x3f803f80u, 0x3f803f80u
 // item's range, each with the next block's keys in registers and values in its own LDS buffer while it
 // computes; their states are merged through LDS in wave order.
 // Items: first those of the shared fixed part (grid: n_split1 ranges x row groups x kv heads), then of each
-// sequence (ranges x row groups x kv heads x sequences).
+// sequence (ranges x row groups x kv heads x sequences). An item normalises and rotates its queries (into LDS)
+// and its new keys itself (into the cache: those in its range, which a token's own row always sees, so
+// every one is in some item's; two items of one write the same).
 template <int D, int RT>
 __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs a, SegPlan pl) {
   constexpr int NW = 4, KB = 32, PARTS = 2;
@@ -360,8 +375,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
   constexpr int CH = D / 8;                    // 16-byte chunks per row
   __shared__ __attribute__((aligned(1024))) char sV0[NW][KB * D * 2];
   __shared__ __attribute__((aligned(1024))) char sV1[NW][KB * D * 2];
+  __shared__ __attribute__((aligned(1024))) char sQ[16 * RT * D * 2];
   __shared__ float sM[NW][16 * RT], sL[NW][16 * RT];
-  __shared__ int sBad[NW];
 
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -390,16 +405,12 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
     item_keys<KB>(a, it, 16 * RT, !pl.shared, true, id / n, pl.split2);
   }
 
-  u32x4 qf[RT][DK];
   RowKeys rk[RT];
   const int p0 = it.packed ? a.F : first_pos(a, it.b);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = it.row0 + rt * 16 + li;
     rk[rt] = row_keys(a, row_pos(a, it, r < it.rows ? r : it.rows - 1, p0));
-    const uint16_t* qp = q_row(a, it, r, D) + 8 * grp;
-#pragma unroll
-    for (int i = 0; i < DK; ++i) qf[rt][i] = ld16(qp + 32 * i);
   }
 
   const uint16_t* const kb[2] = {a.fk + it.b * a.sfb + it.kh * a.sfh, a.ok + it.b * a.sob + it.kh * a.soh};
@@ -425,6 +436,39 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
         kf[kt][i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(kb[own], bytes[own]),
                                                           (uint32_t)(blk * KB + 16 * kt + li) * st + 16 * grp + 64 * i, 0, 0);
   };
+
+  // new keys are in the range (uniform; conservative: from the first token's block to the last's)
+  const int n_new = it.packed ? 0 : count(a, it.b);
+  const bool fresh = n_new > 0 && it.lo < it.hi && new_block<KB>(a, it, p0) < it.hi &&
+                     new_block<KB>(a, it, p0 + n_new - 1) >= it.lo;
+  constexpr int LPH = D / 8;
+  const int hr = threadIdx.x / LPH, hj = threadIdx.x % LPH;
+  for (int r = hr; r < 16 * RT; r += 256 / LPH) {
+    const int rc = it.row0 + r < it.rows ? it.row0 + r : it.rows - 1, n = rc / G;
+    const int b = it.packed ? n / a.T : it.b, t = it.packed ? n - b * a.T : n;
+    const uint16_t* src = a.q + b * a.sqb + t * a.sqt + (int64_t)(it.kh * G + rc - n * G) * D;
+    u32x2 lo = *reinterpret_cast<const u32x2*>(src + 4 * hj);
+    u32x2 hi = *reinterpret_cast<const u32x2*>(src + D / 2 + 4 * hj);
+    if (a.cos)
+      norm_rope_row<D>(lo, hi, a.gq, a.epsq, a.cos + b * a.scb + t * a.sct, a.sin + b * a.ssb + t * a.sst, hj);
+    char* const dst = sQ + r * (D * 2) + (hj & 1) * 8;
+    *reinterpret_cast<u32x2*>(dst + (((hj >> 1) ^ swk<D>(r)) * 16)) = lo;
+    *reinterpret_cast<u32x2*>(dst + (((D / 16 + (hj >> 1)) ^ swk<D>(r)) * 16)) = hi;
+  }
+  if (fresh) {
+    for (int i = hr; i < 2 * n_new; i += 256 / LPH) {
+      const int t = i >> 1, c = new_block<KB>(a, it, p0 + t);
+      if (!in_cache(a, p0 + t) || c < it.lo || c >= it.hi) continue;
+      put_new<D>(a, it.b, it.kh, t, p0 + t, (i & 1) != 0, hj);
+    }
+  }
+  __syncthreads();  // (the keys: read by this workgroup after their writes)
+  u32x4 qf[RT][DK];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int i = 0; i < DK; ++i)
+      qf[rt][i] = *reinterpret_cast<const u32x4*>(sQ + (rt * 16 + li) * (D * 2) + (((4 * i + grp) ^ swk<D>(rt * 16 + li)) * 16));
 
   const float sc = kLog2e / sqrtf((float)D);
   State<D, RT> S;
@@ -972,7 +1016,7 @@ inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 template <int D>
 int launch_prep(const SegArgs& a, hipStream_t s) {
-  const int64_t heads = (int64_t)a.B * a.T * ((a.cos ? a.Hq : 0) + 2 * a.Hk), per = 256 / (D / 8);
+  const int64_t heads = (int64_t)a.B * a.T * ((a.qn ? a.Hq : 0) + 2 * a.Hk), per = 256 / (D / 8);
   hipLaunchKernelGGL(seg_prep_kernel<D>, dim3((unsigned)((heads + per - 1) / per)), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
@@ -1010,7 +1054,7 @@ int64_t seg_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_
                             bool rope) {
   const SegPlan p = seg_plan(B, T, Hq, Hk, F, keys, shared);
   const int64_t rows = B * T * Hq;
-  int64_t b = rope ? up256(rows * D * 2) : 0;
+  int64_t b = rope && (p.tiles1 || p.tiles2) ? up256(rows * D * 2) : 0;
   if (p.planes > 1) b += up256(rows * p.planes * 8) + rows * p.planes * D * 4;
   return b;
 }
@@ -1024,7 +1068,8 @@ int launch_seg_attention(SegArgs a, int64_t D, int64_t keys, bool shared, void* 
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
   char* w = (char*)ws;
   a.qsrc = a.q, a.sqsb = a.sqb, a.sqst = a.sqt;
-  if (a.cos) {
+  const bool tiles = p.tiles1 || p.tiles2;
+  if (tiles && a.cos) {
     a.qn = (uint16_t*)w;
     a.qsrc = a.qn, a.sqst = (int64_t)a.Hq * D, a.sqsb = a.T * a.sqst;
     w += up256(rows * D * 2);
@@ -1032,8 +1077,10 @@ int launch_seg_attention(SegArgs a, int64_t D, int64_t keys, bool shared, void* 
   a.stat = (float*)w;
   if (p.planes > 1) w += up256(rows * p.planes * 8);
   a.part = (float*)w;
-  const int e = launch_seg_write(a, D, s);
-  if (e) return e;
+  if (tiles) {  // (seg_rows_kernel does its own)
+    const int e = launch_seg_write(a, D, s);
+    if (e) return e;
+  }
   return D == 128 ? launch_attend<128>(a, p, s) : launch_attend<64>(a, p, s);
 }
 
