@@ -359,15 +359,15 @@ __device__ __forceinline__ u32x4 ones8() { return u32x4{0x3f803f80u, 0x3f803f80u
 
 // ---- few rows ------------------------------------------------------------------------
 //
-// Bound by the cache's bytes. 16 RT query rows; the four waves take 32-key blocks w, w + 4, ... of the
+// Bound by the cache's bytes. 16 query rows; the four waves take 32-key blocks w, w + 4, ... of the
 // item's range, each with the next block's keys in registers and values in its own LDS buffer while it
 // computes; their states are merged through LDS in wave order.
 // Items: first those of the shared fixed part (grid: n_split1 ranges x row groups x kv heads), then of each
 // sequence (ranges x row groups x kv heads x sequences). An item normalises and rotates its queries (into LDS)
 // and its new keys itself (into the cache: those in its range, which a token's own row always sees, so
 // every one is in some item's; two items of one write the same).
-template <int D, int RT>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs a, SegPlan pl) {
+template <int D>
+__global__ __launch_bounds__(256, 2) void seg_rows_kernel(SegArgs a, SegPlan pl) {
   constexpr int NW = 4, KB = 32, PARTS = 2;
   constexpr int DK = D / 32, DT = D / 16;      // k-steps of q.k, d blocks of p.V
   constexpr int RPI = 1024 / (D * 2);          // V rows per load instruction
@@ -375,8 +375,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
   constexpr int CH = D / 8;                    // 16-byte chunks per row
   __shared__ __attribute__((aligned(1024))) char sV0[NW][KB * D * 2];
   __shared__ __attribute__((aligned(1024))) char sV1[NW][KB * D * 2];
-  __shared__ __attribute__((aligned(1024))) char sQ[16 * RT * D * 2];
-  __shared__ float sM[NW][16 * RT], sL[NW][16 * RT];
+  __shared__ __attribute__((aligned(1024))) char sQ[16 * D * 2];
+  __shared__ float sM[NW][16], sL[NW][16];
 
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -391,27 +391,22 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
   if (it.packed) {
     it.b = 0;
     it.rows = a.B * a.T * G;
-    const int n = (it.rows + 16 * RT - 1) / (16 * RT);
-    it.row0 = id % n * 16 * RT;
+    const int n = (it.rows + 15) / 16;
+    it.row0 = id % n * 16;
     it.plane = id / n;
-    item_keys<KB>(a, it, 16 * RT, true, false, it.plane, pl.split1);
+    item_keys<KB>(a, it, 16, true, false, it.plane, pl.split1);
   } else {
     it.b = id % a.B;
     id /= a.B;
     it.rows = a.T * G;
-    const int n = (it.rows + 16 * RT - 1) / (16 * RT);
-    it.row0 = id % n * 16 * RT;
+    const int n = (it.rows + 15) / 16;
+    it.row0 = id % n * 16;
     it.plane = pl.split1 + id / n;
-    item_keys<KB>(a, it, 16 * RT, !pl.shared, true, id / n, pl.split2);
+    item_keys<KB>(a, it, 16, !pl.shared, true, id / n, pl.split2);
   }
 
-  RowKeys rk[RT];
-  const int p0 = it.packed ? a.F : first_pos(a, it.b);
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = it.row0 + rt * 16 + li;
-    rk[rt] = row_keys(a, row_pos(a, it, r < it.rows ? r : it.rows - 1, p0));
-  }
+  const int p0 = it.packed ? a.F : first_pos(a, it.b), r0 = it.row0 + li;
+  const RowKeys rk = row_keys(a, row_pos(a, it, r0 < it.rows ? r0 : it.rows - 1, p0));
 
   const uint16_t* const kb[2] = {a.fk + it.b * a.sfb + it.kh * a.sfh, a.ok + it.b * a.sob + it.kh * a.soh};
   const uint16_t* const vb[2] = {a.fv + it.b * a.sfb + it.kh * a.sfh, a.ov + it.b * a.sob + it.kh * a.soh};
@@ -443,7 +438,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
                      new_block<KB>(a, it, p0 + n_new - 1) >= it.lo;
   constexpr int LPH = D / 8;
   const int hr = threadIdx.x / LPH, hj = threadIdx.x % LPH;
-  for (int r = hr; r < 16 * RT; r += 256 / LPH) {
+  for (int r = hr; r < 16; r += 256 / LPH) {
     const int rc = it.row0 + r < it.rows ? it.row0 + r : it.rows - 1, n = rc / G;
     const int b = it.packed ? n / a.T : it.b, t = it.packed ? n - b * a.T : n;
     const uint16_t* src = a.q + b * a.sqb + t * a.sqt + (int64_t)(it.kh * G + rc - n * G) * D;
@@ -463,82 +458,57 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
     }
   }
   __syncthreads();  // (the keys: read by this workgroup after their writes)
-  u32x4 qf[RT][DK];
+  u32x4 qf[DK];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-    for (int i = 0; i < DK; ++i)
-      qf[rt][i] = *reinterpret_cast<const u32x4*>(sQ + (rt * 16 + li) * (D * 2) + (((4 * i + grp) ^ swk<D>(rt * 16 + li)) * 16));
+  for (int i = 0; i < DK; ++i)
+    qf[i] = *reinterpret_cast<const u32x4*>(sQ + li * (D * 2) + (((4 * i + grp) ^ swk<D>(li)) * 16));
 
   const float sc = kLog2e / sqrtf((float)D);
-  State<D, RT> S;
+  State<D, 1> S;
   auto compute = [&](u32x4 (&kf)[2][DK], const char* sv, int c, bool careful) {
     const int own = c < it.nf ? 0 : 1;
     const int first = own ? (it.c0 + c - it.nf) * KB : c * KB;
-    f32x4 s[RT][2];
+    const int lo = own ? rk.lo_o : 0, hi = own ? rk.hi_o : rk.hi_f;
+    f32x4 s[1][2], one[2];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int kt = 0; kt < 2; ++kt) {
+      s[0][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < DK; ++i) s[rt][kt] = mfma16(kf[kt][i], qf[rt][i], s[rt][kt]);
-      }
-    u32x4 pf[RT][PARTS], seen[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int lo = own ? rk[rt].lo_o : 0, hi = own ? rk[rt].hi_o : rk[rt].hi_f;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = first + kt * 16 + 4 * grp + r;
-          if (i < lo || i > hi) s[rt][kt][r] = -INFINITY;
-        }
-      if (careful) {
-        f32x4 t[2];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = first + kt * 16 + 4 * grp + r;
-            t[kt][r] = i < lo || i > hi ? 0.f : 1.f;
-          }
-        u32x4 f[1];
-        split_p<1>(t[0], t[1], f);
-        seen[rt] = f[0];
-      }
+      for (int i = 0; i < DK; ++i) s[0][kt] = mfma16(kf[kt][i], qf[i], s[0][kt]);
     }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = first + kt * 16 + 4 * grp + r;
+        const bool hidden = i < lo || i > hi;
+        if (hidden) s[0][kt][r] = -INFINITY;
+        one[kt][r] = hidden ? 0.f : 1.f;
+      }
+    u32x4 pf[PARTS], seen[1];
+    if (careful) split_p<1>(one[0], one[1], seen);
     S.follow(s, sc);
+    const float base = S.mx[0] == -INFINITY ? 0.f : S.mx[0];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float base = S.mx[rt] == -INFINITY ? 0.f : S.mx[rt];
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int r = 0; r < 4; ++r) s[0][kt][r] = exp2_fast(fmaf(s[0][kt][r], sc, -base));
+    split_p<PARTS>(s[0][0], s[0][1], pf);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[rt][kt][r] = exp2_fast(fmaf(s[rt][kt][r], sc, -base));
-      split_p<PARTS>(s[rt][0], s[rt][1], pf[rt]);
-#pragma unroll
-      for (int c2 = 0; c2 < PARTS; ++c2) S.sum[rt] = mfma16(ones8(), pf[rt][c2], S.sum[rt]);
-    }
+    for (int c2 = 0; c2 < PARTS; ++c2) S.sum[0] = mfma16(ones8(), pf[c2], S.sum[0]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       u32x4 vt = read_vt<D>(sv, dt, li, grp);
       if (careful) {
         u32x4 bad;
         take_nonfinite8(vt, bad);
+        const f32x4 n = mfma16(bad, seen[0], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const f32x4 n = mfma16(bad, seen[rt], f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n[r] > 0.f) S.o[dt][rt][r] = __uint_as_float(0x7fc00000u);
-        }
+        for (int r = 0; r < 4; ++r)
+          if (n[r] > 0.f) S.o[dt][0][r] = __uint_as_float(0x7fc00000u);
       }
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int c2 = 0; c2 < PARTS; ++c2) S.o[dt][rt] = mfma16(vt, pf[rt][c2], S.o[dt][rt]);
+      for (int c2 = 0; c2 < PARTS; ++c2) S.o[dt][0] = mfma16(vt, pf[c2], S.o[dt][0]);
     }
   };
 
@@ -571,24 +541,20 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void seg_rows_kernel(SegArgs 
   pass(false);
   if (__any(S.nonfinite())) pass(true);
 
-  // Merge the waves' states in wave order. Row block rt's sums go over the wave's own V buffer rt
-  // (free now), 16-byte chunk q of row r at q ^ r, so 16 rows' stores spread over the banks.
-  static_assert(RT <= 2 && 16 * D * 4 == KB * D * 2, "row sums fit the V buffers");
+  // Merge the waves' states in wave order. A wave's row sums go over its own first V buffer (free now), 16-byte
+  // chunk q of row r at q ^ r, so 16 rows' stores spread over the banks.
+  static_assert(16 * D * 4 == KB * D * 2, "the sums fit the V buffer");
   auto slot = [&](int w, int r, int q) -> f32x4* {
-    char* base = r < 16 ? sV0[w] : sV1[w];
-    return reinterpret_cast<f32x4*>(base + (r & 15) * (D * 4) + ((q ^ (r & 15)) * 16));
+    return reinterpret_cast<f32x4*>(sV0[w] + r * (D * 4) + ((q ^ r) * 16));
   };
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    if (grp == 0) {
-      sM[wave][rt * 16 + li] = S.mx[rt];
-      sL[wave][rt * 16 + li] = S.sum[rt][0];
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *slot(wave, rt * 16 + li, dt * 4 + grp) = S.o[dt][rt];
+  if (grp == 0) {
+    sM[wave][li] = S.mx[0];
+    sL[wave][li] = S.sum[0][0];
   }
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) *slot(wave, li, dt * 4 + grp) = S.o[dt][0];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * RT * (D / 4); i += NW * kWave) {
+  for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * kWave) {
     const int r = i / (D / 4), d = (i % (D / 4)) * 4, rr = it.row0 + r;
     if (rr >= it.rows) continue;
     float m = sM[0][r];
@@ -970,45 +936,50 @@ __global__ __launch_bounds__(256) void seg_combine_kernel(SegArgs a, int planes)
 
 // ---- plan ---------------------------------------------------------------------------
 
-constexpr int kGroups = 512;    // workgroups that a call aims at (two per CU)
-constexpr int64_t kRowsMax = 64;  // query rows per kv head of seg_rows_kernel
+constexpr int kGroups = 512;  // workgroups that a call aims at: two per CU
+// Rows of a sequence and kv head up to which a shared text is read once for all sequences (us at 9000 positions
+// and heads of 128, for all | each by itself: 32 sequences of 20 rows 58 | 164, 8 of 32 rows 40 | 54, 8 of 64
+// rows 50 | 45; past a text that stays in the second level of cache more rows gain too: 8 of 64 at 50000 133 | 154).
+constexpr int64_t kPackedMax = 32;
+// Query rows per kv head that seg_rows_kernel takes, in groups of 16 that each read the keys: up to 32, or up
+// to 64 of up to 1536 keys in all, which the second level of cache then holds (us, it | seg_tiles_kernel: 20 rows
+// of 1024 keys 9.8 | 14.1, of 4 x 4096 21.6 | 23.2, of 16 x 4096 58 | 55; 64 rows of 1000 keys 12 | 15, of
+// 2000 20 | 18).
+constexpr int64_t kRowsMax = 32, kRowsShort = 64, kShort = 1536;
 
 // keys: how many a token may see of its own part.
 SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_t keys, bool shared) {
   SegPlan p{};
-  const int64_t G = Hq / Hk, rows = T * G;
-  const auto clamp = [](int64_t v, int64_t hi) { return v < 1 ? 1 : v > hi ? hi : v; };
-  p.shared = shared && F > 0 && rows <= kRowsMax;
+  const int64_t rows = T * (Hq / Hk), all = B * rows;
+  // Ranges of at least 128 keys (a block for each wave) or four tiles: shorter ones cost more in partial sums than
+  // the waiting that they save (us: 20 rows of 4 x 1024 keys in 128s 14 | 64s 15; 64 rows of 4000 in 256s
+  // 18 | 128s 20 | 512s 20).
+  const auto cut = [](int64_t n, int64_t keys, int64_t least) {
+    const int64_t v = kGroups / n, most = (keys + least - 1) / least;
+    return (int)(v < 1 ? 1 : v > most ? most : v);
+  };
+  p.shared = shared && F > 0 && rows <= kPackedMax;
+  const int64_t most = p.shared ? all : rows;
+  const bool few = most <= kRowsMax || (most <= kRowsShort && (p.shared ? F : B * (F + keys)) <= kShort);
+  // Two row blocks a wave read the tiles half as often from LDS; one makes twice the workgroups, and is taken
+  // while they all run at once (us, two | one, a window of 2048: 2000 tokens of 8 kv heads 82 | 103, 1000 tokens
+  // 88 | 56; 128 packed rows 44 | 49).
+  if (!few) p.tiles = p.shared ? (all > 64 ? 2 : 1) : B * Hk * ((rows + 63) / 64) > kGroups ? 2 : 1;
+  // (the second part costs 20% where products bound the call: 8 x 64 rows of 9000 keys 52 | 43 us)
+  p.parts = all <= 64 ? 2 : 1;
+  const int64_t unit = p.tiles ? 64 * p.tiles : 16, least = p.tiles ? 256 : 128;
+  const int64_t n2 = B * Hk * ((rows + unit - 1) / unit);
+  p.split2 = cut(n2, p.shared ? keys : F + keys, least);
   if (p.shared) {
-    // the fixed part's rows are all sequences', in ranges of at least 128 keys (rows) or four tiles
-    const int64_t all = B * rows;
-    p.tiles1 = all > 32 ? (all > 64 ? 2 : 1) : 0;  // row blocks per wave; 0: seg_rows_kernel
-    p.rt = all > 16 ? 2 : 1;
-    const int64_t unit = p.tiles1 ? 64 * p.tiles1 : 16 * p.rt, n1 = (all + unit - 1) / unit * Hk;
-    const int64_t least = p.tiles1 ? 256 : 128;
-    p.split1 = (int)clamp(kGroups / n1, (F + least - 1) / least);
-    const int64_t n2 = B * Hk * ((rows + unit - 1) / unit);
-    p.split2 = (int)clamp(kGroups / n2, (keys + least - 1) / least);
-    if (p.split1 > kMaxPlanes - 8) p.split1 = kMaxPlanes - 8;
+    const int64_t n1 = Hk * ((all + unit - 1) / unit);
+    p.split1 = cut(n1, F, least);
     if (p.split2 > 8) p.split2 = 8;
+    if (p.split1 > kMaxPlanes - 8) p.split1 = kMaxPlanes - 8;
     p.items1 = (int)(n1 * p.split1);
-    p.items2 = (int)(n2 * p.split2);
-    p.planes = p.split1 + p.split2;
-    return p;
   }
-  const int64_t all = F + keys;
-  if (rows <= kRowsMax) {
-    p.rt = rows <= 16 ? 1 : 2;
-    const int64_t n = B * Hk * ((rows + 16 * p.rt - 1) / (16 * p.rt));
-    p.split2 = (int)clamp(clamp(kGroups / n, (all + 127) / 128), kMaxPlanes);
-    p.items2 = (int)(n * p.split2);
-  } else {
-    p.tiles2 = B * Hk * ((rows + 127) / 128) >= kGroups ? 2 : 1;
-    const int64_t u = p.tiles2 == 2 ? 128 : 64, n = B * Hk * ((rows + u - 1) / u);
-    p.split2 = (int)clamp(clamp(kGroups / n, (all + 255) / 256), kMaxPlanes);
-    p.items2 = (int)(n * p.split2);
-  }
-  p.planes = p.split2;
+  if (p.split2 > kMaxPlanes) p.split2 = kMaxPlanes;
+  p.items2 = (int)(n2 * p.split2);
+  p.planes = p.split1 + p.split2;
   return p;
 }
 
@@ -1024,21 +995,13 @@ int launch_prep(const SegArgs& a, hipStream_t s) {
 template <int D>
 int launch_attend(const SegArgs& a, const SegPlan& p, hipStream_t s) {
   int e = 0;
-  if (p.tiles1 || p.tiles2) {
-    const dim3 grid((unsigned)(p.items1 + p.items2));
-    if (p.tiles1 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 2>), grid, dim3(256), 0, s, a, p);
-    else if (p.tiles1 == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1>), grid, dim3(256), 0, s, a, p);
-    else if (p.tiles2 == 1) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 1>), grid, dim3(256), 0, s, a, p);
-    else hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1>), grid, dim3(256), 0, s, a, p);
-    e = (int)hipGetLastError();
-    if (e) return e;
-  } else {
-    const dim3 grid((unsigned)(p.items1 + p.items2));
-    if (p.rt == 1) hipLaunchKernelGGL((seg_rows_kernel<D, 1>), grid, dim3(256), 0, s, a, p);
-    else hipLaunchKernelGGL((seg_rows_kernel<D, 2>), grid, dim3(256), 0, s, a, p);
-    e = (int)hipGetLastError();
-    if (e) return e;
-  }
+  const dim3 items((unsigned)(p.items1 + p.items2));
+  if (p.tiles == 0) hipLaunchKernelGGL((seg_rows_kernel<D>), items, dim3(256), 0, s, a, p);
+  else if (p.tiles == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1>), items, dim3(256), 0, s, a, p);
+  else if (p.parts == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 2>), items, dim3(256), 0, s, a, p);
+  else hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 1>), items, dim3(256), 0, s, a, p);
+  e = (int)hipGetLastError();
+  if (e) return e;
   if (p.planes > 1) {
     const dim3 grid((unsigned)((int64_t)a.B * a.T * a.Hq));
     if (p.planes <= 16) hipLaunchKernelGGL((seg_combine_kernel<D, 16>), grid, dim3(256), 0, s, a, p.planes);
@@ -1054,7 +1017,7 @@ int64_t seg_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_
                             bool rope) {
   const SegPlan p = seg_plan(B, T, Hq, Hk, F, keys, shared);
   const int64_t rows = B * T * Hq;
-  int64_t b = rope && (p.tiles1 || p.tiles2) ? up256(rows * D * 2) : 0;
+  int64_t b = rope && p.tiles ? up256(rows * D * 2) : 0;
   if (p.planes > 1) b += up256(rows * p.planes * 8) + rows * p.planes * D * 4;
   return b;
 }
@@ -1068,8 +1031,7 @@ int launch_seg_attention(SegArgs a, int64_t D, int64_t keys, bool shared, void* 
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
   char* w = (char*)ws;
   a.qsrc = a.q, a.sqsb = a.sqb, a.sqst = a.sqt;
-  const bool tiles = p.tiles1 || p.tiles2;
-  if (tiles && a.cos) {
+  if (p.tiles && a.cos) {
     a.qn = (uint16_t*)w;
     a.qsrc = a.qn, a.sqst = (int64_t)a.Hq * D, a.sqsb = a.T * a.sqst;
     w += up256(rows * D * 2);
@@ -1077,7 +1039,7 @@ int launch_seg_attention(SegArgs a, int64_t D, int64_t keys, bool shared, void* 
   a.stat = (float*)w;
   if (p.planes > 1) w += up256(rows * p.planes * 8);
   a.part = (float*)w;
-  if (tiles) {  // (seg_rows_kernel does its own)
+  if (p.tiles) {  // (seg_rows_kernel does its own)
     const int e = launch_seg_write(a, D, s);
     if (e) return e;
   }
