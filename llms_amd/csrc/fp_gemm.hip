@@ -415,8 +415,8 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_kernel(StreamArgs a, int
 // loads in one burst 643), 4B QKV 57; a load every second or every MFMA 605, 631;
 // three stages of both operands with all loads in the second half: 4B o 43.5.
 // I8 (four waves): both operands are int8, a 16-bit element of the tile being two of them (a.x holds
-// codes, a.K, a.ldx and a.ldw* count pairs; a.wbytes is a weight row's true length, what lies behind
-// it meets codes of zero). v_mfma_i32_16x16x64_i8 reads the same bytes per lane as the bf16
+// codes, a.K, a.ldx and a.ldw* count pairs; a.wbytes is a weight row's true length in
+// whole dwords, what lies behind it meets codes of zero). v_mfma_i32_16x16x64_i8 reads the same bytes per lane as the bf16
 // instruction, so everything up to the accumulators (int32 bits) is the same, and so is its time:
 // twice the operations. The epilogue multiplies by the scales of weight row (s0, s1) and token (sx).
 // 8B gate-up at 4096 rows (256 x 256): 319 us, 2.59 POP/s (bf16 575 and 1.43 PFLOP/s).

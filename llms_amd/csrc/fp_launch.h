@@ -276,8 +276,8 @@ struct W8A8Args {
 };
 // The int8 x int8 form of the prefill tiles (fp_gemm.hip): codes and weights as pairs of int8 in
 // StreamArgs' 16-bit elements (x: rows of Kp = 2 a.K codes, a multiple of 256; weight rows on 16
-// bytes, a.wbytes long), scales in s0, s1, sx; a.ws holds i8_workspace_bytes. Every operand's byte
-// size is below 2^31.
+// bytes, a.wbytes long in whole dwords, which a buffer's end cuts off or not), scales in s0, s1, sx;
+// a.ws holds i8_workspace_bytes. Every operand's byte size is below 2^31.
 struct I8Args : StreamArgs {
   const float* sx;
   int64_t wbytes;

@@ -223,8 +223,9 @@ struct WeightRows {
     if constexpr (!ALIGNED) {
       const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(p) & 3);
       p -= d;
-      b = (b + d + 3) & ~(int64_t)3;
+      b += d;
     }
+    b = (b + 3) & ~(int64_t)3;  // (a dword that the range ends inside of would read as zero)
     const int64_t far = kOut;
     return {p, b < far ? b : far};
   }
@@ -685,7 +686,7 @@ int launch_w8a8(W8A8Args a, bool gateup, bool aligned, void* ws, hipStream_t s) 
     t.w0 = a.q0, t.ldw0 = a.ldq0 / 2, t.w1 = gateup ? a.q1 : nullptr, t.ldw1 = a.ldq1 / 2;
     t.s0 = a.s0, t.s1 = a.s1, t.y = a.y, t.ldy = a.ldy;
     t.M = a.M, t.N = a.N, t.K = a.Kp / 2;
-    t.sx = a.sx, t.wbytes = a.K;
+    t.sx = a.sx, t.wbytes = (a.K + 3) & ~(int64_t)3;
     t.ws = (float*)((char*)a.sx + up256(a.M * 4));
     return launch_i8(t, gateup, s);
   }

@@ -261,6 +261,22 @@ def test_strides_and_views():
 
 
 @gpu
+@pytest.mark.parametrize("M", [1, 3, 5, 17, 70, 300])
+@pytest.mark.parametrize("K,step", [(1000, 1008), (2541, 2560), (130, 1024)])
+def test_padded_weight_rows(M, K, step):
+    """Rows of any length at a stride of whole 16 bytes: what lies between them has no part."""
+    x, ws = make(M + K, M, K, 130, n=2)
+    xd = x.to(DEV)
+    pad = []
+    for q, s in ws:
+        b = torch.full((130, step), 127, dtype=torch.int8)
+        b[:, :K] = q
+        pad.append((b.to(DEV)[:, :K], s.to(DEV)))
+    check_linear(fk.fused_linear_w8a8(xd, *pad[0]), x, ws[0])
+    check_gate_up(fk.fused_gate_up_silu_w8a8(xd, *pad[0], *pad[1]), x, *ws)
+
+
+@gpu
 @pytest.mark.parametrize("M,K", [(1, 1024), (3, 2541), (12, 2560), (70, 1024), (70, 2541)])
 def test_graph_replays(M, K):
     x, ws = make(M, M, K, 320, n=2)
@@ -328,6 +344,18 @@ def test_swapped_model(fuse_norm, rows):
         assert torch.equal(ffn.down(want), fk.fused_linear_w8a8(want, ffn.down.q, ffn.down.s))
         y = [m(ids, m.alloc_cache(rows + 4), start_pos=0).float() for m in (a, b)]
     assert torch.nn.functional.cosine_similarity(y[0].flatten(), y[1].flatten(), 0) > 0.99
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 6, 40])
+def test_modules_of_odd_sizes(rows):
+    """Weights whose rows are no whole 16 bytes are kept at a stride that is."""
+    lin = torch.nn.Linear(201, 77, bias=False, device=DEV, dtype=torch.bfloat16)
+    f = fk.FusedLinear.from_linear(lin, int8=True, a8=True)
+    assert f.q.shape == (77, 201) and f.q.stride(0) == 208
+    x = make(rows, rows, 201, 1)[0]
+    with torch.inference_mode():
+        check_linear(f(x.to(DEV)), x, (f.q.cpu(), f.s.cpu()))
 
 
 @gpu
