@@ -8,20 +8,20 @@
 // (its keys are read once for all of them); with a fixed part of a few first tokens for each sequence and
 // a ring it is attention with a sliding window and sinks.
 //
-//   - seg_prep_kernel: normalises and rotates q and k (or takes them as they are), writes the new
-//     keys and values into the cache.
 //   - seg_rows_kernel (few rows per kv head) and seg_tiles_kernel (many): a work item is a group of
 //     query rows of one kv head and a range of the key blocks that they see, fixed ones first. Rows are
 //     one sequence's (tokens x heads of the group), or, for a shared fixed part alone, those
 //     of all sequences. An item of all of its rows' keys writes the output, else partial sums.
+//   - seg_prep_kernel, before seg_tiles_kernel: normalises and rotates q and k (or takes them as they are), writes
+//     the new keys and values into the cache. (seg_rows_kernel's items do their own: a launch less.)
 //   - seg_combine_kernel: sums the partials of a row in order.
 //
 // Products as in fp_attn.hip: S^T = K Q^T, so a row's scores lie in one lane column and are the B
 // operand of O^T = V^T P^T as they come. Softmax in fp32 with the maximum followed in steps: p is taken
 // about a reference that is raised (and the sums scaled) when a score passes it by 2^kLift. The
 // sums of p come from the matrix core too, with a row of ones, so they are of p as it enters: in one bf16 part
-// (seg_tiles_kernel where it is bound by the products: 2^-9 of each p, no more than the rounding of the
-// values' own sums to bf16 costs) or two (2^-17; where keys are what bounds, they cost nothing).
+// where more than 64 query rows per kv head read the keys and products bound the call (2^-9 of each p, no more
+// than the rounding of the output itself), else in two (2^-17; where keys bound it, they cost little).
 //
 // An entry that a row does not see has no part in it, whatever it holds. An infinity or a NaN among
 // the values would (0 inf): the sums show it, and then the item is done again with such entries taken
@@ -965,8 +965,8 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
   // while they all run at once (us, two | one, a window of 2048: 2000 tokens of 8 kv heads 82 | 103, 1000 tokens
   // 88 | 56; 128 packed rows 44 | 49).
   if (!few) p.tiles = p.shared ? (all > 64 ? 2 : 1) : B * Hk * ((rows + 63) / 64) > kGroups ? 2 : 1;
-  // (the second part costs 20% where products bound the call: 8 x 64 rows of 9000 keys 52 | 43 us)
-  p.parts = all <= 64 ? 2 : 1;
+  // (the second part costs 20% where products bound the call, as for 8 x 64 rows of 9000 shared keys: 52 | 43 us)
+  p.parts = (shared ? all : rows) <= 64 ? 2 : 1;
   const int64_t unit = p.tiles ? 64 * p.tiles : 16, least = p.tiles ? 256 : 128;
   const int64_t n2 = B * Hk * ((rows + unit - 1) / unit);
   p.split2 = cut(n2, p.shared ? keys : F + keys, least);

@@ -211,7 +211,7 @@ def attention_shared(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: K
         ``[B, T, heads, D]`` bfloat16: attention of the token at position p over positions 0 .. p. Rows past
         a sequence's length, and at device positions outside its own part (whose tokens are not
         written), are zero. Keys of the text are read once for all sequences while they have few tokens
-        each (64 query rows per kv head).
+        each (32 query rows per kv head).
     """
     return _attend("attention_shared", q, k, v, (None, None, 0.0, 0.0), None, None, cache, layer, start_pos, lengths)
 

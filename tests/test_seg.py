@@ -235,6 +235,20 @@ def test_shared_prompts(Hq, Hk, D, B, T, P):
 
 
 @gpu
+@pytest.mark.parametrize("Hq,Hk,D", [(16, 8, 128), (8, 2, 64), (16, 4, 128)])
+@pytest.mark.parametrize("B", [1, 3, 20])
+@pytest.mark.parametrize("P", [300, 1600])
+def test_shared_drafts(Hq, Hk, D, B, P):
+    """Steps of a few tokens: one to five groups of 16 rows, short and longer texts."""
+    g = torch.Generator().manual_seed(B + P + Hq)
+    c, hist = new_shared(g, Hk, P, D, B, 70)
+    starts = [0] * B
+    for i, T in enumerate((4, 8, 9, 16, 17)):
+        counts = [T if (b + i) % 3 else (T * b) // B for b in range(B)]
+        starts = step_shared(g, c, hist, starts, counts, T, Hq, True, True)
+
+
+@gpu
 def test_shared_positions_outside():
     """Rows at device positions before the own part or past it are zero and write nothing."""
     g = torch.Generator().manual_seed(5)
@@ -352,6 +366,61 @@ def test_window_ragged(Hq, Hk, D, window, sinks, B):
     for i, T in enumerate((40, 1, 200, 5, 1, 64, 1, 90, 2)):
         counts = [T if (b + i) % 4 == 0 else (T * (b % 5)) // 4 % (T + 1) for b in range(B)]
         starts = step_window(g, c, hist, starts, counts, T, Hq, True, True)
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hk,D", [(16, 8, 128), (8, 2, 64), (16, 4, 128)])
+@pytest.mark.parametrize("window,sinks", [(300, 4), (1700, 0)])
+@pytest.mark.parametrize("B", [1, 3])
+def test_window_drafts(Hq, Hk, D, window, sinks, B):
+    """Steps of a few tokens: one to five groups of 16 rows, short and longer windows."""
+    g = torch.Generator().manual_seed(B + window + Hq)
+    c, hist = new_window(window, sinks, Hk, D, B)
+    starts = step_window(g, c, hist, [0] * B, [1750 - 30 * b for b in range(B)], 1750, Hq, True, True)
+    for i, T in enumerate((4, 8, 9, 16, 17)):
+        counts = [T if (b + i) % 3 else T // 2 for b in range(B)]
+        starts = step_window(g, c, hist, starts, counts, T, Hq, True, True)
+
+
+@gpu
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("Hq,Hk,D", [(16, 4, 128), (8, 2, 64)])
+def test_norm_and_rope_in_the_call(Hq, Hk, D, window):
+    """The same tokens in one call and in calls of all sizes: the same keys, bit for bit, and of each call the
+    outputs for them. (The queries as the kernels normalise them: a cache's keys, with q in k's place.)"""
+    g = torch.Generator().manual_seed(Hq + window)
+    B, T, P, ops = 3, 60, 20, _lib.ops()
+    gm, cos, sin = ((torch.rand(*s, generator=g) * 2 - 0.5).bfloat16().to(DEV) for s in ((D,), (B, T, D), (B, T, D)))
+    q, k, v = (randn(g, B, T, h, D).to(DEV) for h in (Hq, Hk, Hk))
+    text = [randn(g, Hq, P, D).to(DEV) for _ in range(2)]
+
+    def new(heads):
+        if window:
+            return fk.KVCacheWindow.alloc(1, window, sinks=3, max_step=T, max_batch=B, n_kv_heads=heads, head_dim=D,
+                                          device=DEV)
+        return fk.KVCacheShared([text[0][:heads]], [text[1][:heads]], max_batch=B, max_new=T)
+
+    def call(c, q, k, v, lo, hi):
+        cut = [t[:, lo:hi] for t in (q, k, v, cos, sin)]
+        at = torch.full((B,), (0 if window else P) + lo, device=DEV)
+        return ops.attention_seg(*cut[:3], gm, gm, 1e-6, 1e-5, *cut[3:], *c.parts(0), window, 0, at, None)
+
+    a, b, d = new(Hk), new(Hk), new(Hq)
+    d_call = ops.attention_seg(q, q, q, gm, gm, 1e-6, 1e-6, cos, sin, *d.parts(0), window, 0 if window else P, None, None)
+    assert d_call.shape == q.shape
+    y = [call(a, q, k, v, 0, T)]
+    ends = (1, 4, 12, 28, 45, 60)
+    y.append(torch.cat([call(b, q, k, v, lo, hi) for lo, hi in zip((0, *ends), ends)], 1))
+    assert torch.equal(a.k[0], b.k[0]) and torch.equal(a.v[0], b.v[0])
+    for i in range(B):
+        qn, kn = (c.k[0][i, :, :T].transpose(0, 1).cpu() for c in (d, a))
+        vn = v[i].cpu()
+        if not window:
+            kn, vn = (torch.cat([t[:Hk].transpose(0, 1).cpu(), n]) for t, n in zip(text, (kn, vn)))
+        at = torch.arange(T) + (0 if window else P)
+        e = exact(qn, kn, vn, at, torch.arange(len(kn)), window, 3 if window else 0)
+        check(y[0][i], e, 1)
+        check(y[1][i], e, 1)
 
 
 @gpu
