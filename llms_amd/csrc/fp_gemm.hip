@@ -419,7 +419,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void gemm_kernel(StreamArgs a, int
 // whole dwords, what lies behind it meets codes of zero). v_mfma_i32_16x16x64_i8 reads the same bytes per lane as the bf16
 // instruction, so everything up to the accumulators (int32 bits) is the same, and so is its time:
 // twice the operations. The epilogue multiplies by the scales of weight row (s0, s1) and token (sx).
-// 8B gate-up at 4096 rows (256 x 256): 319 us, 2.59 POP/s (bf16 575 and 1.43 PFLOP/s).
+// 8B gate-up at 4096 rows (256 x 256): 330 us, 2.50 POP/s (bf16 575 and 1.43 PFLOP/s).
 template <int BN, int BM, int WN, int WM, bool GATEUP, bool W8, int BK = kBK, int NS = 2,
           bool SPLIT = false, bool W3 = false, bool I8 = false>
 __global__ __launch_bounds__(WN * WM * kWave) void gemm_tiles_kernel(std::conditional_t<I8, I8Args, StreamArgs> a,
