@@ -737,45 +737,54 @@ __global__ __launch_bounds__(256, RT > 2 ? 1 : 2) void seg_tiles_kernel(SegArgs 
     const int at = own ? (it.c0 + c - it.nf) * KB : c * KB;
     // whether a row of this wave does not see some key (uniform)
     const bool mask = at + KB - 1 > (own ? first.hi_o : first.hi_f) || (own && at < last.lo_o);
-    u32x4 seen[RT][2];
-    if (mask || careful) {
+    u32x4 seen[RT][2], pf[RT][2][PARTS];
+    const auto softmax = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int lo = own ? rk[rt].lo_o : 0, hi = own ? rk[rt].hi_o : rk[rt].hi_f;
-        f32x4 one[4];
+        const float base = S.mx[rt] == -INFINITY ? 0.f : S.mx[rt];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < 4; ++n) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = at + n * 16 + 4 * grp + r;
-            const bool hidden = i < lo || i > hi;
-            if (hidden) s[rt][n][r] = -INFINITY;
-            one[n][r] = hidden ? 0.f : 1.f;
-          }
-        if (careful)
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            u32x4 f[1];
-            split_p<1>(one[2 * n], one[2 * n + 1], f);
-            seen[rt][n] = f[0];
-          }
+          for (int r = 0; r < 4; ++r) s[rt][n][r] = exp2_fast(fmaf(s[rt][n][r], sc, -base));
+          if (n & 1) split_p<PARTS>(s[rt][n - 1], s[rt][n], pf[rt][n / 2]);
+        }
       }
-    }
+    };
     // A row's reference comes from the first tiles that it sees keys of. After one that all of the wave's rows
     // see whole, only the careful pass follows it: exponents then may reach 2^127 (floating point, so p
     // is no less exact for that), and past it the sums are infinite and the item is done again.
-    if (mask || careful || !ready) S.follow(s, sc);
-    if (!mask) ready = true;
-    u32x4 pf[RT][2][PARTS];
+    // (The two ways have their own softmax, and the empty statement keeps them apart: where they meet before it
+    // the scores are moved twice, 64 of 150 instructions beside the products.)
+    if (careful || mask || !ready) {
+      if (mask || careful) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float base = S.mx[rt] == -INFINITY ? 0.f : S.mx[rt];
+        for (int rt = 0; rt < RT; ++rt) {
+          const int lo = own ? rk[rt].lo_o : 0, hi = own ? rk[rt].hi_o : rk[rt].hi_f;
+          f32x4 one[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+          for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[rt][n][r] = exp2_fast(fmaf(s[rt][n][r], sc, -base));
-        if (n & 1) split_p<PARTS>(s[rt][n - 1], s[rt][n], pf[rt][n / 2]);
+            for (int r = 0; r < 4; ++r) {
+              const int i = at + n * 16 + 4 * grp + r;
+              const bool hidden = i < lo || i > hi;
+              if (hidden) s[rt][n][r] = -INFINITY;
+              one[n][r] = hidden ? 0.f : 1.f;
+            }
+          if (careful)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              u32x4 f[1];
+              split_p<1>(one[2 * n], one[2 * n + 1], f);
+              seen[rt][n] = f[0];
+            }
+        }
       }
+      S.follow(s, sc);
+      if (!mask) ready = true;
+      softmax();
+    } else {
+      softmax();
+      asm volatile("");
     }
     // these values have landed (behind them: the next keys and values), and every wave is done with the keys
     __builtin_amdgcn_sched_barrier(0);
@@ -869,9 +878,11 @@ __global__ __launch_bounds__(256, RT > 2 ? 1 : 2) void seg_tiles_kernel(SegArgs 
     pass(std::true_type{});
   }
 
+  int lj = li;
+  asm volatile("" : "+v"(lj));  // (so that no address of this is kept from before the tiles)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = row0 + rt * 16 + li;
+    const int r = row0 + rt * 16 + lj;
     if (r >= it.rows) continue;
     const float l = S.sum[rt][0];
     if (pl.planes > 1) {
