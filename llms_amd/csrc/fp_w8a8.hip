@@ -452,6 +452,9 @@ __global__ __launch_bounds__(256, 3) void w8a8_rows_kernel(W8A8Args a) {
 // go through registers into LDS (rows of any alignment cannot take the direct way), the next step's
 // loads in flight while one is computed. 16-byte chunk c of row r lies at c ^ (r & 7): the eight
 // rows that a fragment read touches at once are on distinct banks.
+// Bound by the way through registers (two stages of them; four are slower, 36 us against 33). 64 weight rows and
+// 128 tokens (us, 128 x 64 | 128 x 128 | this: 9700 x 2541 at 64 tokens 22 | 26 | 19, at 300 31 | 29 | 27, at 2000
+// 132 | 95 | 108; 2600 x 4097 at 300 31 | 37 | 26); with a column tile's workgroups spread over the XCDs 36 at 300.
 template <int BN, int BM, bool GATEUP>
 __global__ __launch_bounds__(256, 2) void w8a8_general_kernel(W8A8Args a) {
   constexpr int FN = BN / 32, FM = BM / 32;       // MFMA blocks per wave
@@ -463,7 +466,8 @@ __global__ __launch_bounds__(256, 2) void w8a8_general_kernel(W8A8Args a) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wn = wave >> 1, wm = wave & 1, li = lane & 15, grp = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.x * BM, c0 = (int64_t)blockIdx.y * COLS;
+  const int64_t m0 = (int64_t)(blockIdx.x / 8) * BM, c0 = ((int64_t)blockIdx.y * 8 + blockIdx.x % 8) * COLS;
+  if (c0 >= a.N) return;
   const int nk = (int)((a.K + 2 * kStep - 1) / (2 * kStep)) * 2;  // an even count: codes of zero behind K
 
   const WeightRows rows[2] = {WeightRows::at<false>(a.q0, a.ldq0, c0, a.N, a.K),
@@ -607,9 +611,10 @@ int launch_prep(const W8A8Args& a, hipStream_t s) {
 
 template <bool GATEUP>
 int launch_general(const W8A8Args& a, hipStream_t s) {
-  constexpr int BN = 128, BM = 64;
+  constexpr int BN = 64, BM = 128;
+  // (a column tile's workgroups are eight apart: on one XCD, whose cache then has its weights once)
   const int64_t cols = GATEUP ? BN / 2 : BN;
-  const dim3 grid((unsigned)((a.M + BM - 1) / BM), (unsigned)((a.N + cols - 1) / cols));
+  const dim3 grid((unsigned)((a.M + BM - 1) / BM * 8), (unsigned)((a.N + 8 * cols - 1) / (8 * cols)));
   hipLaunchKernelGGL((w8a8_general_kernel<BN, BM, GATEUP>), grid, dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
