@@ -332,11 +332,13 @@ struct State {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const float mn = fmaxf(mx[rt], col_max(m[rt]) * sc);
-        const float al = mn == -INFINITY ? 1.f : exp2_fast(mx[rt] - mn);
+        // The factor in two halves: the sums may be up to 2^127 about the old reference, so one below 2^-126,
+        // which v_exp_f32 gives as 0, can still leave them a part of the row.
+        const float al = mn == -INFINITY ? 1.f : exp2_fast(0.5f * (mx[rt] - mn));
         mx[rt] = mn;
-        sum[rt] *= al;
+        sum[rt] = sum[rt] * al * al;
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) o[dt][rt] *= al;
+        for (int dt = 0; dt < D / 16; ++dt) o[dt][rt] = o[dt][rt] * al * al;
       }
     }
   }
