@@ -926,18 +926,21 @@ __global__ __launch_bounds__(256) void seg_combine_kernel(SegArgs a, int planes)
   it.b = (int)(t / a.T);
   const int rr = (int)(r - (int64_t)it.b * a.T * G);
   const bool live = row_live(a, it, rr);
-  float m = lane < planes ? st.x : -INFINITY;
+  // A plane's sums may be up to 2^127 about its reference, so the base is above all of the planes' sums, not
+  // their references alone, and the factors are applied in halves (e, twice): so neither does a large sum about a low
+  // reference fall out (below 2^-126 v_exp_f32 gives 0), nor do several pass the largest number together.
+  float m = lane < planes ? st.x + (float)__builtin_amdgcn_frexp_expf(st.y) : -INFINITY;
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
   const float base = m == -INFINITY ? 0.f : m;
-  const float e = lane < planes ? exp2_fast(st.x - base) : 0.f;
-  const float l = wave_sum(lane < planes ? e * st.y : 0.f);
+  const float e = lane < planes ? exp2_fast(0.5f * (st.x - base)) : 0.f;
+  const float l = wave_sum(lane < planes ? st.y * e * e : 0.f);
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int s = n * NG + grp;
     const float w = __shfl(e, s < kWave ? s : 0);  // every lane takes part in the exchange
-    if (s < planes) v += p[n] * w;
+    if (s < planes) v += p[n] * w * w;
   }
   part[grp][q] = v;
   __syncthreads();

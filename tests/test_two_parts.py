@@ -58,3 +58,36 @@ def test_a_score_far_above_those_before(early, late):
     """Of 200 keys one at position 100 counts beside a later one in the tile that the last rows see in part: sums of
     up to 2^127 meet a reference that rises by as much, or by more than an exponential can say."""
     window_apart(200, 200, {100: early, 195: late})
+
+
+@gpu
+@pytest.mark.parametrize("n,spikes", [
+    (1065, {130: 30.75, 260: 31.125}),  # the first range's largest comes late, the second's early
+    (1065, {130: 31.0, 260: 31.25, 700: 30.875}),
+    (1065, {130: 31.25, 386: 31.25, 642: 31.25, 898: 31.25}),  # each range's sum is near the largest number
+    (1065, {130: 31.25, 140: 45.0, 386: 31.25, 642: 45.0}),
+    (16449, {320 * i + 130: 30.25 for i in range(51)}),  # and together they are past it
+])
+def test_scores_apart_in_ranges(n, spikes):
+    """The same where a row's keys are cut into ranges."""
+    window_apart(n, 65, spikes)
+
+
+@gpu
+@pytest.mark.parametrize("spikes", [{130: 30.75, 270: 31.125}, {256 * i + 130: 31.25 for i in range(8)}])
+@pytest.mark.parametrize("B", [20, 40])
+def test_scores_apart_in_a_shared_text(B, spikes):
+    """And of rows of all sequences over one text."""
+    g = torch.Generator().manual_seed(B)
+    P, Hq = 2048, 8
+    k, v, own = along(P, 128, spikes), randn(g, P, 1, 128), randn(g, B, 1, 1, 128)
+    for p in spikes:
+        v[p] = v[p].sign() / 2
+    c = fk.KVCacheShared([k.transpose(0, 1).to(DEV)], [v.transpose(0, 1).to(DEV)], max_batch=B, max_new=4)
+    q = torch.zeros(B, 1, Hq, 128).bfloat16()
+    q[..., 0] = 32
+    y = fk.attention_shared(q.to(DEV), torch.zeros_like(own).to(DEV), own.to(DEV), c, 0, P)
+    for b in range(B):
+        e = exact(q[b], torch.cat([k, torch.zeros_like(own[b])]), torch.cat([v, own[b]]), torch.tensor([P]),
+                  torch.arange(P + 1))
+        check_apart(y[b], e)
