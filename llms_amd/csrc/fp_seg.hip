@@ -753,8 +753,9 @@ __global__ __launch_bounds__(256, RT > 2 ? 1 : 2) void seg_tiles_kernel(SegArgs 
       }
     };
     // A row's reference comes from the first tiles that it sees keys of. After one that all of the wave's rows
-    // see whole, only the careful pass follows it: exponents then may reach 2^127 (floating point, so p
-    // is no less exact for that), and past it the sums are infinite and the item is done again.
+    // see whole, and that has given each a reference, only the careful pass follows it: exponents then may reach
+    // 2^127 (floating point, so p is no less exact for that), and past it the sums are infinite and the item is
+    // done again.
     // (The two ways have their own softmax, and the empty statement keeps them apart: where they meet before it
     // the scores are moved twice, 64 of 150 instructions beside the products.)
     if (careful || mask || !ready) {
@@ -782,7 +783,12 @@ __global__ __launch_bounds__(256, RT > 2 ? 1 : 2) void seg_tiles_kernel(SegArgs 
         }
       }
       S.follow(s, sc);
-      if (!mask) ready = true;
+      if (!mask) {  // (scores of the negative infinity alone give no reference)
+        bool all = true;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) all &= S.mx[rt] > -INFINITY;
+        ready = __all(all);
+      }
       softmax();
     } else {
       softmax();

@@ -91,3 +91,19 @@ def test_scores_apart_in_a_shared_text(B, spikes):
         e = exact(q[b], torch.cat([k, torch.zeros_like(own[b])]), torch.cat([v, own[b]]), torch.tensor([P]),
                   torch.arange(P + 1))
         check_apart(y[b], e)
+
+
+@gpu
+@pytest.mark.parametrize("n,T", [(200, 5), (200, 100), (1065, 65)])
+@pytest.mark.parametrize("x", [float("-inf"), torch.finfo(torch.bfloat16).min])
+def test_first_keys_of_no_weight(n, T, x):
+    """A whole tile whose scores are all the negative infinity comes before the others."""
+    g = torch.Generator().manual_seed(n)
+    c, _ = new_window(n, 0, 1, 128, 1, max_step=n)
+    q, k, v = randn(g, T, 1, 128), randn(g, n, 1, 128), randn(g, n, 1, 128)
+    k[:70, :, 0] = x
+    q[:, :, 0] = q[:, :, 0].abs() + 32
+    c.write(0, k[None].to(DEV), v[None].to(DEV), 0)
+    y = fk.attention_window(q[None].to(DEV), k[None, n - T :].to(DEV), v[None, n - T :].to(DEV), c, 0, n - T)
+    at = torch.arange(n)
+    check_apart(y[0], exact(q, k, v, at[n - T :], at))
