@@ -324,10 +324,9 @@ struct SegArgs {
   float *part, *stat;  // partial sums [planes][Hk][B T G][D] and their {max, sum}
 };
 // How a call's work is cut: items of the fixed part for all sequences together (shared), then of each
-// sequence; planes of partial sums (1: none); row blocks per wave of seg_tiles_kernel (tiles; 0: seg_rows_kernel)
-// and the bf16 parts of p.
+// sequence; planes of partial sums (1: none); row blocks per wave of seg_tiles_kernel (tiles; 0: seg_rows_kernel).
 struct SegPlan {
-  int items1, split1, items2, split2, planes, tiles, parts, shared;
+  int items1, split1, items2, split2, planes, tiles, shared;
 };
 // keys: how many positions of the own part a token may see.
 int64_t seg_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t F, int64_t keys, bool shared,

@@ -18,10 +18,9 @@
 //
 // Products as in fp_attn.hip: S^T = K Q^T, so a row's scores lie in one lane column and are the B
 // operand of O^T = V^T P^T as they come. Softmax in fp32 with the maximum followed in steps: p is taken
-// about a reference that is raised (and the sums scaled) when a score passes it by 2^kLift. The
-// sums of p come from the matrix core too, with a row of ones, so they are of p as it enters: in one bf16 part
-// where more than 64 query rows per kv head read the keys and products bound the call (2^-9 of each p, no more
-// than the rounding of the output itself), else in two (2^-17; where keys bound it, they cost little).
+// about a reference that is raised (and the sums scaled) when a score passes it by 2^kLift. p enters the
+// matrix core in two bf16 parts (off by 2^-17 of each, so that a row's error is its output's rounding), whatever
+// the call's size. The sums of p come from the matrix core too, with a row of ones, so they are of p as it enters.
 //
 // An entry that a row does not see has no part in it, whatever it holds. An infinity or a NaN among
 // the values would (0 inf): the sums show it, and then the item is done again with such entries taken
@@ -51,6 +50,7 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLift = 6.f;
+constexpr int kParts = 2;       // bf16 parts of p
 constexpr int kMaxPlanes = 64;  // one lane per plane in seg_combine_kernel
 
 constexpr int vmcnt_imm(int v) { return (v & 15) | (7 << 4) | (15 << 8) | ((v >> 4) << 14); }
@@ -370,7 +370,7 @@ __device__ __forceinline__ u32x4 ones8() { return u32x4{0x3f803f80u, 0x3f803f80u
 // every one is in some item's; two items of one write the same).
 template <int D>
 __global__ __launch_bounds__(256, 2) void seg_rows_kernel(SegArgs a, SegPlan pl) {
-  constexpr int NW = 4, KB = 32, PARTS = 2;
+  constexpr int NW = 4, KB = 32, PARTS = kParts;
   constexpr int DK = D / 32, DT = D / 16;      // k-steps of q.k, d blocks of p.V
   constexpr int RPI = 1024 / (D * 2);          // V rows per load instruction
   constexpr int NV = KB / RPI, NK = 2 * DK;    // V and K load instructions per block
@@ -587,9 +587,9 @@ __global__ __launch_bounds__(256, 2) void seg_rows_kernel(SegArgs a, SegPlan pl)
 // loads in flight while one is computed.
 // Items: ranges x row tiles (of one sequence, or of all where only a shared fixed part is read) with the kv
 // head fastest, so that one XCD runs a head's tiles.
-template <int D, int RT, int PARTS>
+template <int D, int RT>
 __global__ __launch_bounds__(256, RT > 2 ? 1 : 2) void seg_tiles_kernel(SegArgs a, SegPlan pl) {
-  constexpr int NW = 4, KB = 64;
+  constexpr int NW = 4, KB = 64, PARTS = kParts;
   constexpr int DK = D / 32, DT = D / 16;
   constexpr int RPI = 1024 / (D * 2);          // rows per load instruction
   constexpr int NL = KB / RPI / NW;            // load instructions per wave of a tile's keys
@@ -987,8 +987,6 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
   // while they all run at once (us, two | one, a window of 2048: 2000 tokens of 8 kv heads 82 | 103, 1000 tokens
   // 88 | 56; 128 packed rows 44 | 49).
   if (!few) p.tiles = p.shared ? (all > 64 ? 2 : 1) : B * Hk * ((rows + 63) / 64) > kGroups ? 2 : 1;
-  // (the second part costs 20% where products bound the call, as for 8 x 64 rows of 9000 shared keys: 52 | 43 us)
-  p.parts = (shared ? all : rows) <= 64 ? 2 : 1;
   const int64_t unit = p.tiles ? 64 * p.tiles : 16, least = p.tiles ? 256 : 128;
   const int64_t n2 = B * Hk * ((rows + unit - 1) / unit);
   p.split2 = cut(n2, p.shared ? keys : F + keys, least);
@@ -1019,9 +1017,8 @@ int launch_attend(const SegArgs& a, const SegPlan& p, hipStream_t s) {
   int e = 0;
   const dim3 items((unsigned)(p.items1 + p.items2));
   if (p.tiles == 0) hipLaunchKernelGGL((seg_rows_kernel<D>), items, dim3(256), 0, s, a, p);
-  else if (p.tiles == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2, 1>), items, dim3(256), 0, s, a, p);
-  else if (p.parts == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 2>), items, dim3(256), 0, s, a, p);
-  else hipLaunchKernelGGL((seg_tiles_kernel<D, 1, 1>), items, dim3(256), 0, s, a, p);
+  else if (p.tiles == 2) hipLaunchKernelGGL((seg_tiles_kernel<D, 2>), items, dim3(256), 0, s, a, p);
+  else hipLaunchKernelGGL((seg_tiles_kernel<D, 1>), items, dim3(256), 0, s, a, p);
   e = (int)hipGetLastError();
   if (e) return e;
   if (p.planes > 1) {

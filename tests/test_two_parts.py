@@ -107,3 +107,51 @@ def test_first_keys_of_no_weight(n, T, x):
     y = fk.attention_window(q[None].to(DEV), k[None, n - T :].to(DEV), v[None, n - T :].to(DEV), c, 0, n - T)
     at = torch.arange(n)
     check_apart(y[0], exact(q, k, v, at[n - T :], at))
+
+
+# ------------------------------------------------------------- precision
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hk,D", [(16, 8, 128), (8, 2, 64), (7, 1, 128)])
+@pytest.mark.parametrize("B,T", [(1, 200), (2, 90), (1, 1000)])
+def test_prompts_take_p_in_two_parts(Hq, Hk, D, B, T):
+    g = torch.Generator().manual_seed(T + Hq)
+    c, _ = new_window(400, 3, Hk, D, B, max_step=1000)
+    s, text = new_shared(g, Hk, 333, D, B, T)
+    q, k, v = randn(g, B, T, Hq, D, scale=1.5), randn(g, B, T, Hk, D), randn(g, B, T, Hk, D)
+    on = [t.to(DEV) for t in (q, k, v)]
+    y, z = fk.attention_window(*on, c, 0, 0), fk.attention_shared(*on, s, 0, 333)
+    at = torch.arange(T)
+    for b in range(B):
+        check(y[b], exact(q[b], k[b], v[b], at, at, 400, 3), 2)
+        kv = [torch.cat([text[b][n], t[b]]) for n, t in (("k", k), ("v", v))]
+        check(z[b], exact(q[b], *kv, 333 + at, torch.arange(333 + T)), 2)
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hk,D", [(32, 8, 128), (8, 2, 64)])
+@pytest.mark.parametrize("B", [2, 17, 33, 64])
+def test_precision_of_a_sequence_does_not_depend_on_the_batch(Hq, Hk, D, B):
+    g = torch.Generator().manual_seed(B)
+    P, T = 700, 3
+    s, text = new_shared(g, Hk, P, D, B, 8)
+    q, k, v = randn(g, B, T, Hq, D, scale=1.5), randn(g, B, T, Hk, D), randn(g, B, T, Hk, D)
+    y = fk.attention_shared(q.to(DEV), k.to(DEV), v.to(DEV), s, 0, P)
+    at = torch.arange(T)
+    for b in (0, 1, B - 1):
+        kv = [torch.cat([text[b][n], t[b]]) for n, t in (("k", k), ("v", v))]
+        check(y[b], exact(q[b], *kv, P + at, torch.arange(P + T)), 2)
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hk,D,B,T", [(32, 8, 128, 128, 9), (16, 8, 64, 70, 30), (12, 4, 128, 150, 16)])
+def test_few_rows_of_many_sequences(Hq, Hk, D, B, T):
+    """More than 512 row tiles, each of 33 to 64 rows."""
+    g = torch.Generator().manual_seed(B)
+    c, _ = new_window(300, 4, Hk, D, B)
+    q, k, v = randn(g, B, T, Hq, D, scale=1.5), randn(g, B, 400 + T, Hk, D), randn(g, B, 400 + T, Hk, D)
+    c.write(0, k[:, :400].to(DEV), v[:, :400].to(DEV), 0)
+    y = fk.attention_window(q.to(DEV), k[:, 400:].to(DEV), v[:, 400:].to(DEV), c, 0, 400)
+    for b in (0, 1, B // 2, B - 1):
+        check(y[b], exact(q[b], k[b], v[b], 400 + torch.arange(T), torch.arange(400 + T), 300, 4), 2)
