@@ -984,9 +984,10 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
   const int64_t most = p.shared ? all : rows;
   const bool few = most <= kRowsMax || (most <= kRowsShort && (p.shared ? F : B * (F + keys)) <= kShort);
   // Two row blocks a wave read the tiles half as often from LDS; one makes twice the workgroups, and is taken
-  // while they all run at once (us, two | one, a window of 2048: 2000 tokens of 8 kv heads 82 | 103, 1000 tokens
-  // 88 | 56; 128 packed rows 44 | 49).
-  if (!few) p.tiles = p.shared ? (all > 64 ? 2 : 1) : B * Hk * ((rows + 63) / 64) > kGroups ? 2 : 1;
+  // while they all run at once (us, two | one, a window of 2048: 2000 tokens of 8 kv heads 104 | 120, 1000 tokens
+  // 97 | 64; 256 packed rows 73 | 78, 128 52 | 52, 160 59 | 57).
+  // Up to 64 rows one is all that there is (128 sequences of 36 rows on a window of 300: 51 | 43).
+  if (!few) p.tiles = most > 64 && (p.shared || B * Hk * ((rows + 63) / 64) > kGroups) ? 2 : 1;
   const int64_t unit = p.tiles ? 64 * p.tiles : 16, least = p.tiles ? 256 : 128;
   const int64_t n2 = B * Hk * ((rows + unit - 1) / unit);
   p.split2 = cut(n2, p.shared ? keys : F + keys, least);
