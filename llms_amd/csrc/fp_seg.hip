@@ -959,18 +959,22 @@ __global__ __launch_bounds__(256) void seg_combine_kernel(SegArgs a, int planes)
 // ---- plan ---------------------------------------------------------------------------
 
 constexpr int kGroups = 512;  // workgroups that a call aims at: two per CU
-// Rows of a sequence and kv head up to which a shared text is read once for all sequences (us at 9000 positions
-// and heads of 128, for all | each by itself: 32 sequences of 20 rows 58 | 164, 8 of 32 rows 40 | 54, 8 of 64
-// rows 50 | 45; past a text that stays in the second level of cache more rows gain too: 8 of 64 at 50000 133 | 154).
+// Rows of a sequence and kv head up to which a shared text is read once for all sequences (us, for all | each by
+// itself, heads of 128: 32 sequences of 20 rows of 9000 positions 61 | 162, 8 of 32 rows 40 | 51, 8 of 40 rows 41 | 40,
+// 8 of 64 rows 50 | 46). It does not weigh the text's length: past what the second level of cache holds more rows
+// can gain (8 of 64 rows of 25000 90 | 92, of 50000 151 | 166, but 32 of 64 rows of 50000 729 | 620), and with many
+// rows of a short one packing loses (32 of 32 rows of 2000 48 | 42).
 constexpr int64_t kPackedMax = 32;
-// Query rows per kv head that seg_rows_kernel takes, in groups of 16 that each read the keys: up to 32, or up
-// to 64 of up to 1536 keys in all, which the second level of cache then holds (us, it | seg_tiles_kernel: 20 rows
-// of 1024 keys 9.8 | 14.1, of 4 x 4096 21.6 | 23.2, of 16 x 4096 58 | 55; 64 rows of 1000 keys 12 | 15, of
-// 2000 20 | 18).
-constexpr int64_t kRowsMax = 32, kRowsShort = 64, kShort = 1536;
+// Query rows per kv head that seg_rows_kernel takes, in groups of 16 that each read the keys: one group; two of up to
+// 4 M elements of keys and while all of their workgroups run at once; up to four of up to 1536 keys in all,
+// which the second level of cache then holds (us, it | seg_tiles_kernel, windows and heads of 128: 16 rows of 16 x 4096
+// keys 49 | 52; 20 rows of 1024 9.5 | 14, of 4 x 4096 21.7 | 22.4, of 8 x 4096 31.9 | 31.9, of 12 x 4096 58 | 43, of
+// 16 x 4096 57 | 53, of 64 x 300 34 | 25, heads of 64: of 32 x 1024 19 | 27; 64 rows of 1000 11 | 16.5, 36 of 2000
+// 13 | 16, of 4 x 2000 19.5 | 19.0; a shared text: 20 rows of 1000 9.8 | 13.4, of 9000 20.1 | 18.4, of 50000 41 | 41).
+constexpr int64_t kRowsOne = 16, kRowsMax = 32, kRowsShort = 64, kKeys = 1 << 22, kShort = 1536;
 
 // keys: how many a token may see of its own part.
-SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_t keys, bool shared) {
+SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t F, int64_t keys, bool shared) {
   SegPlan p{};
   const int64_t rows = T * (Hq / Hk), all = B * rows;
   // Ranges of at least 128 keys (a block for each wave) or four tiles: shorter ones cost more in partial sums than
@@ -982,7 +986,9 @@ SegPlan seg_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t F, int64_
   };
   p.shared = shared && F > 0 && rows <= kPackedMax;
   const int64_t most = p.shared ? all : rows;
-  const bool few = most <= kRowsMax || (most <= kRowsShort && (p.shared ? F : B * (F + keys)) <= kShort);
+  const int64_t in_all = p.shared ? F : B * (F + keys), heads = p.shared ? Hk : B * Hk;
+  const bool few = most <= kRowsOne || (most <= kRowsMax && in_all * D <= kKeys && 2 * heads <= kGroups) ||
+                   (most <= kRowsShort && in_all <= kShort);
   // Two row blocks a wave read the tiles half as often from LDS; one makes twice the workgroups, and is taken
   // while they all run at once (us, two | one, a window of 2048: 2000 tokens of 8 kv heads 104 | 120, 1000 tokens
   // 97 | 64; 256 packed rows 73 | 78, 128 52 | 52, 160 59 | 57).
@@ -1035,7 +1041,7 @@ int launch_attend(const SegArgs& a, const SegPlan& p, hipStream_t s) {
 
 int64_t seg_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t F, int64_t keys, bool shared,
                             bool rope) {
-  const SegPlan p = seg_plan(B, T, Hq, Hk, F, keys, shared);
+  const SegPlan p = seg_plan(B, T, Hq, Hk, D, F, keys, shared);
   const int64_t rows = B * T * Hq;
   int64_t b = rope && p.tiles ? up256(rows * D * 2) : 0;
   if (p.planes > 1) b += up256(rows * p.planes * 8) + rows * p.planes * D * 4;
@@ -1047,7 +1053,7 @@ int launch_seg_write(const SegArgs& a, int64_t D, hipStream_t s) {
 }
 
 int launch_seg_attention(SegArgs a, int64_t D, int64_t keys, bool shared, void* ws, hipStream_t s) {
-  const SegPlan p = seg_plan(a.B, a.T, a.Hq, a.Hk, a.F, keys, shared);
+  const SegPlan p = seg_plan(a.B, a.T, a.Hq, a.Hk, D, a.F, keys, shared);
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
   char* w = (char*)ws;
   a.qsrc = a.q, a.sqsb = a.sqb, a.sqst = a.sqt;

@@ -145,9 +145,9 @@ def test_precision_of_a_sequence_does_not_depend_on_the_batch(Hq, Hk, D, B):
 
 
 @gpu
-@pytest.mark.parametrize("Hq,Hk,D,B,T", [(32, 8, 128, 128, 9), (16, 8, 64, 70, 30), (12, 4, 128, 150, 16)])
+@pytest.mark.parametrize("Hq,Hk,D,B,T", [(32, 8, 128, 128, 9), (16, 8, 64, 70, 30), (12, 4, 128, 150, 16), (32, 8, 128, 64, 5)])
 def test_few_rows_of_many_sequences(Hq, Hk, D, B, T):
-    """More than 512 row tiles, each of 33 to 64 rows."""
+    """More than 512 row tiles, each of 20 to 64 rows."""
     g = torch.Generator().manual_seed(B)
     c, _ = new_window(300, 4, Hk, D, B)
     q, k, v = randn(g, B, T, Hq, D, scale=1.5), randn(g, B, 400 + T, Hk, D), randn(g, B, 400 + T, Hk, D)
