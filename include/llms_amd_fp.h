@@ -407,7 +407,8 @@ int fp_kv8_read(const fp_kv8_args* args, float* k_out, float* v_out, void* strea
  * fp_seg_attention writes the new keys and values (of the tokens that there are), then attends with scale
  * head_dim^-0.5, softmax in fp32. Rows past a sequence's length, or at a position outside the cache (a
  * ring takes 0 .. 2^30 - 1), are zero and write nothing; an entry that a row does not see has no part
- * in it, a value that is not finite makes the rows that see it NaN in its column. fp_seg_write only writes
+ * in it, a value that is not finite makes the rows that see it NaN in its column, a score that is NaN or the
+ * positive infinity all of its row (the negative infinity has no weight). fp_seg_write only writes
  * (q, y unused). A text shared by all is not written to: its positions are outside the cache.
  * head_dim 64 or 128; rows, strides and pointers on 16 bytes (cos, sin: 2); each head's part under 2^31
  * bytes. workspace: at least fp_seg_workspace_bytes(..., keys, shared, rope), 16-byte aligned, with

@@ -7,8 +7,9 @@ The reference has neither (its cache is one tensor per layer, ``src/engine/kv_ca
 Both caches are bf16 and have a fixed part, positions ``0 .. n - 1`` (the shared text, or
 the first tokens), and an own part of each sequence. One kernel family attends over both
 (``llms_amd/csrc/fp_seg.hip``): softmax in fp32 with scale ``D ** -0.5`` over the entries that
-a token sees. What it does not see has no part in it, whatever it holds. A key that is not finite
-spoils the rows that see it, such a value its column in them (NaN).
+a token sees. What it does not see has no part in it, whatever it holds. A row that sees a score that is NaN or
+the positive infinity is NaN (a score of the negative one has no weight, as in torch), and so is the column of a value
+that is not finite in the rows that see it.
 
 Path: wrapper -> ``torch.ops.llms_amd.attention_seg`` / ``write_seg`` -> C ABI
 ``fp_seg_attention`` / ``fp_seg_write`` -> HIP kernels on torch's current stream.

@@ -155,3 +155,29 @@ def test_few_rows_of_many_sequences(Hq, Hk, D, B, T):
     y = fk.attention_window(q.to(DEV), k[:, 400:].to(DEV), v[:, 400:].to(DEV), c, 0, 400)
     for b in (0, 1, B // 2, B - 1):
         check(y[b], exact(q[b], k[b], v[b], 400 + torch.arange(T), torch.arange(400 + T), 300, 4), 2)
+
+
+# ------------------------------------------------------------- keys that are not finite
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 5, 100])
+@pytest.mark.parametrize("x", [float("inf"), float("-inf"), float("nan")])
+def test_keys_that_are_not_finite(T, x):
+    """A row that sees one is NaN where its score is NaN or the positive infinity; a score of the negative one has no
+    weight."""
+    g = torch.Generator().manual_seed(T)
+    n, Hq, Hk, D = 200, 4, 2, 64
+    for dim in (1, D):
+        c, _ = new_window(300, 2, Hk, D, 1, max_step=n)
+        q, k, v = randn(g, T, Hq, D, scale=1.5), randn(g, n, Hk, D), randn(g, n, Hk, D)
+        k[120, 0, :dim] = x
+        k[n - 1, 1, :dim] = x  # seen by the last row alone
+        c.write(0, k[None].to(DEV), v[None].to(DEV), 0)
+        y = fk.attention_window(q[None].to(DEV), k[None, n - T :].to(DEV), v[None, n - T :].to(DEV), c, 0, n - T)
+        at = torch.arange(n)
+        want, size, _ = exact(q, k, v, at[n - T :], at, 300, 2)
+        bad = want.isnan()
+        assert torch.equal(y[0].isnan(), bad)
+        err = (y[0].double() - want).abs()
+        assert (err <= want.abs() * 2.0**-8 + size * (2 * 2.0**-8 + 2.0**-17))[~bad].all()
