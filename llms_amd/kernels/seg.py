@@ -140,8 +140,9 @@ class KVCacheWindow(_TwoParts):
     other in slot ``sinks + (p - sinks) % ring``, with ``ring`` the multiple of 64 that holds a window and a
     step of ``max_step`` tokens. Longer calls are done in steps of that.
 
-    Tokens are written in order. A call may start up to ``max_step`` tokens before the last one written (a
-    rejected draft), not further back: the window there is gone. Positions are under 2^30.
+    Tokens are written in order. A call may take back up to ``max_step`` tokens (a rejected draft): start at
+    ``n - max_step`` or later, where ``n - 1`` is the furthest position written so far, by this call's
+    predecessors or by tokens that were taken back since. Further back the window is gone. Positions are under 2^30.
     """
 
     def __init__(self, k: list, v: list, window: int, sinks: int, max_step: int) -> None:

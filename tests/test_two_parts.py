@@ -181,3 +181,26 @@ def test_keys_that_are_not_finite(T, x):
         assert torch.equal(y[0].isnan(), bad)
         err = (y[0].double() - want).abs()
         assert (err <= want.abs() * 2.0**-8 + size * (2 * 2.0**-8 + 2.0**-17))[~bad].all()
+
+
+# ------------------------------------------------------------- positions
+
+
+@gpu
+@pytest.mark.parametrize("window,max_step", [(65, 64), (1, 64), (1, 128), (129, 128)])
+@pytest.mark.parametrize("again", [1, 5, 64])
+def test_the_furthest_step_back(window, max_step, again):
+    """max_step tokens taken back from a ring that has not a slot to spare, and written anew in steps of any size."""
+    g = torch.Generator().manual_seed(window)
+    Hq, Hk, D, n = 4, 2, 64, 500
+    c, _ = new_window(window, 2, Hk, D, 1, max_step=max_step)
+    assert c.ring == window + max_step - 1
+    k, v = randn(g, n, Hk, D), randn(g, n, Hk, D)
+    c.write(0, k[None].to(DEV), v[None].to(DEV), 0)
+    at = torch.arange(n)
+    for start in range(n - max_step, n, again):
+        T = min(again, n - start)
+        q, k[start : start + T], v[start : start + T] = randn(g, T, Hq, D), randn(g, T, Hk, D), randn(g, T, Hk, D)
+        end = start + T
+        y = fk.attention_window(q[None].to(DEV), *(t[None, start:end].to(DEV) for t in (k, v)), c, 0, start)
+        check(y[0], exact(q, k[:end], v[:end], at[start:end], at[:end], window, 2), 1)
