@@ -176,9 +176,10 @@ class Qwen3Model(nn.Module):
         T = input_ids.shape[1]
         h = self.embed(input_ids)
         if torch.is_tensor(start_pos):
-            if start_pos.dim() and not isinstance(kv_cache, (KVCacheShared, KVCacheWindow)):
+            each = start_pos.dim() > 0 and isinstance(kv_cache, (KVCacheShared, KVCacheWindow))
+            if start_pos.numel() != 1 and not each:
                 raise TypeError(f"positions of each sequence over a {type(kv_cache).__name__}: one is taken for all")
-            rows = start_pos[..., None] + torch.arange(T, device=input_ids.device)
+            rows = (start_pos[..., None] if each else start_pos) + torch.arange(T, device=input_ids.device)
             cos, sin = (t.index_select(0, rows.flatten()).view(*rows.shape, -1) for t in (self.rope_cos, self.rope_sin))
         else:
             cos = self.rope_cos[start_pos:start_pos + T]

@@ -141,8 +141,8 @@ class KVCacheWindow(_TwoParts):
     step of ``max_step`` tokens. Longer calls are done in steps of that.
 
     Tokens are written in order. A call may take back up to ``max_step`` tokens (a rejected draft): start at
-    ``n - max_step`` or later, where ``n - 1`` is the furthest position written so far, by this call's
-    predecessors or by tokens that were taken back since. Further back the window is gone. Positions are under 2^30.
+    ``n - max_step`` or later, where ``n - 1`` is the furthest position written so far (tokens that were taken back
+    count). Further back the window is gone. Positions are under 2^30.
     """
 
     def __init__(self, k: list, v: list, window: int, sinks: int, max_step: int) -> None:

@@ -204,3 +204,27 @@ def test_the_furthest_step_back(window, max_step, again):
         end = start + T
         y = fk.attention_window(q[None].to(DEV), *(t[None, start:end].to(DEV) for t in (k, v)), c, 0, start)
         check(y[0], exact(q, k[:end], v[:end], at[start:end], at[:end], window, 2), 1)
+
+
+def model_of(**kw):
+    c = harness.Cfg(vocab_size=211, hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                    intermediate_size=512, max_position_embeddings=700)
+    m = harness.tiny_model(c, state=harness.tiny_state(c, embed_scale=0.3), device=DEV)
+    return fk.apply_triton_kernels(m, **kw)
+
+
+@gpu
+@pytest.mark.parametrize("kv8", [False, True])
+def test_a_position_in_one_element(kv8):
+    """One sequence's position as [1] is the one for all, over every cache."""
+    f = model_of()
+    ids = torch.randint(0, 211, (1, 40), generator=torch.Generator().manual_seed(1)).to(DEV)
+    with torch.inference_mode():
+        ys = []
+        for shape in ((), (1,)):
+            c = f.alloc_cache(64, kv8=kv8)
+            f(ids[:, :30], c)
+            at = torch.full(shape, 30, device=DEV)
+            ys.append((f(ids[:, 30:31], c, start_pos=at), f(ids[:, 31:], c, start_pos=at + 1)))
+        for a, b in zip(*ys):
+            assert a.shape == b.shape and (a.float() - b.float()).abs().max() <= 0.02 * a.float().std()
