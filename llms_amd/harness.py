@@ -170,18 +170,24 @@ class Qwen3Model(nn.Module):
         """Logits for ``input_ids`` [B, T] at positions start_pos ..; an int
         start_pos (default ``kv_cache.cur_len``) advances ``cur_len``, a 0-dim
         device tensor (graph mode) leaves it to the caller, as one of [B] positions
-        does (sequences of different lengths; a ``KVCacheShared`` or ``KVCacheWindow``)."""
+        does (sequences of different lengths; a ``KVCacheShared`` or ``KVCacheWindow``). A
+        device position outside the RoPE table takes the table's nearest row."""
         if start_pos is None:
             start_pos = kv_cache.cur_len
-        T = input_ids.shape[1]
+        T, table = input_ids.shape[1], self.rope_cos.shape[0]
         h = self.embed(input_ids)
         if torch.is_tensor(start_pos):
             each = start_pos.dim() > 0 and isinstance(kv_cache, (KVCacheShared, KVCacheWindow))
             if start_pos.numel() != 1 and not each:
                 raise TypeError(f"positions of each sequence over a {type(kv_cache).__name__}: one is taken for all")
-            rows = (start_pos[..., None] if each else start_pos) + torch.arange(T, device=input_ids.device)
+            rows = start_pos[..., None] if each else start_pos.reshape(1)
+            if T > 1:
+                rows = rows + torch.arange(T, device=input_ids.device)
+            rows = rows.clamp(0, table - 1)
             cos, sin = (t.index_select(0, rows.flatten()).view(*rows.shape, -1) for t in (self.rope_cos, self.rope_sin))
         else:
+            if not 0 <= start_pos <= table - T:
+                raise ValueError(f"positions {start_pos} .. {start_pos + T - 1} are outside the RoPE table of {table}")
             cos = self.rope_cos[start_pos:start_pos + T]
             sin = self.rope_sin[start_pos:start_pos + T]
         for i, layer in enumerate(self.layers):
@@ -331,6 +337,9 @@ class StepGraph:
         torch.cuda.synchronize(dev)
 
     def __call__(self, ids: torch.Tensor, pos) -> torch.Tensor:
+        table = self.model.rope_cos.shape[0]
+        if not torch.is_tensor(pos) and not 0 <= pos <= table - self.T:
+            raise ValueError(f"positions {pos} .. {pos + self.T - 1} are outside the RoPE table of {table}")
         self.ids.copy_(ids)
         self.pos.copy_(pos) if torch.is_tensor(pos) else self.pos.fill_(pos)
         self.graph.replay()

@@ -228,3 +228,53 @@ def test_a_position_in_one_element(kv8):
             ys.append((f(ids[:, 30:31], c, start_pos=at), f(ids[:, 31:], c, start_pos=at + 1)))
         for a, b in zip(*ys):
             assert a.shape == b.shape and (a.float() - b.float()).abs().max() <= 0.02 * a.float().std()
+
+
+def small(device="cpu", **kw):
+    c = harness.Cfg(vocab_size=40, hidden_size=64, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=1,
+                    head_dim=64, intermediate_size=64, **{"max_position_embeddings": 20, **kw})
+    return harness.tiny_model(c, device=device)
+
+
+def test_positions_past_the_rope_table():
+    """Host positions are refused; device ones read no row that is not there (here the eager attention's refusal of the
+    cache, not an index out of range, ends the call)."""
+    m = small()
+    ids = torch.zeros(1, 3, dtype=torch.long)
+    with torch.inference_mode():
+        assert m(ids, m.alloc_cache(30), start_pos=17).shape == (1, 3, 40)
+        for at in (18, 19, 20, 1000, -1):
+            with pytest.raises(ValueError, match="RoPE table of 20"):
+                m(ids, m.alloc_cache(30), start_pos=at)
+        cache = m.alloc_cache(30, window=4)
+        for at in ([18], [-1], [1 << 40]):
+            with pytest.raises(TypeError, match="apply_triton_kernels"):
+                m(ids, cache, start_pos=torch.tensor(at))
+        # within the table a device position is the host's
+        a, b = m.alloc_cache(20), m.alloc_cache(20)
+        for c, at in ((a, 0), (b, torch.tensor(0))):
+            m(ids, c, start_pos=at)
+        for n in (1, 2):
+            y, z = m(ids[:, :n], a, start_pos=3), m(ids[:, :n], b, start_pos=torch.tensor(3))
+            assert (y - z).abs().max() <= 0.02 * y.float().std()
+
+
+@gpu
+def test_a_window_model_at_its_table_s_end():
+    f = model_of()
+    ids = torch.randint(0, 211, (1, 698), generator=torch.Generator().manual_seed(1)).to(DEV)
+    with torch.inference_mode():
+        c = f.alloc_cache(900, window=100)
+        f(ids, c)
+        with pytest.raises(ValueError, match="RoPE table"):
+            f(ids[:, :3], c)
+        step = harness.StepGraph(f, c, T=2)
+        with pytest.raises(ValueError, match="RoPE table"):
+            step(ids[:, :2], 699)
+        y = step(ids[:, :2], 698).clone()
+        assert torch.equal(y, f(ids[:, :2], c))
+        s = harness.StepGraph(f, c, T=1, per_sequence=True)
+        s(ids[:, :1], torch.tensor([700], device=DEV))  # past the table: its last row
+        s(ids[:, :1], torch.tensor([-3], device=DEV))
+    with pytest.raises(ValueError, match="RoPE table"):
+        harness.greedy_generate(f, ids[0].tolist(), 8, DEV, window=100)
