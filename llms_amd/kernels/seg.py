@@ -237,10 +237,12 @@ def attention_core_seg(q, k, v, *, q_norm, k_norm, num_heads: int, cache: _TwoPa
     are ``[T, D]``, or ``[B, T, D]`` for sequences at different positions. Returns ``[B, T, num_heads * D]``."""
     fn, D = "attention_window" if cache.window else "attention_shared", cache.head_dim
     B, T, _ = q.shape
+    if any(t.shape not in ((T, D), (B, T, D)) for t in (cos, sin)):  # (one row would be every token's in torch)
+        raise ValueError(f"{fn}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be {(T, D)} or {(B, T, D)}")
     fused = (plain_norm(q_norm) and plain_norm(k_norm) and not autocast()
              and all(t.dtype == torch.bfloat16 and t.shape == (D,) and t.is_contiguous() and t.data_ptr() % 16 == 0
                      for t in (q_norm.weight, k_norm.weight))
-             and all(t.dtype == torch.bfloat16 and t.shape in ((T, D), (B, T, D)) and t.stride(-1) == 1
+             and all(t.dtype == torch.bfloat16 and t.stride(-1) == 1
                      and t.device == q.device and (T == 1 or t.stride(-2) >= D) for t in (cos, sin))
              and not transformed(q_norm.weight, k_norm.weight, cos, sin))
     if not fused:

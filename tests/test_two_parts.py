@@ -259,6 +259,18 @@ def test_positions_past_the_rope_table():
             assert (y - z).abs().max() <= 0.02 * y.float().std()
 
 
+def test_rope_rows_of_another_length():
+    """cos and sin must have a row for each token, whatever computes the rotation."""
+    norm = small().layers[0].attn.q_norm
+    c = fk.KVCacheWindow.alloc(1, 8, n_kv_heads=1, head_dim=64, device="cpu")
+    q, k = torch.zeros(1, 3, 128).bfloat16(), torch.zeros(1, 3, 64).bfloat16()
+    for n in (1, 2, 4):
+        for t in (torch.ones(n, 64).bfloat16(), torch.ones(n, 64), torch.ones(1, n, 64)):
+            with pytest.raises(ValueError, match=r"must be \(3, 64\)"), torch.inference_mode():
+                fk.seg.attention_core_seg(q, k, k, q_norm=norm, k_norm=norm, num_heads=2, cache=c, layer=0, cos=t, sin=t,
+                                          start_pos=0)
+
+
 @gpu
 def test_a_window_model_at_its_table_s_end():
     f = model_of()
