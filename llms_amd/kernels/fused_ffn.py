@@ -20,7 +20,7 @@ from torch import nn
 
 from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
-from .quant import pack_weight
+from .quant import PaddedRows, pack_weight
 from .w4 import fused_gate_up_silu_w4, fused_rmsnorm_gate_up_silu_w4
 from .w8a8 import fused_gate_up_silu_w8a8, fused_rmsnorm_gate_up_silu_w8a8
 
@@ -101,7 +101,7 @@ def fused_gate_up_silu_w8(
     return y.reshape(*leading_shape, N)
 
 
-class TritonFFN(nn.Module):
+class TritonFFN(PaddedRows, nn.Module):
     """Drop-in for the reference's ``TritonFFN`` (``src/kernels/fused_ffn.py:155-185``):
     ``down(fused_gate_up_silu(x, gate.weight, up.weight))``; parameter names
     ``gate``/``up``/``down`` match the eager ``FFN``.
@@ -119,6 +119,7 @@ class TritonFFN(nn.Module):
     w4_group = 0
     # Whether int8 modules take their tokens in 8 bits too (on the class for the same reason).
     a8 = False
+    codes = ("qg", "qu")
 
     def __init__(self, hidden_size: int, intermediate_size: int) -> None:
         super().__init__()

@@ -19,7 +19,7 @@ from ._checks import inner_contiguous, require_bf16_hip, require_device
 from ._eager import RMSNorm, apply_rope, attend, write_kv
 from .fused_attention import attention_core
 from .kv8 import KVCache8, attention_core_kv8
-from .quant import pack_weight
+from .quant import PaddedRows, pack_weight
 from .seg import KVCacheShared, KVCacheWindow, attention_core_seg
 from .w4 import fused_qkv_w4, fused_rmsnorm_qkv_w4
 from .w8a8 import fused_qkv_w8a8, fused_rmsnorm_qkv_w8a8
@@ -129,7 +129,7 @@ def fused_qkv_w8(
     return q, k, v
 
 
-class TritonAttention(nn.Module):
+class TritonAttention(PaddedRows, nn.Module):
     """Drop-in for the reference's ``TritonAttention``
     (``src/kernels/fused_qkv.py:152-282``): stores one stacked ``W_qkv``
     instead of ``q``/``k``/``v`` Linears and runs the fused HIP projection.
@@ -155,6 +155,7 @@ class TritonAttention(nn.Module):
     w4_group = 0
     # Whether int8 modules take their tokens in 8 bits too (on the class for the same reason).
     a8 = False
+    codes = ("q_qkv",)
 
     def __init__(
         self,

@@ -18,7 +18,7 @@ from torch import nn
 
 from .. import _lib
 from ._checks import inner_contiguous, require_bf16_hip, require_device
-from .quant import pack_weight
+from .quant import PaddedRows, pack_weight
 from .w4 import fused_linear_w4
 from .w8a8 import fused_linear_w8a8
 
@@ -73,7 +73,7 @@ def fused_linear_w8(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.
     return y.reshape(*leading_shape, N)
 
 
-class FusedLinear(nn.Module):
+class FusedLinear(PaddedRows, nn.Module):
     """A bias-free ``nn.Linear`` replacement on the HIP projection kernels.
 
     bf16: keeps the wrapped Linear's ``weight`` Parameter (same state-dict
@@ -86,6 +86,7 @@ class FusedLinear(nn.Module):
     w4_group = 0
     # Whether int8 modules take their tokens in 8 bits too (on the class for the same reason).
     a8 = False
+    codes = ("q",)
 
     def __init__(self, in_features: int, out_features: int) -> None:
         super().__init__()

@@ -63,7 +63,31 @@ def pack_weight(W: torch.Tensor, w4_group: int, a8: bool = False) -> tuple[torch
     if w4_group:
         return quantize_w4(W, w4_group)
     q, s = quantize_w8_per_row(W)
+    return (padded_rows(q) if a8 else q), s
+
+
+def padded_rows(q: torch.Tensor) -> torch.Tensor:
+    """``q [N, K]`` with its rows at a stride of whole 16 bytes (itself where they are)."""
     K = q.shape[1]
-    if a8 and K % 16:
-        q = torch.nn.functional.pad(q, (0, -K % 16))[:, :K]
-    return q, s
+    return q if q.stride(0) % 16 == 0 or K % 16 == 0 else torch.nn.functional.pad(q, (0, -K % 16))[:, :K]
+
+
+class PaddedRows:
+    """Base of the modules that hold int8 codes: with ``a8`` the buffers named in ``codes`` lie at padded strides
+    again after ``module.to(..)``, ``load_state_dict(assign=True)`` and the like, which make them dense."""
+
+    a8 = False
+    codes: tuple = ()
+
+    def _repad(self) -> None:
+        for name in self.codes if self.a8 else ():
+            setattr(self, name, padded_rows(getattr(self, name)))
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._repad()
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._repad()
