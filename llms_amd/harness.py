@@ -147,16 +147,17 @@ class Qwen3Model(nn.Module):
         self.register_buffer("rope_sin", sin, persistent=False)
 
     def alloc_cache(self, max_seq_len: int, *, max_batch: int = 1, kv8: bool = False, window: int = 0,
-                    sinks: int = 4) -> KVCache | KVCache8 | KVCacheWindow:
+                    sinks: int = 4, max_step: int = 256) -> KVCache | KVCache8 | KVCacheWindow:
         """A cache for up to ``max_batch`` sequences; ``kv8``: in 8 bits, ``window``: of the last
-        ``window`` tokens and the first ``sinks``, whatever ``max_seq_len`` (both: a swapped model
-        on a HIP device)."""
+        ``window`` tokens and the first ``sinks``, whatever ``max_seq_len``, written in steps of up to
+        ``max_step`` (both: a swapped model on a HIP device). Positions run to the RoPE table's end
+        (``max_position_embeddings``) over every cache."""
         c = self.cfg
         w = self.embed.weight
         if window:
             if kv8:
                 raise ValueError("alloc_cache: window and kv8 exclude each other")
-            return KVCacheWindow.alloc(c.num_hidden_layers, window, sinks=sinks, max_batch=max_batch,
+            return KVCacheWindow.alloc(c.num_hidden_layers, window, sinks=sinks, max_step=max_step, max_batch=max_batch,
                                        n_kv_heads=c.num_key_value_heads, head_dim=c.head_dim, device=w.device)
         if kv8:
             return KVCache8.alloc(c.num_hidden_layers, max_seq_len, max_batch=max_batch,
@@ -252,10 +253,11 @@ def random_model(c: Cfg, *, device="cuda", seed: int = 0, dtype=torch.bfloat16) 
 
 
 def greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device, *,
-                    kv8: bool = False, window: int = 0) -> list[int]:
-    """Prefill the prompt, then decode n_new tokens one at a time (argmax)."""
+                    kv8: bool = False, window: int = 0, sinks: int = 4, max_step: int = 256) -> list[int]:
+    """Prefill the prompt, then decode n_new tokens one at a time (argmax). The cache is
+    ``model.alloc_cache``'s of these arguments."""
     ids = torch.tensor([prompt], dtype=torch.long, device=device)
-    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8, window=window)
+    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8, window=window, sinks=sinks, max_step=max_step)
     out: list[int] = []
     with torch.inference_mode():
         logits = model(ids, cache, start_pos=0)
@@ -347,13 +349,13 @@ class StepGraph:
 
 
 def graph_greedy_generate(model: Qwen3Model, prompt: list[int], n_new: int, device, *,
-                          kv8: bool = False, window: int = 0) -> list[int]:
+                          kv8: bool = False, window: int = 0, sinks: int = 4, max_step: int = 256) -> list[int]:
     """``greedy_generate`` with every decode step replayed from one captured
     ``StepGraph`` (the prefill runs eagerly)."""
     ids = torch.tensor([prompt], dtype=torch.long, device=device)
     if window and len(prompt) + n_new > model.cfg.max_position_embeddings:
         raise ValueError(f"{len(prompt) + n_new} positions, the model has {model.cfg.max_position_embeddings}")
-    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8, window=window)
+    cache = model.alloc_cache(len(prompt) + n_new + 4, kv8=kv8, window=window, sinks=sinks, max_step=max_step)
     with torch.inference_mode():
         logits = model(ids, cache, start_pos=0)
     step = StepGraph(model, cache, T=1)

@@ -290,3 +290,26 @@ def test_a_window_model_at_its_table_s_end():
         s(ids[:, :1], torch.tensor([-3], device=DEV))
     with pytest.raises(ValueError, match="RoPE table"):
         harness.greedy_generate(f, ids[0].tolist(), 8, DEV, window=100)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(sinks=0), dict(sinks=9, max_step=100)])
+def test_a_model_s_window_has_all_of_the_operator_s_sizes(kw):
+    c = small().alloc_cache(50, window=30, max_batch=2, **kw)
+    assert (c.window, c.sinks, c.max_step) == (30, kw.get("sinks", 4), kw.get("max_step", 256))
+    with pytest.raises(ValueError, match="KVCacheWindow"):
+        small().alloc_cache(50, window=30, max_step=0)
+
+
+@gpu
+def test_generation_over_a_window_of_any_sizes():
+    """Steps of another size are the same attention; sinks are not."""
+    f = model_of()
+    prompt = torch.randint(0, 211, (300,), generator=torch.Generator().manual_seed(7)).tolist()
+    kw = dict(window=64, sinks=7)
+    out = harness.greedy_generate(f, prompt, 20, DEV, **kw)
+    assert out == harness.graph_greedy_generate(f, prompt, 20, DEV, **kw)
+    with torch.inference_mode():
+        ids = torch.tensor([prompt], device=DEV)
+        a, b, c = (f(ids, f.alloc_cache(300, window=64, **k)).float() for k in (dict(sinks=7), dict(sinks=7, max_step=300),
+                                                                               dict(sinks=0)))
+        assert (a - b).abs().max() <= 0.05 * a.std() < (a - c).abs().max()
