@@ -115,6 +115,8 @@ class KVCacheShared(_TwoParts):
     def of(cls, cache, length: int, *, max_batch: int, max_new: int) -> "KVCacheShared":
         """The first ``length`` tokens of sequence 0 in a plain cache (``harness.KVCache``: lists ``k``, ``v`` of
         ``[batch, n_kv_heads, max_seq, D]``) as the shared text: views of its tensors."""
+        if isinstance(cache, _TwoParts):  # (its tensors do not hold position p at p)
+            raise TypeError(f"KVCacheShared.of: a text is taken from a plain cache, not a {type(cache).__name__}")
         if not 1 <= length <= cache.k[0].shape[2]:
             raise ValueError(f"KVCacheShared.of: length {length} of a cache of {cache.k[0].shape[2]}")
         return cls([t[0, :, :length] for t in cache.k], [t[0, :, :length] for t in cache.v], max_batch=max_batch,

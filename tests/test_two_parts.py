@@ -313,3 +313,11 @@ def test_generation_over_a_window_of_any_sizes():
         a, b, c = (f(ids, f.alloc_cache(300, window=64, **k)).float() for k in (dict(sinks=7), dict(sinks=7, max_step=300),
                                                                                dict(sinks=0)))
         assert (a - b).abs().max() <= 0.05 * a.std() < (a - c).abs().max()
+
+
+def test_a_shared_text_is_taken_from_a_plain_cache():
+    m = small()
+    text = fk.KVCacheShared.of(m.alloc_cache(30), 10, max_batch=2, max_new=20)
+    for cache in (m.alloc_cache(30, window=16), text):
+        with pytest.raises(TypeError, match="plain cache"):
+            fk.KVCacheShared.of(cache, 5, max_batch=1, max_new=1)
