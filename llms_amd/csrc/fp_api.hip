@@ -306,13 +306,17 @@ int check_attention(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
 
 // ---- a cache of two parts ----
 
+constexpr int64_t kSegMost = (int64_t)1 << 28;  // positions of a part
+// A caller's bound of the keys that a token sees, as the plan takes it.
+int64_t seg_keys(int64_t keys) { return keys < kSegMost ? keys : kSegMost; }
+
 // The checks and the kernels' form of such a call: queries (q, y) or only new tokens (k, v).
 int seg_args(const fp_seg_args& g, bool queries, SegArgs* out) {
   const int64_t D = g.head_dim, F = g.n_fixed, S = g.own_len, Hk = g.n_kv_heads;
   const int st = check_attention(g.B, g.T, queries ? g.n_heads : Hk, Hk, D);
   if (st) return st;
-  constexpr int64_t kMost = (int64_t)1 << 28, kLim = (int64_t)1 << 31;
-  if (F < 0 || F > kMost || S < 1 || S > kMost) return FP_ERR_SHAPE;
+  constexpr int64_t kLim = (int64_t)1 << 31;
+  if (F < 0 || F > kSegMost || S < 1 || S > kSegMost) return FP_ERR_SHAPE;
   if (g.ring ? g.window < 1 || S % 64 != 0 || g.T + g.window - 1 > S : g.window != 0) return FP_ERR_SHAPE;
   const int64_t end = g.ring ? (int64_t)1 << 30 : F + S, first = g.ring ? 0 : F;
   if (!g.pos_dev && (g.pos < first || g.pos > end - g.T)) return FP_ERR_SHAPE;
@@ -343,7 +347,7 @@ int seg_args(const fp_seg_args& g, bool queries, SegArgs* out) {
   a.ok = (uint16_t*)g.own_k, a.ov = (uint16_t*)g.own_v, a.sob = g.own_s_b, a.soh = g.own_s_h, a.sos = g.own_s_p;
   a.y = (uint16_t*)g.y, a.syb = g.y_s_b;
   a.B = (int)g.B, a.T = (int)g.T, a.Hq = (int)g.n_heads, a.Hk = (int)Hk;
-  a.F = (int)F, a.S = (int)S, a.ring = g.ring != 0, a.W = (int)(g.window < kMost ? g.window : kMost);
+  a.F = (int)F, a.S = (int)S, a.ring = g.ring != 0, a.W = (int)(g.window < kSegMost ? g.window : kSegMost);
   a.pos = g.pos, a.pos_dev = g.pos_dev, a.pos_stride = g.pos_stride, a.lengths = g.lengths;
   *out = a;
   return FP_OK;
@@ -788,8 +792,9 @@ int fp_kv8_read(const fp_kv8_args* g, float* k_out, float* v_out, void* stream) 
 
 int64_t fp_seg_workspace_bytes(int64_t B, int64_t T, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
                                int64_t n_fixed, int64_t keys, int shared, int rope) {
-  if (fp::check_attention(B, T, n_heads, n_kv_heads, head_dim) || n_fixed < 0 || keys < 1) return 0;
-  return fp::seg_workspace_bytes(B, T, n_heads, n_kv_heads, head_dim, n_fixed, keys, shared != 0, rope != 0);
+  if (fp::check_attention(B, T, n_heads, n_kv_heads, head_dim) || n_fixed < 0 || n_fixed > fp::kSegMost || keys < 1)
+    return 0;
+  return fp::seg_workspace_bytes(B, T, n_heads, n_kv_heads, head_dim, n_fixed, fp::seg_keys(keys), shared != 0, rope != 0);
 }
 
 int fp_seg_attention(const fp_seg_args* g, int64_t keys, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -798,6 +803,7 @@ int fp_seg_attention(const fp_seg_args* g, int64_t keys, void* workspace, int64_
   const int st = fp::seg_args(*g, true, &a);
   if (st) return st;
   if (keys < 1) return FP_ERR_SHAPE;
+  keys = fp::seg_keys(keys);
   const bool shared = !g->ring && g->n_fixed > 0 && g->fix_s_b == 0;
   const int64_t need = fp::seg_workspace_bytes(g->B, g->T, g->n_heads, g->n_kv_heads, g->head_dim, g->n_fixed, keys,
                                                shared, g->cos != nullptr);

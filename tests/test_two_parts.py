@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from llms_amd import harness
+from llms_amd import _lib, harness
 from llms_amd import kernels as fk
 from tests.test_seg import check, exact, new_shared, new_window, randn
 
@@ -321,3 +321,15 @@ def test_a_shared_text_is_taken_from_a_plain_cache():
     for cache in (m.alloc_cache(30, window=16), text):
         with pytest.raises(TypeError, match="plain cache"):
             fk.KVCacheShared.of(cache, 5, max_batch=1, max_new=1)
+
+
+def test_key_counts_beyond_any_cache():
+    """The C entry plans for at most as many keys as a cache may hold (2^28), whatever it is told."""
+    need = _lib.capi().fp_seg_workspace_bytes
+    for B, T, Hq, Hk, shared in ((1, 1, 4, 2, 0), (3, 5, 4, 2, 1), (2, 100, 4, 4, 0)):
+        most = need(B, T, Hq, Hk, 64, 100, 1 << 28, shared, 0)
+        assert most > 0
+        for keys in ((1 << 28) + 1, 1 << 40, 1 << 61, (1 << 63) - 300, (1 << 63) - 1):
+            assert need(B, T, Hq, Hk, 64, 100, keys, shared, 0) == most, keys
+        for fixed in ((1 << 28) + 1, 1 << 60, (1 << 63) - 1):
+            assert need(B, T, Hq, Hk, 64, fixed, 100, shared, 0) == 0
