@@ -317,7 +317,7 @@ int seg_args(const fp_seg_args& g, bool queries, SegArgs* out) {
   if (st) return st;
   constexpr int64_t kLim = (int64_t)1 << 31;
   if (F < 0 || F > kSegMost || S < 1 || S > kSegMost) return FP_ERR_SHAPE;
-  if (g.ring ? g.window < 1 || S % 64 != 0 || g.T + g.window - 1 > S : g.window != 0) return FP_ERR_SHAPE;
+  if (g.ring ? g.window < 1 || S % 64 != 0 || g.window > S || g.T + g.window - 1 > S : g.window != 0) return FP_ERR_SHAPE;
   const int64_t end = g.ring ? (int64_t)1 << 30 : F + S, first = g.ring ? 0 : F;
   if (!g.pos_dev && (g.pos < first || g.pos > end - g.T)) return FP_ERR_SHAPE;
   if (g.pos_dev && g.pos_stride != 0 && g.pos_stride != 1) return FP_ERR_STRIDE;
@@ -332,7 +332,9 @@ int seg_args(const fp_seg_args& g, bool queries, SegArgs* out) {
   if (F > 0) any |= g.fix_s_b | g.fix_s_h | g.fix_s_p;
   if (queries) any |= g.q_s_b | g.q_s_t | g.y_s_b;
   if (any < 0 || (any & 7) != 0 || (g.cos && (g.cos_s_b < 0 || g.sin_s_b < 0))) return FP_ERR_STRIDE;
-  if ((S + 64) * g.own_s_p * 2 >= kLim || (F > 0 && (F + 64) * g.fix_s_p * 2 >= kLim)) return FP_ERR_SHAPE;
+  if (g.own_s_p >= kLim || (S + 64) * g.own_s_p * 2 >= kLim ||
+      (F > 0 && (g.fix_s_p >= kLim || (F + 64) * g.fix_s_p * 2 >= kLim)))
+    return FP_ERR_SHAPE;
   for (const void* p : {g.q, g.k, g.v, (const void*)g.fix_k, (const void*)g.fix_v, (const void*)g.own_k,
                         (const void*)g.own_v, (const void*)g.y, g.q_gamma, g.k_gamma})
     if (!al16(p)) return FP_ERR_STRIDE;

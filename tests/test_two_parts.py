@@ -3,12 +3,14 @@ the size of a call, positions at a window's and at a table's end."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 from llms_amd import _lib, harness
 from llms_amd import kernels as fk
-from tests.test_seg import check, exact, new_shared, new_window, randn
+from tests.test_seg import SegArgs, check, exact, new_shared, new_window, randn
 
 DEV = "cuda"
 gpu = pytest.mark.gpu
@@ -333,3 +335,16 @@ def test_key_counts_beyond_any_cache():
             assert need(B, T, Hq, Hk, 64, 100, keys, shared, 0) == most, keys
         for fixed in ((1 << 28) + 1, 1 << 60, (1 << 63) - 1):
             assert need(B, T, Hq, Hk, 64, fixed, 100, shared, 0) == 0
+
+
+def test_sizes_that_overflow_are_refused():
+    """Before a launch (there is no GPU here: a launch would not be FP_ERR_SHAPE either)."""
+    a = dict(q=64, k=64, v=64, q_s_b=256, q_s_t=256, k_s_b=128, k_s_t=128, v_s_b=128, v_s_t=128, own_k=64, own_v=64,
+             own_s_b=2 * 128 * 64, own_s_h=128 * 64, own_s_p=64, y=64, y_s_b=256, B=3, T=1, n_heads=4, n_kv_heads=2,
+             head_dim=64, n_fixed=0, own_len=128)
+    fixed = dict(fix_k=64, fix_v=64, fix_s_h=6400, n_fixed=100, pos=100)
+    for kw in (dict(ring=1, window=(1 << 63) - 1), dict(ring=1, window=(1 << 63) - 129, T=128), dict(own_s_p=1 << 60),
+               dict(own_s_p=1 << 62), dict(fixed, fix_s_p=1 << 61), dict(fixed, fix_s_p=(1 << 63) - 8)):
+        for call in (lambda p: _lib.capi().fp_seg_attention(p, 100, 64, 1 << 40, None),
+                     lambda p: _lib.capi().fp_seg_write(p, None)):
+            assert call(ctypes.byref(SegArgs(**(a | kw)))) == 2, kw
