@@ -24,6 +24,7 @@ from ._checks import autocast, plain_norm, refuse_grad, transformed
 from .kv8 import _place
 
 MAX_LEN = 1 << 28
+MAX_POS = 1 << 30  # of a window's cache
 
 
 class _TwoParts:
@@ -46,7 +47,7 @@ class _TwoParts:
         fn = f"{type(self).__name__}.write"
         start, pos = _place(fn, start_pos, lengths)
         refuse_grad(fn, k, v)
-        _check_tokens(fn, k, self)
+        _check_tokens(fn, k, self, start, pos)
         for lo, hi in self._pieces(k.shape[1]):
             s, p, n = _at(lo, hi, k.shape[1], start, pos, lengths)
             _lib.ops().write_seg(k[:, lo:hi], v[:, lo:hi], *self.parts(layer), self.window, s, p, n)
@@ -64,9 +65,12 @@ def _at(lo: int, hi: int, T: int, start: int, pos, lengths):
             None if lengths is None else (lengths - lo).clamp(0, hi - lo))
 
 
-def _check_tokens(fn: str, k: torch.Tensor, cache: _TwoParts) -> None:
+def _check_tokens(fn: str, k: torch.Tensor, cache: _TwoParts, start: int, pos) -> None:
+    """What the operator would find only after some of a call's steps were done (it checks the rest)."""
     if k.dim() not in (3, 4):
         raise ValueError(f"{fn}: k {tuple(k.shape)} must be (B, T, {cache.n_kv_heads}, {cache.head_dim})")
+    if cache.window and pos is None and start + k.shape[1] > MAX_POS:
+        raise ValueError(f"{fn}: positions {start} .. {start + k.shape[1] - 1} are outside 0 .. {MAX_POS - 1}")
 
 
 class KVCacheShared(_TwoParts):
@@ -186,7 +190,7 @@ class KVCacheWindow(_TwoParts):
 def _attend(fn, q, k, v, norms, cos, sin, cache, layer, start_pos, lengths):
     start, pos = _place(fn, start_pos, lengths)
     refuse_grad(fn, q, k, v)
-    _check_tokens(fn, k, cache)
+    _check_tokens(fn, k, cache, start, pos)
     T, out = k.shape[1], []
     for lo, hi in cache._pieces(T):
         s, p, n = _at(lo, hi, T, start, pos, lengths)

@@ -348,3 +348,18 @@ def test_sizes_that_overflow_are_refused():
         for call in (lambda p: _lib.capi().fp_seg_attention(p, 100, 64, 1 << 40, None),
                      lambda p: _lib.capi().fp_seg_write(p, None)):
             assert call(ctypes.byref(SegArgs(**(a | kw)))) == 2, kw
+
+
+@gpu
+@pytest.mark.parametrize("T", [200, 129, 64])
+def test_a_call_in_steps_past_the_last_position_writes_nothing(T):
+    g = torch.Generator().manual_seed(0)
+    c, _ = new_window(50, 4, 2, 64, 1)
+    q, k = randn(g, 1, T, 4, 64).to(DEV), randn(g, 1, T, 2, 64).to(DEV)
+    start = (1 << 30) - T + 1
+    for call in (lambda: fk.attention_window(q, k, k, c, 0, start), lambda: c.write(0, k, k, start)):
+        with pytest.raises(ValueError, match="outside"):
+            call()
+    assert not c.k[0].any() and not c.v[0].any()
+    fk.attention_window(q, k, k, c, 0, start - 1)
+    assert c.k[0].any()
