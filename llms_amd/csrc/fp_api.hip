@@ -273,9 +273,9 @@ int check_w4(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t 
 bool off2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }
 bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) != 0; }
 
-// Arguments of an 8-bit integer call but for its pointers. Sums stay within int32 (127^2 K), 128 weight
-// rows within 32-bit offsets, the
-// grids' column workgroups (64 columns at least) within 65535 and their threads under 2^32.
+// Arguments of an 8-bit integer call but for its pointers. Sums stay within int32 (127^2 K, and with codes of -128),
+// 128 weight rows within 32-bit offsets. The general kernel's grid is eight column tiles (of 32 columns at least) by
+// row tiles of 128 in x and the rest of the columns in y: y within 65535, the threads of each under 2^32.
 int check_w8a8(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldy, int64_t ldq) {
   if (M < 0 || N < 1 || K < 1) return FP_ERR_SHAPE;
   if (N > 65535 * 64 || K > (int64_t)1 << 17 || M >= (int64_t)1 << 24 ||

@@ -757,7 +757,7 @@ __global__ __launch_bounds__(256, RT > 2 ? 1 : 2) void seg_tiles_kernel(SegArgs 
     // 2^127 (floating point, so p is no less exact for that), and past it the sums are infinite and the item is
     // done again.
     // (The two ways have their own softmax, and the empty statement keeps them apart: where they meet before it
-    // the scores are moved twice, 64 of 150 instructions beside the products.)
+    // the scores are moved twice, 64 instructions a tile.)
     if (careful || mask || !ready) {
       if (mask || careful) {
 #pragma unroll

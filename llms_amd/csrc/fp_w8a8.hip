@@ -18,7 +18,7 @@
 // times a power of two, r exact and the tie rounded as one).
 //
 //   - w8a8_prep_kernel: tokens into codes in the workspace, rows of whole 128 (zeros behind K).
-//   - w8a8_rows_kernel: up to 16 tokens.
+//   - w8a8_rows_kernel: up to 16 tokens, 32 on narrow weights with long rows.
 //   - w8a8_general_kernel: more tokens, weight rows of any alignment.
 #include "fp_common.h"
 #include "fp_launch.h"
